@@ -23,6 +23,7 @@ HX_E_TOO_LARGE = -5
 
 HX_DTYPE_BF16 = 0
 HX_DTYPE_FP16 = 1
+HX_DTYPE_FP32 = 2
 
 HX_WERR_BAD_PAGE = 1
 HX_WERR_CLAMPED_LEN = 2
@@ -209,6 +210,43 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ctypes.c_int,
         [_c_void_p, _i64, _i64, _c_void_p, _i64, _i32, _i32, _i32,
          _c_void_p, _f32, _c_void_p, _i64, _i32, _c_void_p, _i64, _c_void_p],
+    ),
+    "hx_int4_gemm": (
+        ctypes.c_int,
+        [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _i32, _i32,
+         _c_void_p, _f32, _c_void_p, _i64, _i32, _c_void_p, _i64, _c_void_p],
+    ),
+    "hx_int4_dequantize": (
+        ctypes.c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _i32, _i32, _i32, _i32, _c_void_p, _i64, _c_void_p],
+    ),
+    "hx_kv_block_bounds": (
+        ctypes.c_int,
+        [_c_void_p, _c_void_p, _i32, _i32, _i32, _i32, _i32, _i32,
+         _c_void_p, _i64, _i32, _c_void_p, _c_void_p, _i32, _i32, _c_void_p],
+    ),
+    "hx_select_blocks": (
+        ctypes.c_int,
+        [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i64,
+         _i32, _i32, _i32, _i32, _c_void_p, _i32, _i32, _i32,
+         _c_void_p, _i64, _i32, _i32, _i32, _i32, _i32, _c_void_p, _c_void_p],
+    ),
+    "hx_block_sparse_workspace_bytes": (_size, [_i64, _i32, _i32, _i32, _i32, _i32]),
+    "hx_block_sparse_attn": (
+        ctypes.c_int,
+        [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i64,
+         _c_void_p, _c_void_p, _i32, _i32, _i32, _c_void_p, _i32,
+         _c_void_p, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _i32,
+         _c_void_p, _i64, _i64, _c_void_p, _size, _c_void_p],
+    ),
+    "hx_logit_rules_workspace_bytes": (_size, [_i64, _i64]),
+    "hx_logit_rules": (
+        ctypes.c_int,
+        [_c_void_p, _i64, _i64, _i64, _i32,
+         _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
+         _c_void_p, _c_void_p, _c_void_p,
+         _c_void_p, _c_void_p, _i64, _i32, _c_void_p, _i64,
+         _c_void_p, _i64, _c_void_p, _c_void_p, _size, _c_void_p],
     ),
     "hx_logits_workspace_bytes": (_size, [_i64, _i64, _i32]),
     "hx_final_norm_logits_argmax": (

@@ -19,7 +19,7 @@ CSRC = PACKAGE_DIR / "csrc"
 INCLUDE = PACKAGE_DIR.parent / "include"
 LIBRARY = PACKAGE_DIR / "libhelios_paged.so"
 SOURCES = ("kv_ops.hip", "paged_attn.hip", "tick_meta.hip", "qk_rope.hip", "block_ops.hip", "skinny_gemm.hip",
-           "logits.hip")
+           "logits.hip", "int4_gemm.hip", "logit_rules.hip", "block_sparse.hip")
 ARCH = "gfx950"
 
 

@@ -1,0 +1,782 @@
+// Attention over selected blocks of the paged KV cache (gfx950): the key bounds of each block,
+// the selection by them, and the attention that reads the selected blocks only.
+//
+// A block is `block` consecutive tokens of a page (a power of two from 16 that divides the
+// page). Per block and KV head
+//   lower[d] = min_j k_j[d],  upper[d] = max_j k_j[d]           (block_bounds_kernel)
+// bound the scores of its keys: q . k_j <= sum_d max(q[d] lower[d], q[d] upper[d]). Summed over
+// the G query heads that share the KV head the bound is linear in two vectors,
+//   s = sum_d (sum_g min(q_g[d], 0)) lower[d] + (sum_g max(q_g[d], 0)) upper[d],
+// and the blocks with the largest s, with the first `sink` and the last `recent` ones, are the
+// row's selection for that KV head (select_blocks_kernel). The attention is the softmax over
+// the keys of those blocks alone (sparse_attn_kernel).
+
+#include "hx_common.h"
+
+namespace {
+
+// ------------------------------------------------------------------------- key bounds
+//
+// The bounds of every block that a tick's new tokens touched, from all of its keys so far and
+// never from its former bounds: a dropped draft or a reused page leaves no trace in them, and
+// the order of ticks none either. At most `block` keys are read for a sequence's first block.
+// A workgroup takes one block and 32 16-byte pieces of the key rows, eight tokens at a time.
+
+constexpr int kBdThreads = 256;
+constexpr int kBdPieces = 32, kBdTokens = kBdThreads / kBdPieces;
+
+typedef short s16x2_t __attribute__((ext_vector_type(2)));
+
+struct BoundsArgs {
+  const uint16_t* k;
+  uint16_t* bounds;  // [num_pages][page / block][heads][2][head_dim]
+  int32_t num_pages, page, block, pieces, pieces_head;  // 16-byte pieces of a token row, of a head
+  const int32_t* table;
+  int64_t table_stride;
+  int32_t table_width;
+  const int32_t* cu_q;
+  const int32_t* used;
+  int32_t groups, chunks;  // workgroups along a sequence's blocks and along the pieces
+  uint16_t inf;            // bits of the type's infinity
+};
+
+// bf16 / fp16 bits in the order of their values as signed integers, and back (an involution).
+__device__ __forceinline__ s16x2_t ordered(s16x2_t x) { return x ^ ((x >> 15) & (short)0x7fff); }
+
+__global__ __launch_bounds__(kBdThreads) void block_bounds_kernel(BoundsArgs a) {
+  __shared__ s16x2_t s_low[kBdTokens][kBdPieces][4], s_high[kBdTokens][kBdPieces][4], s_mag[kBdTokens][kBdPieces][4];
+  const int tid = hx::tid_x(), at = tid % kBdPieces, tl = tid / kBdPieces;
+  int wg = hx::wg_x();
+  const int piece = wg % a.chunks * kBdPieces + at;
+  wg /= a.chunks;
+  const int g = wg % a.groups, b = wg / a.groups;
+  const int len = a.used[b], fresh = min(a.cu_q[b + 1] - a.cu_q[b], len);
+  if (fresh <= 0) return;
+  const int per_page = a.page / a.block, last = (len - 1) / a.block;
+  for (int j = (len - fresh) / a.block + g; j <= last; j += a.groups) {
+    if (j / per_page >= a.table_width) return;
+    const int page = a.table[(int64_t)b * a.table_stride + j / per_page];
+    if (page < 0 || page >= a.num_pages) continue;  // uniform over the workgroup
+    const int64_t block0 = (int64_t)page * per_page + j % per_page;
+    const int keys = min(a.block, len - j * a.block);
+    s16x2_t low[4], high[4], mag[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      low[q] = s16x2_t{0x7fff, 0x7fff};
+      high[q] = s16x2_t{(short)0x8000, (short)0x8000};
+      mag[q] = s16x2_t{0, 0};
+    }
+    if (piece < a.pieces) {
+      const uint4* p = reinterpret_cast<const uint4*>(a.k) + block0 * a.block * a.pieces + piece;
+#pragma unroll 8
+      for (int i = tl; i < keys; i += kBdTokens) {
+        const uint4 u = p[(int64_t)i * a.pieces];
+        const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const s16x2_t x = __builtin_bit_cast(s16x2_t, wd[q]), o = ordered(x);
+          low[q] = __builtin_elementwise_min(low[q], o);
+          high[q] = __builtin_elementwise_max(high[q], o);
+          mag[q] = __builtin_elementwise_max(mag[q], (s16x2_t)(x & (short)0x7fff));
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      s_low[tl][at][q] = low[q];
+      s_high[tl][at][q] = high[q];
+      s_mag[tl][at][q] = mag[q];
+    }
+    __syncthreads();
+    if (tl == 0 && piece < a.pieces) {
+      uint32_t lo[4], hi[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+#pragma unroll
+        for (int t = 1; t < kBdTokens; ++t) {
+          low[q] = __builtin_elementwise_min(low[q], s_low[t][at][q]);
+          high[q] = __builtin_elementwise_max(high[q], s_high[t][at][q]);
+          mag[q] = __builtin_elementwise_max(mag[q], s_mag[t][at][q]);
+        }
+        s16x2_t l = ordered(low[q]), h = ordered(high[q]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if ((uint16_t)mag[q][e] > a.inf) l[e] = h[e] = 0x7fff;  // a NaN key: both bounds NaN
+        lo[q] = __builtin_bit_cast(uint32_t, l);
+        hi[q] = __builtin_bit_cast(uint32_t, h);
+      }
+      const int64_t row = block0 * (a.pieces / a.pieces_head) + piece / a.pieces_head;
+      uint4* out = reinterpret_cast<uint4*>(a.bounds) + row * 2 * a.pieces_head + piece % a.pieces_head;
+      out[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      out[a.pieces_head] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    }
+    __syncthreads();
+  }
+}
+
+// -------------------------------------------------------------------------- selection
+//
+// A workgroup takes one query row and KV head. The scores are 64-bit sums: the blocks at the
+// border of a selection lie close together, and a sum in another order would choose others.
+// The r-th largest of the free blocks' keys is found bit by bit (a bit is set when r keys
+// still reach it), from the highest bit in which the keys differ.
+
+constexpr int kSelThreads = 256;
+constexpr int kSelMaxBlocks = 16384;  // 64-bit keys in LDS
+
+struct SelectArgs {
+  const uint16_t* q;
+  int64_t q_row, q_head, q_rows;
+  const int64_t* rows;     // query row of each selection (null: itself)
+  const int32_t* row_seq;  // its sequence (null: itself)
+  const int32_t* keys;
+  int32_t n_heads, group, head_dim;
+  const uint16_t* bounds;
+  int32_t num_pages, page, block;
+  const int32_t* table;
+  int64_t table_stride;
+  int32_t batch, table_width;
+  int32_t budget, sink, recent;
+  int32_t* out;
+};
+
+__device__ __forceinline__ uint64_t ordered_key(double s) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, s + 0.0);  // -0 like 0
+  if ((u & 0x7fffffffffffffffull) > 0x7ff0000000000000ull) return 0xfff0000000000000ull;  // NaN like +inf
+  return (u >> 63) ? ~u : u | 0x8000000000000000ull;
+}
+
+__device__ __forceinline__ double add_xor(double v, int m) { return v + __shfl_xor(v, m); }
+
+template <typename T>
+__global__ __launch_bounds__(kSelThreads) void select_blocks_kernel(SelectArgs a) {
+  typedef hx::Elem<T> E;
+  extern __shared__ __attribute__((aligned(16))) uint64_t s_key[];
+  __shared__ double s_q[2][256];  // sums over the group of min(q, 0) and of max(q, 0)
+  const int tid = hx::tid_x();
+  const int64_t i = hx::wg_x() / a.n_heads;
+  const int h = hx::wg_x() % a.n_heads;
+  int32_t* out = a.out + (int64_t)hx::wg_x() * a.budget;
+  const int64_t row = a.rows != nullptr ? a.rows[i] : i;
+  const int64_t seq = a.row_seq != nullptr ? a.row_seq[i] : i;
+  int64_t n = max(a.keys[i], 0);
+  n = min(n, (int64_t)a.table_width * a.page);
+  if (seq < 0 || seq >= a.batch || row < 0 || row >= a.q_rows) n = 0;
+  const int count = (int)((n + a.block - 1) / a.block);
+  if (count <= a.budget) {
+    for (int j = tid; j < a.budget; j += kSelThreads) out[j] = j < count ? j : -1;
+    return;
+  }
+  for (int d = tid; d < a.head_dim; d += kSelThreads) {
+    double neg = 0.0, pos = 0.0;
+    for (int g = 0; g < a.group; ++g) {
+      const float x = E::lo(a.q[row * a.q_row + (int64_t)(h * a.group + g) * a.q_head + d]);
+      // By the sign bit: a NaN counts in one of the sums.
+      if (__float_as_uint(x) >> 31) neg += (double)x;
+      else pos += (double)x;
+    }
+    s_q[0][d] = neg;
+    s_q[1][d] = pos;
+  }
+  __syncthreads();
+  // 16 lanes a block, 8 dims a lane.
+  const int li = tid & 15, per_page = a.page / a.block;
+  const int free_end = count - a.recent;
+  for (int j = tid >> 4; j < count; j += kSelThreads / 16) {
+    const int page = a.table[seq * a.table_stride + j / per_page];
+    double s = 0.0;
+    const bool bad = page < 0 || page >= a.num_pages;
+    if (!bad) {
+      const uint16_t* lo = a.bounds + (((int64_t)page * per_page + j % per_page) * a.n_heads + h) * 2 * a.head_dim;
+      for (int d = 8 * li; d < a.head_dim; d += 128) {
+        const uint4 l4 = *reinterpret_cast<const uint4*>(lo + d), h4 = *reinterpret_cast<const uint4*>(lo + a.head_dim + d);
+        const uint32_t lw[4] = {l4.x, l4.y, l4.z, l4.w}, hw[4] = {h4.x, h4.y, h4.z, h4.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          s = fma((double)E::lo(lw[q]), s_q[0][d + 2 * q], s);
+          s = fma((double)E::hi(lw[q]), s_q[0][d + 2 * q + 1], s);
+          s = fma((double)E::lo(hw[q]), s_q[1][d + 2 * q], s);
+          s = fma((double)E::hi(hw[q]), s_q[1][d + 2 * q + 1], s);
+        }
+      }
+    }
+    s = add_xor(add_xor(add_xor(add_xor(s, 1), 2), 4), 8);
+    // Blocks taken in any case stay out of the search (0 is below every key); a page
+    // outside the pool comes last.
+    if (li == 0) s_key[j] = j < a.sink || j >= free_end ? 0 : bad ? 1 : ordered_key(s);
+  }
+  __syncthreads();
+  if (tid >= 64) return;
+  const int need = a.budget - a.sink - a.recent;
+  uint64_t any = 0, all = ~0ull;
+  for (int j = a.sink + tid; j < free_end; j += 64) {
+    any |= s_key[j];
+    all &= s_key[j];
+  }
+  for (int m = 1; m < 64; m <<= 1) {
+    any |= __shfl_xor((unsigned long long)any, m);
+    all &= __shfl_xor((unsigned long long)all, m);
+  }
+  const uint64_t differ = any ^ all;
+  // The bits above the first difference are everyone's.
+  uint64_t least = differ == 0 ? all : all & ~((2ull << (63 - __builtin_clzll(differ))) - 1ull);
+  int reach = free_end - a.sink;  // keys >= least
+  if (need == 0) least = ~0ull, reach = 0;
+  for (int bit = differ == 0 ? -1 : 63 - __builtin_clzll(differ); bit >= 0 && reach > need; --bit) {
+    const uint64_t cand = least | 1ull << bit;
+    int c = 0;
+    for (int j = a.sink + tid; j < free_end; j += 64) c += s_key[j] >= cand;
+    for (int m = 1; m < 64; m <<= 1) c += __shfl_xor(c, m);
+    if (c >= need) {
+      least = cand;
+      reach = c;
+    }
+  }
+  // Of the keys equal to the threshold the first ones are taken.
+  int above = 0;
+  for (int j = a.sink + tid; j < free_end; j += 64) above += s_key[j] > least;
+  for (int m = 1; m < 64; m <<= 1) above += __shfl_xor(above, m);
+  int ties = need - above, at = 0;
+  for (int j0 = 0; j0 < count; j0 += 64) {
+    const int j = j0 + tid;
+    const bool kept = j < count && (j < a.sink || j >= free_end);
+    const bool free_block = j < count && !kept;
+    const bool tie = free_block && s_key[j] == least;
+    const uint64_t before = (1ull << tid) - 1ull;
+    const uint64_t tied = __builtin_amdgcn_ballot_w64(tie);
+    const bool take = kept || (free_block && s_key[j] > least) || (tie && __builtin_popcountll(tied & before) < ties);
+    ties -= __builtin_popcountll(tied);  // at 0 or below no later tie is taken
+    const uint64_t taken = __builtin_amdgcn_ballot_w64(take);
+    const int to = at + __builtin_popcountll(taken & before);
+    if (take && to < a.budget) out[to] = j;
+    at += __builtin_popcountll(taken);
+  }
+}
+
+// -------------------------------------------------------------------------- attention
+//
+// One query row and KV head to a workgroup and split: the G query heads (8 at a time) share
+// each K / V read, which HBM bounds. The list's blocks are cut into units of 16 tokens; a wave
+// takes two units (32 keys) at a time through its own part of LDS, the next two in flight in
+// registers meanwhile, so the waves never wait for one another. Rows past a sequence's keys
+// are read past the end of the unit's buffer resource and come back as zeros: what a page
+// holds behind its last key never reaches the sums.
+//
+// S^T = K Q^T has the query heads as its columns, twice: of each key's weight p, columns 0-7
+// carry the leading bits of the element type into P V and columns 8-15 the remainder, so one
+// MFMA sums both, and P has 16 (fp16: 22) bits. S^T's registers are the P operand as they are.
+// bf16 weights are scaled down by 2^24, which their range has room for: values up to the
+// type's largest then cannot leave fp32 in the sums over a list's keys.
+
+constexpr int kSpWaves = 4;
+constexpr int kSpHeads = 8;       // query heads of a workgroup
+constexpr int kSpMaxUnits = 64;   // 16-token units of a split
+constexpr float kSpLog2e = 1.44269504088896340736f;
+
+struct SparseArgs {
+  const uint16_t* q;
+  int64_t q_row, q_head, q_rows;
+  const int64_t* rows;
+  const int32_t* row_seq;
+  const int32_t* keys;
+  const uint16_t* k;
+  const uint16_t* v;
+  int32_t num_pages, page, block;
+  const int32_t* blocks;  // [n][n_heads][budget]
+  int32_t budget;
+  const int32_t* table;
+  int64_t table_stride;
+  int32_t batch, table_width;
+  int32_t n_heads, group, head_dim, head_blocks;
+  float scale_log2;
+  uint16_t* out;
+  int64_t out_row, out_head;
+  float* part_o;  // [n][query heads][splits][head_dim]
+  float* part_ml; // [n][query heads][splits][2]
+  int32_t splits, units;  // units of a split, even
+};
+
+// LDS slot of 16-byte piece p of tile row r: a fragment read (16 rows, one piece each) and a
+// transposing read (4 rows, two pieces each) then spread over the banks.
+template <int DP>
+__device__ __forceinline__ int sp_piece(int r, int p) {
+  return DP == 64 ? p ^ ((r >> 1) & 7) : p ^ (r & 15);
+}
+
+// The leading bits of p >= 0 in the element type, rounded down.
+template <typename T>
+__device__ __forceinline__ float leading(float p);
+template <>
+__device__ __forceinline__ float leading<__bf16>(float p) { return __uint_as_float(__float_as_uint(p) & 0xffff0000u); }
+template <>
+__device__ __forceinline__ float leading<_Float16>(float p) {
+  return (float)__builtin_amdgcn_cvt_pkrtz(p, 0.f)[0];
+}
+
+// Powers of two by which the weights are scaled down (fp16 values never sum beyond fp32).
+template <typename T>
+__device__ __forceinline__ constexpr float weight_bias() { return __is_same(T, __bf16) ? 24.f : 0.f; }
+
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a) {
+  typedef hx::Elem<T> E;
+  typedef typename E::v8 v8;
+  constexpr int kRowBytes = 2 * DP, kPieces = DP / 8, kSteps = DP / 32, kDims = DP / 16;
+  constexpr int kPerLoad = 64 / kPieces, kLoads = 16 / kPerLoad;  // tokens a load, loads a unit
+  constexpr int kTile = 32 * kRowBytes;
+  constexpr int kStage = 2 * kTile;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kSpWaves * kStage];
+  __shared__ int64_t s_row[kSpMaxUnits];
+  __shared__ int s_cnt[kSpMaxUnits];
+  __shared__ float s_m[kSpWaves][kSpHeads], s_l[kSpWaves][kSpHeads];
+  const int tid = hx::tid_x(), lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int wg = hx::wg_x();
+  const int split = wg % a.splits;
+  wg /= a.splits;
+  const int hb = wg % a.head_blocks;
+  wg /= a.head_blocks;
+  const int h = wg % a.n_heads;
+  const int64_t i = wg / a.n_heads;
+  const int64_t row = a.rows != nullptr ? a.rows[i] : i;
+  const int64_t seq = a.row_seq != nullptr ? a.row_seq[i] : i;
+  if (row < 0 || row >= a.q_rows) return;  // no such query, and no such output row
+  int64_t n = min((int64_t)max(a.keys[i], 0), (int64_t)a.table_width * a.page);
+  if (seq < 0 || seq >= a.batch) n = 0;
+  const int per_page = a.page / a.block, per_block = a.block / 16;
+  const int64_t row_elems = (int64_t)a.n_heads * a.head_dim;
+
+  if (tid < a.units) {
+    const int u = split * a.units + tid, e = u / per_block;
+    int64_t at = 0;
+    int cnt = 0;
+    if (e < a.budget) {
+      const int64_t j = a.blocks[((int64_t)i * a.n_heads + h) * a.budget + e];
+      const int64_t token = j * a.block + u % per_block * 16;
+      if (j >= 0 && token < n) {
+        const int page = a.table[seq * a.table_stride + j / per_page];
+        if (page >= 0 && page < a.num_pages) {
+          at = (int64_t)page * a.page + token % a.page;
+          cnt = (int)min((int64_t)16, n - token);
+        }
+      }
+    }
+    s_row[tid] = at;
+    s_cnt[tid] = cnt;
+  }
+
+  const int heads = min(kSpHeads, a.group - hb * kSpHeads);
+  const int head0 = h * a.group + hb * kSpHeads;
+  v8 qf[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    uint4 u = hx::zero4();
+    const int d = 32 * s + 8 * lg;
+    if ((lr & 7) < heads && d < a.head_dim)
+      u = *reinterpret_cast<const uint4*>(a.q + row * a.q_row + (int64_t)(head0 + (lr & 7)) * a.q_head + d);
+    qf[s] = hx::as_v8<T>(u);
+  }
+  __syncthreads();
+
+  // Lane l of a load takes piece l % kPieces of token l / kPieces; a piece past the head's
+  // dims is read past the buffer's end (zeros).
+  const uint32_t row_bytes = (uint32_t)row_elems * 2;
+  const int piece = lane % kPieces, ltok = lane / kPieces;
+  const uint32_t voff = 8 * piece < a.head_dim ? ltok * row_bytes + 16 * piece : 0x7ffffff0u;
+  uint4 kb[2][kLoads], vb[2][kLoads];
+  auto load = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int64_t at = s_row[2 * tile + u];
+      const int cnt = __builtin_amdgcn_readfirstlane(s_cnt[2 * tile + u]);
+      const int64_t pool_row = (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at) |
+                               (int64_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32;
+      const int64_t base = pool_row * row_elems + (int64_t)h * a.head_dim;
+      const uint32_t bytes = cnt > 0 ? (uint32_t)(cnt - 1) * row_bytes + 2 * a.head_dim : 0u;
+      const __amdgpu_buffer_rsrc_t kr = hx::buffer_rsrc(a.k + base, bytes), vr = hx::buffer_rsrc(a.v + base, bytes);
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) {
+        // All of the offset in the vector part: the range check is on it alone.
+        kb[u][q] = hx::ld16_stream(kr, voff + q * kPerLoad * row_bytes, 0);
+        vb[u][q] = hx::ld16_stream(vr, voff + q * kPerLoad * row_bytes, 0);
+      }
+    }
+  };
+
+  uint8_t* const kt = smem + w * kStage;
+  uint8_t* const vt = kt + kTile;
+  float m_run = -INFINITY, l_run = 0.f;
+  hx::f32x4_t o[kDims];
+#pragma unroll
+  for (int d = 0; d < kDims; ++d) o[d] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  const int tiles = a.units / 2;
+  auto live = [&](int tile) __attribute__((always_inline)) {
+    return __builtin_amdgcn_readfirstlane(s_cnt[2 * tile] | s_cnt[2 * tile + 1]) != 0;
+  };
+  // The wave's next tile with a key in it.
+  auto next = [&](int tile) __attribute__((always_inline)) {
+    while (tile < tiles && !live(tile)) tile += kSpWaves;
+    return tile;
+  };
+  int tile = next(w);
+  if (tile < tiles) load(tile);
+  while (tile < tiles) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) {
+        const int r = 16 * u + q * kPerLoad + ltok;
+        const int to = r * kRowBytes + 16 * sp_piece<DP>(r, piece);
+        *reinterpret_cast<uint4*>(kt + to) = kb[u][q];
+        *reinterpret_cast<uint4*>(vt + to) = vb[u][q];
+      }
+    // Lanes read what other lanes of the wave stored: a wave's LDS accesses complete in order,
+    // the fences hold the compiler to it.
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    int cnt[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) cnt[u] = __builtin_amdgcn_readfirstlane(s_cnt[2 * tile + u]);
+    tile = next(tile + kSpWaves);
+    if (tile < tiles) load(tile);
+
+    hx::f32x4_t sc[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      sc[u] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int r = 16 * u + lr;
+        const uint4 kf = *reinterpret_cast<const uint4*>(kt + r * kRowBytes + 16 * sp_piece<DP>(r, 4 * s + lg));
+        sc[u] = E::mfma16x16x32(hx::as_v8<T>(kf), qf[s], sc[u]);
+      }
+    }
+    float mx = m_run;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sc[u][e] = 4 * lg + e < cnt[u] ? sc[u][e] * a.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, sc[u][e]);
+      }
+    mx = hx::max_xor32(hx::max_xor16(mx));
+    const float alpha = mx == -INFINITY ? 1.f : hx::fast_exp2(m_run - mx);
+    const float neg = mx == -INFINITY ? 0.f : -mx - weight_bias<T>();
+    m_run = mx;
+    l_run *= alpha;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) o[d] *= alpha;
+    uint32_t pw[4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = hx::fast_exp2(sc[u][e] + neg);
+        l_run += p;
+        const float top = leading<T>(p);
+        x[e] = lr < 8 ? top : p - top;
+      }
+      pw[2 * u] = hx::pack2_round<T>(x[0], x[1]);
+      pw[2 * u + 1] = hx::pack2_round<T>(x[2], x[3]);
+    }
+    const v8 pf = hx::as_v8<T>(make_uint4(pw[0], pw[1], pw[2], pw[3]));
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) {
+      uint2 f[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int r = 16 * u + 4 * lg + (lr >> 2);
+        f[u] = hx::ld8_lds_tr16(vt + r * kRowBytes + 16 * sp_piece<DP>(r, 2 * d + ((lr & 3) >> 1)) + 8 * (lr & 1));
+      }
+      o[d] = E::mfma16x16x32(hx::as_v8<T>(make_uint4(f[0].x, f[0].y, f[1].x, f[1].y)), pf, o[d]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+
+  // Lane: dims 16 d + 4 lg .. + 3 of head lr % 8; both halves of P summed.
+  l_run = hx::add_xor32(hx::add_xor16(l_run));
+#pragma unroll
+  for (int d = 0; d < kDims; ++d)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[d][e] += hx::dpp<0x128>(o[d][e]);  // the lane 8 apart in its row of 16
+  __syncthreads();  // every wave is done with its stage
+  float (*const s_o)[kSpHeads][DP] = reinterpret_cast<float (*)[kSpHeads][DP]>(smem);
+  if (lr < kSpHeads) {
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+      *reinterpret_cast<float4*>(&s_o[w][lr][16 * d + 4 * lg]) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+    if (lg == 0) {
+      s_m[w][lr] = m_run;
+      s_l[w][lr] = l_run;
+    }
+  }
+  __syncthreads();
+  const int half = a.head_dim / 2;  // head_dim is a multiple of 8
+  for (int e = tid; e < heads * half; e += 64 * kSpWaves) {
+    const int hd = e / half, d = 2 * (e % half);
+    float m = s_m[0][hd];
+#pragma unroll
+    for (int ww = 1; ww < kSpWaves; ++ww) m = fmaxf(m, s_m[ww][hd]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+    for (int ww = 0; ww < kSpWaves; ++ww) {
+      const float f = hx::fast_exp2(s_m[ww][hd] - ref);
+      l = fmaf(f, s_l[ww][hd], l);
+      x = fmaf(f, s_o[ww][hd][d], x);
+      y = fmaf(f, s_o[ww][hd][d + 1], y);
+    }
+    const int64_t head = head0 + hd;
+    if (a.splits == 1) {
+      const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+      *reinterpret_cast<uint32_t*>(a.out + row * a.out_row + head * a.out_head + d) = hx::pack2_round<T>(x * inv, y * inv);
+    } else {
+      const int64_t p = (i * a.n_heads * a.group + head) * a.splits + split;
+      *reinterpret_cast<float2*>(a.part_o + p * a.head_dim + d) = make_float2(x, y);
+      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * p) = make_float2(m, l);
+    }
+  }
+}
+
+// The splits of a row and query head, in order; one wave each.
+template <typename T>
+__global__ __launch_bounds__(256) void sparse_combine_kernel(SparseArgs a, int64_t heads_total) {
+  const int lane = hx::tid_x() & 63;
+  const int64_t t = (int64_t)hx::wg_x() * 4 + (hx::tid_x() >> 6);
+  if (t >= heads_total) return;
+  const int64_t n_q = (int64_t)a.n_heads * a.group, i = t / n_q, head = t % n_q;
+  const int64_t row = a.rows != nullptr ? a.rows[i] : i;
+  if (row < 0 || row >= a.q_rows) return;
+  const float* ml = a.part_ml + 2 * t * a.splits;
+  float m = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[2 * s]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  for (int d = 2 * lane; d < a.head_dim; d += 128) {
+    float l = 0.f, x = 0.f, y = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+      const float f = hx::fast_exp2(ml[2 * s] - ref);
+      const float2 o = *reinterpret_cast<const float2*>(a.part_o + (t * a.splits + s) * a.head_dim + d);
+      l = fmaf(f, ml[2 * s + 1], l);
+      x = fmaf(f, o.x, x);
+      y = fmaf(f, o.y, y);
+    }
+    const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+    *reinterpret_cast<uint32_t*>(a.out + row * a.out_row + head * a.out_head + d) = hx::pack2_round<T>(x * inv, y * inv);
+  }
+}
+
+struct Split {
+  int32_t units, splits;
+};
+
+// Splits of a row's list: about four workgroups a CU where the rows and heads alone give fewer,
+// of at least 128 and at most 1024 keys.
+Split sparse_split(int64_t n, int32_t n_heads, int32_t head_blocks, int32_t budget, int32_t block) {
+  const int64_t row_heads = n * n_heads * head_blocks, total = (int64_t)budget * (block / 16);
+  const int64_t want = (1024 + row_heads - 1) / row_heads;
+  int64_t units = ((total + want - 1) / want + 7) / 8 * 8;
+  units = units < 8 ? 8 : units > kSpMaxUnits ? kSpMaxUnits : units;
+  return {(int32_t)units, (int32_t)((total + units - 1) / units)};
+}
+
+template <typename T, int DP>
+void launch_sparse(const SparseArgs& a, int64_t n, hipStream_t s) {
+  const dim3 grid((unsigned)(n * a.n_heads * a.head_blocks * a.splits));
+  hipLaunchKernelGGL((sparse_attn_kernel<T, DP>), grid, dim3(64 * kSpWaves), 0, s, a);
+}
+
+template <typename T>
+void launch_sparse_dims(const SparseArgs& a, int64_t n, hipStream_t s) {
+  if (a.head_dim <= 64) launch_sparse<T, 64>(a, n, s);
+  else if (a.head_dim <= 128) launch_sparse<T, 128>(a, n, s);
+  else launch_sparse<T, 256>(a, n, s);
+  if (a.splits > 1) {
+    const int64_t heads = n * a.n_heads * a.group;
+    hipLaunchKernelGGL(sparse_combine_kernel<T>, dim3((unsigned)((heads + 3) / 4)), dim3(256), 0, s, a, heads);
+  }
+}
+
+bool power_of_two(int32_t x) { return x > 0 && (x & (x - 1)) == 0; }
+
+int check_layout(int32_t num_pages, int32_t page, int32_t block, int32_t n_heads, int32_t head_dim, int32_t dtype) {
+  if (dtype != HX_DTYPE_BF16 && dtype != HX_DTYPE_FP16) return HX_E_UNSUPPORTED;
+  if (num_pages < 1 || page < 1 || n_heads < 1 || head_dim < 1) return HX_E_INVALID_ARG;
+  if (head_dim % 8 || head_dim > 256 || !power_of_two(block) || block < 16 || block > 1024 || page % block)
+    return HX_E_UNSUPPORTED;
+  if ((int64_t)n_heads * head_dim > (1 << 24)) return HX_E_UNSUPPORTED;  // a unit within a buffer resource
+  return HX_OK;
+}
+
+}  // namespace
+
+extern "C" int hx_kv_block_bounds(const void* k_pool, void* bounds, int32_t num_pages, int32_t page_size,
+                                  int32_t block_size, int32_t n_kv_heads, int32_t head_dim, int32_t dtype,
+                                  const int32_t* block_table, int64_t block_table_stride, int32_t block_table_width,
+                                  const int32_t* cu_seq_q, const int32_t* seqused_k, int32_t batch, int32_t max_q,
+                                  void* stream) {
+  const int bad = check_layout(num_pages, page_size, block_size, n_kv_heads, head_dim, dtype);
+  if (bad != HX_OK) return bad;
+  if (batch < 0 || max_q < 0 || block_table_width < 1 || block_table_stride < block_table_width)
+    return HX_E_INVALID_ARG;
+  if (batch == 0 || max_q == 0) return HX_OK;
+  if (!k_pool || !bounds || !block_table || !cu_seq_q || !seqused_k ||
+      ((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(bounds)) & 15))
+    return HX_E_INVALID_ARG;
+  BoundsArgs a;
+  a.k = static_cast<const uint16_t*>(k_pool);
+  a.bounds = static_cast<uint16_t*>(bounds);
+  a.num_pages = num_pages;
+  a.page = page_size;
+  a.block = block_size;
+  a.pieces = n_kv_heads * head_dim / 8;
+  a.pieces_head = head_dim / 8;
+  a.table = block_table;
+  a.table_stride = block_table_stride;
+  a.table_width = block_table_width;
+  a.cu_q = cu_seq_q;
+  a.used = seqused_k;
+  a.groups = (max_q - 1) / block_size + 2;
+  a.chunks = (a.pieces + kBdPieces - 1) / kBdPieces;
+  a.inf = dtype == HX_DTYPE_BF16 ? 0x7f80 : 0x7c00;
+  const int64_t wgs = (int64_t)batch * a.groups * a.chunks;
+  if (wgs > 0x7fffffff) return HX_E_UNSUPPORTED;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(block_bounds_kernel, dim3((unsigned)wgs), dim3(kBdThreads), 0, s, a);
+  return hx::status_from_hip(hipGetLastError());
+}
+
+extern "C" int hx_select_blocks(const void* q, int64_t q_row_stride, int64_t q_head_stride, int64_t q_rows,
+                                const int64_t* rows, const int32_t* row_seq, const int32_t* key_counts, int64_t n,
+                                int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t dtype,
+                                const void* bounds, int32_t num_pages, int32_t page_size, int32_t block_size,
+                                const int32_t* block_table, int64_t block_table_stride, int32_t batch,
+                                int32_t block_table_width, int32_t budget, int32_t sink, int32_t recent,
+                                int32_t* blocks, void* stream) {
+  const int bad = check_layout(num_pages, page_size, block_size, n_kv_heads, head_dim, dtype);
+  if (bad != HX_OK) return bad;
+  if (n < 0 || q_rows < 0 || n_q_heads < 1 || n_q_heads % n_kv_heads || batch < 0 || block_table_width < 1 ||
+      block_table_stride < block_table_width || budget < 1 || sink < 0 || recent < 1 ||
+      (int64_t)sink + recent > budget)
+    return HX_E_INVALID_ARG;
+  const int64_t most = (int64_t)block_table_width * (page_size / block_size);
+  if (most > kSelMaxBlocks || n > 0x7fffffff / n_kv_heads) return HX_E_UNSUPPORTED;
+  if (n == 0) return HX_OK;
+  if (!q || !key_counts || !bounds || !block_table || !blocks || (reinterpret_cast<uintptr_t>(q) & 1) ||
+      (reinterpret_cast<uintptr_t>(bounds) & 15) || (rows == nullptr && n > q_rows) ||
+      (row_seq == nullptr && n > batch))
+    return HX_E_INVALID_ARG;
+  SelectArgs a;
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_row = q_row_stride;
+  a.q_head = q_head_stride;
+  a.q_rows = q_rows;
+  a.rows = rows;
+  a.row_seq = row_seq;
+  a.keys = key_counts;
+  a.n_heads = n_kv_heads;
+  a.group = n_q_heads / n_kv_heads;
+  a.head_dim = head_dim;
+  a.bounds = static_cast<const uint16_t*>(bounds);
+  a.num_pages = num_pages;
+  a.page = page_size;
+  a.block = block_size;
+  a.table = block_table;
+  a.table_stride = block_table_stride;
+  a.batch = batch;
+  a.table_width = block_table_width;
+  a.budget = budget;
+  a.sink = sink;
+  a.recent = recent;
+  a.out = blocks;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)(n * n_kv_heads));
+  const size_t lds = (size_t)most * sizeof(uint64_t);
+  const void* fn = dtype == HX_DTYPE_BF16 ? reinterpret_cast<const void*>(select_blocks_kernel<__bf16>)
+                                          : reinterpret_cast<const void*>(select_blocks_kernel<_Float16>);
+  if (lds > 60 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return hx::status_from_hip(e);
+  }
+  if (dtype == HX_DTYPE_BF16) hipLaunchKernelGGL(select_blocks_kernel<__bf16>, grid, dim3(kSelThreads), lds, s, a);
+  else hipLaunchKernelGGL(select_blocks_kernel<_Float16>, grid, dim3(kSelThreads), lds, s, a);
+  return hx::status_from_hip(hipGetLastError());
+}
+
+extern "C" size_t hx_block_sparse_workspace_bytes(int64_t n, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                                  int32_t budget, int32_t block_size) {
+  if (n < 1 || n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads || head_dim < 1 || budget < 1 ||
+      block_size < 16)
+    return 0;
+  const int32_t head_blocks = (n_q_heads / n_kv_heads + kSpHeads - 1) / kSpHeads;
+  const Split sp = sparse_split(n, n_kv_heads, head_blocks, budget, block_size);
+  return sp.splits == 1 ? 0 : (size_t)n * n_q_heads * sp.splits * (head_dim + 2) * sizeof(float);
+}
+
+extern "C" int hx_block_sparse_attn(const void* q, int64_t q_row_stride, int64_t q_head_stride, int64_t q_rows,
+                                    const int64_t* rows, const int32_t* row_seq, const int32_t* key_counts, int64_t n,
+                                    const void* k_pool, const void* v_pool, int32_t num_pages, int32_t page_size,
+                                    int32_t block_size, const int32_t* blocks, int32_t budget,
+                                    const int32_t* block_table, int64_t block_table_stride, int32_t batch,
+                                    int32_t block_table_width, int32_t n_q_heads, int32_t n_kv_heads,
+                                    int32_t head_dim, float scale, int32_t dtype, void* out, int64_t out_row_stride,
+                                    int64_t out_head_stride, void* workspace, size_t workspace_bytes, void* stream) {
+  const int bad = check_layout(num_pages, page_size, block_size, n_kv_heads, head_dim, dtype);
+  if (bad != HX_OK) return bad;
+  if (n < 0 || q_rows < 0 || n_q_heads < 1 || n_q_heads % n_kv_heads || batch < 0 || block_table_width < 1 ||
+      block_table_stride < block_table_width || budget < 1 || budget > (1 << 24))
+    return HX_E_INVALID_ARG;
+  if (n == 0) return HX_OK;
+  if (!q || !key_counts || !k_pool || !v_pool || !blocks || !block_table || !out || (rows == nullptr && n > q_rows) ||
+      (row_seq == nullptr && n > batch))
+    return HX_E_INVALID_ARG;
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) &
+       15) ||
+      q_row_stride % 8 || q_head_stride % 8 || (reinterpret_cast<uintptr_t>(out) & 3) || out_row_stride % 2 ||
+      out_head_stride % 2)
+    return HX_E_INVALID_ARG;
+  SparseArgs a;
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_row = q_row_stride;
+  a.q_head = q_head_stride;
+  a.q_rows = q_rows;
+  a.rows = rows;
+  a.row_seq = row_seq;
+  a.keys = key_counts;
+  a.k = static_cast<const uint16_t*>(k_pool);
+  a.v = static_cast<const uint16_t*>(v_pool);
+  a.num_pages = num_pages;
+  a.page = page_size;
+  a.block = block_size;
+  a.blocks = blocks;
+  a.budget = budget;
+  a.table = block_table;
+  a.table_stride = block_table_stride;
+  a.batch = batch;
+  a.table_width = block_table_width;
+  a.n_heads = n_kv_heads;
+  a.group = n_q_heads / n_kv_heads;
+  a.head_dim = head_dim;
+  a.head_blocks = (a.group + kSpHeads - 1) / kSpHeads;
+  a.scale_log2 = scale * kSpLog2e;
+  a.out = static_cast<uint16_t*>(out);
+  a.out_row = out_row_stride;
+  a.out_head = out_head_stride;
+  const Split sp = sparse_split(n, n_kv_heads, a.head_blocks, budget, block_size);
+  a.splits = sp.splits;
+  a.units = sp.units;
+  a.part_o = a.part_ml = nullptr;
+  if (a.splits > 1) {
+    const size_t parts = (size_t)n * n_q_heads * a.splits;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+        workspace_bytes < parts * (head_dim + 2) * sizeof(float))
+      return HX_E_WORKSPACE;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + parts * head_dim;
+  }
+  if ((double)n * n_kv_heads * a.head_blocks * a.splits > 2147483647.0) return HX_E_UNSUPPORTED;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == HX_DTYPE_BF16) launch_sparse_dims<__bf16>(a, n, s);
+  else launch_sparse_dims<_Float16>(a, n, s);
+  return hx::status_from_hip(hipGetLastError());
+}

@@ -416,6 +416,453 @@ def block_linear(x: torch.Tensor, weight: torch.Tensor, *, norm_weight: torch.Te
     return out
 
 
+# ------------------------------------------- attention over selected blocks of the cache
+def _check_blocks(pool_name: str, pool: torch.Tensor, block_table: torch.Tensor, block_size: int) -> int:
+    """Checks shared by the block operators; the pool's dtype code."""
+    if pool.ndim != 4 or not pool.is_contiguous() or min(pool.shape) < 1:
+        raise ValueError(f"{pool_name} must be a contiguous [pages, page_size, kv_heads, head_dim] pool.")
+    dtype = _SUPPORTED.get(pool.dtype)
+    if dtype is None:
+        raise ValueError(f"{pool_name} must be bfloat16 or float16.")
+    _check_block_size(block_size, pool.shape[1])
+    if pool.shape[3] % 8 or pool.shape[3] > 256:
+        raise ValueError("head_dim must be a multiple of 8 from 8 to 256.")
+    _check_table(block_table)
+    return dtype
+
+
+def _check_block_size(block_size: int, page_size: int) -> None:
+    if not 16 <= block_size <= 1024 or block_size & (block_size - 1) or page_size % block_size:
+        raise ValueError("block_size must be a power of two from 16 to 1024 that divides the page size.")
+
+
+def _check_table(block_table: torch.Tensor) -> None:
+    if block_table.dtype != torch.int32 or block_table.ndim != 2 or block_table.shape[1] < 1 \
+            or (block_table.shape[1] > 1 and block_table.stride(1) != 1) \
+            or (block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]):
+        raise ValueError("block_table must be int32 [batch, width] with contiguous rows.")
+
+
+def _table_stride(block_table: torch.Tensor) -> int:
+    return block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1]
+
+
+def _check_rows(query: torch.Tensor, key_counts: torch.Tensor, rows: torch.Tensor | None,
+                row_seq: torch.Tensor | None, block_table: torch.Tensor) -> int:
+    """Checks of the query rows of a selection; their number."""
+    n = key_counts.numel()
+    for name, t, dtype in (("key_counts", key_counts, torch.int32), ("row_seq", row_seq, torch.int32),
+                           ("rows", rows, torch.int64)):
+        if t is not None and (t.dtype != dtype or t.ndim != 1 or t.numel() != n or not t.is_contiguous()
+                              or t.device != query.device):
+            raise ValueError(f"{name} must be a contiguous {dtype} vector, one entry per query row, on the device.")
+    if rows is None and n != query.shape[0]:
+        raise ValueError("without rows, key_counts must have one entry per query.")
+    if row_seq is None and n > block_table.shape[0]:
+        raise ValueError("without row_seq, the block table must have a row per query row.")
+    return n
+
+
+def kv_block_bounds(k_cache: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, cu_seq_q: torch.Tensor,
+                    seqused_k: torch.Tensor, *, max_q: int) -> None:
+    """Key bounds of the blocks that a tick's new tokens touched, in place, after those tokens
+    are in the pool: ``bounds[page, block, h, 0] / [..., 1]`` is the elementwise lowest /
+    highest key of head h among the block's tokens so far.
+
+    ``k_cache`` ``[pages, page_size, kv_heads, head_dim]`` contiguous, bfloat16 or float16;
+    ``bounds`` ``[pages, page_size // block_size, kv_heads, 2, head_dim]`` contiguous, of its
+    dtype (a block is a power of two of 16 to 1024 tokens); ``block_table`` / ``cu_seq_q`` /
+    ``seqused_k`` as for ``varlen_attn``. A block is read whole and its former bounds never,
+    so a page that was reused or truncated needs no clearing. A NaN key makes both bounds
+    NaN."""
+    device = _require_gpu(k_cache, bounds, block_table, cu_seq_q, seqused_k)
+    if bounds.ndim != 5 or bounds.shape[1] < 1 or k_cache.ndim != 4 or k_cache.shape[1] % bounds.shape[1]:
+        raise ValueError("bounds must be [pages, blocks per page, kv_heads, 2, head_dim].")
+    block_size = k_cache.shape[1] // bounds.shape[1]
+    dtype = _check_blocks("k_cache", k_cache, block_table, block_size)
+    pages, page_size, n_kv, head_dim = k_cache.shape
+    if tuple(bounds.shape) != (pages, page_size // block_size, n_kv, 2, head_dim) or bounds.dtype != k_cache.dtype \
+            or not bounds.is_contiguous():
+        raise ValueError("bounds must be contiguous [pages, blocks per page, kv_heads, 2, head_dim] of the pool's dtype.")
+    batch = seqused_k.numel()
+    for name, t, count in (("cu_seq_q", cu_seq_q, batch + 1), ("seqused_k", seqused_k, batch)):
+        if t.dtype != torch.int32 or t.ndim != 1 or t.numel() != count or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 vector of {count} values.")
+    if block_table.shape[0] != batch:
+        raise ValueError("block_table must have a row per sequence.")
+    if max_q < 0:
+        raise ValueError("max_q must be non-negative.")
+    code = _launch(device, _capi.lib().hx_kv_block_bounds, k_cache.data_ptr(), bounds.data_ptr(), pages, page_size,
+                   block_size, n_kv, head_dim, dtype, block_table.data_ptr(), _table_stride(block_table),
+                   block_table.shape[1], cu_seq_q.data_ptr(), seqused_k.data_ptr(), batch, max_q)
+    _capi.check(code, "hx_kv_block_bounds")
+
+
+def select_blocks(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, key_counts: torch.Tensor,
+                  budget: int, *, block_size: int, sink: int = 1, recent: int = 2, row_seq: torch.Tensor | None = None,
+                  rows: torch.Tensor | None = None) -> torch.Tensor:
+    """The blocks each query row attends to, per KV head: int32 ``[n, kv_heads, budget]``,
+    ascending, -1 behind a row's last.
+
+    ``query`` ``[T, Hq, d]``; entry i of ``key_counts`` (int32 ``[n]``) is the number of keys
+    that query row ``rows[i]`` (int64; None: i) sees of sequence ``row_seq[i]`` (int32; None:
+    i), whose pages are ``block_table[row_seq[i]]``. The first ``sink`` and the last
+    ``recent`` (at least 1) blocks are always among them; the others are those with the largest
+    ``sum_g sum_d max(q_g[d] * lower[d], q_g[d] * upper[d])`` over the query heads g of the KV
+    head, an upper bound of their summed scores, computed in 64 bits (equal ones: the
+    earlier block; NaN: as infinity). A row with no more than ``budget`` blocks gets them all."""
+    device = _require_gpu(query, bounds, block_table, key_counts)
+    if query.ndim != 3 or query.shape[2] < 1 or query.stride(2) != 1:
+        raise ValueError("query must be [rows, n_q_heads, head_dim] with a contiguous head_dim.")
+    dtype = _SUPPORTED.get(query.dtype)
+    if dtype is None or bounds.dtype != query.dtype:
+        raise ValueError("query and bounds must be bfloat16 or float16, of one dtype.")
+    if bounds.ndim != 5 or bounds.shape[3] != 2 or bounds.shape[4] != query.shape[2] or not bounds.is_contiguous() \
+            or min(bounds.shape) < 1:
+        raise ValueError("bounds must be contiguous [pages, blocks per page, kv_heads, 2, head_dim].")
+    n_kv, page_size = bounds.shape[2], bounds.shape[1] * block_size
+    _check_block_size(block_size, page_size)
+    if query.shape[2] % 8 or query.shape[2] > 256:
+        raise ValueError("head_dim must be a multiple of 8 from 8 to 256.")
+    if query.shape[1] < 1 or query.shape[1] % n_kv:
+        raise ValueError(f"GQA needs n_q_heads ({query.shape[1]}) to be a multiple of n_kv_heads ({n_kv}).")
+    _check_table(block_table)
+    if sink < 0 or recent < 1 or sink + recent > budget:
+        raise ValueError("budget must cover sink (at least 0) and recent (at least 1) blocks.")
+    if block_table.shape[1] * bounds.shape[1] > 16384:
+        raise ValueError("a block table may cover at most 16384 blocks; use larger ones.")
+    n = _check_rows(query, key_counts, rows, row_seq, block_table)
+    blocks = torch.empty((n, n_kv, budget), dtype=torch.int32, device=device)
+    code = _launch(
+        device, _capi.lib().hx_select_blocks, query.data_ptr(), query.stride(0), query.stride(1), query.shape[0],
+        None if rows is None else rows.data_ptr(), None if row_seq is None else row_seq.data_ptr(),
+        key_counts.data_ptr(), n, query.shape[1], n_kv, query.shape[2], dtype, bounds.data_ptr(), bounds.shape[0],
+        page_size, block_size, block_table.data_ptr(), _table_stride(block_table), block_table.shape[0],
+        block_table.shape[1], budget, sink, recent, blocks.data_ptr())
+    _capi.check(code, "hx_select_blocks")
+    return blocks
+
+
+def block_sparse_attn(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, blocks: torch.Tensor,
+                      block_table: torch.Tensor, key_counts: torch.Tensor, *, block_size: int,
+                      scale: float | None = None, row_seq: torch.Tensor | None = None,
+                      rows: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of each query row over its listed blocks: ``softmax(scale * q . k) v`` over
+    the keys of ``blocks[i, h // group]`` (int32 ``[n, kv_heads, budget]``, as ``select_blocks``
+    gives them) below ``key_counts[i]``, in fp32, rounded once. Returns ``[T, Hq, d]`` like
+    ``query``.
+
+    ``rows`` / ``row_seq`` / ``key_counts`` / ``block_table`` as for ``select_blocks``; the
+    pools ``[pages, page_size, kv_heads, head_dim]`` contiguous. Entries that are negative or
+    past the keys are skipped, a block listed twice counts twice, a row without any key gets
+    zeros. With ``rows`` (each at most once) only those rows of ``out`` are written: the
+    others stay as they were (zeros when ``out`` is not given). Whatever the pool holds behind
+    a sequence's last key is not read; an infinite or NaN element of a key or value that a
+    row does see makes that row's result infinite or NaN."""
+    device = _require_gpu(query, k_cache, v_cache, blocks, block_table, key_counts)
+    dtype = _check_blocks("k_cache", k_cache, block_table, block_size)
+    if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype or not v_cache.is_contiguous():
+        raise ValueError("Key and value pools must be contiguous, of one shape and dtype.")
+    pages, page_size, n_kv, head_dim = k_cache.shape
+    if query.ndim != 3 or query.shape[2] != head_dim or query.dtype != k_cache.dtype:
+        raise ValueError("query must be [rows, n_q_heads, head_dim] of the pools' dtype.")
+    if query.shape[1] < 1 or query.shape[1] % n_kv:
+        raise ValueError(f"GQA needs n_q_heads ({query.shape[1]}) to be a multiple of n_kv_heads ({n_kv}).")
+    n = _check_rows(query, key_counts, rows, row_seq, block_table)
+    if blocks.dtype != torch.int32 or blocks.ndim != 3 or tuple(blocks.shape[:2]) != (n, n_kv) \
+            or blocks.shape[2] < 1 or not blocks.is_contiguous():
+        raise ValueError("blocks must be contiguous int32 [n, kv_heads, budget].")
+    if out is None:
+        new = torch.empty if rows is None else torch.zeros
+        out = new(query.shape, dtype=query.dtype, device=device)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.device != device or out.stride(2) != 1 \
+            or out.data_ptr() % 4 or out.stride(0) % 2 or out.stride(1) % 2:
+        raise ValueError("out must have the query's shape, dtype and device, a contiguous head_dim and even strides.")
+    if n == 0:
+        return out
+    if query.stride(2) != 1 or query.data_ptr() % 16 or query.stride(0) % 8 or query.stride(1) % 8:
+        query = query.clone(memory_format=torch.contiguous_format)  # 16-byte loads
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+    budget = blocks.shape[2]
+    lib = _capi.lib()
+    ws_bytes = lib.hx_block_sparse_workspace_bytes(n, query.shape[1], n_kv, head_dim, budget, block_size)
+    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
+    code = _launch(
+        device, lib.hx_block_sparse_attn, query.data_ptr(), query.stride(0), query.stride(1), query.shape[0],
+        None if rows is None else rows.data_ptr(), None if row_seq is None else row_seq.data_ptr(),
+        key_counts.data_ptr(), n, k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, block_size,
+        blocks.data_ptr(), budget, block_table.data_ptr(), _table_stride(block_table), block_table.shape[0],
+        block_table.shape[1], query.shape[1], n_kv, head_dim, scale, dtype, out.data_ptr(), out.stride(0),
+        out.stride(1), None if workspace is None else workspace.data_ptr(), ws_bytes)
+    _capi.check(code, "hx_block_sparse_attn")
+    return out
+
+
+# ------------------------------------------------------- products with 4-bit weights
+class Int4Weight(NamedTuple):
+    """A weight matrix ``[rows, k]`` in 4 bits with a scale and a zero point per ``group``
+    elements of k: ``W[n, k] = scales[k // group, n] * (q[n, k] - zeros[k // group, n])``.
+    ``packed`` holds q in the order the kernel reads it (hx_int4_gemm); ``scales`` (bfloat16
+    or float16: the products' dtype) and ``zeros`` (uint8) are ``[groups, rows]``, rows
+    rounded up to 16. Made by ``int4_quantize`` or ``int4_pack``."""
+
+    packed: torch.Tensor
+    scales: torch.Tensor
+    zeros: torch.Tensor
+    rows: int
+    k: int
+    group: int
+
+
+def int4_pack(values: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor) -> Int4Weight:
+    """``Int4Weight`` of integers 0..15 ``values`` ``[rows, k]`` (uint8), ``scales``
+    ``[k / group, rows]`` (bfloat16 or float16) and ``zeros`` (uint8, 0..15) of the same
+    shape; the group (32, 64 or 128) follows from the shapes. Done once per weight, in torch
+    operations, on the tensors' device."""
+    if values.ndim != 2 or values.dtype != torch.uint8 or min(values.shape) < 1:
+        raise ValueError("values must be uint8 [rows, k].")
+    rows, k = values.shape
+    if scales.ndim != 2 or scales.shape[1] != rows or scales.dtype not in _SUPPORTED:
+        raise ValueError("scales must be bfloat16 or float16 [k / group, rows].")
+    if zeros.shape != scales.shape or zeros.dtype != torch.uint8:
+        raise ValueError("zeros must be uint8, of the scales' shape.")
+    if scales.device != values.device or zeros.device != values.device:
+        raise ValueError("All tensors must be on the same device.")
+    group = k // scales.shape[0] if scales.shape[0] else 0
+    if group not in (32, 64, 128) or group * scales.shape[0] != k:
+        raise ValueError(f"{k} elements in {scales.shape[0]} groups: a group is 32, 64 or 128 elements.")
+    if int(values.max()) > 15 or int(zeros.max()) > 15:
+        raise ValueError("values and zeros must lie in 0..15.")
+    more_k, more_rows = -k % 128, -rows % 16
+    q = torch.nn.functional.pad(values, (0, more_k, 0, more_rows)).to(torch.int64)
+    q = q.view(-1, 16, q.shape[1] // 128, 4, 4, 8)  # tile, row, block, word, k group of a lane, element
+    shift = torch.tensor([4 * (j // 2) + 16 * (j % 2) for j in range(8)], device=q.device)
+    words = (q << shift).sum(dim=-1)
+    words = torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+    packed = words.permute(0, 2, 4, 1, 3).contiguous().view(torch.uint8)
+    pad = (0, more_rows, 0, more_k // group)
+    return Int4Weight(packed.view(packed.shape[0], packed.shape[1], 64, 16),
+                      torch.nn.functional.pad(scales, pad).contiguous(),
+                      torch.nn.functional.pad(zeros, pad).contiguous(), rows, k, group)
+
+
+def int4_quantize(weight: torch.Tensor, group: int = 128) -> Int4Weight:
+    """``weight`` ``[rows, k]`` (bfloat16 or float16) in 4 bits: per row and ``group`` (32, 64
+    or 128) elements the 16 steps from the smallest (or 0) to the largest (or 0), each
+    element to the nearest. Done once per weight, in torch operations."""
+    if weight.ndim != 2 or weight.dtype not in _SUPPORTED or min(weight.shape) < 1:
+        raise ValueError("weight must be bfloat16 or float16 [rows, k].")
+    rows, k = weight.shape
+    if group not in (32, 64, 128) or k % group:
+        raise ValueError("group must be 32, 64 or 128 and divide k.")
+    w = weight.float().view(rows, k // group, group) if weight.is_contiguous() else \
+        weight.float().reshape(rows, k // group, group)
+    if not bool(torch.isfinite(w).all()):
+        raise ValueError("weight must be finite.")
+    low, high = w.amin(dim=-1).clamp(max=0), w.amax(dim=-1).clamp(min=0)
+    scale = ((high - low) / 15).to(weight.dtype)
+    step = scale.float().masked_fill(scale == 0, 1.0)[..., None]  # a group of zeros
+    zero = (-low[..., None] / step).round().clamp(0, 15)
+    values = ((w / step).round() + zero).clamp(0, 15).to(torch.uint8).view(rows, k)
+    return int4_pack(values, scale.t().contiguous(), zero[..., 0].t().to(torch.uint8).contiguous())
+
+
+def _check_int4(weight: Int4Weight, device: torch.device) -> int:
+    """Checks of a packed weight; its dtype code."""
+    blocks, tiles = -(-weight.k // 128), -(-weight.rows // 16)
+    if weight.group not in (32, 64, 128) or weight.k % weight.group or weight.k < 1 or weight.rows < 1:
+        raise ValueError("the weight's group must be 32, 64 or 128 and divide its k.")
+    shape = (blocks * 128 // weight.group, tiles * 16)
+    if weight.packed.dtype != torch.uint8 or tuple(weight.packed.shape) != (tiles, blocks, 64, 16) \
+            or weight.zeros.dtype != torch.uint8 or tuple(weight.zeros.shape) != shape \
+            or weight.scales.dtype not in _SUPPORTED or tuple(weight.scales.shape) != shape:
+        raise ValueError("an Int4Weight's tensors do not have the shapes and dtypes that int4_pack gives.")
+    for t in (weight.packed, weight.scales, weight.zeros):
+        if t.device != device or not t.is_contiguous():
+            raise ValueError("an Int4Weight's tensors must be contiguous, on the product's device.")
+    return _SUPPORTED[weight.scales.dtype]
+
+
+def _launch(device: torch.device, fn, *args) -> int:
+    """``fn(*args, stream)`` on ``device``'s current stream, with ``device`` the current one."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if device.index == torch._C._cuda_getDevice():
+        return fn(*args, stream)
+    with torch.cuda.device(device):
+        return fn(*args, stream)
+
+
+INT4_MAX_ROWS = 64  # rows of x that one int4_linear takes
+
+
+def int4_linear(x: torch.Tensor, weight: Int4Weight, *, norm_weight: torch.Tensor | None = None, eps: float = 0.0,
+                residual: torch.Tensor | None = None, swiglu: bool = False) -> torch.Tensor:
+    """``block_linear`` with 4-bit weights, for up to 64 rows: ``x @ W.t()`` with ``x``
+    RMSNormed first by ``norm_weight``, ``residual`` added, or, with ``swiglu`` (``W`` holds
+    gate, then up rows), ``silu(gate) * up``, in one launch. In fp32 and rounded once, at the
+    end. ``x`` ``[..., k]`` and ``residual`` ``[..., n]`` contiguous, in the scales' dtype, ``x``
+    16-byte aligned. More rows: ``int4_dequantize`` and a library product."""
+    device = _require_gpu(x)
+    dtype = _check_int4(weight, device)
+    if x.ndim < 1 or x.dtype != weight.scales.dtype or x.shape[-1] != weight.k or not x.is_contiguous():
+        raise ValueError("x must be contiguous [..., k], in the weight's dtype.")
+    cols = weight.rows
+    if swiglu:
+        if cols % 2 or residual is not None:
+            raise ValueError("swiglu takes a weight of gate and up rows and no residual.")
+        cols //= 2
+    shape = (*x.shape[:-1], cols)
+    if residual is not None and (residual.shape != shape or residual.dtype != x.dtype or residual.device != device
+                                 or not residual.is_contiguous()):
+        raise ValueError("residual must be contiguous, of the result's shape and dtype.")
+    if norm_weight is not None:
+        if tuple(norm_weight.shape) != (weight.k,) or norm_weight.device != device \
+                or not norm_weight.is_floating_point():
+            raise ValueError("norm_weight must be floating-point [k].")
+        norm_weight = norm_weight.float().contiguous()  # no copy for the usual float32 vector
+        if norm_weight.data_ptr() % 16:
+            norm_weight = norm_weight.clone()  # a slice of a larger buffer
+    out = torch.empty(shape, dtype=x.dtype, device=device)
+    code = _launch(
+        device, _capi.lib().hx_int4_gemm, x.data_ptr(), weight.k, x.numel() // weight.k, weight.packed.data_ptr(),
+        weight.scales.data_ptr(), weight.zeros.data_ptr(), cols, weight.k, weight.group, dtype,
+        None if norm_weight is None else norm_weight.data_ptr(), eps,
+        None if residual is None else residual.data_ptr(), cols, 1 if swiglu else 0, out.data_ptr(), cols)
+    _capi.check(code, "hx_int4_gemm")
+    return out
+
+
+def int4_dequantize(weight: Int4Weight) -> torch.Tensor:
+    """``[rows, k]`` in the scales' dtype: ``scales * (q - zeros)``, rounded once."""
+    device = _require_gpu(weight.packed)
+    dtype = _check_int4(weight, device)
+    # Rows of a multiple of 8 elements (k is one of 32), so every row is 16-byte aligned.
+    out = torch.empty((weight.rows, weight.k), dtype=weight.scales.dtype, device=device)
+    code = _launch(device, _capi.lib().hx_int4_dequantize, weight.packed.data_ptr(), weight.scales.data_ptr(),
+                   weight.zeros.data_ptr(), weight.rows, weight.k, weight.group, dtype, out.data_ptr(), weight.k)
+    _capi.check(code, "hx_int4_dequantize")
+    return out
+
+
+# --------------------------------------------------------------- rules on the logits
+class LogitRules(NamedTuple):
+    """What the requests of a tick ask of their logit rows, all on the device, None: not asked.
+
+    ``tokens`` int32 ``[rows, cap]`` with ``lengths`` int32 ``[rows]``: the tokens row r knows
+    are ``tokens[r, :lengths[r]]`` (a server appends a column a tick), the first
+    ``prompt_lens[r]`` (int32, None: 0) its prompt, the others said. ``repetition`` (of
+    known tokens), ``presence`` and ``frequency`` (of said ones): float32 ``[rows]``.
+    ``bias_ids`` int32 and ``bias_values`` float32 ``[rows, n]``: added to those tokens; of an
+    id listed twice in a row the last counts. ``allowed`` int32 ``[rows, ceil(vocab / 32)]``:
+    bit ``v % 32`` of word ``v // 32`` allows token v. Token and bias ids outside the
+    vocabulary (-1: padding) are skipped."""
+
+    tokens: torch.Tensor | None = None
+    lengths: torch.Tensor | None = None
+    prompt_lens: torch.Tensor | None = None
+    repetition: torch.Tensor | None = None
+    presence: torch.Tensor | None = None
+    frequency: torch.Tensor | None = None
+    bias_ids: torch.Tensor | None = None
+    bias_values: torch.Tensor | None = None
+    allowed: torch.Tensor | None = None
+
+
+class RuledLogits(NamedTuple):
+    """Result of ``apply_logit_rules``: ``logits`` in the input's shape and dtype (None when
+    not asked for) and the greedy ``token_ids`` int64 ``[rows]``."""
+
+    logits: torch.Tensor | None
+    token_ids: torch.Tensor
+
+
+def _check_rules(rules: LogitRules, rows: int, vocab: int, device: torch.device) -> None:
+    per_row = (("lengths", torch.int32), ("prompt_lens", torch.int32), ("repetition", torch.float32),
+               ("presence", torch.float32), ("frequency", torch.float32))
+    for name, dtype in per_row:
+        t = getattr(rules, name)
+        if t is not None and (t.dtype != dtype or tuple(t.shape) != (rows,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous {dtype} [{rows}].")
+    tables = (("tokens", torch.int32), ("bias_ids", torch.int32), ("bias_values", torch.float32),
+              ("allowed", torch.int32))
+    for name, dtype in tables:
+        t = getattr(rules, name)
+        if t is not None and (t.dtype != dtype or t.ndim != 2 or t.shape[0] != rows
+                              or (t.shape[1] > 1 and t.stride(1) != 1)
+                              or (rows > 1 and t.stride(0) < t.shape[1])):
+            raise ValueError(f"{name} must be {dtype} [{rows}, n] with contiguous rows.")
+    if (rules.tokens is None) != (rules.lengths is None):
+        raise ValueError("tokens and lengths go together.")
+    if rules.tokens is None and any(t is not None for t in (rules.prompt_lens, rules.repetition, rules.presence,
+                                                            rules.frequency)):
+        raise ValueError("prompt_lens, repetition, presence and frequency need tokens.")
+    if (rules.bias_ids is None) != (rules.bias_values is None) \
+            or (rules.bias_ids is not None and rules.bias_ids.shape != rules.bias_values.shape):
+        raise ValueError("bias_ids and bias_values go together, in one shape.")
+    if rules.bias_ids is not None and rules.bias_ids.stride(0) != rules.bias_values.stride(0):
+        raise ValueError("bias_ids and bias_values must have the same row stride.")
+    if rules.allowed is not None and rules.allowed.shape[1] < -(-vocab // 32):
+        raise ValueError("allowed needs a bit for every token of the vocabulary.")
+    for name, t in zip(rules._fields, rules):
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} must be on the logits' device.")
+
+
+def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, *, out: torch.Tensor | None = None,
+                      return_logits: bool = True) -> RuledLogits:
+    """Penalties, biases and allowed tokens on ``logits`` ``[rows, vocab]`` (bfloat16, float16
+    or float32, contiguous rows), and the greedy ids of the result.
+
+    In fp32, each step rounded, for a token v of row r with logit l: known,
+    ``l / repetition`` if l > 0, else ``l * repetition``; said c times,
+    ``l - (frequency * c + presence)``; listed, ``l + bias``; not allowed, ``-inf``; then
+    rounded to the dtype. ``token_ids[r]`` is the smallest allowed token with the largest
+    result (a NaN counts as the largest, as in ``torch.argmax``), -1 in a row that nothing
+    is allowed in. ``out`` may be ``logits`` itself (in place), or memory that does not
+    overlap it; with ``return_logits=False`` and no ``out`` only the ids are written."""
+    device = _require_gpu(logits)
+    dtype = _capi.HX_DTYPE_FP32 if logits.dtype == torch.float32 else _SUPPORTED.get(logits.dtype)
+    if dtype is None or logits.ndim != 2 or logits.shape[1] < 1:
+        raise ValueError("logits must be bfloat16, float16 or float32 [rows, vocab].")
+    rows, vocab = logits.shape
+    if (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
+        raise ValueError("logits need contiguous rows that do not overlap.")
+    _check_rules(rules, rows, vocab, device)
+    if out is None:
+        if return_logits:
+            out = torch.empty((rows, vocab), dtype=logits.dtype, device=device)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != device \
+            or (vocab > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < vocab):
+        raise ValueError("out must have the logits' shape, dtype and device, and contiguous rows.")
+    elif out.data_ptr() == logits.data_ptr() and rows > 1 and out.stride(0) != logits.stride(0):
+        raise ValueError("out must be the logits or memory that does not overlap them.")
+    token_ids = torch.empty(rows, dtype=torch.int64, device=device)
+    if rows == 0:
+        return RuledLogits(out, token_ids)
+    lib = _capi.lib()
+    ws_bytes = lib.hx_logit_rules_workspace_bytes(rows, vocab)
+    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+
+    def ptr(t):
+        return None if t is None else t.data_ptr()
+
+    def row_stride(t, width):  # a single row's stride may be anything
+        return 0 if t is None else t.stride(0) if rows > 1 else width
+
+    tokens, bias, allowed = rules.tokens, rules.bias_ids, rules.allowed
+    cap = 0 if tokens is None else tokens.shape[1]
+    n_bias = 0 if bias is None else bias.shape[1]
+    code = _launch(
+        device, lib.hx_logit_rules, logits.data_ptr(), row_stride(logits, vocab), rows, vocab, dtype,
+        ptr(tokens) if cap else None, row_stride(tokens, cap), cap, ptr(rules.lengths), ptr(rules.prompt_lens),
+        ptr(rules.repetition), ptr(rules.presence), ptr(rules.frequency),
+        ptr(bias) if n_bias else None, ptr(rules.bias_values), row_stride(bias, n_bias), n_bias,
+        ptr(allowed), row_stride(allowed, 0 if allowed is None else allowed.shape[1]),
+        ptr(out), row_stride(out, vocab), token_ids.data_ptr(), workspace.data_ptr(), ws_bytes)
+    _capi.check(code, "hx_logit_rules")
+    return RuledLogits(out, token_ids)
+
+
 # --------------------------------------------------------------- logits and argmax
 class GreedyHeads(NamedTuple):
     """Result of ``final_norm_logits_argmax``: ``token_ids`` int64 ``[n]`` (-1 for an index

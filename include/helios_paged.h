@@ -48,6 +48,7 @@ extern "C" {
 /* ---- element types -------------------------------------------------------- */
 #define HX_DTYPE_BF16 0
 #define HX_DTYPE_FP16 1
+#define HX_DTYPE_FP32 2 /* hx_logit_rules only */
 
 /* ---- bits of the workspace error word (hx_varlen_attn_error_word) --------- */
 #define HX_WERR_BAD_PAGE 1        /* a block-table entry outside [0, num_pages)     */
@@ -564,6 +565,123 @@ int hx_skinny_gemm(const void* x, int64_t x_row_stride, int64_t rows, const void
                    const float* norm_weight, float eps, const void* residual,
                    int64_t residual_row_stride, int32_t swiglu, void* out,
                    int64_t out_row_stride, void* stream);
+
+/* The same products with 4-bit weights and group scales, for up to 64 rows:
+ *   W[n][k] = scales[g][n] * (q[n][k] - zeros[g][n]),  q and zeros in 0..15, g = k / group
+ *   y = h W^T with h = x, or its RMSNorm when norm_weight is given
+ *   out = y; residual + y; or silu(y[:, :cols]) * y[:, cols:] with swiglu (W then holds
+ *   2 * cols rows, gate first; not together with residual)
+ * in fp32, rounded to the element type once, at the end. group is 32, 64 or 128, k a
+ * multiple of it, cols any number. With w_pad and k_pad the rows of W and k rounded up to
+ * 16 and 128:
+ *   packed  uint8 [w_pad / 16][k_pad / 128][64][16], 16-byte aligned: byte group (c, r) =
+ *           lane 16 c + r of a tile holds four words of row r; word s holds the k elements
+ *           128 b + 32 s + 8 c + j, j = 0..7, element j at bits 4 (j / 2) + 16 (j % 2)
+ *   scales  element type [k_pad / group][w_pad], 0 where W has no row or k
+ *   zeros   uint8 [k_pad / group][w_pad]
+ * x and norm_weight 16-byte aligned, x_row_stride a multiple of 8. out must not overlap x or
+ * the weights; it may be the residual. HX_E_UNSUPPORTED for more than 64 rows or another
+ * group. hx_int4_dequantize writes round(W), rows of k elements, out 16-byte aligned and
+ * out_row_stride a multiple of 8. */
+int hx_int4_gemm(const void* x, int64_t x_row_stride, int64_t rows, const void* packed,
+                 const void* scales, const void* zeros, int32_t cols, int32_t k,
+                 int32_t group, int32_t dtype, const float* norm_weight, float eps,
+                 const void* residual, int64_t residual_row_stride, int32_t swiglu,
+                 void* out, int64_t out_row_stride, void* stream);
+int hx_int4_dequantize(const void* packed, const void* scales, const void* zeros,
+                       int32_t weight_rows, int32_t k, int32_t group, int32_t dtype,
+                       void* out, int64_t out_row_stride, void* stream);
+
+/*
+ * Attention over selected blocks of the paged KV cache. A block is block_size consecutive
+ * tokens of a page: a power of two from 16 to 1024 that divides page_size; block j of a
+ * sequence holds its tokens j * block_size .. + block_size - 1. bf16 and fp16, head_dim a
+ * multiple of 8 up to 256, any number of query heads per KV head.
+ *
+ * hx_kv_block_bounds: after a tick's new keys are in the pool, for every block that they
+ * touched (tokens seqused_k[b] - n_b .. seqused_k[b] - 1, n_b = cu_seq_q[b + 1] - cu_seq_q[b])
+ * and every KV head
+ *   bounds[page][block of the page][h][0][d] = min, [1][d] = max of k[j][h][d]
+ * over the block's tokens below seqused_k[b], both NaN where one of them is. Former bounds
+ * are not read. bounds is [num_pages][page_size / block_size][n_kv_heads][2][head_dim],
+ * contiguous like the pool, 16-byte aligned both. max_q sizes the grid only. Two sequences
+ * that touch one block in one call write it in no particular order.
+ *
+ * hx_select_blocks: entry i < n is query row rows[i] of q (i itself when rows is NULL; q_rows
+ * rows in all) of sequence row_seq[i] (NULL: i), which sees its first key_counts[i] keys. For
+ * KV head h and its query heads g the blocks are ordered by
+ *   s_j = sum_g sum_d max(q[g][d] bounds[j][h][0][d], q[g][d] bounds[j][h][1][d])
+ * in 64 bits (a NaN counts as +inf, a page outside the pool comes last, equal ones by j);
+ * blocks[i][h] = the first `sink` blocks, the last `recent` (at least 1) and the best others,
+ * `budget` in all, ascending; all of them, then -1, when there are no more. Of an entry whose
+ * row or sequence is not there: -1. HX_E_UNSUPPORTED when the table's width covers more than
+ * 16384 blocks.
+ *
+ * hx_block_sparse_attn: out[rows[i]][h] = softmax(scale q . k) V over the keys of blocks[i]
+ * [h / group] below key_counts[i], in fp32 with weights of 16 (fp16: 22) bits, rounded once.
+ * Entries of a list that are negative, past the keys or on a page outside the pool are
+ * skipped; a block listed twice counts twice. Without any key the row is zeros. Entries whose
+ * row is outside [0, q_rows) are skipped, and rows not listed are left as they were; a row
+ * must not be listed twice. q and the pools 16-byte aligned, q's strides multiples of 8; out
+ * 4-byte aligned, its strides even. The workspace is hx_block_sparse_workspace_bytes bytes
+ * (may be 0), 16-byte aligned; calls that share one must be ordered.
+ */
+int hx_kv_block_bounds(const void* k_pool, void* bounds, int32_t num_pages,
+                       int32_t page_size, int32_t block_size, int32_t n_kv_heads,
+                       int32_t head_dim, int32_t dtype, const int32_t* block_table,
+                       int64_t block_table_stride, int32_t block_table_width,
+                       const int32_t* cu_seq_q, const int32_t* seqused_k, int32_t batch,
+                       int32_t max_q, void* stream);
+int hx_select_blocks(const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                     int64_t q_rows, const int64_t* rows, const int32_t* row_seq,
+                     const int32_t* key_counts, int64_t n, int32_t n_q_heads,
+                     int32_t n_kv_heads, int32_t head_dim, int32_t dtype,
+                     const void* bounds, int32_t num_pages, int32_t page_size,
+                     int32_t block_size, const int32_t* block_table,
+                     int64_t block_table_stride, int32_t batch, int32_t block_table_width,
+                     int32_t budget, int32_t sink, int32_t recent, int32_t* blocks,
+                     void* stream);
+size_t hx_block_sparse_workspace_bytes(int64_t n, int32_t n_q_heads, int32_t n_kv_heads,
+                                       int32_t head_dim, int32_t budget, int32_t block_size);
+int hx_block_sparse_attn(const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                         int64_t q_rows, const int64_t* rows, const int32_t* row_seq,
+                         const int32_t* key_counts, int64_t n, const void* k_pool,
+                         const void* v_pool, int32_t num_pages, int32_t page_size,
+                         int32_t block_size, const int32_t* blocks, int32_t budget,
+                         const int32_t* block_table, int64_t block_table_stride,
+                         int32_t batch, int32_t block_table_width, int32_t n_q_heads,
+                         int32_t n_kv_heads, int32_t head_dim, float scale, int32_t dtype,
+                         void* out, int64_t out_row_stride, int64_t out_head_stride,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Penalties, biases and allowed-token masks on logits [rows, vocab], and the greedy ids.
+ * For row r and token v, l the logit in fp32, each step rounded to fp32:
+ *   v among the row's known tokens:   l = l > 0 ? l / repetition[r] : l * repetition[r]
+ *   v said c > 0 times:               l = l - (frequency[r] * c + presence[r])
+ *   v in the row's bias list:         l = l + bias_values[r][i], i its last entry there
+ *   v not allowed:                    l = -inf
+ * out = l rounded to the element type (it may be the logits themselves; NULL: none);
+ * token_ids[r] = the smallest allowed v with the largest rounded l (a NaN counts as the
+ * largest), -1 when nothing is allowed. Row r knows tokens[r][0 .. lengths[r] - 1] (at most
+ * token_cap), the first prompt_lens[r] of them its prompt, the others said. Token and bias
+ * ids outside the vocabulary are skipped. Bit v % 32 of allowed[r][v / 32] allows v. tokens
+ * (with lengths and prompt_lens), prompt_lens, repetition, presence, frequency, bias_ids
+ * (with bias_values) and allowed may be NULL: no known tokens, none of them a prompt, 1, 0,
+ * 0, no bias, all allowed. dtype: bf16, fp16 or fp32. The workspace is
+ * hx_logit_rules_workspace_bytes(rows, vocab) bytes, 8-byte aligned; calls that share one
+ * must be ordered.
+ */
+size_t hx_logit_rules_workspace_bytes(int64_t rows, int64_t vocab);
+int hx_logit_rules(const void* logits, int64_t logits_row_stride, int64_t rows,
+                   int64_t vocab, int32_t dtype, const int32_t* tokens,
+                   int64_t token_row_stride, int64_t token_cap, const int32_t* lengths,
+                   const int32_t* prompt_lens, const float* repetition,
+                   const float* presence, const float* frequency, const int32_t* bias_ids,
+                   const float* bias_values, int64_t bias_row_stride, int32_t n_bias,
+                   const uint32_t* allowed, int64_t allowed_row_stride, void* out,
+                   int64_t out_row_stride, int64_t* token_ids, void* workspace,
+                   size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
