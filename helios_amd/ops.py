@@ -417,6 +417,9 @@ def block_linear(x: torch.Tensor, weight: torch.Tensor, *, norm_weight: torch.Te
 
 
 # ------------------------------------------- attention over selected blocks of the cache
+MAX_SELECT_BLOCKS = 16384  # blocks of a sequence that select_blocks can order
+
+
 def _check_blocks(pool_name: str, pool: torch.Tensor, block_table: torch.Tensor, block_size: int) -> int:
     """Checks shared by the block operators; the pool's dtype code."""
     if pool.ndim != 4 or not pool.is_contiguous() or min(pool.shape) < 1:
@@ -529,8 +532,8 @@ def select_blocks(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.
     _check_table(block_table)
     if sink < 0 or recent < 1 or sink + recent > budget:
         raise ValueError("budget must cover sink (at least 0) and recent (at least 1) blocks.")
-    if block_table.shape[1] * bounds.shape[1] > 16384:
-        raise ValueError("a block table may cover at most 16384 blocks; use larger ones.")
+    if block_table.shape[1] * bounds.shape[1] > MAX_SELECT_BLOCKS:
+        raise ValueError(f"a block table may cover at most {MAX_SELECT_BLOCKS} blocks; use larger ones.")
     n = _check_rows(query, key_counts, rows, row_seq, block_table)
     blocks = torch.empty((n, n_kv, budget), dtype=torch.int32, device=device)
     code = _launch(

@@ -21,7 +21,8 @@ this module unchanged. How they are computed is this module's own design:
   only the bookkeeping works.
 * Extensions, all off the reference's call path: ``restore_blocks(copy=...,
   private_tail=...)`` (copying restores on the page-copy kernel), ``attend_projected``
-  (q/k RMSNorm + RoPE fused with the append) and the shared-prefix cascade.
+  (q/k RMSNorm + RoPE fused with the append), the shared-prefix cascade, and attention
+  over selected blocks (``KVPagePool(block_size=...)``, ``BlockSparse``).
 """
 
 from __future__ import annotations
@@ -82,14 +83,26 @@ class KVPagePool:
 
     ``keys[l]`` / ``values[l]`` are ``[num_pages, page_size, n_kv_heads, head_dim]``
     contiguous views of ``storage``. On a fresh pool ids are handed out from 0 upwards;
-    the id released last is the next one handed out."""
+    the id released last is the next one handed out.
+
+    With ``block_size`` (a power of two from 16 to 1024 that divides the page) the pool
+    also keeps each block's key bounds, ``bounds[l]`` ``[num_pages, page_size //
+    block_size, n_kv_heads, 2, head_dim]`` (2 / block_size of the keys' memory): every append
+    of a batch brings them up to date, so that ``BlockSparse`` batches can select by them.
+    Keys written into the pool by other means need ``PagedKVCache.refresh_bounds``."""
 
     def __init__(self, config: Qwen3Config, num_pages: int, *, device: torch.device,
-                 page_size: int = 256) -> None:
+                 page_size: int = 256, block_size: int | None = None) -> None:
         if num_pages < 1:
             raise ValueError(f"a KV page pool needs at least one page, not {num_pages}")
         if page_size < 1 or page_size % 256 != 0:
             raise ValueError(f"page_size must be a positive multiple of 256, not {page_size}")
+        if block_size is not None:
+            if not 16 <= block_size <= 1024 or block_size & (block_size - 1) or page_size % block_size:
+                raise ValueError(
+                    f"block_size must be a power of two from 16 to 1024 that divides the page, not {block_size}")
+            if config.dtype not in (torch.bfloat16, torch.float16) or config.head_dim % 8 or config.head_dim > 256:
+                raise ValueError("key bounds need bfloat16 or float16 heads of a multiple of 8 up to 256 elements")
         self.config = config
         self.num_pages = int(num_pages)
         self.page_size = int(page_size)
@@ -100,6 +113,12 @@ class KVPagePool:
         )
         self.keys = tuple(self.storage[0].unbind(0))
         self.values = tuple(self.storage[1].unbind(0))
+        self.block_size = block_size
+        self.bounds: tuple[torch.Tensor, ...] | None = None
+        if block_size is not None:
+            self.bounds = tuple(torch.zeros(
+                (config.n_layers, self.num_pages, self.page_size // block_size, config.n_kv_heads, 2, config.head_dim),
+                dtype=config.dtype, device=self.device).unbind(0))
         # _stack[:_top] holds the free ids; _stack[_top - 1] is handed out next. Released
         # ids wait in _released (in release order) until the next acquire or free-page
         # count moves them onto the stack: a release can run inside the garbage
@@ -155,8 +174,11 @@ class KVPagePool:
             n = len(released)
 
     def copy_pages(self, src_pages: Sequence[int], dst_pages: Sequence[int]) -> None:
-        """Bit-copy pages for every layer, keys and values, on the page-copy kernel."""
+        """Bit-copy pages for every layer, keys, values and any key bounds, on the page-copy
+        kernel."""
         ops.kv_copy_pages(self.keys, self.values, src_pages, dst_pages)
+        if self.bounds is not None:
+            ops.kv_copy_pages(self.bounds, None, src_pages, dst_pages)
 
 
 # ----------------------------------------------------------------- request cache
@@ -259,6 +281,21 @@ class PagedKVCache:
                 + (", an append is in flight" if self._pending_tokens is not None else ""))
         del self.pages[_page_count(length, self.pool.page_size):]
         self.length = length
+
+    def refresh_bounds(self) -> None:
+        """Key bounds of all committed tokens from the pool's keys, every layer: for keys that
+        came into the pool otherwise than by a batch's append."""
+        pool = self.pool
+        if pool.bounds is None:
+            raise RuntimeError("the pool keeps no key bounds; create it with block_size")
+        if self._pending_tokens is not None:
+            raise RuntimeError("refresh_bounds needs the append in flight to be committed")
+        if not self.length:
+            return
+        table = torch.tensor([[page.index for page in self.pages]], dtype=torch.int32, device=pool.device)
+        ends = torch.tensor([0, self.length], dtype=torch.int32, device=pool.device)
+        for keys, bounds in zip(pool.keys, pool.bounds):
+            ops.kv_block_bounds(keys, bounds, table, ends, ends[1:], max_q=self.length)
 
     def close(self) -> None:
         self.pages = []
@@ -656,6 +693,73 @@ class _PrefixCascade:
         return out
 
 
+# --------------------------------------------------- attention over selected blocks
+@dataclass(frozen=True)
+class BlockSparse:
+    """How the decode rows of a batch attend to long caches: each row, per KV head, to
+    ``budget`` blocks of the pool's ``block_size`` tokens, the first ``sink``, the last
+    ``recent`` and otherwise those whose key bounds promise the highest scores
+    (``ops.select_blocks``). Rows of at most ``budget`` blocks attend to all of their keys."""
+
+    budget: int
+    sink: int = 1
+    recent: int = 2
+
+    def __post_init__(self) -> None:
+        if self.sink < 0 or self.recent < 1 or self.sink + self.recent > self.budget:
+            raise ValueError("a sparse budget must cover its sink (at least 0) and recent (at least 1) blocks")
+
+
+class _SparseTick:
+    """One tick's sparse attention: its decode rows (one new token) over selected blocks, its
+    other rows over all of their keys with a plan of their own. ``None`` tensors mean all
+    sequences are decode rows, in order."""
+
+    def __init__(self, batch: PagedBatchCache, sparse: BlockSparse, counts: list[int], ends: list[int]) -> None:
+        self.sparse, self.batch = sparse, batch
+        self.rows = self.row_seq = self.plan = None
+        self.keys = batch.seqused_k
+        if max(counts) == 1:
+            return
+        pool, config = batch.pool, batch.pool.config
+        starts = [0, *accumulate(counts)]
+        decode = [b for b, n in enumerate(counts) if n == 1]
+        chunks = [b for b, n in enumerate(counts) if n > 1]
+        chunk_counts, chunk_ends = [counts[b] for b in chunks], [ends[b] for b in chunks]
+        chunk_rows = [r for b in chunks for r in range(starts[b], starts[b + 1])]
+        parts = [decode, [ends[b] for b in decode], [0, *accumulate(chunk_counts)], chunk_ends, chunks]
+        pin32, i32 = _pinned(sum(map(len, parts)), torch.int32)
+        pin64, i64 = _pinned(len(decode) + len(chunk_rows), torch.int64)
+        i32[:] = [x for part in parts for x in part]
+        i64[:] = [starts[b] for b in decode] + chunk_rows
+        dev32 = torch.empty(pin32.shape, dtype=torch.int32, device=pool.device)
+        dev32.copy_(pin32, non_blocking=True)
+        dev64 = torch.empty(pin64.shape, dtype=torch.int64, device=pool.device)
+        dev64.copy_(pin64, non_blocking=True)
+        self.row_seq, self.keys, cu_q, used, ids = dev32.split([len(part) for part in parts])
+        self.rows, self.chunk_rows = dev64.split([len(decode), len(chunk_rows)])
+        self.table = batch.block_table.index_select(0, ids)
+        self.plan = ops.VarlenAttnPlan(
+            cu_q, None, used, total_q=len(chunk_rows), max_q=max(chunk_counts), max_k=max(chunk_ends),
+            n_q_heads=config.n_heads, n_kv_heads=config.n_kv_heads, head_dim=config.head_dim,
+            page_size=pool.page_size, block_table_stride=self.table.shape[1], window=(-1, 0),
+            q_lens=chunk_counts, k_lens=chunk_ends)
+
+    def attend(self, rows: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+               bounds: torch.Tensor) -> torch.Tensor:
+        """Attention of every packed row, the new K/V and bounds already in the pool."""
+        sparse, block, table = self.sparse, self.batch.pool.block_size, self.batch.block_table
+        out = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
+        blocks = ops.select_blocks(rows, bounds, table, self.keys, sparse.budget, block_size=block, sink=sparse.sink,
+                                   recent=sparse.recent, row_seq=self.row_seq, rows=self.rows)
+        ops.block_sparse_attn(rows, k_pool, v_pool, blocks, table, self.keys, block_size=block,
+                              row_seq=self.row_seq, rows=self.rows, out=out)
+        if self.plan is not None:
+            chunk_out = self.plan.run(rows, k_pool, v_pool, self.table, query_rows=self.chunk_rows)
+            out.index_copy_(0, self.chunk_rows, chunk_out)
+        return out
+
+
 # ------------------------------------------------------------------- batches
 class PagedBatchCache:
     """Request caches of one pool stepping together (paged_cache.py:177-345).
@@ -672,10 +776,13 @@ class PagedBatchCache:
     stream while decode rows (HBM-bound) run on the current one. It is off by default: on
     MI355X the decode grid fills every CU and a chunk workgroup cannot share a CU with
     decode workgroups, so the kernels interleave rather than overlap (the full Qwen3-4B
-    tick measured 12.5 ms of attention with it, 12.0 ms without)."""
+    tick measured 12.5 ms of attention with it, 12.0 ms without). ``sparse`` lets decode rows
+    of long caches attend to selected blocks; a tick in which one does runs on one stream
+    and without the cascade."""
 
     def __init__(self, caches: Sequence[PagedKVCache], *, device_metadata: bool | None = None,
-                 prefix_cascade: bool | None = None, overlap: bool = False) -> None:
+                 prefix_cascade: bool | None = None, overlap: bool = False,
+                 sparse: BlockSparse | None = None) -> None:
         caches = tuple(caches)
         if not caches:
             raise ValueError("a paged batch needs at least one request cache")
@@ -691,8 +798,16 @@ class PagedBatchCache:
             raise ValueError("device metadata needs a pool on a ROCm device")
         if overlap and not on_gpu:
             raise ValueError("overlapped streams need a pool on a ROCm device")
+        if sparse is not None and pool.bounds is None:
+            raise ValueError("block-sparse attention needs a pool with key bounds (block_size)")
+        if sparse is not None and _page_count(pool.config.context_length, pool.page_size) \
+                * (pool.page_size // pool.block_size) > ops.MAX_SELECT_BLOCKS:
+            raise ValueError(f"block-sparse attention covers {ops.MAX_SELECT_BLOCKS} blocks of a context; "
+                             "use larger ones")
         self.pool = pool
         self.caches = caches
+        self._sparse = sparse
+        self._sparse_tick: _SparseTick | None = None
         self.batch_size = len(caches)
         self._staged: dict[str, tuple[torch.Tensor, np.ndarray]] = {}
         self._table_key: tuple | None = None
@@ -778,6 +893,7 @@ class PagedBatchCache:
         the reference's exception types."""
         caches = self.caches
         size = self.pool.page_size
+        on_gpu = self.pool.device.type == "cuda"
         short: list[int] = []
         for cache, n in zip(caches, counts):
             if cache._pending_tokens is not None:
@@ -805,7 +921,12 @@ class PagedBatchCache:
             ends = self._host_tick(lengths, counts, tails, tables, width)
         self._plan = None
         self._lens = (list(counts), ends)
-        self._cascade = _PrefixCascade.build(self, list(counts), ends) if self._use_cascade else None
+        self._sparse_tick = self._cascade = None
+        if self._sparse is not None and on_gpu and any(
+                n == 1 and end > self._sparse.budget * self.pool.block_size for n, end in zip(counts, ends)):
+            self._sparse_tick = _SparseTick(self, self._sparse, list(counts), ends)
+        elif self._use_cascade:
+            self._cascade = _PrefixCascade.build(self, list(counts), ends)
 
     def _host_tick(self, lengths, counts, tails, tables, width) -> list[int]:
         tick = _HostTick(lengths, counts, tails, tables, width, self.pool.page_size)
@@ -916,7 +1037,7 @@ class PagedBatchCache:
             queries, keys, values, config.n_heads, q_norm_weight, k_norm_weight, cos, sin, self._positions_for_rows(),
             k_pool, v_pool, self.write_slots, eps)
         if q_rot is not None:
-            out = self._attend_rows(q_rot, k_pool, v_pool)
+            out = self._attend_rows(q_rot, layer)
             return out.view(1, rows, config.n_heads, config.head_dim).transpose(1, 2)
         q = queries.reshape(rows, config.n_heads, config.head_dim)
         k = keys.reshape(rows, config.n_kv_heads, config.head_dim)
@@ -924,7 +1045,7 @@ class PagedBatchCache:
         q_rot = ops.qk_norm_rope_append(q, k, v, q_norm_weight, k_norm_weight, cos, sin,
                                         self._positions_for_rows(), k_pool, v_pool,
                                         self.write_slots, eps)
-        out = self._attend_rows(q_rot, k_pool, v_pool)
+        out = self._attend_rows(q_rot, layer)
         return out.view(queries.shape[0], queries.shape[1], config.n_heads, config.head_dim).transpose(1, 2)
 
     def _positions_for_rows(self) -> torch.Tensor:
@@ -933,8 +1054,18 @@ class PagedBatchCache:
             self._row_positions = self.metadata("row_positions", self._host_positions, torch.long)
         return self._row_positions
 
-    def _attend_rows(self, rows: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor) -> torch.Tensor:
+    def _update_bounds(self, layer: int) -> None:
+        """Key bounds of the blocks this tick's new keys went to, if the pool keeps them."""
+        if self.pool.bounds is not None:
+            ops.kv_block_bounds(self.pool.keys[layer], self.pool.bounds[layer], self.block_table, self.cu_seq_q,
+                                self.seqused_k, max_q=self.max_q)
+
+    def _attend_rows(self, rows: torch.Tensor, layer: int) -> torch.Tensor:
         """Attention of packed query rows whose new K/V is already in the pool."""
+        k_pool, v_pool = self.pool.keys[layer], self.pool.values[layer]
+        self._update_bounds(layer)
+        if self._sparse_tick is not None:
+            return self._sparse_tick.attend(rows, k_pool, v_pool, self.pool.bounds[layer])
         if self._cascade is not None:
             return self._cascade.attend(rows, k_pool, v_pool, self._side())
         plan = self._attention_plan(rows.shape[0])
@@ -956,14 +1087,15 @@ class PagedBatchCache:
         loads (always, for contiguous projections), else the append kernel first."""
         k_rows, v_rows = _as_rows(keys), _as_rows(values)
         k_pool, v_pool = self.pool.keys[layer], self.pool.values[layer]
-        fused = (self._cascade is None and self._side() is None
+        fused = (self._cascade is None and self._sparse_tick is None and self._side() is None
                  and _vector_aligned(k_rows) and _vector_aligned(v_rows))
         if fused:
             plan = self._attention_plan(rows.shape[0])
-            return plan.run(rows, k_pool, v_pool, self.block_table,
-                            append=(k_rows, v_rows, self.write_slots))
+            out = plan.run(rows, k_pool, v_pool, self.block_table, append=(k_rows, v_rows, self.write_slots))
+            self._update_bounds(layer)
+            return out
         ops.kv_append(k_pool, v_pool, self.write_slots, k_rows, v_rows)
-        return self._attend_rows(rows, k_pool, v_pool)
+        return self._attend_rows(rows, layer)
 
 
 class PackedBatchCache(PagedBatchCache):
@@ -994,11 +1126,12 @@ class PackedBatchCache(PagedBatchCache):
                 f"packed attention takes [1, heads, {sum(self.counts)}, head_dim] queries, "
                 f"not {list(queries.shape)}")
         self._require_device()
-        if self._cascade is None and not self._overlap:
+        if self._cascade is None and self._sparse_tick is None and not self._overlap:
             out = self._attention_plan(queries.shape[2]).append_attend(
                 queries, keys, values, self.pool.keys[layer], self.pool.values[layer], self.block_table,
                 self.write_slots)
             if out is not None:
+                self._update_bounds(layer)
                 return out
         out = self._append_and_attend(layer, queries[0].transpose(0, 1), keys, values)
         return out.transpose(0, 1).unsqueeze(0)
