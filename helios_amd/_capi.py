@@ -213,12 +213,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "hx_int4_gemm": (
         ctypes.c_int,
-        [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _i32, _i32,
-         _c_void_p, _f32, _c_void_p, _i64, _i32, _c_void_p, _i64, _c_void_p],
+        [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i32, _i32, _i32, _i32,
+         _c_void_p, _f32, _c_void_p, _i64, _i32, _c_void_p, _i64, _c_void_p, _size, _c_void_p],
     ),
+    "hx_int4_workspace_bytes": (_size, [_i64, _i32, _i32]),
     "hx_int4_dequantize": (
         ctypes.c_int,
-        [_c_void_p, _c_void_p, _c_void_p, _i32, _i32, _i32, _i32, _c_void_p, _i64, _c_void_p],
+        [_c_void_p, _c_void_p, _i32, _i32, _i32, _i32, _c_void_p, _i64, _c_void_p],
     ),
     "hx_kv_block_bounds": (
         ctypes.c_int,

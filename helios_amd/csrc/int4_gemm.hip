@@ -8,19 +8,26 @@
 // A product of few rows is a stream of W: a quarter of the bytes of 16-bit weights. Per group
 //   sum_k h_k s (q_k - z) = s (sum_k h_k (16 + q_k) - (16 + z) sum_k h_k):
 // 16 + q is a bf16 (fp16) number with q in its upper mantissa bits, so a pair of weights costs
-// a shift and one and-or, and the sums of h come from one more MFMA against ones. Both sums
+// a rotation and one and-or, and the sums of h come from one more MFMA against ones. Both sums
 // are fp32; the offset 16 makes the terms at most 31 / 15 times as large as they have to be.
 //
 // Weights are packed in the order in which the MFMA takes them: 1 KiB holds 16 rows x 128 k,
 // lane l = 16 c + r of a wave reads 16 bytes, the k elements 32 s + 8 c .. + 7 of row r in its
-// word s. Element j of a word sits at bits 4 (j / 2) + 16 (j % 2), where the shift above finds
-// elements 2 i and 2 i + 1 at once.
+// word s. Element j of a word sits at bits 3 + 4 (j / 2) + 16 (j % 2), modulo 32: turned by 4 i,
+// elements 2 i and 2 i + 1 lie in the upper mantissa bits of a bf16 pair.
 //
 // The norm's row factor 1 / rms multiplies y at the end; x * norm_weight is split into two
-// bf16 (their sum has 16 bits), each with an MFMA of its own.
+// bf16 (their sum has 16 bits), each an operand row of its own: of up to eight rows the leading
+// parts are rows 0-7 of one MFMA operand and the rest rows 8-15, at no further cost.
 //
-// A workgroup owns 16 columns of y (SwiGLU: 16 gate and the 16 up columns they multiply) and
-// all rows; its waves split K and merge through LDS in wave order.
+// A workgroup owns 16 or 32 columns of y (SwiGLU: 16 gate and the 16 up columns they multiply)
+// and 16 (8) rows; its waves split K and merge through LDS in wave order.
+//
+// A layer of hidden 2560, 32/8 heads of 128 and ffn 9728, W from HBM, 1 / 8 / 16 rows (us): qkv
+// 5.5 / 6.0 / 8.0, o 4.0 / 4.5 / 5.3, gate_up 10.2 / 11.1 / 15.0, down 6.6 / 7.4 / 9.4, in all 26 /
+// 29 / 38 where the 16-bit products take 60 / 62 / 71. gate_up's 26 MB are 2.6 TB/s at one row:
+// about 4 us of each launch are its start, the first loads' way and the merge, as for the
+// 16-bit products; the rest is bound by the address unit (x and W: 104 cycles a block at 8 rows).
 
 #include <type_traits>
 
@@ -30,15 +37,14 @@ namespace {
 
 constexpr int kI4Block = 128;  // k elements per packed block: one 16-byte load a lane
 
-enum : int { kEpiPlain = 0, kEpiResidual = 1, kEpiSwiglu = 2 };
-
 struct Int4Args {
   const uint16_t* x;
+  const uint16_t* h;  // normalised rows (int4_norm_kernel)
   int64_t x_row;
   const uint8_t* w;       // [rows of W / 16][blocks][64][16]
-  const uint16_t* scale;  // [k_pad / group][w_rows_pad]
-  const uint8_t* zero;
+  const uint32_t* steps;  // [k_pad / group][w_pad]: the scale, and 16 + zero in the high half
   int32_t rows, cols, k, blocks, w_pad;  // cols: of the output; w_pad: rows of W, padded to 16
+  int32_t row_tiles, col_tiles;
   const float* norm_w;
   float eps;
   const uint16_t* res;
@@ -47,186 +53,326 @@ struct Int4Args {
   int64_t out_row;
 };
 
+// Constants of widen, kept in registers: v_and_or_b32 takes no literals, and one scalar operand.
+template <typename T>
+struct WidenBits {
+  uint32_t mask, one;
+  __device__ __forceinline__ WidenBits() {
+    asm("s_mov_b32 %0, %1" : "=s"(mask) : "n"(__is_same(T, __bf16) ? 0x00780078 : 0x03c003c0));
+    asm("v_mov_b32 %0, %1" : "=v"(one) : "n"(__is_same(T, __bf16) ? 0x41804180 : 0x4c004c00));
+  }
+};
+
 // Eight weights of a packed word as 16 + q in the MFMA's element type.
 template <typename T>
-__device__ __forceinline__ uint4 widen(uint32_t w);
-template <>
-__device__ __forceinline__ uint4 widen<__bf16>(uint32_t w) {
-  constexpr uint32_t m = 0x00780078u, o = 0x41804180u;
-  return make_uint4(((w << 3) & m) | o, ((w >> 1) & m) | o, ((w >> 5) & m) | o, ((w >> 9) & m) | o);
-}
-template <>
-__device__ __forceinline__ uint4 widen<_Float16>(uint32_t w) {
-  constexpr uint32_t m = 0x03c003c0u, o = 0x4c004c00u;
-  return make_uint4(((w << 6) & m) | o, ((w << 2) & m) | o, ((w >> 2) & m) | o, ((w >> 6) & m) | o);
+__device__ __forceinline__ uint4 widen(uint32_t w, const WidenBits<T>& c) {
+  constexpr int kAt = __is_same(T, __bf16) ? 0 : 29;  // fp16's upper mantissa bits lie three further up
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t turned = (kAt + 4 * i) % 32 == 0 ? w : __builtin_amdgcn_alignbit(w, w, (kAt + 4 * i) % 32);
+    o[i] = (turned & c.mask) | c.one;
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// MT: row tiles of 16. G: k elements per group (32, 64 or 128).
-template <typename T, bool NORM, int EPI, int MT, int G, int WAVES>
+// Eight elements of x times norm_weight times r, each as two bf16 numbers: their sum has 16 bits.
+template <typename T>
+__device__ __forceinline__ void split_pair(uint4 u, const float (&nw)[8], float r, uint4& high, uint4& low) {
+  typedef hx::Elem<T> E;
+  typedef hx::Elem<__bf16> B;
+  const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float p0 = E::lo(wd[q]) * r * nw[2 * q], p1 = E::hi(wd[q]) * r * nw[2 * q + 1];
+    h[q] = hx::pack2_round<__bf16>(p0, p1);
+    l[q] = hx::pack2_round<__bf16>(p0 - B::lo(h[q]), p1 - B::hi(h[q]));
+  }
+  high = make_uint4(h[0], h[1], h[2], h[3]);
+  low = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+// RMSNorm of row r as two bf16 parts, for more rows than one tile: h holds, per row tile, block of
+// 128 k, part and step, the MFMA's operand [lane][8]. The first kHold x 256 pieces of a row stay
+// in registers.
+template <typename T>
+__global__ __launch_bounds__(256) void int4_norm_kernel(Int4Args a, uint16_t* h) {
+  constexpr int kHold = 2;
+  __shared__ float s_part[4];
+  const int row = hx::wg_x(), tid = hx::tid_x(), pieces = a.k / 8, padded = a.blocks * (kI4Block / 8);
+  const uint4* x = reinterpret_cast<const uint4*>(a.x + (int64_t)row * a.x_row);
+  const float4* n = reinterpret_cast<const float4*>(a.norm_w);
+  uint4 held[kHold];
+  float4 nw[kHold][2];
+#pragma unroll
+  for (int i = 0; i < kHold; ++i) {
+    const int p = tid + 256 * i;
+    held[i] = hx::zero4();
+    nw[i][0] = nw[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p >= pieces) continue;
+    held[i] = x[p];
+    nw[i][0] = n[2 * p];
+    nw[i][1] = n[2 * p + 1];
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < kHold; ++i) ss = hx::dot8<T>(held[i], held[i], ss);
+  for (int p = tid + 256 * kHold; p < pieces; p += 256) {
+    const uint4 u = x[p];
+    ss = hx::dot8<T>(u, u, ss);
+  }
+  ss = hx::wave_sum_xor(ss, 1, 32);
+  if ((tid & 63) == 0) s_part[tid >> 6] = ss;
+  __syncthreads();
+  ss = (s_part[0] + s_part[1]) + (s_part[2] + s_part[3]);
+  const float r = rsqrtf(__fadd_rn(__fdiv_rn(ss, (float)a.k), a.eps));
+  uint4* tile = reinterpret_cast<uint4*>(h) + (int64_t)(row >> 4) * 2 * padded * 16 + (row & 15);
+  auto put = [&](int p, uint4 u, float4 na, float4 nb) __attribute__((always_inline)) {
+    const float w[8] = {na.x, na.y, na.z, na.w, nb.x, nb.y, nb.z, nb.w};
+    uint4* to = tile + (p / 16 * 8 + p / 4 % 4) * 64 + 16 * (p % 4);
+    split_pair<T>(u, w, r, to[0], to[256]);
+  };
+#pragma unroll
+  for (int i = 0; i < kHold; ++i)
+    if (tid + 256 * i < padded) put(tid + 256 * i, held[i], nw[i][0], nw[i][1]);
+  const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p = tid + 256 * kHold; p < padded; p += 256)
+    put(p, p < pieces ? x[p] : hx::zero4(), p < pieces ? n[2 * p] : none, p < pieces ? n[2 * p + 1] : none);
+}
+
+// 16-byte buffer load at byte offset voff + soff.
+__device__ __forceinline__ uint4 ld16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) {
+  const hx::u32x4_t v =
+      __builtin_bit_cast(hx::u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, (int)soff, 0));
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// How x reaches the MFMA: as it is, up to 4, 8 or 16 rows a tile; normalised on the way, the same;
+// or as int4_norm_kernel's parts.
+enum : int { kRaw4, kRaw8, kRaw16, kNorm4, kNorm8, kNorm16, kParts16 };
+
+// LDS slot of 16-byte piece p of row r: the 16 rows of a fragment read spread over the banks.
+__device__ __forceinline__ int turn_piece(int r, int p) { return p ^ (r & 15); }
+
+// G: k elements per group (32, 64 or 128). NV: W tiles of a wave (SWIGLU: a gate and the up tile
+// it multiplies). D: packed blocks in flight per wave.
+template <typename T, int IN, bool SWIGLU, int G, int NV, int WAVES, int D>
 __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
-  // The normalised rows are bf16 pairs whatever the element type: x * norm_weight may leave
-  // fp16's range, and 16 + q is exact in either.
-  typedef typename std::conditional<NORM, __bf16, T>::type M;
+  constexpr bool kRaw = IN <= kRaw16, kNorm = IN >= kNorm4 && IN <= kNorm16, kTurn = kRaw || kNorm;
+  // Normalised rows are bf16 parts whatever the element type: 16 + q is exact in either.
+  typedef typename std::conditional<kRaw, T, __bf16>::type M;
   typedef hx::Elem<T> E;
   typedef hx::Elem<M> EM;
-  constexpr int NV = EPI == kEpiSwiglu ? 2 : 1;
+  typedef typename EM::v8 v8;
   constexpr int kSteps = kI4Block / 32, kGroups = kI4Block / G;
-  __shared__ __attribute__((aligned(16))) float red[WAVES][MT * NV][256];
-  __shared__ float s_ss[WAVES][MT * 16];
+  constexpr int kCols = SWIGLU ? 16 : 16 * NV;  // of the output
+  constexpr int kRows = IN == kNorm4 || IN == kNorm8 ? 8 : 16;  // of a row tile
+  constexpr int kOps = IN == kNorm16 || IN == kParts16 ? 2 : 1;  // MFMA operands of a tile's rows
+  // Up to eight normalised rows share one operand: leading parts in rows 0-7, the rest in 8-15.
+  constexpr bool kPaired = IN == kNorm4 || IN == kNorm8;
+  constexpr int kLoads = IN == kParts16 ? 2 * kSteps : IN == kRaw4 || IN == kNorm4 ? 1 : IN == kRaw8 || IN == kNorm8 ? 2 : 4;
+  __shared__ __attribute__((aligned(16))) float red[WAVES][NV][256];
+  __shared__ __attribute__((aligned(16))) uint8_t turn[kTurn ? WAVES : 1][kTurn ? 4096 * kOps : 16];
+  __shared__ float s_ss[WAVES][16];
   const int tid = hx::tid_x(), lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n0 = hx::wg_x() * 16;
+  // Workgroups go to the XCDs in turn: the row tiles of a column tile share one, and its L2.
+  const int xcd = hx::wg_x() % 8, j = hx::wg_x() / 8;
+  const int rt = j % a.row_tiles, ct = j / a.row_tiles * 8 + xcd;
+  if (ct >= a.col_tiles) return;
+  const int n0 = ct * kCols;
   const int b_begin = (int)((int64_t)a.blocks * w / WAVES), b_end = (int)((int64_t)a.blocks * (w + 1) / WAVES);
 
-  const uint8_t* wp[NV];
-  int wrow[NV];
+  // Buffer loads: what varies over the lanes is one offset, what varies over the blocks a scalar
+  // one. (With an address per load a third of the instructions were additions.)
+  __amdgpu_buffer_rsrc_t wr[NV];
+  uint32_t woff[NV], soff[NV];
+  const uint32_t sbytes = (uint32_t)(a.blocks * kGroups) * a.w_pad * 4, wbytes = 2u * a.blocks * 1024;
+  const __amdgpu_buffer_rsrc_t sr = hx::buffer_rsrc(a.steps, sbytes);
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     // A column past the last reads a row of W that is there; its sums are not stored.
-    wrow[v] = min(n0 + lr, a.cols - 1) + v * a.cols;
-    wp[v] = a.w + ((int64_t)(wrow[v] >> 4) * a.blocks * 64 + (wrow[v] & 15) + 16 * lg) * 16;
+    const int first = SWIGLU ? n0 + v * a.cols : min(n0 + 16 * v, a.cols - 1);
+    const int row = min(first + lr, (SWIGLU ? (v + 1) * a.cols : a.cols) - 1);
+    wr[v] = hx::buffer_rsrc(a.w + (int64_t)(first >> 4) * a.blocks * 1024, wbytes);
+    woff[v] = (uint32_t)((row >> 4) - (first >> 4)) * a.blocks * 1024 + ((row & 15) + 16 * lg) * 16;
+    soff[v] = 4u * row;
   }
-  hx::f32x4_t acc[MT][NV];
-  float ss[MT];
+  // x is read in whole lines, 16 lanes to the 256 bytes of a row's block, and turned into the
+  // MFMA's layout through the wave's part of LDS: lanes next to each other in that layout are
+  // different rows, and a load straight into it costs an access per lane (64 cycles of the
+  // address unit instead of 16: what bounded this kernel). Rows that are not there are read
+  // past the buffer's end (zeros).
+  const int rows = min(a.rows - rt * kRows, kRows);
+  const uint16_t* xbase = kTurn ? a.x + (int64_t)rt * kRows * a.x_row : a.h + (int64_t)rt * 32 * a.blocks * kI4Block;
+  const uint32_t xbytes = kTurn ? (uint32_t)((rows - 1) * a.x_row + a.k) * 2 : (uint32_t)a.blocks * 8192;
+  const __amdgpu_buffer_rsrc_t xr = hx::buffer_rsrc(xbase, xbytes);
+  const uint32_t nbytes = 4u * a.k;
+  const __amdgpu_buffer_rsrc_t nr = hx::buffer_rsrc(kNorm ? a.norm_w : nullptr, kNorm ? nbytes : 0u);
+  uint32_t xoff[kLoads];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    ss[t] = 0.f;
+  for (int q = 0; q < kLoads; ++q)
+    xoff[q] = !kTurn ? 16u * lane + 1024u * q : 4 * q + lg < rows ? (uint32_t)((4 * q + lg) * a.x_row) * 2 + 16 * lr
+                                                                  : 0x80000000u;
+  // Loads complete in the order they were issued, so a block's x goes with its weights. Blocks
+  // past the wave's last are loaded too, from the end of each buffer: zeros, and no traffic.
+  // (With a branch around these loads every trip through the loop waited for all of them.)
+  uint4 wq[D][NV], xb[D][kLoads], nb[D][kNorm ? 2 : 1];
+  uint32_t st[D][NV][kGroups];
+  auto load = [&](int i, int b) __attribute__((always_inline)) {
+    const bool in = b < b_end;
+    const uint32_t at = in ? (kTurn ? 256u : 8192u) * b : xbytes;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) acc[t][v] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
-  }
-  const typename EM::v8 ones = hx::as_v8<M>(hx::ones8<M>());
-
-  for (int b = b_begin; b < b_end; ++b) {
-    uint4 wq[NV];
-    float sc[NV][kGroups], zp[NV][kGroups];
+    for (int q = 0; q < kLoads; ++q) xb[i][q] = ld16(xr, xoff[q], at);
+    if constexpr (kNorm) {
+      nb[i][0] = ld16(nr, 32u * lr, in ? 512u * b : nbytes);
+      nb[i][1] = ld16(nr, 32u * lr + 16, in ? 512u * b : nbytes);
+    }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      wq[v] = hx::ld16_stream(wp[v] + (int64_t)b * 1024);
+      wq[i][v] = hx::ld16_stream(wr[v], woff[v], in ? 1024u * b : wbytes);
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const int64_t at = (int64_t)(b * kGroups + g) * a.w_pad + wrow[v];
-        sc[v][g] = E::lo(a.scale[at]);
-        zp[v][g] = 16.f + (float)a.zero[at];
-      }
+      for (int g = 0; g < kGroups; ++g)
+        st[i][v][g] = __builtin_amdgcn_raw_buffer_load_b32(
+            sr, (int)soff[v], (int)(in ? (uint32_t)(b * kGroups + g) * a.w_pad * 4 : sbytes), 0);
     }
-    hx::f32x4_t ga[MT][NV], gx[MT];
+  };
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int k0 = b * kI4Block + 32 * s + 8 * lg;
-      const bool in = k0 < a.k;
-      uint4 wf[NV];
+  for (int i = 0; i < D; ++i) load(i, b_begin + i);
+
+  // The first output element's residual, in flight with the weights.
+  const int r_row = rt * kRows + tid / 16, r_col = n0 + tid % 16;
+  uint16_t r_first = 0;
+  if constexpr (!SWIGLU)
+    if (a.res != nullptr && tid < kRows * 16 && r_row < a.rows && r_col < a.cols)
+      r_first = a.res[(int64_t)r_row * a.res_row + r_col];
+
+  hx::f32x4_t acc[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) acc[v] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float ss[kLoads];
+#pragma unroll
+  for (int q = 0; q < kLoads; ++q) ss[q] = 0.f;
+  const v8 ones = hx::as_v8<M>(hx::ones8<M>());
+  const WidenBits<M> bits;
+  auto consume = [&](int i, int b) __attribute__((always_inline)) {
+    uint4 xf[kSteps][kOps];
+    if constexpr (kTurn) {
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) {
+        uint4 u = xb[i][q];
+        if (G < kI4Block && b * kI4Block + 8 * lr >= a.k) u = hx::zero4();  // the next row's
+        const int r = 4 * q + lg;
+        uint8_t* to = turn[w] + 256 * r + 16 * turn_piece(r, lr);
+        if constexpr (kNorm) {
+          // x * norm_weight in two parts; 1 / rms multiplies the sums at the end.
+          const uint32_t nw4[8] = {nb[i][0].x, nb[i][0].y, nb[i][0].z, nb[i][0].w,
+                                   nb[i][kNorm].x, nb[i][kNorm].y, nb[i][kNorm].z, nb[i][kNorm].w};
+          float nw[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) nw[e] = __uint_as_float(nw4[e]);
+          uint4 h, l;
+          split_pair<T>(u, nw, 1.f, h, l);
+          ss[q] = hx::dot8<T>(u, u, ss[q]);
+          *reinterpret_cast<uint4*>(to) = h;
+          const int r2 = kPaired ? r + 8 : r;  // the same slot of another row, or another operand
+          *reinterpret_cast<uint4*>(turn[w] + 256 * r2 + 16 * turn_piece(r2, lr) + (kPaired ? 0 : 4096)) = l;
+        } else {
+          *reinterpret_cast<uint4*>(to) = u;
+        }
+      }
+      // One wave's LDS accesses complete in order: the fences hold the compiler to it. Rows that
+      // are not stored here hold anything: their sums are not used, and rows do not mix.
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int o = 0; o < kOps; ++o)
+        xf[s][o] = kTurn ? *reinterpret_cast<const uint4*>(turn[w] + 4096 * o + 256 * lr + 16 * turn_piece(lr, 4 * s + lg))
+                         : xb[i][(kSteps * o + s) % kLoads];
+    if constexpr (kTurn) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      hx::f32x4_t ga[NV], gx{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int v = 0; v < NV; ++v) ga[v] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = g * (G / 32); s < (g + 1) * (G / 32); ++s) {
+#pragma unroll
+        for (int o = 0; o < kOps; ++o) gx = EM::mfma16x16x32(hx::as_v8<M>(xf[s][o]), ones, gx);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const uint32_t wd[4] = {wq[i][v].x, wq[i][v].y, wq[i][v].z, wq[i][v].w};
+          const v8 wf = hx::as_v8<M>(widen<M>(wd[s], bits));
+#pragma unroll
+          for (int o = 0; o < kOps; ++o) ga[v] = EM::mfma16x16x32(hx::as_v8<M>(xf[s][o]), wf, ga[v]);
+        }
+      }
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const uint32_t wd[4] = {wq[v].x, wq[v].y, wq[v].z, wq[v].w};
-        wf[v] = widen<M>(wd[s]);
+        const float sc = E::lo(st[i][v][g]), zp = E::hi(st[i][v][g]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[v][e] = fmaf(sc, fmaf(-zp, gx[e], ga[v][e]), acc[v][e]);
       }
-      float nw[8];
-      if constexpr (NORM) {
+    }
+  };
+  for (int b = b_begin; b < b_end; b += D) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) nw[i] = 0.f;
-        if (in) {
-          const float4 lo = *reinterpret_cast<const float4*>(a.norm_w + k0);
-          const float4 hi = *reinterpret_cast<const float4*>(a.norm_w + k0 + 4);
-          nw[0] = lo.x, nw[1] = lo.y, nw[2] = lo.z, nw[3] = lo.w;
-          nw[4] = hi.x, nw[5] = hi.y, nw[6] = hi.z, nw[7] = hi.w;
-        }
-      }
-      if (s % (G / 32) == 0) {
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          gx[t] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int v = 0; v < NV; ++v) ga[t][v] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const int row = 16 * t + lr;
-        uint4 xv = hx::zero4();
-        if (in && row < a.rows) xv = *reinterpret_cast<const uint4*>(a.x + (int64_t)row * a.x_row + k0);
-        if constexpr (NORM) {
-          const uint32_t wd[4] = {xv.x, xv.y, xv.z, xv.w};
-          uint32_t h[4], l[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float e0 = E::lo(wd[q]), e1 = E::hi(wd[q]);
-            ss[t] = fmaf(e0, e0, ss[t]);
-            ss[t] = fmaf(e1, e1, ss[t]);
-            const float p0 = e0 * nw[2 * q], p1 = e1 * nw[2 * q + 1];
-            h[q] = hx::pack2_round<M>(p0, p1);
-            l[q] = hx::pack2_round<M>(p0 - EM::lo(h[q]), p1 - EM::hi(h[q]));
-          }
-          const typename EM::v8 xh = hx::as_v8<M>(make_uint4(h[0], h[1], h[2], h[3]));
-          const typename EM::v8 xl = hx::as_v8<M>(make_uint4(l[0], l[1], l[2], l[3]));
-          gx[t] = EM::mfma16x16x32(xh, ones, gx[t]);
-          gx[t] = EM::mfma16x16x32(xl, ones, gx[t]);
-#pragma unroll
-          for (int v = 0; v < NV; ++v) {
-            ga[t][v] = EM::mfma16x16x32(xh, hx::as_v8<M>(wf[v]), ga[t][v]);
-            ga[t][v] = EM::mfma16x16x32(xl, hx::as_v8<M>(wf[v]), ga[t][v]);
-          }
-        } else {
-          const typename EM::v8 xf = hx::as_v8<M>(xv);
-          gx[t] = EM::mfma16x16x32(xf, ones, gx[t]);
-#pragma unroll
-          for (int v = 0; v < NV; ++v) ga[t][v] = EM::mfma16x16x32(xf, hx::as_v8<M>(wf[v]), ga[t][v]);
-        }
-      }
-      if (s % (G / 32) == G / 32 - 1) {
-        const int g = s / (G / 32);
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              acc[t][v][i] = fmaf(sc[v][g], fmaf(-zp[v][g], gx[t][i], ga[t][v][i]), acc[t][v][i]);
-      }
+    for (int i = 0; i < D; ++i) {
+      if (b + i < b_end) consume(i, b + i);  // wave-uniform
+      load(i, b + i + D);
     }
   }
 
-  // Lane holds column lr of rows 4 lg .. + 3 of each tile.
+  // Lane holds column lr of rows 4 lg .. + 3.
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
+  for (int v = 0; v < NV; ++v)
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int i = 0; i < 4; ++i) red[w][v][16 * (4 * lg + i) + lr] = acc[v][i];
+  if constexpr (kNorm) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) red[w][t * NV + v][16 * (4 * lg + i) + lr] = acc[t][v][i];
-    if constexpr (NORM) {
-      const float sum = hx::add_xor32(hx::add_xor16(ss[t]));
-      if (lane < 16) s_ss[w][16 * t + lr] = sum;
+    for (int q = 0; q < kLoads; ++q) {
+      const float sum = hx::wave_sum_xor(ss[q], 1, 8);  // over the row's 16 lanes
+      if (lr == 0) s_ss[w][4 * q + lg] = sum;
     }
   }
   __syncthreads();
-  for (int e = tid; e < MT * 256; e += 64 * WAVES) {
-    const int t = e >> 8, row = e >> 4, n = n0 + (e & 15);
+  constexpr int kOut = SWIGLU ? 1 : NV;  // output tiles of kRows x 16
+  for (int e = tid; e < kOut * kRows * 16; e += 64 * WAVES) {
+    const int v0 = e / (kRows * 16), at = e % (kRows * 16);
+    const int row = rt * kRows + at / 16, n = n0 + 16 * v0 + at % 16;
     if (row >= a.rows || n >= a.cols) continue;
-    float y[NV];
+    constexpr int kSums = SWIGLU ? NV : 1;
+    float y[kSums];
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
+    for (int v = 0; v < kSums; ++v) {
       y[v] = 0.f;
 #pragma unroll
-      for (int ww = 0; ww < WAVES; ++ww) y[v] += red[ww][t * NV + v][e & 255];
+      for (int ww = 0; ww < WAVES; ++ww) {
+        y[v] += red[ww][v0 + v][at];
+        if constexpr (kPaired) y[v] += red[ww][v0 + v][at + 128];  // the other part
+      }
     }
-    if constexpr (NORM) {
+    if constexpr (kNorm) {
       float sum = 0.f;
 #pragma unroll
-      for (int ww = 0; ww < WAVES; ++ww) sum += s_ss[ww][row];
+      for (int ww = 0; ww < WAVES; ++ww) sum += s_ss[ww][at / 16];
       const float r = rsqrtf(__fadd_rn(__fdiv_rn(sum, (float)a.k), a.eps));
 #pragma unroll
-      for (int v = 0; v < NV; ++v) y[v] *= r;
+      for (int v = 0; v < kSums; ++v) y[v] *= r;
     }
     float o = y[0];
-    if constexpr (EPI == kEpiSwiglu) o = hx::silu(o) * y[NV - 1];
-    if constexpr (EPI == kEpiResidual) o += E::lo(a.res[(int64_t)row * a.res_row + n]);
+    if constexpr (SWIGLU) o = hx::silu(o) * y[kSums - 1];
+    else if (a.res != nullptr) o += E::lo(e < kRows * 16 && e == tid ? r_first : a.res[(int64_t)row * a.res_row + n]);
     a.out[(int64_t)row * a.out_row + n] = E::bits(o);
   }
 }
 
 struct DequantArgs {
   const uint8_t* w;
-  const uint16_t* scale;
-  const uint8_t* zero;
+  const uint32_t* steps;
   int32_t w_rows, k, blocks, w_pad, group;
   uint16_t* out;
   int64_t out_row;
@@ -249,64 +395,90 @@ __global__ __launch_bounds__(256) void int4_dequant_kernel(DequantArgs a, int64_
     const int k0 = b * kI4Block + 32 * s + 8 * lg;
     if (k0 >= a.k) return;
     const int64_t at = (int64_t)(k0 / a.group) * a.w_pad + row;
-    const float sc = E::lo(a.scale[at]), zp = (float)a.zero[at];
+    const uint32_t step = a.steps[at];
+    const float sc = E::lo(step), zp = E::hi(step) - 16.f;
+    const uint32_t turned = __builtin_amdgcn_alignbit(wd[s], wd[s], 3);
     uint32_t o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      o[i] = hx::pack2_round<T>(sc * ((float)(wd[s] >> (4 * i) & 15u) - zp),
-                                sc * ((float)(wd[s] >> (4 * i + 16) & 15u) - zp));
+      o[i] = hx::pack2_round<T>(sc * ((float)(turned >> (4 * i) & 15u) - zp),
+                                sc * ((float)(turned >> (4 * i + 16) & 15u) - zp));
     *reinterpret_cast<uint4*>(a.out + (int64_t)row * a.out_row + k0) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
-template <typename T, bool NORM, int EPI, int MT, int G>
-void launch_one(const Int4Args& a, hipStream_t s) {
-  constexpr int kWaves = MT * (EPI == kEpiSwiglu ? 2 : 1) > 4 ? 4 : 8;  // the sums fit 64 KiB of LDS
-  hipLaunchKernelGGL((int4_gemm_kernel<T, NORM, EPI, MT, G, kWaves>), dim3((unsigned)((a.cols + 15) / 16)),
-                     dim3(64 * kWaves), 0, s, a);
+template <typename T, int IN, bool SWIGLU, int G, int NV>
+int launch_tiles(Int4Args a, hipStream_t s) {
+  constexpr int kCols = SWIGLU ? 16 : 16 * NV, kRows = IN == kNorm4 || IN == kNorm8 ? 8 : 16;
+  a.row_tiles = (a.rows + kRows - 1) / kRows;
+  a.col_tiles = (a.cols + kCols - 1) / kCols;
+  // Waves that split K, and blocks in flight. bf16, 1 / 8 / 16 rows, W from HBM (us): 9728 + 9728
+  // columns of 2560 with SwiGLU, 4 waves and 1 block 10.2 / 11.1 / 15.0, 2 blocks 10.1 / 12.2 /
+  // 15.2, 8 waves 9.9 / 11.7 / 21.8 (their LDS leaves one workgroup to a CU at 16 rows); 2560
+  // columns of 9728, 8 waves and 2 blocks 6.6 / 7.4 / 9.4, 3 blocks 6.3 / 7.3 / 9.8, 4 waves
+  // 9.1 / 10.0 / 11.0.
+  constexpr int kWaves = SWIGLU ? 4 : 8, kDepth = SWIGLU ? 1 : 2;
+  const auto fn = int4_gemm_kernel<T, IN, SWIGLU, G, NV, kWaves, kDepth>;
+  hipLaunchKernelGGL(fn, dim3((unsigned)((a.col_tiles + 7) / 8 * 8 * a.row_tiles)), dim3(64 * kWaves), 0, s, a);
+  return hx::status_from_hip(hipGetLastError());
 }
 
-template <typename T, bool NORM, int EPI, int MT>
-void launch_group(const Int4Args& a, int group, hipStream_t s) {
-  if (group == 128) launch_one<T, NORM, EPI, MT, 128>(a, s);
-  else if (group == 64) launch_one<T, NORM, EPI, MT, 64>(a, s);
-  else launch_one<T, NORM, EPI, MT, 32>(a, s);
+// Two W tiles a wave where x costs more than a load (6144 columns of 2560, normalised, 1 / 8 / 16
+// rows: 5.5 / 6.0 / 8.0 us, one tile 6.2 / 7.6 / 10.6), one where it does not (2560 columns of
+// 9728: 6.4 / 7.3 / 9.3, two tiles 8.2 / 9.2 / 11.0), two again for several row tiles, which
+// fill the chip (64 rows: 16.8, one tile 18.7).
+template <typename T, int IN, bool SWIGLU, int NV = SWIGLU || IN >= kNorm4 ? 2 : 1>
+int launch_group(const Int4Args& a, int group, hipStream_t s) {
+  if (group == 128) return launch_tiles<T, IN, SWIGLU, 128, NV>(a, s);
+  if (group == 64) return launch_tiles<T, IN, SWIGLU, 64, NV>(a, s);
+  return launch_tiles<T, IN, SWIGLU, 32, NV>(a, s);
 }
 
-template <typename T, bool NORM, int EPI>
-void launch_rows(const Int4Args& a, int group, hipStream_t s) {
-  if (a.rows <= 16) launch_group<T, NORM, EPI, 1>(a, group, s);
-  else if (a.rows <= 32) launch_group<T, NORM, EPI, 2>(a, group, s);
-  else launch_group<T, NORM, EPI, 4>(a, group, s);
+// Rows that each workgroup normalises on their way in; more of them are normalised once, in a
+// launch of about 3 us (6144 columns of 2560: 16 rows 8.0 us, 17 rows 12.6; 64 rows 16.5 us, and
+// 32.1 normalised by every workgroup's own row tiles of 8).
+constexpr int kFusedNormRows = 16;
+
+template <typename T, bool SWIGLU>
+int launch_in(const Int4Args& a, int group, hipStream_t s) {
+  if (a.norm_w == nullptr) {
+    if (a.rows <= 4) return launch_group<T, kRaw4, SWIGLU>(a, group, s);
+    if (a.rows <= 8) return launch_group<T, kRaw8, SWIGLU>(a, group, s);
+    if (a.rows <= 16) return launch_group<T, kRaw16, SWIGLU>(a, group, s);
+    return launch_group<T, kRaw16, SWIGLU, 2>(a, group, s);
+  }
+  if (a.rows <= 4) return launch_group<T, kNorm4, SWIGLU>(a, group, s);
+  if (a.rows <= 8) return launch_group<T, kNorm8, SWIGLU>(a, group, s);
+  if (a.rows <= kFusedNormRows) return launch_group<T, kNorm16, SWIGLU>(a, group, s);
+  hipLaunchKernelGGL(int4_norm_kernel<T>, dim3((unsigned)a.rows), dim3(256), 0, s, a, const_cast<uint16_t*>(a.h));
+  return launch_group<T, kParts16, SWIGLU>(a, group, s);
 }
 
-template <typename T>
-void launch_epi(const Int4Args& a, int group, bool swiglu, hipStream_t s) {
-  const bool norm = a.norm_w != nullptr;
-  if (swiglu && norm) launch_rows<T, true, kEpiSwiglu>(a, group, s);
-  else if (swiglu) launch_rows<T, false, kEpiSwiglu>(a, group, s);
-  else if (a.res != nullptr && norm) launch_rows<T, true, kEpiResidual>(a, group, s);
-  else if (a.res != nullptr) launch_rows<T, false, kEpiResidual>(a, group, s);
-  else if (norm) launch_rows<T, true, kEpiPlain>(a, group, s);
-  else launch_rows<T, false, kEpiPlain>(a, group, s);
-}
-
-bool bad_weight(const void* w, const void* scale, const void* zero, int32_t k, int32_t group) {
-  return !w || !scale || !zero || (reinterpret_cast<uintptr_t>(w) & 15) || (reinterpret_cast<uintptr_t>(scale) & 1) ||
-         k % group;
+bool bad_weight(const void* w, const void* steps, int32_t k, int32_t group) {
+  return !w || !steps || (reinterpret_cast<uintptr_t>(w) & 15) || (reinterpret_cast<uintptr_t>(steps) & 3) || k % group;
 }
 
 }  // namespace
 
-extern "C" int hx_int4_gemm(const void* x, int64_t x_row_stride, int64_t rows, const void* packed, const void* scales,
-                            const void* zeros, int32_t cols, int32_t k, int32_t group, int32_t dtype,
+extern "C" size_t hx_int4_workspace_bytes(int64_t rows, int32_t k, int32_t norm) {
+  const int64_t blocks = ((int64_t)k + kI4Block - 1) / kI4Block;
+  if (!norm || rows <= kFusedNormRows || k < 1) return 0;
+  return (size_t)((rows + 15) / 16 * 32) * (size_t)blocks * kI4Block * 2;
+}
+
+extern "C" int hx_int4_gemm(const void* x, int64_t x_row_stride, int64_t rows, const void* packed, const void* steps,
+                            int32_t cols, int32_t k, int32_t group, int32_t dtype,
                             const float* norm_weight, float eps, const void* residual, int64_t residual_row_stride,
-                            int32_t swiglu, void* out, int64_t out_row_stride, void* stream) {
+                            int32_t swiglu, void* out, int64_t out_row_stride, void* workspace,
+                            size_t workspace_bytes, void* stream) {
   if (dtype != HX_DTYPE_BF16 && dtype != HX_DTYPE_FP16) return HX_E_UNSUPPORTED;
   if (group != 32 && group != 64 && group != 128) return HX_E_UNSUPPORTED;
   if (rows < 0 || cols < 1 || k < 1 || (norm_weight != nullptr && !(eps >= 0.f))) return HX_E_INVALID_ARG;
-  if (rows > 64 || cols > (1 << 29) || k > (1 << 29)) return HX_E_UNSUPPORTED;
-  if (bad_weight(packed, scales, zeros, k, group) || (swiglu && residual)) return HX_E_INVALID_ARG;
+  // 32-bit buffer offsets within a row tile of x, a column tile of W and the steps.
+  if (rows > 64 || cols > (1 << 26) || k > (1 << 20) || x_row_stride > (1 << 26) ||
+      ((int64_t)k / group + 4) * (2 * (int64_t)cols + 16) * 4 > 0x7fffffff)
+    return HX_E_UNSUPPORTED;
+  if (bad_weight(packed, steps, k, group) || (swiglu && residual)) return HX_E_INVALID_ARG;
   if (rows == 0) return HX_OK;
   if (!x || !out) return HX_E_INVALID_ARG;
   if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(norm_weight)) & 15) || x_row_stride % 8 ||
@@ -315,12 +487,15 @@ extern "C" int hx_int4_gemm(const void* x, int64_t x_row_stride, int64_t rows, c
   if (((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(residual)) & 1) || out_row_stride < cols ||
       (residual != nullptr && residual_row_stride < cols))
     return HX_E_INVALID_ARG;
+  const size_t need = hx_int4_workspace_bytes(rows, k, norm_weight != nullptr);
+  if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need))
+    return HX_E_WORKSPACE;
   Int4Args a;
   a.x = static_cast<const uint16_t*>(x);
+  a.h = static_cast<const uint16_t*>(workspace);
   a.x_row = x_row_stride;
   a.w = static_cast<const uint8_t*>(packed);
-  a.scale = static_cast<const uint16_t*>(scales);
-  a.zero = static_cast<const uint8_t*>(zeros);
+  a.steps = static_cast<const uint32_t*>(steps);
   a.rows = (int32_t)rows;
   a.cols = cols;
   a.k = k;
@@ -333,24 +508,23 @@ extern "C" int hx_int4_gemm(const void* x, int64_t x_row_stride, int64_t rows, c
   a.out = static_cast<uint16_t*>(out);
   a.out_row = out_row_stride;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == HX_DTYPE_BF16) launch_epi<__bf16>(a, group, swiglu != 0, s);
-  else launch_epi<_Float16>(a, group, swiglu != 0, s);
-  return hx::status_from_hip(hipGetLastError());
+  if (dtype == HX_DTYPE_BF16)
+    return swiglu ? launch_in<__bf16, true>(a, group, s) : launch_in<__bf16, false>(a, group, s);
+  return swiglu ? launch_in<_Float16, true>(a, group, s) : launch_in<_Float16, false>(a, group, s);
 }
 
-extern "C" int hx_int4_dequantize(const void* packed, const void* scales, const void* zeros, int32_t weight_rows,
-                                  int32_t k, int32_t group, int32_t dtype, void* out, int64_t out_row_stride,
+extern "C" int hx_int4_dequantize(const void* packed, const void* steps, int32_t weight_rows, int32_t k, int32_t group,
+                                  int32_t dtype, void* out, int64_t out_row_stride,
                                   void* stream) {
   if (dtype != HX_DTYPE_BF16 && dtype != HX_DTYPE_FP16) return HX_E_UNSUPPORTED;
   if (group != 32 && group != 64 && group != 128) return HX_E_UNSUPPORTED;
   if (weight_rows < 1 || k < 1 || weight_rows > (1 << 30) || k > (1 << 29)) return HX_E_INVALID_ARG;
-  if (bad_weight(packed, scales, zeros, k, group) || !out || (reinterpret_cast<uintptr_t>(out) & 15) ||
+  if (bad_weight(packed, steps, k, group) || !out || (reinterpret_cast<uintptr_t>(out) & 15) ||
       out_row_stride % 8 || out_row_stride < k)
     return HX_E_INVALID_ARG;
   DequantArgs a;
   a.w = static_cast<const uint8_t*>(packed);
-  a.scale = static_cast<const uint16_t*>(scales);
-  a.zero = static_cast<const uint8_t*>(zeros);
+  a.steps = static_cast<const uint32_t*>(steps);
   a.w_rows = weight_rows;
   a.k = k;
   a.blocks = (k + kI4Block - 1) / kI4Block;

@@ -604,17 +604,18 @@ def block_sparse_attn(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
 # ------------------------------------------------------- products with 4-bit weights
 class Int4Weight(NamedTuple):
     """A weight matrix ``[rows, k]`` in 4 bits with a scale and a zero point per ``group``
-    elements of k: ``W[n, k] = scales[k // group, n] * (q[n, k] - zeros[k // group, n])``.
-    ``packed`` holds q in the order the kernel reads it (hx_int4_gemm); ``scales`` (bfloat16
-    or float16: the products' dtype) and ``zeros`` (uint8) are ``[groups, rows]``, rows
-    rounded up to 16. Made by ``int4_quantize`` or ``int4_pack``."""
+    elements of k: ``W[n, k] = scale[k // group, n] * (q[n, k] - zero[k // group, n])``.
+    ``packed`` holds q in the order the kernel reads it (hx_int4_gemm), ``steps`` (int32
+    ``[groups, rows]``, rows rounded up to 16) a scale's bits in the low half and those of 16
+    + a zero point in the high one; ``dtype`` is the scales' and the products' type. Made by
+    ``int4_quantize`` or ``int4_pack``."""
 
     packed: torch.Tensor
-    scales: torch.Tensor
-    zeros: torch.Tensor
+    steps: torch.Tensor
     rows: int
     k: int
     group: int
+    dtype: torch.dtype
 
 
 def int4_pack(values: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor) -> Int4Weight:
@@ -640,13 +641,15 @@ def int4_pack(values: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor) -
     q = torch.nn.functional.pad(values, (0, more_k, 0, more_rows)).to(torch.int64)
     q = q.view(-1, 16, q.shape[1] // 128, 4, 4, 8)  # tile, row, block, word, k group of a lane, element
     shift = torch.tensor([4 * (j // 2) + 16 * (j % 2) for j in range(8)], device=q.device)
-    words = (q << shift).sum(dim=-1)
+    words = (q << shift).sum(dim=-1) << 3
+    words = (words & 0xffffffff) | words >> 32  # turned by 3
     words = torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
     packed = words.permute(0, 2, 4, 1, 3).contiguous().view(torch.uint8)
-    pad = (0, more_rows, 0, more_k // group)
-    return Int4Weight(packed.view(packed.shape[0], packed.shape[1], 64, 16),
-                      torch.nn.functional.pad(scales, pad).contiguous(),
-                      torch.nn.functional.pad(zeros, pad).contiguous(), rows, k, group)
+    low, high = (t.contiguous().view(torch.int16).to(torch.int32) & 0xffff
+                 for t in (scales, (zeros.to(torch.float32) + 16).to(scales.dtype)))
+    steps = low | high << 16
+    steps = torch.nn.functional.pad(steps, (0, more_rows, 0, more_k // group)).contiguous()
+    return Int4Weight(packed.view(packed.shape[0], packed.shape[1], 64, 16), steps, rows, k, group, scales.dtype)
 
 
 def int4_quantize(weight: torch.Tensor, group: int = 128) -> Int4Weight:
@@ -677,13 +680,13 @@ def _check_int4(weight: Int4Weight, device: torch.device) -> int:
         raise ValueError("the weight's group must be 32, 64 or 128 and divide its k.")
     shape = (blocks * 128 // weight.group, tiles * 16)
     if weight.packed.dtype != torch.uint8 or tuple(weight.packed.shape) != (tiles, blocks, 64, 16) \
-            or weight.zeros.dtype != torch.uint8 or tuple(weight.zeros.shape) != shape \
-            or weight.scales.dtype not in _SUPPORTED or tuple(weight.scales.shape) != shape:
+            or weight.steps.dtype != torch.int32 or tuple(weight.steps.shape) != shape \
+            or weight.dtype not in _SUPPORTED:
         raise ValueError("an Int4Weight's tensors do not have the shapes and dtypes that int4_pack gives.")
-    for t in (weight.packed, weight.scales, weight.zeros):
+    for t in (weight.packed, weight.steps):
         if t.device != device or not t.is_contiguous():
             raise ValueError("an Int4Weight's tensors must be contiguous, on the product's device.")
-    return _SUPPORTED[weight.scales.dtype]
+    return _SUPPORTED[weight.dtype]
 
 
 def _launch(device: torch.device, fn, *args) -> int:
@@ -703,11 +706,11 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, norm_weight: torch.Tenso
     """``block_linear`` with 4-bit weights, for up to 64 rows: ``x @ W.t()`` with ``x``
     RMSNormed first by ``norm_weight``, ``residual`` added, or, with ``swiglu`` (``W`` holds
     gate, then up rows), ``silu(gate) * up``, in one launch. In fp32 and rounded once, at the
-    end. ``x`` ``[..., k]`` and ``residual`` ``[..., n]`` contiguous, in the scales' dtype, ``x``
+    end. ``x`` ``[..., k]`` and ``residual`` ``[..., n]`` contiguous, in the weight's dtype, ``x``
     16-byte aligned. More rows: ``int4_dequantize`` and a library product."""
     device = _require_gpu(x)
     dtype = _check_int4(weight, device)
-    if x.ndim < 1 or x.dtype != weight.scales.dtype or x.shape[-1] != weight.k or not x.is_contiguous():
+    if x.ndim < 1 or x.dtype != weight.dtype or x.shape[-1] != weight.k or not x.is_contiguous():
         raise ValueError("x must be contiguous [..., k], in the weight's dtype.")
     cols = weight.rows
     if swiglu:
@@ -726,23 +729,27 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, norm_weight: torch.Tenso
         if norm_weight.data_ptr() % 16:
             norm_weight = norm_weight.clone()  # a slice of a larger buffer
     out = torch.empty(shape, dtype=x.dtype, device=device)
+    rows, lib = x.numel() // weight.k, _capi.lib()
+    ws_bytes = 0 if norm_weight is None else lib.hx_int4_workspace_bytes(rows, weight.k, 1)
+    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
     code = _launch(
-        device, _capi.lib().hx_int4_gemm, x.data_ptr(), weight.k, x.numel() // weight.k, weight.packed.data_ptr(),
-        weight.scales.data_ptr(), weight.zeros.data_ptr(), cols, weight.k, weight.group, dtype,
+        device, lib.hx_int4_gemm, x.data_ptr(), weight.k, rows, weight.packed.data_ptr(),
+        weight.steps.data_ptr(), cols, weight.k, weight.group, dtype,
         None if norm_weight is None else norm_weight.data_ptr(), eps,
-        None if residual is None else residual.data_ptr(), cols, 1 if swiglu else 0, out.data_ptr(), cols)
+        None if residual is None else residual.data_ptr(), cols, 1 if swiglu else 0, out.data_ptr(), cols,
+        None if workspace is None else workspace.data_ptr(), ws_bytes)
     _capi.check(code, "hx_int4_gemm")
     return out
 
 
 def int4_dequantize(weight: Int4Weight) -> torch.Tensor:
-    """``[rows, k]`` in the scales' dtype: ``scales * (q - zeros)``, rounded once."""
+    """``[rows, k]`` in the weight's dtype: ``scale * (q - zero)``, rounded once."""
     device = _require_gpu(weight.packed)
     dtype = _check_int4(weight, device)
     # Rows of a multiple of 8 elements (k is one of 32), so every row is 16-byte aligned.
-    out = torch.empty((weight.rows, weight.k), dtype=weight.scales.dtype, device=device)
-    code = _launch(device, _capi.lib().hx_int4_dequantize, weight.packed.data_ptr(), weight.scales.data_ptr(),
-                   weight.zeros.data_ptr(), weight.rows, weight.k, weight.group, dtype, out.data_ptr(), weight.k)
+    out = torch.empty((weight.rows, weight.k), dtype=weight.dtype, device=device)
+    code = _launch(device, _capi.lib().hx_int4_dequantize, weight.packed.data_ptr(), weight.steps.data_ptr(),
+                   weight.rows, weight.k, weight.group, dtype, out.data_ptr(), weight.k)
     _capi.check(code, "hx_int4_dequantize")
     return out
 

@@ -576,20 +576,24 @@ int hx_skinny_gemm(const void* x, int64_t x_row_stride, int64_t rows, const void
  * 16 and 128:
  *   packed  uint8 [w_pad / 16][k_pad / 128][64][16], 16-byte aligned: byte group (c, r) =
  *           lane 16 c + r of a tile holds four words of row r; word s holds the k elements
- *           128 b + 32 s + 8 c + j, j = 0..7, element j at bits 4 (j / 2) + 16 (j % 2)
- *   scales  element type [k_pad / group][w_pad], 0 where W has no row or k
- *   zeros   uint8 [k_pad / group][w_pad]
+ *           128 b + 32 s + 8 c + j, j = 0..7, element j at bits 3 + 4 (j / 2) + 16 (j % 2)
+ *           modulo 32
+ *   steps   uint32 [k_pad / group][w_pad]: in the element type, the scale in the low half and
+ *           16 + zero in the high one; 0 where W has no row or k
  * x and norm_weight 16-byte aligned, x_row_stride a multiple of 8. out must not overlap x or
  * the weights; it may be the residual. HX_E_UNSUPPORTED for more than 64 rows or another
- * group. hx_int4_dequantize writes round(W), rows of k elements, out 16-byte aligned and
+ * group. The workspace is hx_int4_workspace_bytes(rows, k, norm_weight given) bytes (may be
+ * 0), 16-byte aligned; calls that share one must be ordered. hx_int4_dequantize writes round(W), rows of k elements, out 16-byte aligned and
  * out_row_stride a multiple of 8. */
+size_t hx_int4_workspace_bytes(int64_t rows, int32_t k, int32_t norm);
 int hx_int4_gemm(const void* x, int64_t x_row_stride, int64_t rows, const void* packed,
-                 const void* scales, const void* zeros, int32_t cols, int32_t k,
-                 int32_t group, int32_t dtype, const float* norm_weight, float eps,
+                 const void* steps, int32_t cols, int32_t k, int32_t group, int32_t dtype,
+                 const float* norm_weight, float eps,
                  const void* residual, int64_t residual_row_stride, int32_t swiglu,
-                 void* out, int64_t out_row_stride, void* stream);
-int hx_int4_dequantize(const void* packed, const void* scales, const void* zeros,
-                       int32_t weight_rows, int32_t k, int32_t group, int32_t dtype,
+                 void* out, int64_t out_row_stride, void* workspace,
+                 size_t workspace_bytes, void* stream);
+int hx_int4_dequantize(const void* packed, const void* steps, int32_t weight_rows,
+                       int32_t k, int32_t group, int32_t dtype,
                        void* out, int64_t out_row_stride, void* stream);
 
 /*

@@ -18,14 +18,14 @@ def _call(name, base, **change):
     return getattr(_capi.lib(), name)(*args.values())
 
 
-INT4 = dict(x=P, x_row=256, rows=4, packed=P, scales=P, zeros=P, cols=16, k=256, group=64, dtype=0, norm=None, eps=0.0,
+INT4 = dict(x=P, x_row=256, rows=4, packed=P, steps=P, cols=16, k=256, group=64, dtype=0, norm=None, eps=0.0,
             residual=None, residual_row=16, swiglu=0, out=P, out_row=16, stream=None)
 
 
 @pytest.mark.parametrize("change,code", [
     (dict(dtype=2), NO), (dict(group=16), NO), (dict(group=48), NO), (dict(rows=65), NO), (dict(rows=-1), BAD),
     (dict(cols=0), BAD), (dict(k=0), BAD), (dict(k=96), BAD), (dict(x=None), BAD), (dict(packed=None), BAD),
-    (dict(scales=None), BAD), (dict(zeros=None), BAD), (dict(out=None), BAD), (dict(packed=P + 8), BAD),
+    (dict(steps=None), BAD), (dict(steps=P + 2), BAD), (dict(out=None), BAD), (dict(packed=P + 8), BAD),
     (dict(x=P + 2), BAD), (dict(x_row=255), BAD), (dict(x_row=252), BAD), (dict(norm=P, eps=-1.0), BAD),
     (dict(norm=P, eps=float("nan")), BAD), (dict(norm=P + 4), BAD), (dict(out=P + 1), BAD), (dict(out_row=15), BAD),
     (dict(residual=P, swiglu=1), BAD), (dict(residual=P, residual_row=15), BAD), (dict(rows=0), 0)])
@@ -33,7 +33,7 @@ def test_int4_gemm(change, code):
     assert _call("hx_int4_gemm", INT4, **change) == code
 
 
-DEQUANT = dict(packed=P, scales=P, zeros=P, rows=20, k=256, group=64, dtype=0, out=P, out_row=256, stream=None)
+DEQUANT = dict(packed=P, steps=P, rows=20, k=256, group=64, dtype=0, out=P, out_row=256, stream=None)
 
 
 @pytest.mark.parametrize("change,code", [

@@ -134,7 +134,8 @@ def test_int4_quantize(device, group, dtype):
     q = ops.int4_quantize(w.to(device), group)
     assert (q.rows, q.k, q.group) == (33, 384, group)
     back = ops.int4_dequantize(q).cpu().double()
-    step = q.scales.cpu().double()[:, :33].t().repeat_interleave(group, 1)[:, :384]
+    scales = (q.steps & 0xffff).to(torch.int16).view(dtype)
+    step = scales.cpu().double()[:, :33].t().repeat_interleave(group, 1)[:, :384]
     # half a step; the scale's own rounding (half an eps of 15 steps) may push an end past the
     # last value; and the result's rounding
     most = step * (0.5 + 15 * torch.finfo(dtype).eps) + torch.finfo(dtype).eps / 2 * w.double().abs()
@@ -187,8 +188,9 @@ def test_int4_refusals(device):
         lambda: ops.int4_linear(x, w, norm_weight=torch.ones(255, device=device)),
         lambda: ops.int4_linear(x, w, norm_weight=torch.ones(256, device=device), eps=-1.0),
         lambda: ops.int4_linear(x, w._replace(packed=w.packed[:1])),
-        lambda: ops.int4_linear(x, w._replace(scales=w.scales.float())),
-        lambda: ops.int4_linear(x, w._replace(zeros=w.zeros.cpu())),
+        lambda: ops.int4_linear(x, w._replace(steps=w.steps.float())),
+        lambda: ops.int4_linear(x, w._replace(steps=w.steps.cpu())),
+        lambda: ops.int4_linear(x, w._replace(dtype=torch.float32)),
         lambda: ops.int4_dequantize(w._replace(rows=64)),
         lambda: ops.int4_pack(parts[0].to(device), parts[1].to(device), parts[2].to(device) + 16),
         lambda: ops.int4_quantize(torch.full((16, 128), float("nan"), dtype=torch.bfloat16, device=device)),
