@@ -19,7 +19,7 @@ def _call(name, base, **change):
 
 
 INT4 = dict(x=P, x_row=256, rows=4, packed=P, steps=P, cols=16, k=256, group=64, dtype=0, norm=None, eps=0.0,
-            residual=None, residual_row=16, swiglu=0, out=P, out_row=16, stream=None)
+            residual=None, residual_row=16, swiglu=0, out=P, out_row=16, ws=P, ws_bytes=1 << 20, stream=None)
 
 
 @pytest.mark.parametrize("change,code", [
@@ -28,7 +28,9 @@ INT4 = dict(x=P, x_row=256, rows=4, packed=P, steps=P, cols=16, k=256, group=64,
     (dict(steps=None), BAD), (dict(steps=P + 2), BAD), (dict(out=None), BAD), (dict(packed=P + 8), BAD),
     (dict(x=P + 2), BAD), (dict(x_row=255), BAD), (dict(x_row=252), BAD), (dict(norm=P, eps=-1.0), BAD),
     (dict(norm=P, eps=float("nan")), BAD), (dict(norm=P + 4), BAD), (dict(out=P + 1), BAD), (dict(out_row=15), BAD),
-    (dict(residual=P, swiglu=1), BAD), (dict(residual=P, residual_row=15), BAD), (dict(rows=0), 0)])
+    (dict(residual=P, swiglu=1), BAD), (dict(residual=P, residual_row=15), BAD), (dict(rows=0), 0),
+    (dict(norm=P, rows=17, ws=None), WS), (dict(norm=P, rows=17, ws=P + 8), WS), (dict(norm=P, rows=17, ws_bytes=16), WS),
+    (dict(k=1 << 21, x_row=1 << 21), NO), (dict(x_row=1 << 27), NO), (dict(cols=1 << 26), NO)])
 def test_int4_gemm(change, code):
     assert _call("hx_int4_gemm", INT4, **change) == code
 
@@ -104,6 +106,9 @@ def test_workspace_sizes():
     lib = _capi.lib()
     assert lib.hx_logit_rules_workspace_bytes(3, 4097) == 3 * 2 * 8
     assert lib.hx_logit_rules_workspace_bytes(0, 10) == 0
+    # normalised rows past one tile: two parts of each row tile of 16, k rounded up to 128
+    assert lib.hx_int4_workspace_bytes(16, 2560, 1) == lib.hx_int4_workspace_bytes(64, 2560, 0) == 0
+    assert lib.hx_int4_workspace_bytes(17, 200, 1) == 2 * 32 * 256 * 2
     # Few rows: their lists are split, each part with its sums and two statistics per head.
     small = lib.hx_block_sparse_workspace_bytes(1, 32, 8, 128, 32, 64)
     assert small > 0 and small % (32 * 130 * 4) == 0
