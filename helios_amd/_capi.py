@@ -230,8 +230,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ctypes.c_int,
         [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i64,
          _i32, _i32, _i32, _i32, _c_void_p, _i32, _i32, _i32,
-         _c_void_p, _i64, _i32, _i32, _i32, _i32, _i32, _c_void_p, _c_void_p],
+         _c_void_p, _i64, _i32, _i32, _i32, _i32, _i32, _c_void_p, _c_void_p, _size, _c_void_p],
     ),
+    "hx_select_blocks_workspace_bytes": (_size, [_i64, _i32, _i64]),
     "hx_block_sparse_workspace_bytes": (_size, [_i64, _i32, _i32, _i32, _i32, _i32]),
     "hx_block_sparse_attn": (
         ctypes.c_int,

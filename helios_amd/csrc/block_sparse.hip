@@ -8,12 +8,18 @@
 // the G query heads that share the KV head the bound is linear in two vectors,
 //   s = sum_d (sum_g min(q_g[d], 0)) lower[d] + (sum_g max(q_g[d], 0)) upper[d],
 // and the blocks with the largest s, with the first `sink` and the last `recent` ones, are the
-// row's selection for that KV head (select_blocks_kernel). The attention is the softmax over
+// row's selection for that KV head (block_scores_kernel, select_blocks_kernel). The attention is the softmax over
 // the keys of those blocks alone (sparse_attn_kernel).
 
 #include "hx_common.h"
 
 namespace {
+
+// HIP's min and max go through double for some mixes of 64-bit types.
+template <typename I>
+__device__ __forceinline__ I least_of(I a, I b) { return b < a ? b : a; }
+template <typename I>
+__device__ __forceinline__ I most_of(I a, I b) { return a < b ? b : a; }
 
 // ------------------------------------------------------------------------- key bounds
 //
@@ -116,13 +122,17 @@ __global__ __launch_bounds__(kBdThreads) void block_bounds_kernel(BoundsArgs a) 
 
 // -------------------------------------------------------------------------- selection
 //
-// A workgroup takes one query row and KV head. The scores are 64-bit sums: the blocks at the
-// border of a selection lie close together, and a sum in another order would choose others.
-// The r-th largest of the free blocks' keys is found bit by bit (a bit is set when r keys
-// still reach it), from the highest bit in which the keys differ.
+// block_scores_kernel reads the bounds once, HBM-bound: LANES lanes hold a query row's sums for
+// one KV head, eight dims each, and take kScPer blocks, all in flight at once. The sums are
+// 64-bit: the blocks at the border of a selection lie close together, and a sum in another order
+// would choose others. Their keys (64-bit integers in the scores' order) go to the workspace.
+// select_blocks_kernel holds a row's keys in registers and finds the r-th largest free one by
+// counting keys in bins.
 
-constexpr int kSelThreads = 256;
-constexpr int kSelMaxBlocks = 16384;  // 64-bit keys in LDS
+constexpr int kScThreads = 256;
+constexpr int kScPer = 4;
+constexpr int kSelMaxBlocks = 16384;  // keys in the registers of one workgroup
+constexpr int kSelBins = 1024, kSelPasses = 7;  // 10 bits of the range a pass
 
 struct SelectArgs {
   const uint16_t* q;
@@ -137,8 +147,15 @@ struct SelectArgs {
   int64_t table_stride;
   int32_t batch, table_width;
   int32_t budget, sink, recent;
+  uint32_t page_magic;             // 2^32 / blocks of a page, rounded up
+  int32_t chunks, stretch, most;  // workgroups along a row's blocks, blocks of one; blocks the table covers
+  uint64_t* order;       // [n][n_heads][most]
   int32_t* out;
 };
+
+// Keys of blocks that are taken in any case, and of those on a page outside the pool; every
+// other block's is above both.
+constexpr uint64_t kKeyTaken = 0, kKeyLast = 1;
 
 __device__ __forceinline__ uint64_t ordered_key(double s) {
   const uint64_t u = __builtin_bit_cast(uint64_t, s + 0.0);  // -0 like 0
@@ -146,111 +163,305 @@ __device__ __forceinline__ uint64_t ordered_key(double s) {
   return (u >> 63) ? ~u : u | 0x8000000000000000ull;
 }
 
-__device__ __forceinline__ double add_xor(double v, int m) { return v + __shfl_xor(v, m); }
+// Blocks that row i sees: 0 where its row or sequence is not there.
+__device__ __forceinline__ int selected_from(const SelectArgs& a, int64_t i, int64_t& row, int64_t& seq) {
+  row = a.rows != nullptr ? a.rows[i] : i;
+  seq = a.row_seq != nullptr ? a.row_seq[i] : i;
+  if (seq < 0 || seq >= a.batch || row < 0 || row >= a.q_rows) return 0;
+  const int64_t n = least_of<int64_t>(max(a.keys[i], 0), (int64_t)a.table_width * a.page);
+  return (int)((n + a.block - 1) / a.block);
+}
 
-template <typename T>
-__global__ __launch_bounds__(kSelThreads) void select_blocks_kernel(SelectArgs a) {
+// Sum over LANES lanes next to each other, in all of them (pairings as in hx::dpp).
+template <int CTRL>
+__device__ __forceinline__ double add_dpp(double v) {
+  typedef int i2 __attribute__((ext_vector_type(2)));
+  i2 u = __builtin_bit_cast(i2, v);
+  u.x = __builtin_amdgcn_update_dpp(0, u.x, CTRL, 0xF, 0xF, false);
+  u.y = __builtin_amdgcn_update_dpp(0, u.y, CTRL, 0xF, 0xF, false);
+  return v + __builtin_bit_cast(double, u);
+}
+template <int LANES>
+__device__ __forceinline__ double lanes_sum(double v) {
+  v = add_dpp<hx::kDppHalfMirror>(add_dpp<hx::kDppXor2>(add_dpp<hx::kDppXor1>(v)));
+  if constexpr (LANES >= 16) v = add_dpp<hx::kDppMirror>(v);
+  if constexpr (LANES >= 32) v += __shfl_xor(v, 16);
+  return v;
+}
+
+// A workgroup takes a stretch of a row's blocks for one KV head, kGroups x kScPer at a time.
+template <typename T, int LANES>
+__global__ __launch_bounds__(kScThreads) void block_scores_kernel(SelectArgs a) {
   typedef hx::Elem<T> E;
-  extern __shared__ __attribute__((aligned(16))) uint64_t s_key[];
-  __shared__ double s_q[2][256];  // sums over the group of min(q, 0) and of max(q, 0)
-  const int tid = hx::tid_x();
-  const int64_t i = hx::wg_x() / a.n_heads;
-  const int h = hx::wg_x() % a.n_heads;
-  int32_t* out = a.out + (int64_t)hx::wg_x() * a.budget;
-  const int64_t row = a.rows != nullptr ? a.rows[i] : i;
-  const int64_t seq = a.row_seq != nullptr ? a.row_seq[i] : i;
-  int64_t n = max(a.keys[i], 0);
-  n = min(n, (int64_t)a.table_width * a.page);
-  if (seq < 0 || seq >= a.batch || row < 0 || row >= a.q_rows) n = 0;
-  const int count = (int)((n + a.block - 1) / a.block);
-  if (count <= a.budget) {
-    for (int j = tid; j < a.budget; j += kSelThreads) out[j] = j < count ? j : -1;
-    return;
-  }
-  for (int d = tid; d < a.head_dim; d += kSelThreads) {
-    double neg = 0.0, pos = 0.0;
-    for (int g = 0; g < a.group; ++g) {
-      const float x = E::lo(a.q[row * a.q_row + (int64_t)(h * a.group + g) * a.q_head + d]);
-      // By the sign bit: a NaN counts in one of the sums.
-      if (__float_as_uint(x) >> 31) neg += (double)x;
-      else pos += (double)x;
+  constexpr int kGroups = kScThreads / LANES, kPass = kGroups * kScPer;
+  __shared__ double2 s_q[256];
+  const int tid = hx::tid_x(), li = tid % LANES, g = tid / LANES;
+  const int begin = hx::wg_x() % a.chunks * a.stretch;
+  const int64_t ih = hx::wg_x() / a.chunks, i = ih / a.n_heads;
+  const int h = (int)(ih % a.n_heads);
+  int64_t row, seq;
+  const int count = selected_from(a, i, row, seq);
+  if (count <= a.budget || begin >= count) return;
+  const int end = min(begin + a.stretch, count);
+  const int32_t* table = a.table + seq * a.table_stride;
+  const int per_page = a.page / a.block, d = 8 * li;
+  const bool dims = d < a.head_dim;
+  const uint32_t block_elems = (uint32_t)a.n_heads * 2 * a.head_dim;
+  const uint16_t* const bounds = a.bounds + h * 2 * a.head_dim + d;
+  uint4 low[kScPer], high[kScPer];
+  uint32_t bad = 0;
+  auto load = [&](int j0) __attribute__((always_inline)) {
+    int page[kScPer], in_page[kScPer];
+#pragma unroll
+    for (int p = 0; p < kScPer; ++p) {
+      const uint32_t j = min(j0 + g + p * kGroups, count - 1);
+      const uint32_t k = per_page == 1 ? j : (uint32_t)((uint64_t)j * a.page_magic >> 32);  // j / per_page
+      in_page[p] = j - k * per_page;
+      page[p] = table[k];
     }
-    s_q[0][d] = neg;
-    s_q[1][d] = pos;
+    bad = 0;
+#pragma unroll
+    for (int p = 0; p < kScPer; ++p) {
+      const bool off = page[p] < 0 || page[p] >= a.num_pages;
+      bad |= (uint32_t)off << p;
+      low[p] = high[p] = hx::zero4();
+      if (off || !dims) continue;
+      const uint16_t* at = bounds + ((int64_t)page[p] * per_page + in_page[p]) * block_elems;
+      low[p] = hx::ld16_stream(at);
+      high[p] = hx::ld16_stream(at + a.head_dim);
+    }
+  };
+  load(begin);
+  // Sums over the group of min(q, 0) and max(q, 0), by the sign bit: a NaN counts in one of them.
+  for (int e = tid; e < a.head_dim; e += kScThreads) {
+    const uint16_t* q = a.q + row * a.q_row + (int64_t)h * a.group * a.q_head + e;
+    double neg = 0.0, pos = 0.0;
+    for (int k = 0; k < a.group; ++k) {
+      const uint32_t bits = __float_as_uint(E::lo(q[k * a.q_head])), minus = (uint32_t)((int32_t)bits >> 31);
+      neg += (double)__uint_as_float(bits & minus);
+      pos += (double)__uint_as_float(bits & ~minus);
+    }
+    s_q[e] = make_double2(neg, pos);
   }
   __syncthreads();
-  // 16 lanes a block, 8 dims a lane.
-  const int li = tid & 15, per_page = a.page / a.block;
-  const int free_end = count - a.recent;
-  for (int j = tid >> 4; j < count; j += kSelThreads / 16) {
-    const int page = a.table[seq * a.table_stride + j / per_page];
-    double s = 0.0;
-    const bool bad = page < 0 || page >= a.num_pages;
-    if (!bad) {
-      const uint16_t* lo = a.bounds + (((int64_t)page * per_page + j % per_page) * a.n_heads + h) * 2 * a.head_dim;
-      for (int d = 8 * li; d < a.head_dim; d += 128) {
-        const uint4 l4 = *reinterpret_cast<const uint4*>(lo + d), h4 = *reinterpret_cast<const uint4*>(lo + a.head_dim + d);
-        const uint32_t lw[4] = {l4.x, l4.y, l4.z, l4.w}, hw[4] = {h4.x, h4.y, h4.z, h4.w};
+  double neg[8], pos[8];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          s = fma((double)E::lo(lw[q]), s_q[0][d + 2 * q], s);
-          s = fma((double)E::hi(lw[q]), s_q[0][d + 2 * q + 1], s);
-          s = fma((double)E::lo(hw[q]), s_q[1][d + 2 * q], s);
-          s = fma((double)E::hi(hw[q]), s_q[1][d + 2 * q + 1], s);
-        }
+  for (int e = 0; e < 8; ++e) {
+    const double2 v = s_q[dims ? d + e : 0];
+    neg[e] = dims ? v.x : 0.0;
+    pos[e] = dims ? v.y : 0.0;
+  }
+  uint64_t* const order = a.order + ih * a.most;
+  for (int j0 = begin;;) {
+    double s[kScPer];
+#pragma unroll
+    for (int p = 0; p < kScPer; ++p) {
+      const uint32_t lw[4] = {low[p].x, low[p].y, low[p].z, low[p].w};
+      const uint32_t hw[4] = {high[p].x, high[p].y, high[p].z, high[p].w};
+      s[p] = 0.0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s[p] = fma((double)(e % 2 ? E::hi(lw[e / 2]) : E::lo(lw[e / 2])), neg[e], s[p]);
+        s[p] = fma((double)(e % 2 ? E::hi(hw[e / 2]) : E::lo(hw[e / 2])), pos[e], s[p]);
       }
     }
-    s = add_xor(add_xor(add_xor(add_xor(s, 1), 2), 4), 8);
-    // Blocks taken in any case stay out of the search (0 is below every key); a page
-    // outside the pool comes last.
-    if (li == 0) s_key[j] = j < a.sink || j >= free_end ? 0 : bad ? 1 : ordered_key(s);
+    const uint32_t was_bad = bad;
+    const int j1 = j0 + kPass;
+    if (j1 < end) load(j1);
+#pragma unroll
+    for (int p = 0; p < kScPer; ++p) {
+      s[p] = lanes_sum<LANES>(s[p]);
+      const int j = j0 + g + p * kGroups;
+      if (li == 0 && j < end)
+        order[j] = j < a.sink || j >= count - a.recent ? kKeyTaken : was_bad >> p & 1 ? kKeyLast : ordered_key(s[p]);
+    }
+    if (j1 >= end) return;
+    j0 = j1;
   }
-  __syncthreads();
-  if (tid >= 64) return;
-  const int need = a.budget - a.sink - a.recent;
-  uint64_t any = 0, all = ~0ull;
-  for (int j = a.sink + tid; j < free_end; j += 64) {
-    any |= s_key[j];
-    all &= s_key[j];
+}
+
+// The largest of a wave's values, in all lanes.
+template <int CTRL>
+__device__ __forceinline__ uint64_t max_dpp(uint64_t v) {
+  const uint32_t x = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, 0xF, 0xF, false);
+  const uint32_t y = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, 0xF, 0xF, false);
+  return most_of<uint64_t>(v, (uint64_t)y << 32 | x);
+}
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+  v = max_dpp<hx::kDppHalfMirror>(max_dpp<hx::kDppXor2>(max_dpp<hx::kDppXor1>(v)));
+  v = max_dpp<hx::kDppMirror>(v);  // of each row of 16 lanes
+  uint64_t best = 0;
+#pragma unroll
+  for (int r = 0; r < 64; r += 16)
+    best = most_of<uint64_t>(best, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), r) << 32 |
+                                       (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, r));
+  return best;
+}
+
+// Sum of the lanes' values up to and with each lane's own.
+__device__ __forceinline__ int wave_prefix(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // the row before's last, into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // lane 31's, into rows 2 and 3
+  return v;
+}
+
+// Wave w holds blocks 64 PER w .. + 64 PER - 1, block 64 PER w + 64 t + lane in key[t].
+template <int WAVES, int PER>
+__global__ __launch_bounds__(64 * WAVES) void select_blocks_kernel(SelectArgs a) {
+  __shared__ uint64_t s_ends[2][WAVES];
+  __shared__ __attribute__((aligned(16))) int s_bins[kSelBins];
+  __shared__ int s_above[WAVES], s_ties[WAVES], s_taken[WAVES];
+  const int tid = hx::tid_x(), lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t ih = hx::wg_x();
+  int32_t* out = a.out + ih * a.budget;
+  int64_t row, seq;
+  const int count = selected_from(a, ih / a.n_heads, row, seq);
+  if (count <= a.budget) {
+    for (int j = tid; j < a.budget; j += 64 * WAVES) out[j] = j < count ? j : -1;
+    return;
   }
-  for (int m = 1; m < 64; m <<= 1) {
-    any |= __shfl_xor((unsigned long long)any, m);
-    all &= __shfl_xor((unsigned long long)all, m);
+  const int first = 64 * PER * w + lane;
+  uint64_t key[PER], hi = 0, lo = ~0ull;
+#pragma unroll
+  for (int t = 0; t < PER; ++t) {
+    key[t] = kKeyTaken;
+    if (first + 64 * t < count) key[t] = a.order[ih * a.most + first + 64 * t];
   }
-  const uint64_t differ = any ^ all;
-  // The bits above the first difference are everyone's.
-  uint64_t least = differ == 0 ? all : all & ~((2ull << (63 - __builtin_clzll(differ))) - 1ull);
-  int reach = free_end - a.sink;  // keys >= least
-  if (need == 0) least = ~0ull, reach = 0;
-  for (int bit = differ == 0 ? -1 : 63 - __builtin_clzll(differ); bit >= 0 && reach > need; --bit) {
-    const uint64_t cand = least | 1ull << bit;
-    int c = 0;
-    for (int j = a.sink + tid; j < free_end; j += 64) c += s_key[j] >= cand;
-    for (int m = 1; m < 64; m <<= 1) c += __shfl_xor(c, m);
-    if (c >= need) {
-      least = cand;
-      reach = c;
+#pragma unroll
+  for (int t = 0; t < PER; ++t) {
+    hi = most_of(hi, key[t]);
+    if (key[t] != kKeyTaken) lo = least_of(lo, key[t]);
+  }
+  hi = wave_max(hi);
+  lo = ~wave_max(~lo);
+  if constexpr (WAVES > 1) {
+    if (lane == 0) {
+      s_ends[0][w] = hi;
+      s_ends[1][w] = lo;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int ww = 0; ww < WAVES; ++ww) {
+      hi = most_of(hi, s_ends[0][ww]);
+      lo = least_of(lo, s_ends[1][ww]);
     }
   }
-  // Of the keys equal to the threshold the first ones are taken.
-  int above = 0;
-  for (int j = a.sink + tid; j < free_end; j += 64) above += s_key[j] > least;
-  for (int m = 1; m < 64; m <<= 1) above += __shfl_xor(above, m);
-  int ties = need - above, at = 0;
-  for (int j0 = 0; j0 < count; j0 += 64) {
-    const int j = j0 + tid;
-    const bool kept = j < count && (j < a.sink || j >= free_end);
-    const bool free_block = j < count && !kept;
-    const bool tie = free_block && s_key[j] == least;
-    const uint64_t before = (1ull << tid) - 1ull;
-    const uint64_t tied = __builtin_amdgcn_ballot_w64(tie);
-    const bool take = kept || (free_block && s_key[j] > least) || (tie && __builtin_popcountll(tied & before) < ties);
-    ties -= __builtin_popcountll(tied);  // at 0 or below no later tie is taken
-    const uint64_t taken = __builtin_amdgcn_ballot_w64(take);
-    const int to = at + __builtin_popcountll(taken & before);
-    if (take && to < a.budget) out[to] = j;
-    at += __builtin_popcountll(taken);
+  // The need-th largest free key: counts of the keys between lo and hi in up to 1024 equal bins,
+  // then of those in the bin it lies in, until that bin is wanted whole or is a single key. Two or
+  // three passes of keys that spread out, at most seven.
+  const int need = a.budget - a.sink - a.recent;
+  uint64_t least = ~0ull;  // above every key
+  for (int want = need, pass = 0; want > 0 && pass < kSelPasses; ++pass) {
+    const int bits = lo == hi ? 0 : 64 - __builtin_clzll(hi - lo), shift = bits > 10 ? bits - 10 : 0;
+    for (int e = tid; e < kSelBins / 4; e += 64 * WAVES) reinterpret_cast<uint4*>(s_bins)[e] = hx::zero4();
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < PER; ++t)
+      if (key[t] >= lo && key[t] <= hi) atomicAdd(&s_bins[(key[t] - lo) >> shift], 1);
+    __syncthreads();
+    int in[16], sum = 0;  // every wave reads them all: bins 16 lane .. + 15
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int4 u = reinterpret_cast<const int4*>(s_bins)[4 * lane + e / 4];
+      in[e] = u.x, in[e + 1] = u.y, in[e + 2] = u.z, in[e + 3] = u.w;
+      sum += (u.x + u.y) + (u.z + u.w);
+    }
+    const int upto = wave_prefix(sum), all = __builtin_amdgcn_readlane(upto, 63);
+    // Keys in the lane's bins and above, and above them alone.
+    int from = all - upto + sum, above = all - upto, bin = 0, count_of = 0;
+    const int owner = __builtin_ctzll(__builtin_amdgcn_ballot_w64(from >= want && above < want));
+    bool found = false;
+#pragma unroll
+    for (int e = 15; e >= 0; --e) {
+      const bool here = !found && above + in[e] >= want;
+      bin = here ? 16 * lane + e : bin;
+      count_of = here ? in[e] : count_of;
+      found |= here;
+      above += found ? 0 : in[e];
+    }
+    bin = __builtin_amdgcn_readlane(bin, owner);
+    count_of = __builtin_amdgcn_readlane(count_of, owner);
+    want -= __builtin_amdgcn_readlane(above, owner);
+    lo += (uint64_t)bin << shift;
+    if (shift == 0 || count_of == want) {
+      least = lo;
+      break;
+    }
+    hi = lo + least_of<uint64_t>(hi - lo, (1ull << shift) - 1);  // lo + 2^shift may pass 2^64
+    __syncthreads();
   }
+  // Keys above the threshold, and of those equal to it the first ones, make up the rest.
+  int above = 0, tied = 0, taken = 0;
+#pragma unroll
+  for (int t = 0; t < PER; ++t) {
+    above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[t] > least));
+    tied += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[t] == least));
+    taken += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[t] == kKeyTaken && first + 64 * t < count));
+  }
+  int ties = need - above, at = 0;
+  if constexpr (WAVES > 1) {
+    if (lane == 0) {
+      s_above[w] = above;
+      s_ties[w] = tied;
+      s_taken[w] = above + taken;
+    }
+    __syncthreads();
+    ties = need;
+#pragma unroll
+    for (int ww = 0; ww < WAVES; ++ww) ties -= s_above[ww];
+    for (int ww = 0; ww < w; ++ww) {
+      const int had = min(max(ties, 0), s_ties[ww]);
+      at += s_taken[ww] + had;
+      ties -= s_ties[ww];
+    }
+  }
+  const uint64_t before = (1ull << lane) - 1ull;
+#pragma unroll
+  for (int t = 0; t < PER; ++t) {
+    const int j = first + 64 * t;
+    const bool there = j < count;
+    const bool tie = there && key[t] == least;
+    const uint64_t equal = __builtin_amdgcn_ballot_w64(tie);
+    const bool take = there && (key[t] == kKeyTaken || key[t] > least ||
+                                (tie && __builtin_popcountll(equal & before) < ties));
+    ties -= __builtin_popcountll(equal);  // at 0 or below no later tie is taken
+    const uint64_t goes = __builtin_amdgcn_ballot_w64(take);
+    const int to = at + __builtin_popcountll(goes & before);
+    if (take && to < a.budget) out[to] = j;
+    at += __builtin_popcountll(goes);
+  }
+}
+
+template <typename T, int LANES>
+void launch_scores(SelectArgs a, int64_t n, hipStream_t s) {
+  constexpr int kPass = kScThreads / LANES * kScPer;
+  const int64_t passes = (a.most + kPass - 1) / kPass;
+  // Several passes a workgroup, one in flight while the last is summed, where that leaves
+  // workgroups enough.
+  int64_t loops = n * a.n_heads * passes / 2048;
+  loops = loops < 1 ? 1 : loops > 8 ? 8 : loops;
+  a.stretch = (int32_t)(loops * kPass);
+  a.chunks = (int32_t)((passes + loops - 1) / loops);
+  hipLaunchKernelGGL((block_scores_kernel<T, LANES>), dim3((unsigned)(n * a.n_heads * a.chunks)), dim3(kScThreads), 0,
+                     s, a);
+}
+
+template <typename T>
+void launch_select(const SelectArgs& a, int64_t n, hipStream_t s) {
+  if (a.most > a.budget) {
+    if (a.head_dim <= 64) launch_scores<T, 8>(a, n, s);
+    else if (a.head_dim <= 128) launch_scores<T, 16>(a, n, s);
+    else launch_scores<T, 32>(a, n, s);
+  }
+  const dim3 grid((unsigned)(n * a.n_heads));
+  // Few keys a thread: 512 rows of 448 blocks take 5.9 us with four waves, 7.1 with one.
+  if (a.most <= 1024) hipLaunchKernelGGL((select_blocks_kernel<4, 4>), grid, dim3(256), 0, s, a);
+  else if (a.most <= 4096) hipLaunchKernelGGL((select_blocks_kernel<16, 4>), grid, dim3(1024), 0, s, a);
+  else hipLaunchKernelGGL((select_blocks_kernel<16, 16>), grid, dim3(1024), 0, s, a);
 }
 
 // -------------------------------------------------------------------------- attention
@@ -341,7 +552,7 @@ __global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a
   const int64_t row = a.rows != nullptr ? a.rows[i] : i;
   const int64_t seq = a.row_seq != nullptr ? a.row_seq[i] : i;
   if (row < 0 || row >= a.q_rows) return;  // no such query, and no such output row
-  int64_t n = min((int64_t)max(a.keys[i], 0), (int64_t)a.table_width * a.page);
+  int64_t n = least_of<int64_t>(max(a.keys[i], 0), (int64_t)a.table_width * a.page);
   if (seq < 0 || seq >= a.batch) n = 0;
   const int per_page = a.page / a.block, per_block = a.block / 16;
   const int64_t row_elems = (int64_t)a.n_heads * a.head_dim;
@@ -357,7 +568,7 @@ __global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a
         const int page = a.table[seq * a.table_stride + j / per_page];
         if (page >= 0 && page < a.num_pages) {
           at = (int64_t)page * a.page + token % a.page;
-          cnt = (int)min((int64_t)16, n - token);
+          cnt = (int)least_of<int64_t>(16, n - token);
         }
       }
     }
@@ -646,13 +857,17 @@ extern "C" int hx_kv_block_bounds(const void* k_pool, void* bounds, int32_t num_
   return hx::status_from_hip(hipGetLastError());
 }
 
+extern "C" size_t hx_select_blocks_workspace_bytes(int64_t n, int32_t n_kv_heads, int64_t blocks) {
+  return n < 1 || n_kv_heads < 1 || blocks < 1 ? 0 : (size_t)n * n_kv_heads * (size_t)blocks * sizeof(uint64_t);
+}
+
 extern "C" int hx_select_blocks(const void* q, int64_t q_row_stride, int64_t q_head_stride, int64_t q_rows,
                                 const int64_t* rows, const int32_t* row_seq, const int32_t* key_counts, int64_t n,
                                 int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t dtype,
                                 const void* bounds, int32_t num_pages, int32_t page_size, int32_t block_size,
                                 const int32_t* block_table, int64_t block_table_stride, int32_t batch,
                                 int32_t block_table_width, int32_t budget, int32_t sink, int32_t recent,
-                                int32_t* blocks, void* stream) {
+                                int32_t* blocks, void* workspace, size_t workspace_bytes, void* stream) {
   const int bad = check_layout(num_pages, page_size, block_size, n_kv_heads, head_dim, dtype);
   if (bad != HX_OK) return bad;
   if (n < 0 || q_rows < 0 || n_q_heads < 1 || n_q_heads % n_kv_heads || batch < 0 || block_table_width < 1 ||
@@ -660,12 +875,16 @@ extern "C" int hx_select_blocks(const void* q, int64_t q_row_stride, int64_t q_h
       (int64_t)sink + recent > budget)
     return HX_E_INVALID_ARG;
   const int64_t most = (int64_t)block_table_width * (page_size / block_size);
-  if (most > kSelMaxBlocks || n > 0x7fffffff / n_kv_heads) return HX_E_UNSUPPORTED;
+  if (most > kSelMaxBlocks || page_size / block_size > (1 << 16) || n > 0x7fffffff / n_kv_heads / (most + 1)) return HX_E_UNSUPPORTED;
   if (n == 0) return HX_OK;
-  if (!q || !key_counts || !bounds || !block_table || !blocks || (reinterpret_cast<uintptr_t>(q) & 1) ||
-      (reinterpret_cast<uintptr_t>(bounds) & 15) || (rows == nullptr && n > q_rows) ||
+  if (!q || !key_counts || !bounds || !block_table || !blocks ||
+      ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(bounds)) & 15) || q_row_stride % 8 ||
+      q_head_stride % 8 || (rows == nullptr && n > q_rows) ||
       (row_seq == nullptr && n > batch))
     return HX_E_INVALID_ARG;
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 7) ||
+      workspace_bytes < hx_select_blocks_workspace_bytes(n, n_kv_heads, most))
+    return HX_E_WORKSPACE;
   SelectArgs a;
   a.q = static_cast<const uint16_t*>(q);
   a.q_row = q_row_stride;
@@ -688,18 +907,15 @@ extern "C" int hx_select_blocks(const void* q, int64_t q_row_stride, int64_t q_h
   a.budget = budget;
   a.sink = sink;
   a.recent = recent;
+  a.most = (int32_t)most;
+  // j * magic >> 32 = j / per_page while j * per_page < 2^32: j is below 16384.
+  const uint32_t per_page = (uint32_t)(page_size / block_size);
+  a.page_magic = per_page > 1 ? (uint32_t)(((1ull << 32) + per_page - 1) / per_page) : 0;
+  a.order = static_cast<uint64_t*>(workspace);
   a.out = blocks;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)(n * n_kv_heads));
-  const size_t lds = (size_t)most * sizeof(uint64_t);
-  const void* fn = dtype == HX_DTYPE_BF16 ? reinterpret_cast<const void*>(select_blocks_kernel<__bf16>)
-                                          : reinterpret_cast<const void*>(select_blocks_kernel<_Float16>);
-  if (lds > 60 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return hx::status_from_hip(e);
-  }
-  if (dtype == HX_DTYPE_BF16) hipLaunchKernelGGL(select_blocks_kernel<__bf16>, grid, dim3(kSelThreads), lds, s, a);
-  else hipLaunchKernelGGL(select_blocks_kernel<_Float16>, grid, dim3(kSelThreads), lds, s, a);
+  if (dtype == HX_DTYPE_BF16) launch_select<__bf16>(a, n, s);
+  else launch_select<_Float16>(a, n, s);
   return hx::status_from_hip(hipGetLastError());
 }
 

@@ -126,7 +126,7 @@ __global__ __launch_bounds__(256) void int4_norm_kernel(Int4Args a, uint16_t* h)
   if ((tid & 63) == 0) s_part[tid >> 6] = ss;
   __syncthreads();
   ss = (s_part[0] + s_part[1]) + (s_part[2] + s_part[3]);
-  const float r = rsqrtf(__fadd_rn(__fdiv_rn(ss, (float)a.k), a.eps));
+  const float r = __builtin_amdgcn_rsqf(__fadd_rn(__fdiv_rn(ss, (float)a.k), a.eps));
   uint4* tile = reinterpret_cast<uint4*>(h) + (int64_t)(row >> 4) * 2 * padded * 16 + (row & 15);
   auto put = [&](int p, uint4 u, float4 na, float4 nb) __attribute__((always_inline)) {
     const float w[8] = {na.x, na.y, na.z, na.w, nb.x, nb.y, nb.z, nb.w};
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
       float sum = 0.f;
 #pragma unroll
       for (int ww = 0; ww < WAVES; ++ww) sum += s_ss[ww][at / 16];
-      const float r = rsqrtf(__fadd_rn(__fdiv_rn(sum, (float)a.k), a.eps));
+      const float r = __builtin_amdgcn_rsqf(__fadd_rn(__fdiv_rn(sum, (float)a.k), a.eps));
 #pragma unroll
       for (int v = 0; v < kSums; ++v) y[v] *= r;
     }

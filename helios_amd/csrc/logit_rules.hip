@@ -83,7 +83,7 @@ __global__ __launch_bounds__(kLrThreads) void logit_rules_kernel(RuleArgs a) {
   const int tid = hx::tid_x();
   const int64_t row = hx::wg_x() / a.slices;
   const int64_t v0 = (int64_t)(hx::wg_x() % a.slices) * kLrSlice;
-  const int n = (int)min((int64_t)kLrSlice, a.vocab - v0);
+  const int n = a.vocab - v0 < kLrSlice ? (int)(a.vocab - v0) : kLrSlice;
   const bool hist = a.tokens != nullptr, biased = a.bias_ids != nullptr;
   for (int i = tid; i < kLrSlice; i += kLrThreads) {
     if (hist) s_count[i] = 0;
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(kLrThreads) void logit_rules_kernel(RuleArgs a) {
   }
   __syncthreads();
   if (hist) {
-    const int64_t len = min((int64_t)max(a.lengths[row], 0), a.token_cap);
+    const int64_t given = max(a.lengths[row], 0), len = given < a.token_cap ? given : a.token_cap;
     const int64_t prompt = a.prompt_lens != nullptr ? a.prompt_lens[row] : 0;
     const int32_t* t = a.tokens + row * a.token_stride;
     for (int64_t i = tid; i < len; i += kLrThreads) {

@@ -466,6 +466,13 @@ def _check_rows(query: torch.Tensor, key_counts: torch.Tensor, rows: torch.Tenso
     return n
 
 
+def _vector_rows(query: torch.Tensor) -> torch.Tensor:
+    """``query`` with heads that 16-byte loads may take: itself, or a contiguous copy."""
+    if query.stride(2) != 1 or query.data_ptr() % 16 or query.stride(0) % 8 or query.stride(1) % 8:
+        return query.clone(memory_format=torch.contiguous_format)
+    return query
+
+
 def kv_block_bounds(k_cache: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, cu_seq_q: torch.Tensor,
                     seqused_k: torch.Tensor, *, max_q: int) -> None:
     """Key bounds of the blocks that a tick's new tokens touched, in place, after those tokens
@@ -515,8 +522,8 @@ def select_blocks(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.
     head, an upper bound of their summed scores, computed in 64 bits (equal ones: the
     earlier block; NaN: as infinity). A row with no more than ``budget`` blocks gets them all."""
     device = _require_gpu(query, bounds, block_table, key_counts)
-    if query.ndim != 3 or query.shape[2] < 1 or query.stride(2) != 1:
-        raise ValueError("query must be [rows, n_q_heads, head_dim] with a contiguous head_dim.")
+    if query.ndim != 3 or query.shape[2] < 1:
+        raise ValueError("query must be [rows, n_q_heads, head_dim].")
     dtype = _SUPPORTED.get(query.dtype)
     if dtype is None or bounds.dtype != query.dtype:
         raise ValueError("query and bounds must be bfloat16 or float16, of one dtype.")
@@ -536,12 +543,18 @@ def select_blocks(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.
         raise ValueError(f"a block table may cover at most {MAX_SELECT_BLOCKS} blocks; use larger ones.")
     n = _check_rows(query, key_counts, rows, row_seq, block_table)
     blocks = torch.empty((n, n_kv, budget), dtype=torch.int32, device=device)
+    if n == 0:
+        return blocks
+    query = _vector_rows(query)
+    lib = _capi.lib()
+    ws_bytes = lib.hx_select_blocks_workspace_bytes(n, n_kv, block_table.shape[1] * bounds.shape[1])
+    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
     code = _launch(
-        device, _capi.lib().hx_select_blocks, query.data_ptr(), query.stride(0), query.stride(1), query.shape[0],
+        device, lib.hx_select_blocks, query.data_ptr(), query.stride(0), query.stride(1), query.shape[0],
         None if rows is None else rows.data_ptr(), None if row_seq is None else row_seq.data_ptr(),
         key_counts.data_ptr(), n, query.shape[1], n_kv, query.shape[2], dtype, bounds.data_ptr(), bounds.shape[0],
         page_size, block_size, block_table.data_ptr(), _table_stride(block_table), block_table.shape[0],
-        block_table.shape[1], budget, sink, recent, blocks.data_ptr())
+        block_table.shape[1], budget, sink, recent, blocks.data_ptr(), workspace.data_ptr(), ws_bytes)
     _capi.check(code, "hx_select_blocks")
     return blocks
 
@@ -583,8 +596,7 @@ def block_sparse_attn(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         raise ValueError("out must have the query's shape, dtype and device, a contiguous head_dim and even strides.")
     if n == 0:
         return out
-    if query.stride(2) != 1 or query.data_ptr() % 16 or query.stride(0) % 8 or query.stride(1) % 8:
-        query = query.clone(memory_format=torch.contiguous_format)  # 16-byte loads
+    query = _vector_rows(query)
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
     budget = blocks.shape[2]
     lib = _capi.lib()

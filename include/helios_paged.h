@@ -619,7 +619,9 @@ int hx_int4_dequantize(const void* packed, const void* steps, int32_t weight_row
  * blocks[i][h] = the first `sink` blocks, the last `recent` (at least 1) and the best others,
  * `budget` in all, ascending; all of them, then -1, when there are no more. Of an entry whose
  * row or sequence is not there: -1. HX_E_UNSUPPORTED when the table's width covers more than
- * 16384 blocks.
+ * 16384 blocks. q and bounds 16-byte aligned, q's strides multiples of 8. The workspace is
+ * hx_select_blocks_workspace_bytes(n, n_kv_heads, blocks the table's width covers) bytes, 8-byte
+ * aligned; calls that share one must be ordered.
  *
  * hx_block_sparse_attn: out[rows[i]][h] = softmax(scale q . k) V over the keys of blocks[i]
  * [h / group] below key_counts[i], in fp32 with weights of 16 (fp16: 22) bits, rounded once.
@@ -636,6 +638,7 @@ int hx_kv_block_bounds(const void* k_pool, void* bounds, int32_t num_pages,
                        int64_t block_table_stride, int32_t block_table_width,
                        const int32_t* cu_seq_q, const int32_t* seqused_k, int32_t batch,
                        int32_t max_q, void* stream);
+size_t hx_select_blocks_workspace_bytes(int64_t n, int32_t n_kv_heads, int64_t blocks);
 int hx_select_blocks(const void* q, int64_t q_row_stride, int64_t q_head_stride,
                      int64_t q_rows, const int64_t* rows, const int32_t* row_seq,
                      const int32_t* key_counts, int64_t n, int32_t n_q_heads,
@@ -644,7 +647,7 @@ int hx_select_blocks(const void* q, int64_t q_row_stride, int64_t q_head_stride,
                      int32_t block_size, const int32_t* block_table,
                      int64_t block_table_stride, int32_t batch, int32_t block_table_width,
                      int32_t budget, int32_t sink, int32_t recent, int32_t* blocks,
-                     void* stream);
+                     void* workspace, size_t workspace_bytes, void* stream);
 size_t hx_block_sparse_workspace_bytes(int64_t n, int32_t n_q_heads, int32_t n_kv_heads,
                                        int32_t head_dim, int32_t budget, int32_t block_size);
 int hx_block_sparse_attn(const void* q, int64_t q_row_stride, int64_t q_head_stride,

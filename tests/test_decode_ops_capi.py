@@ -75,10 +75,12 @@ def test_kv_block_bounds(change, code):
 
 SELECT = dict(q=P, q_row=4096, q_head=128, q_rows=2, rows=None, row_seq=None, keys=P, n=2, hq=32, hkv=8, dim=128, dtype=0,
               bounds=P, pages=4, page=256, block=64, table=P, stride=4, batch=2, width=4, budget=8, sink=1, recent=2,
-              blocks=P, stream=None)
+              blocks=P, ws=P, ws_bytes=1 << 20, stream=None)
 
 
 @pytest.mark.parametrize("change,code", [
+    (dict(ws=None), WS), (dict(ws=P + 4), WS), (dict(ws_bytes=2 * 8 * 16 * 8 - 1), WS), (dict(q=P + 8), BAD),
+    (dict(q_row=4092), BAD), (dict(q_head=132), BAD),
     (dict(dtype=2), NO), (dict(block=24), NO), (dict(hq=30), BAD), (dict(budget=0), BAD), (dict(sink=-1), BAD),
     (dict(recent=0), BAD), (dict(sink=7, recent=2), BAD), (dict(sink=2 ** 31 - 1, recent=2 ** 31 - 1), BAD),
     (dict(width=4097, stride=4097), NO), (dict(n=3), BAD), (dict(n=-1), BAD), (dict(q=None), BAD),
