@@ -54,7 +54,7 @@ RULES = dict(logits=P, row=64, rows=2, vocab=64, dtype=0, tokens=P, token_row=8,
     (dict(dtype=3), NO), (dict(rows=-1), BAD), (dict(vocab=0), BAD), (dict(row=63), BAD), (dict(logits=None), BAD),
     (dict(ids=None), BAD), (dict(out_row=63), BAD), (dict(lengths=None), BAD), (dict(token_row=7), BAD),
     (dict(bias_values=None), BAD), (dict(bias_row=3), BAD), (dict(n_bias=-1), BAD), (dict(allowed_row=1), BAD),
-    (dict(ws=None), WS), (dict(ws=P + 4), WS), (dict(ws_bytes=15), WS), (dict(rows=0), 0),
+    (dict(ws=None), WS), (dict(ws=P + 4), WS), (dict(ws_bytes=15), WS), (dict(rows=0), 0), (dict(logits=P + 1), BAD), (dict(dtype=2, out=P + 2), BAD),
     (dict(rows=1 << 31, ws_bytes=1 << 40), NO)])
 def test_logit_rules(change, code):
     assert _call("hx_logit_rules", RULES, **change) == code
@@ -106,7 +106,9 @@ def test_block_sparse_attn(change, code):
 
 def test_workspace_sizes():
     lib = _capi.lib()
-    assert lib.hx_logit_rules_workspace_bytes(3, 4097) == 3 * 2 * 8
+    # slices of 4096, a row's first up to 7 elements before it
+    assert lib.hx_logit_rules_workspace_bytes(3, 4089) == 3 * 8
+    assert lib.hx_logit_rules_workspace_bytes(3, 4090) == 3 * 2 * 8
     assert lib.hx_logit_rules_workspace_bytes(0, 10) == 0
     # normalised rows past one tile: two parts of each row tile of 16, k rounded up to 128
     assert lib.hx_int4_workspace_bytes(16, 2560, 1) == lib.hx_int4_workspace_bytes(64, 2560, 0) == 0
