@@ -552,7 +552,7 @@ __global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a
   const int64_t row = a.rows != nullptr ? a.rows[i] : i;
   const int64_t seq = a.row_seq != nullptr ? a.row_seq[i] : i;
   if (row < 0 || row >= a.q_rows) return;  // no such query, and no such output row
-  int64_t n = least_of<int64_t>(max(a.keys[i], 0), (int64_t)a.table_width * a.page);
+  int n = (int)least_of<int64_t>(max(a.keys[i], 0), (int64_t)a.table_width * a.page);
   if (seq < 0 || seq >= a.batch) n = 0;
   const int per_page = a.page / a.block, per_block = a.block / 16;
   const int64_t row_elems = (int64_t)a.n_heads * a.head_dim;
@@ -562,13 +562,13 @@ __global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a
     int64_t at = 0;
     int cnt = 0;
     if (e < a.budget) {
-      const int64_t j = a.blocks[((int64_t)i * a.n_heads + h) * a.budget + e];
-      const int64_t token = j * a.block + u % per_block * 16;
-      if (j >= 0 && token < n) {
+      // A block that starts below n has a first token that fits 32 bits, as n does.
+      const int j = a.blocks[((int64_t)i * a.n_heads + h) * a.budget + e], in = u % per_block * 16;
+      if (n > 0 && j >= 0 && j <= (n - 1) / a.block && j * a.block < n - in) {
         const int page = a.table[seq * a.table_stride + j / per_page];
         if (page >= 0 && page < a.num_pages) {
-          at = (int64_t)page * a.page + token % a.page;
-          cnt = (int)least_of<int64_t>(16, n - token);
+          at = (int64_t)page * a.page + j % per_page * a.block + in;
+          cnt = min(16, n - in - j * a.block);
         }
       }
     }
@@ -750,30 +750,63 @@ __global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a
   }
 }
 
-// The splits of a row and query head, in order; one wave each.
+// The splits of a row and query head, in order; one wave each, with the first kCbAtOnce splits'
+// sums on their way before the maxima are known.
+constexpr int kCbAtOnce = 16;
+
 template <typename T>
-__global__ __launch_bounds__(256) void sparse_combine_kernel(SparseArgs a, int64_t heads_total) {
-  const int lane = hx::tid_x() & 63;
-  const int64_t t = (int64_t)hx::wg_x() * 4 + (hx::tid_x() >> 6);
-  if (t >= heads_total) return;
-  const int64_t n_q = (int64_t)a.n_heads * a.group, i = t / n_q, head = t % n_q;
+__global__ __launch_bounds__(64) void sparse_combine_kernel(SparseArgs a) {
+  const int lane = hx::tid_x();
+  const int64_t t = hx::wg_x();
+  const int n_q = a.n_heads * a.group, i = hx::wg_x() / n_q, head = hx::wg_x() % n_q;
   const int64_t row = a.rows != nullptr ? a.rows[i] : i;
   if (row < 0 || row >= a.q_rows) return;
-  const float* ml = a.part_ml + 2 * t * a.splits;
-  float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[2 * s]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  for (int d = 2 * lane; d < a.head_dim; d += 128) {
+  const float2* const ml = reinterpret_cast<const float2*>(a.part_ml) + t * a.splits;
+  const float* const sums = a.part_o + t * a.splits * a.head_dim;
+  for (int d0 = 0; d0 < a.head_dim; d0 += 128) {
+    const int d = d0 + 2 * lane, from = d < a.head_dim ? d : 0;
+    float2 o[kCbAtOnce];
+    auto load = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < kCbAtOnce; ++k) {
+        const int at = s0 + k < a.splits ? s0 + k : a.splits - 1;
+        o[k] = *reinterpret_cast<const float2*>(sums + (int64_t)at * a.head_dim + from);
+      }
+    };
+    load(0);
+    float m = -INFINITY;
+    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, ml[s].x);
+    m = fmaxf(m, hx::dpp<hx::kDppXor1>(m));
+    m = fmaxf(m, hx::dpp<hx::kDppXor2>(m));
+    m = fmaxf(m, hx::dpp<hx::kDppHalfMirror>(m));
+    m = fmaxf(m, hx::dpp<hx::kDppMirror>(m));
+    m = hx::max_xor32(hx::max_xor16(m));
+    const float ref = m == -INFINITY ? 0.f : m;
     float l = 0.f, x = 0.f, y = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-      const float f = hx::fast_exp2(ml[2 * s] - ref);
-      const float2 o = *reinterpret_cast<const float2*>(a.part_o + (t * a.splits + s) * a.head_dim + d);
-      l = fmaf(f, ml[2 * s + 1], l);
-      x = fmaf(f, o.x, x);
-      y = fmaf(f, o.y, y);
+    for (int s0 = 0; s0 < a.splits; s0 += 64) {
+      const float2 mine = s0 + lane < a.splits ? ml[s0 + lane] : make_float2(-INFINITY, 0.f);
+      const float f = hx::fast_exp2(mine.x - ref);
+      l = fmaf(f, mine.y, l);
+      for (int k0 = 0; k0 < 64 && s0 + k0 < a.splits; k0 += kCbAtOnce) {
+#pragma unroll
+        for (int k = 0; k < kCbAtOnce; ++k) {
+          const float fk = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(f), k0 + k));
+          if (s0 + k0 + k < a.splits) {
+            x = fmaf(fk, o[k].x, x);
+            y = fmaf(fk, o[k].y, y);
+          }
+        }
+        if (s0 + k0 + kCbAtOnce < a.splits) load(s0 + k0 + kCbAtOnce);
+      }
     }
+    l += hx::dpp<hx::kDppXor1>(l);
+    l += hx::dpp<hx::kDppXor2>(l);
+    l += hx::dpp<hx::kDppHalfMirror>(l);
+    l += hx::dpp<hx::kDppMirror>(l);
+    l = hx::add_xor32(hx::add_xor16(l));
     const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-    *reinterpret_cast<uint32_t*>(a.out + row * a.out_row + head * a.out_head + d) = hx::pack2_round<T>(x * inv, y * inv);
+    if (d < a.head_dim)
+      *reinterpret_cast<uint32_t*>(a.out + row * a.out_row + head * a.out_head + d) = hx::pack2_round<T>(x * inv, y * inv);
   }
 }
 
@@ -803,8 +836,7 @@ void launch_sparse_dims(const SparseArgs& a, int64_t n, hipStream_t s) {
   else if (a.head_dim <= 128) launch_sparse<T, 128>(a, n, s);
   else launch_sparse<T, 256>(a, n, s);
   if (a.splits > 1) {
-    const int64_t heads = n * a.n_heads * a.group;
-    hipLaunchKernelGGL(sparse_combine_kernel<T>, dim3((unsigned)((heads + 3) / 4)), dim3(256), 0, s, a, heads);
+    hipLaunchKernelGGL(sparse_combine_kernel<T>, dim3((unsigned)(n * a.n_heads * a.group)), dim3(64), 0, s, a);
   }
 }
 
@@ -990,7 +1022,7 @@ extern "C" int hx_block_sparse_attn(const void* q, int64_t q_row_stride, int64_t
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + parts * head_dim;
   }
-  if ((double)n * n_kv_heads * a.head_blocks * a.splits > 2147483647.0) return HX_E_UNSUPPORTED;
+  if ((double)n * n_q_heads * a.splits > 2147483647.0) return HX_E_UNSUPPORTED;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == HX_DTYPE_BF16) launch_sparse_dims<__bf16>(a, n, s);
   else launch_sparse_dims<_Float16>(a, n, s);

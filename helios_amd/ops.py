@@ -420,18 +420,22 @@ def block_linear(x: torch.Tensor, weight: torch.Tensor, *, norm_weight: torch.Te
 MAX_SELECT_BLOCKS = 16384  # blocks of a sequence that select_blocks can order
 
 
-def _check_blocks(pool_name: str, pool: torch.Tensor, block_table: torch.Tensor, block_size: int) -> int:
-    """Checks shared by the block operators; the pool's dtype code."""
-    if pool.ndim != 4 or not pool.is_contiguous() or min(pool.shape) < 1:
-        raise ValueError(f"{pool_name} must be a contiguous [pages, page_size, kv_heads, head_dim] pool.")
+def _pool_layout(name: str, pool: torch.Tensor) -> tuple[int, int, int, int, int]:
+    """A pool's dtype code, pages, page size, KV heads and head dim, checked for the block operators."""
+    shape = pool.shape
+    if len(shape) != 4 or not pool.is_contiguous() or 0 in shape:
+        raise ValueError(f"{name} must be a contiguous [pages, page_size, kv_heads, head_dim] pool.")
     dtype = _SUPPORTED.get(pool.dtype)
     if dtype is None:
-        raise ValueError(f"{pool_name} must be bfloat16 or float16.")
-    _check_block_size(block_size, pool.shape[1])
-    if pool.shape[3] % 8 or pool.shape[3] > 256:
+        raise ValueError(f"{name} must be bfloat16 or float16.")
+    pages, page_size, n_kv, head_dim = shape
+    _check_head_dim(head_dim)
+    return dtype, pages, page_size, n_kv, head_dim
+
+
+def _check_head_dim(head_dim: int) -> None:
+    if head_dim % 8 or head_dim > 256:
         raise ValueError("head_dim must be a multiple of 8 from 8 to 256.")
-    _check_table(block_table)
-    return dtype
 
 
 def _check_block_size(block_size: int, page_size: int) -> None:
@@ -439,36 +443,40 @@ def _check_block_size(block_size: int, page_size: int) -> None:
         raise ValueError("block_size must be a power of two from 16 to 1024 that divides the page size.")
 
 
-def _check_table(block_table: torch.Tensor) -> None:
-    if block_table.dtype != torch.int32 or block_table.ndim != 2 or block_table.shape[1] < 1 \
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1) \
-            or (block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]):
-        raise ValueError("block_table must be int32 [batch, width] with contiguous rows.")
+def _table_layout(block_table: torch.Tensor) -> tuple[int, int, int]:
+    """A block table's rows, width and row stride, checked."""
+    shape = block_table.shape
+    if block_table.dtype == torch.int32 and len(shape) == 2 and shape[1] >= 1:
+        batch, width = shape
+        if block_table.is_contiguous():
+            return batch, width, width
+        row, entry = block_table.stride()
+        if batch <= 1:
+            row = width  # a single row's stride may be anything
+        if (width == 1 or entry == 1) and row >= width:
+            return batch, width, row
+    raise ValueError("block_table must be int32 [batch, width] with contiguous rows.")
 
 
-def _table_stride(block_table: torch.Tensor) -> int:
-    return block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1]
-
-
-def _check_rows(query: torch.Tensor, key_counts: torch.Tensor, rows: torch.Tensor | None,
-                row_seq: torch.Tensor | None, block_table: torch.Tensor) -> int:
+def _check_rows(queries: int, key_counts: torch.Tensor, rows: torch.Tensor | None, row_seq: torch.Tensor | None,
+                batch: int, device: torch.device) -> int:
     """Checks of the query rows of a selection; their number."""
     n = key_counts.numel()
     for name, t, dtype in (("key_counts", key_counts, torch.int32), ("row_seq", row_seq, torch.int32),
                            ("rows", rows, torch.int64)):
-        if t is not None and (t.dtype != dtype or t.ndim != 1 or t.numel() != n or not t.is_contiguous()
-                              or t.device != query.device):
+        if t is not None and (t.dtype != dtype or t.shape != (n,) or not t.is_contiguous() or t.device != device):
             raise ValueError(f"{name} must be a contiguous {dtype} vector, one entry per query row, on the device.")
-    if rows is None and n != query.shape[0]:
+    if rows is None and n != queries:
         raise ValueError("without rows, key_counts must have one entry per query.")
-    if row_seq is None and n > block_table.shape[0]:
+    if row_seq is None and n > batch:
         raise ValueError("without row_seq, the block table must have a row per query row.")
     return n
 
 
 def _vector_rows(query: torch.Tensor) -> torch.Tensor:
     """``query`` with heads that 16-byte loads may take: itself, or a contiguous copy."""
-    if query.stride(2) != 1 or query.data_ptr() % 16 or query.stride(0) % 8 or query.stride(1) % 8:
+    row, head, element = query.stride()
+    if element != 1 or row % 8 or head % 8 or query.data_ptr() % 16:
         return query.clone(memory_format=torch.contiguous_format)
     return query
 
@@ -486,25 +494,26 @@ def kv_block_bounds(k_cache: torch.Tensor, bounds: torch.Tensor, block_table: to
     so a page that was reused or truncated needs no clearing. A NaN key makes both bounds
     NaN."""
     device = _require_gpu(k_cache, bounds, block_table, cu_seq_q, seqused_k)
-    if bounds.ndim != 5 or bounds.shape[1] < 1 or k_cache.ndim != 4 or k_cache.shape[1] % bounds.shape[1]:
+    dtype, pages, page_size, n_kv, head_dim = _pool_layout("k_cache", k_cache)
+    layout = bounds.shape
+    if len(layout) != 5 or layout[1] < 1 or page_size % layout[1]:
         raise ValueError("bounds must be [pages, blocks per page, kv_heads, 2, head_dim].")
-    block_size = k_cache.shape[1] // bounds.shape[1]
-    dtype = _check_blocks("k_cache", k_cache, block_table, block_size)
-    pages, page_size, n_kv, head_dim = k_cache.shape
-    if tuple(bounds.shape) != (pages, page_size // block_size, n_kv, 2, head_dim) or bounds.dtype != k_cache.dtype \
-            or not bounds.is_contiguous():
+    block_size = page_size // layout[1]
+    _check_block_size(block_size, page_size)
+    if layout != (pages, layout[1], n_kv, 2, head_dim) or bounds.dtype != k_cache.dtype or not bounds.is_contiguous():
         raise ValueError("bounds must be contiguous [pages, blocks per page, kv_heads, 2, head_dim] of the pool's dtype.")
     batch = seqused_k.numel()
     for name, t, count in (("cu_seq_q", cu_seq_q, batch + 1), ("seqused_k", seqused_k, batch)):
-        if t.dtype != torch.int32 or t.ndim != 1 or t.numel() != count or not t.is_contiguous():
+        if t.dtype != torch.int32 or t.shape != (count,) or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 vector of {count} values.")
-    if block_table.shape[0] != batch:
+    table_rows, width, table_stride = _table_layout(block_table)
+    if table_rows != batch:
         raise ValueError("block_table must have a row per sequence.")
     if max_q < 0:
         raise ValueError("max_q must be non-negative.")
     code = _launch(device, _capi.lib().hx_kv_block_bounds, k_cache.data_ptr(), bounds.data_ptr(), pages, page_size,
-                   block_size, n_kv, head_dim, dtype, block_table.data_ptr(), _table_stride(block_table),
-                   block_table.shape[1], cu_seq_q.data_ptr(), seqused_k.data_ptr(), batch, max_q)
+                   block_size, n_kv, head_dim, dtype, block_table.data_ptr(), table_stride, width,
+                   cu_seq_q.data_ptr(), seqused_k.data_ptr(), batch, max_q)
     _capi.check(code, "hx_kv_block_bounds")
 
 
@@ -522,39 +531,42 @@ def select_blocks(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.
     head, an upper bound of their summed scores, computed in 64 bits (equal ones: the
     earlier block; NaN: as infinity). A row with no more than ``budget`` blocks gets them all."""
     device = _require_gpu(query, bounds, block_table, key_counts)
-    if query.ndim != 3 or query.shape[2] < 1:
+    layout = query.shape
+    if len(layout) != 3 or layout[2] < 1:
         raise ValueError("query must be [rows, n_q_heads, head_dim].")
+    queries, n_q, head_dim = layout
     dtype = _SUPPORTED.get(query.dtype)
     if dtype is None or bounds.dtype != query.dtype:
         raise ValueError("query and bounds must be bfloat16 or float16, of one dtype.")
-    if bounds.ndim != 5 or bounds.shape[3] != 2 or bounds.shape[4] != query.shape[2] or not bounds.is_contiguous() \
-            or min(bounds.shape) < 1:
+    layout = bounds.shape
+    if len(layout) != 5 or layout[3] != 2 or layout[4] != head_dim or 0 in layout or not bounds.is_contiguous():
         raise ValueError("bounds must be contiguous [pages, blocks per page, kv_heads, 2, head_dim].")
-    n_kv, page_size = bounds.shape[2], bounds.shape[1] * block_size
+    pages, per_page, n_kv = layout[:3]
+    page_size = per_page * block_size
     _check_block_size(block_size, page_size)
-    if query.shape[2] % 8 or query.shape[2] > 256:
-        raise ValueError("head_dim must be a multiple of 8 from 8 to 256.")
-    if query.shape[1] < 1 or query.shape[1] % n_kv:
-        raise ValueError(f"GQA needs n_q_heads ({query.shape[1]}) to be a multiple of n_kv_heads ({n_kv}).")
-    _check_table(block_table)
+    _check_head_dim(head_dim)
+    if n_q < 1 or n_q % n_kv:
+        raise ValueError(f"GQA needs n_q_heads ({n_q}) to be a multiple of n_kv_heads ({n_kv}).")
+    batch, width, table_stride = _table_layout(block_table)
     if sink < 0 or recent < 1 or sink + recent > budget:
         raise ValueError("budget must cover sink (at least 0) and recent (at least 1) blocks.")
-    if block_table.shape[1] * bounds.shape[1] > MAX_SELECT_BLOCKS:
+    if width * per_page > MAX_SELECT_BLOCKS:
         raise ValueError(f"a block table may cover at most {MAX_SELECT_BLOCKS} blocks; use larger ones.")
-    n = _check_rows(query, key_counts, rows, row_seq, block_table)
-    blocks = torch.empty((n, n_kv, budget), dtype=torch.int32, device=device)
+    n = _check_rows(queries, key_counts, rows, row_seq, batch, device)
+    blocks = key_counts.new_empty((n, n_kv, budget))
     if n == 0:
         return blocks
     query = _vector_rows(query)
     lib = _capi.lib()
-    ws_bytes = lib.hx_select_blocks_workspace_bytes(n, n_kv, block_table.shape[1] * bounds.shape[1])
+    ws_bytes = lib.hx_select_blocks_workspace_bytes(n, n_kv, width * per_page)
     workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    q_row, q_head, _ = query.stride()
     code = _launch(
-        device, lib.hx_select_blocks, query.data_ptr(), query.stride(0), query.stride(1), query.shape[0],
+        device, lib.hx_select_blocks, query.data_ptr(), q_row, q_head, queries,
         None if rows is None else rows.data_ptr(), None if row_seq is None else row_seq.data_ptr(),
-        key_counts.data_ptr(), n, query.shape[1], n_kv, query.shape[2], dtype, bounds.data_ptr(), bounds.shape[0],
-        page_size, block_size, block_table.data_ptr(), _table_stride(block_table), block_table.shape[0],
-        block_table.shape[1], budget, sink, recent, blocks.data_ptr(), workspace.data_ptr(), ws_bytes)
+        key_counts.data_ptr(), n, n_q, n_kv, head_dim, dtype, bounds.data_ptr(), pages, page_size, block_size,
+        block_table.data_ptr(), table_stride, batch, width, budget, sink, recent, blocks.data_ptr(),
+        workspace.data_ptr(), ws_bytes)
     _capi.check(code, "hx_select_blocks")
     return blocks
 
@@ -576,39 +588,42 @@ def block_sparse_attn(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     a sequence's last key is not read; an infinite or NaN element of a key or value that a
     row does see makes that row's result infinite or NaN."""
     device = _require_gpu(query, k_cache, v_cache, blocks, block_table, key_counts)
-    dtype = _check_blocks("k_cache", k_cache, block_table, block_size)
+    dtype, pages, page_size, n_kv, head_dim = _pool_layout("k_cache", k_cache)
+    _check_block_size(block_size, page_size)
     if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype or not v_cache.is_contiguous():
         raise ValueError("Key and value pools must be contiguous, of one shape and dtype.")
-    pages, page_size, n_kv, head_dim = k_cache.shape
-    if query.ndim != 3 or query.shape[2] != head_dim or query.dtype != k_cache.dtype:
+    shape = query.shape
+    if len(shape) != 3 or shape[2] != head_dim or query.dtype != k_cache.dtype:
         raise ValueError("query must be [rows, n_q_heads, head_dim] of the pools' dtype.")
-    if query.shape[1] < 1 or query.shape[1] % n_kv:
-        raise ValueError(f"GQA needs n_q_heads ({query.shape[1]}) to be a multiple of n_kv_heads ({n_kv}).")
-    n = _check_rows(query, key_counts, rows, row_seq, block_table)
-    if blocks.dtype != torch.int32 or blocks.ndim != 3 or tuple(blocks.shape[:2]) != (n, n_kv) \
-            or blocks.shape[2] < 1 or not blocks.is_contiguous():
+    queries, n_q, _ = shape
+    if n_q < 1 or n_q % n_kv:
+        raise ValueError(f"GQA needs n_q_heads ({n_q}) to be a multiple of n_kv_heads ({n_kv}).")
+    batch, width, table_stride = _table_layout(block_table)
+    n = _check_rows(queries, key_counts, rows, row_seq, batch, device)
+    listed = blocks.shape
+    if blocks.dtype != torch.int32 or len(listed) != 3 or listed[0] != n or listed[1] != n_kv or listed[2] < 1 \
+            or not blocks.is_contiguous():
         raise ValueError("blocks must be contiguous int32 [n, kv_heads, budget].")
     if out is None:
-        new = torch.empty if rows is None else torch.zeros
-        out = new(query.shape, dtype=query.dtype, device=device)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != device or out.stride(2) != 1 \
+        out = (query.new_empty if rows is None else query.new_zeros)(shape)
+    elif out.shape != shape or out.dtype != query.dtype or out.device != device or out.stride(2) != 1 \
             or out.data_ptr() % 4 or out.stride(0) % 2 or out.stride(1) % 2:
         raise ValueError("out must have the query's shape, dtype and device, a contiguous head_dim and even strides.")
     if n == 0:
         return out
     query = _vector_rows(query)
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
-    budget = blocks.shape[2]
-    lib = _capi.lib()
-    ws_bytes = lib.hx_block_sparse_workspace_bytes(n, query.shape[1], n_kv, head_dim, budget, block_size)
+    budget, lib = listed[2], _capi.lib()
+    ws_bytes = lib.hx_block_sparse_workspace_bytes(n, n_q, n_kv, head_dim, budget, block_size)
     workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
+    q_row, q_head, _ = query.stride()
+    out_row, out_head, _ = out.stride()
     code = _launch(
-        device, lib.hx_block_sparse_attn, query.data_ptr(), query.stride(0), query.stride(1), query.shape[0],
+        device, lib.hx_block_sparse_attn, query.data_ptr(), q_row, q_head, queries,
         None if rows is None else rows.data_ptr(), None if row_seq is None else row_seq.data_ptr(),
         key_counts.data_ptr(), n, k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, block_size,
-        blocks.data_ptr(), budget, block_table.data_ptr(), _table_stride(block_table), block_table.shape[0],
-        block_table.shape[1], query.shape[1], n_kv, head_dim, scale, dtype, out.data_ptr(), out.stride(0),
-        out.stride(1), None if workspace is None else workspace.data_ptr(), ws_bytes)
+        blocks.data_ptr(), budget, block_table.data_ptr(), table_stride, batch, width, n_q, n_kv, head_dim, scale,
+        dtype, out.data_ptr(), out_row, out_head, None if workspace is None else workspace.data_ptr(), ws_bytes)
     _capi.check(code, "hx_block_sparse_attn")
     return out
 
@@ -687,18 +702,16 @@ def int4_quantize(weight: torch.Tensor, group: int = 128) -> Int4Weight:
 
 def _check_int4(weight: Int4Weight, device: torch.device) -> int:
     """Checks of a packed weight; its dtype code."""
-    blocks, tiles = -(-weight.k // 128), -(-weight.rows // 16)
-    if weight.group not in (32, 64, 128) or weight.k % weight.group or weight.k < 1 or weight.rows < 1:
+    packed, steps, rows, k, group, dtype = weight
+    if group not in (32, 64, 128) or k % group or k < 1 or rows < 1:
         raise ValueError("the weight's group must be 32, 64 or 128 and divide its k.")
-    shape = (blocks * 128 // weight.group, tiles * 16)
-    if weight.packed.dtype != torch.uint8 or tuple(weight.packed.shape) != (tiles, blocks, 64, 16) \
-            or weight.steps.dtype != torch.int32 or tuple(weight.steps.shape) != shape \
-            or weight.dtype not in _SUPPORTED:
+    blocks, tiles = -(-k // 128), -(-rows // 16)
+    if packed.dtype != torch.uint8 or packed.shape != (tiles, blocks, 64, 16) or steps.dtype != torch.int32 \
+            or steps.shape != (blocks * 128 // group, tiles * 16) or dtype not in _SUPPORTED:
         raise ValueError("an Int4Weight's tensors do not have the shapes and dtypes that int4_pack gives.")
-    for t in (weight.packed, weight.steps):
-        if t.device != device or not t.is_contiguous():
-            raise ValueError("an Int4Weight's tensors must be contiguous, on the product's device.")
-    return _SUPPORTED[weight.dtype]
+    if packed.device != device or steps.device != device or not packed.is_contiguous() or not steps.is_contiguous():
+        raise ValueError("an Int4Weight's tensors must be contiguous, on the product's device.")
+    return _SUPPORTED[dtype]
 
 
 def _launch(device: torch.device, fn, *args) -> int:
@@ -722,32 +735,31 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, norm_weight: torch.Tenso
     16-byte aligned. More rows: ``int4_dequantize`` and a library product."""
     device = _require_gpu(x)
     dtype = _check_int4(weight, device)
-    if x.ndim < 1 or x.dtype != weight.dtype or x.shape[-1] != weight.k or not x.is_contiguous():
+    cols, k = weight.rows, weight.k
+    shape = x.shape
+    if len(shape) < 1 or x.dtype != weight.dtype or shape[-1] != k or not x.is_contiguous():
         raise ValueError("x must be contiguous [..., k], in the weight's dtype.")
-    cols = weight.rows
     if swiglu:
         if cols % 2 or residual is not None:
             raise ValueError("swiglu takes a weight of gate and up rows and no residual.")
         cols //= 2
-    shape = (*x.shape[:-1], cols)
+    shape = (*shape[:-1], cols)
     if residual is not None and (residual.shape != shape or residual.dtype != x.dtype or residual.device != device
                                  or not residual.is_contiguous()):
         raise ValueError("residual must be contiguous, of the result's shape and dtype.")
     if norm_weight is not None:
-        if tuple(norm_weight.shape) != (weight.k,) or norm_weight.device != device \
-                or not norm_weight.is_floating_point():
+        if norm_weight.shape != (k,) or norm_weight.device != device or not norm_weight.is_floating_point():
             raise ValueError("norm_weight must be floating-point [k].")
         norm_weight = norm_weight.float().contiguous()  # no copy for the usual float32 vector
         if norm_weight.data_ptr() % 16:
             norm_weight = norm_weight.clone()  # a slice of a larger buffer
-    out = torch.empty(shape, dtype=x.dtype, device=device)
-    rows, lib = x.numel() // weight.k, _capi.lib()
-    ws_bytes = 0 if norm_weight is None else lib.hx_int4_workspace_bytes(rows, weight.k, 1)
+    out = x.new_empty(shape)
+    rows, lib = x.numel() // k, _capi.lib()
+    ws_bytes = 0 if norm_weight is None else lib.hx_int4_workspace_bytes(rows, k, 1)
     workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
     code = _launch(
-        device, lib.hx_int4_gemm, x.data_ptr(), weight.k, rows, weight.packed.data_ptr(),
-        weight.steps.data_ptr(), cols, weight.k, weight.group, dtype,
-        None if norm_weight is None else norm_weight.data_ptr(), eps,
+        device, lib.hx_int4_gemm, x.data_ptr(), k, rows, weight.packed.data_ptr(), weight.steps.data_ptr(), cols, k,
+        weight.group, dtype, None if norm_weight is None else norm_weight.data_ptr(), eps,
         None if residual is None else residual.data_ptr(), cols, 1 if swiglu else 0, out.data_ptr(), cols,
         None if workspace is None else workspace.data_ptr(), ws_bytes)
     _capi.check(code, "hx_int4_gemm")
@@ -798,36 +810,35 @@ class RuledLogits(NamedTuple):
     token_ids: torch.Tensor
 
 
+_PER_ROW_RULES = frozenset(("lengths", "prompt_lens", "repetition", "presence", "frequency"))
+_INT_RULES = frozenset(("tokens", "lengths", "prompt_lens", "bias_ids", "allowed"))
+
+
 def _check_rules(rules: LogitRules, rows: int, vocab: int, device: torch.device) -> None:
-    per_row = (("lengths", torch.int32), ("prompt_lens", torch.int32), ("repetition", torch.float32),
-               ("presence", torch.float32), ("frequency", torch.float32))
-    for name, dtype in per_row:
-        t = getattr(rules, name)
-        if t is not None and (t.dtype != dtype or tuple(t.shape) != (rows,) or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous {dtype} [{rows}].")
-    tables = (("tokens", torch.int32), ("bias_ids", torch.int32), ("bias_values", torch.float32),
-              ("allowed", torch.int32))
-    for name, dtype in tables:
-        t = getattr(rules, name)
-        if t is not None and (t.dtype != dtype or t.ndim != 2 or t.shape[0] != rows
-                              or (t.shape[1] > 1 and t.stride(1) != 1)
-                              or (rows > 1 and t.stride(0) < t.shape[1])):
+    for name, t in zip(LogitRules._fields, rules):
+        if t is None:
+            continue
+        dtype = torch.int32 if name in _INT_RULES else torch.float32
+        shape = t.shape
+        if name in _PER_ROW_RULES:
+            if t.dtype != dtype or shape != (rows,) or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous {dtype} [{rows}].")
+        elif t.dtype != dtype or len(shape) != 2 or shape[0] != rows or (shape[1] > 1 and t.stride(1) != 1) \
+                or (rows > 1 and t.stride(0) < shape[1]):
             raise ValueError(f"{name} must be {dtype} [{rows}, n] with contiguous rows.")
-    if (rules.tokens is None) != (rules.lengths is None):
-        raise ValueError("tokens and lengths go together.")
-    if rules.tokens is None and any(t is not None for t in (rules.prompt_lens, rules.repetition, rules.presence,
-                                                            rules.frequency)):
-        raise ValueError("prompt_lens, repetition, presence and frequency need tokens.")
-    if (rules.bias_ids is None) != (rules.bias_values is None) \
-            or (rules.bias_ids is not None and rules.bias_ids.shape != rules.bias_values.shape):
-        raise ValueError("bias_ids and bias_values go together, in one shape.")
-    if rules.bias_ids is not None and rules.bias_ids.stride(0) != rules.bias_values.stride(0):
-        raise ValueError("bias_ids and bias_values must have the same row stride.")
-    if rules.allowed is not None and rules.allowed.shape[1] < -(-vocab // 32):
-        raise ValueError("allowed needs a bit for every token of the vocabulary.")
-    for name, t in zip(rules._fields, rules):
-        if t is not None and t.device != device:
+        if t.device != device:
             raise ValueError(f"{name} must be on the logits' device.")
+    tokens, lengths, prompt_lens, repetition, presence, frequency, bias_ids, bias_values, allowed = rules
+    if (tokens is None) != (lengths is None):
+        raise ValueError("tokens and lengths go together.")
+    if tokens is None and any(t is not None for t in (prompt_lens, repetition, presence, frequency)):
+        raise ValueError("prompt_lens, repetition, presence and frequency need tokens.")
+    if (bias_ids is None) != (bias_values is None) or (bias_ids is not None and bias_ids.shape != bias_values.shape):
+        raise ValueError("bias_ids and bias_values go together, in one shape.")
+    if bias_ids is not None and rows > 1 and bias_ids.stride(0) != bias_values.stride(0):
+        raise ValueError("bias_ids and bias_values must have the same row stride.")
+    if allowed is not None and allowed.shape[1] < -(-vocab // 32):
+        raise ValueError("allowed needs a bit for every token of the vocabulary.")
 
 
 def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, *, out: torch.Tensor | None = None,
@@ -865,22 +876,23 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, *, out: torch.Ten
     ws_bytes = lib.hx_logit_rules_workspace_bytes(rows, vocab)
     workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
 
-    def ptr(t):
-        return None if t is None else t.data_ptr()
-
-    def row_stride(t, width):  # a single row's stride may be anything
-        return 0 if t is None else t.stride(0) if rows > 1 else width
-
-    tokens, bias, allowed = rules.tokens, rules.bias_ids, rules.allowed
-    cap = 0 if tokens is None else tokens.shape[1]
-    n_bias = 0 if bias is None else bias.shape[1]
+    tokens, lengths, prompt_lens, repetition, presence, frequency, bias, bias_values, allowed = [
+        None if t is None else t.data_ptr() for t in rules]
+    cap = n_bias = words = token_stride = bias_stride = 0
+    if tokens is not None:
+        cap = rules.tokens.shape[1]
+        token_stride = rules.tokens.stride(0) if rows > 1 else cap  # a single row's stride may be anything
+    if bias is not None:
+        n_bias = rules.bias_ids.shape[1]
+        bias_stride = rules.bias_ids.stride(0) if rows > 1 else n_bias
+    if allowed is not None:
+        words = rules.allowed.stride(0) if rows > 1 else rules.allowed.shape[1]
     code = _launch(
-        device, lib.hx_logit_rules, logits.data_ptr(), row_stride(logits, vocab), rows, vocab, dtype,
-        ptr(tokens) if cap else None, row_stride(tokens, cap), cap, ptr(rules.lengths), ptr(rules.prompt_lens),
-        ptr(rules.repetition), ptr(rules.presence), ptr(rules.frequency),
-        ptr(bias) if n_bias else None, ptr(rules.bias_values), row_stride(bias, n_bias), n_bias,
-        ptr(allowed), row_stride(allowed, 0 if allowed is None else allowed.shape[1]),
-        ptr(out), row_stride(out, vocab), token_ids.data_ptr(), workspace.data_ptr(), ws_bytes)
+        device, lib.hx_logit_rules, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, dtype,
+        tokens if cap else None, token_stride, cap, lengths, prompt_lens, repetition, presence, frequency,
+        bias if n_bias else None, bias_values, bias_stride, n_bias, allowed, words,
+        None if out is None else out.data_ptr(), vocab if out is None or rows == 1 else out.stride(0),
+        token_ids.data_ptr(), workspace.data_ptr(), ws_bytes)
     _capi.check(code, "hx_logit_rules")
     return RuledLogits(out, token_ids)
 
