@@ -315,6 +315,8 @@ __global__ __launch_bounds__(64 * WAVES) void select_blocks_kernel(SelectArgs a)
   __shared__ uint64_t s_ends[2][WAVES];
   __shared__ __attribute__((aligned(16))) int s_bins[kSelBins];
   __shared__ int s_above[WAVES], s_ties[WAVES], s_taken[WAVES];
+  __shared__ uint64_t s_few[64];
+  __shared__ int s_listed;
   const int tid = hx::tid_x(), lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t ih = hx::wg_x();
   int32_t* out = a.out + ih * a.budget;
@@ -351,13 +353,14 @@ __global__ __launch_bounds__(64 * WAVES) void select_blocks_kernel(SelectArgs a)
     }
   }
   // The need-th largest free key: counts of the keys between lo and hi in up to 1024 equal bins,
-  // then of those in the bin it lies in, until that bin is wanted whole or is a single key. Two or
-  // three passes of keys that spread out, at most seven.
+  // then of those in the bin it lies in, until that bin is wanted whole, is a single key or holds
+  // no more than a wave does. One or two passes of keys that spread out, at most seven.
   const int need = a.budget - a.sink - a.recent;
   uint64_t least = ~0ull;  // above every key
   for (int want = need, pass = 0; want > 0 && pass < kSelPasses; ++pass) {
     const int bits = lo == hi ? 0 : 64 - __builtin_clzll(hi - lo), shift = bits > 10 ? bits - 10 : 0;
     for (int e = tid; e < kSelBins / 4; e += 64 * WAVES) reinterpret_cast<uint4*>(s_bins)[e] = hx::zero4();
+    if (tid == 0) s_listed = 0;
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < PER; ++t)
@@ -393,6 +396,22 @@ __global__ __launch_bounds__(64 * WAVES) void select_blocks_kernel(SelectArgs a)
     }
     hi = lo + least_of<uint64_t>(hi - lo, (1ull << shift) - 1);  // lo + 2^shift may pass 2^64
     __syncthreads();
+    if (count_of > 64) continue;
+    // Few enough to compare each with each: a lane's key is the one wanted if fewer than want
+    // lie above it and it is not above want of them; every wave finds it.
+#pragma unroll
+    for (int t = 0; t < PER; ++t)
+      if (key[t] >= lo && key[t] <= hi) s_few[atomicAdd(&s_listed, 1)] = key[t];
+    __syncthreads();
+    const uint64_t mine = lane < count_of ? s_few[lane] : 0;
+    int greater = 0, equal = 0;
+    for (int o = 0; o < count_of; ++o) {
+      greater += s_few[o] > mine ? 1 : 0;
+      equal += s_few[o] == mine ? 1 : 0;
+    }
+    const uint64_t is = __builtin_amdgcn_ballot_w64(lane < count_of && greater < want && greater + equal >= want);
+    least = s_few[__builtin_ctzll(is)];
+    break;
   }
   // Keys above the threshold, and of those equal to it the first ones, make up the rest.
   int above = 0, tied = 0, taken = 0;
