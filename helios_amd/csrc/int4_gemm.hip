@@ -20,14 +20,15 @@
 // bf16 (their sum has 16 bits), each an operand row of its own: of up to eight rows the leading
 // parts are rows 0-7 of one MFMA operand and the rest rows 8-15, at no further cost.
 //
-// A workgroup owns 16 or 32 columns of y (SwiGLU: 16 gate and the 16 up columns they multiply)
-// and 16 (8) rows; its waves split K and merge through LDS in wave order.
+// A workgroup owns 16 to 64 columns of y (SwiGLU: gate and the up columns they multiply) and 16
+// (8) rows; its waves split K and merge through LDS in wave order.
 //
 // A layer of hidden 2560, 32/8 heads of 128 and ffn 9728, W from HBM, 1 / 8 / 16 rows (us): qkv
 // 5.5 / 6.0 / 8.0, o 4.0 / 4.5 / 5.3, gate_up 10.2 / 11.1 / 15.0, down 6.6 / 7.4 / 9.4, in all 26 /
-// 29 / 38 where the 16-bit products take 60 / 62 / 71. gate_up's 26 MB are 2.6 TB/s at one row:
-// about 4 us of each launch are its start, the first loads' way and the merge, as for the
-// 16-bit products; the rest is bound by the address unit (x and W: 104 cycles a block at 8 rows).
+// 29 / 38 where the 16-bit products take 60 / 62 / 71; 17 / 64 rows 46 / 62. gate_up's 26 MB are
+// 2.6 TB/s at one row: about 4 us of each launch are its start, the first loads' way and the
+// merge, as for the 16-bit products; the rest is bound by the address unit (x and W: 104 cycles a
+// block at 8 rows), at 64 rows by x's way from L2 (15 TB/s).
 
 #include <type_traits>
 
@@ -155,8 +156,8 @@ enum : int { kRaw4, kRaw8, kRaw16, kNorm4, kNorm8, kNorm16, kParts16 };
 // LDS slot of 16-byte piece p of row r: the 16 rows of a fragment read spread over the banks.
 __device__ __forceinline__ int turn_piece(int r, int p) { return p ^ (r & 15); }
 
-// G: k elements per group (32, 64 or 128). NV: W tiles of a wave (SWIGLU: a gate and the up tile
-// it multiplies). D: packed blocks in flight per wave.
+// G: k elements per group (32, 64 or 128). NV: W tiles of a wave (SWIGLU: gate tiles, then the up
+// tiles they multiply). D: packed blocks in flight per wave.
 template <typename T, int IN, bool SWIGLU, int G, int NV, int WAVES, int D>
 __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
   constexpr bool kRaw = IN <= kRaw16, kNorm = IN >= kNorm4 && IN <= kNorm16, kTurn = kRaw || kNorm;
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
   typedef hx::Elem<M> EM;
   typedef typename EM::v8 v8;
   constexpr int kSteps = kI4Block / 32, kGroups = kI4Block / G;
-  constexpr int kCols = SWIGLU ? 16 : 16 * NV;  // of the output
+  constexpr int kTiles = SWIGLU ? NV / 2 : NV, kCols = 16 * kTiles;  // of the output
   constexpr int kRows = IN == kNorm4 || IN == kNorm8 ? 8 : 16;  // of a row tile
   constexpr int kOps = IN == kNorm16 || IN == kParts16 ? 2 : 1;  // MFMA operands of a tile's rows
   // Up to eight normalised rows share one operand: leading parts in rows 0-7, the rest in 8-15.
@@ -193,8 +194,8 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     // A column past the last reads a row of W that is there; its sums are not stored.
-    const int first = SWIGLU ? n0 + v * a.cols : min(n0 + 16 * v, a.cols - 1);
-    const int row = min(first + lr, (SWIGLU ? (v + 1) * a.cols : a.cols) - 1);
+    const int part = v / kTiles, first = min(n0 + 16 * (v % kTiles), a.cols - 1) + part * a.cols;
+    const int row = min(first + lr, (part + 1) * a.cols - 1);
     wr[v] = hx::buffer_rsrc(a.w + (int64_t)(first >> 4) * a.blocks * 1024, wbytes);
     woff[v] = (uint32_t)((row >> 4) - (first >> 4)) * a.blocks * 1024 + ((row & 15) + 16 * lg) * 16;
     soff[v] = 4u * row;
@@ -339,20 +340,19 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
     }
   }
   __syncthreads();
-  constexpr int kOut = SWIGLU ? 1 : NV;  // output tiles of kRows x 16
-  for (int e = tid; e < kOut * kRows * 16; e += 64 * WAVES) {
+  for (int e = tid; e < kTiles * kRows * 16; e += 64 * WAVES) {
     const int v0 = e / (kRows * 16), at = e % (kRows * 16);
     const int row = rt * kRows + at / 16, n = n0 + 16 * v0 + at % 16;
     if (row >= a.rows || n >= a.cols) continue;
-    constexpr int kSums = SWIGLU ? NV : 1;
+    constexpr int kSums = SWIGLU ? 2 : 1;
     float y[kSums];
 #pragma unroll
     for (int v = 0; v < kSums; ++v) {
       y[v] = 0.f;
 #pragma unroll
       for (int ww = 0; ww < WAVES; ++ww) {
-        y[v] += red[ww][v0 + v][at];
-        if constexpr (kPaired) y[v] += red[ww][v0 + v][at + 128];  // the other part
+        y[v] += red[ww][v0 + v * kTiles][at];
+        if constexpr (kPaired) y[v] += red[ww][v0 + v * kTiles][at + 128];  // the other part
       }
     }
     if constexpr (kNorm) {
@@ -409,24 +409,30 @@ __global__ __launch_bounds__(256) void int4_dequant_kernel(DequantArgs a, int64_
 
 template <typename T, int IN, bool SWIGLU, int G, int NV>
 int launch_tiles(Int4Args a, hipStream_t s) {
-  constexpr int kCols = SWIGLU ? 16 : 16 * NV, kRows = IN == kNorm4 || IN == kNorm8 ? 8 : 16;
+  constexpr int kCols = SWIGLU ? 8 * NV : 16 * NV, kRows = IN == kNorm4 || IN == kNorm8 ? 8 : 16;
   a.row_tiles = (a.rows + kRows - 1) / kRows;
   a.col_tiles = (a.cols + kCols - 1) / kCols;
   // Waves that split K, and blocks in flight. bf16, 1 / 8 / 16 rows, W from HBM (us): 9728 + 9728
   // columns of 2560 with SwiGLU, 4 waves and 1 block 10.2 / 11.1 / 15.0, 2 blocks 10.1 / 12.2 /
   // 15.2, 8 waves 9.9 / 11.7 / 21.8 (their LDS leaves one workgroup to a CU at 16 rows); 2560
   // columns of 9728, 8 waves and 2 blocks 6.6 / 7.4 / 9.4, 3 blocks 6.3 / 7.3 / 9.8, 4 waves
-  // 9.1 / 10.0 / 11.0.
-  constexpr int kWaves = SWIGLU ? 4 : 8, kDepth = SWIGLU ? 1 : 2;
+  // 9.1 / 10.0 / 11.0. Four W tiles, or 16 loads of x and W a block, are enough in flight at one
+  // block: 64 rows of the columns of 9728 13.5, 2 blocks 14.5; 6144 columns of 2560, normalised, 4
+  // waves and 1 block 14.7, 2 blocks 15.8, 8 waves 16.0.
+  constexpr int kWaves = SWIGLU || IN == kParts16 ? 4 : 8, kDepth = SWIGLU || NV == 4 ? 1 : 2;
   const auto fn = int4_gemm_kernel<T, IN, SWIGLU, G, NV, kWaves, kDepth>;
   hipLaunchKernelGGL(fn, dim3((unsigned)((a.col_tiles + 7) / 8 * 8 * a.row_tiles)), dim3(64 * kWaves), 0, s, a);
   return hx::status_from_hip(hipGetLastError());
 }
 
-// Two W tiles a wave where x costs more than a load (6144 columns of 2560, normalised, 1 / 8 / 16
-// rows: 5.5 / 6.0 / 8.0 us, one tile 6.2 / 7.6 / 10.6), one where it does not (2560 columns of
-// 9728: 6.4 / 7.3 / 9.3, two tiles 8.2 / 9.2 / 11.0), two again for several row tiles, which
-// fill the chip (64 rows: 16.8, one tile 18.7).
+// W tiles of a workgroup. Two where x costs more than a load (6144 columns of 2560, normalised,
+// 1 / 8 / 16 rows: 5.5 / 6.0 / 8.0 us, one tile 6.2 / 7.6 / 10.6), one where it does not (2560
+// columns of 9728: 6.4 / 7.3 / 9.3, two tiles 8.2 / 9.2 / 11.0). Past one row tile, x's way from
+// L2 bounds the kernel and more tiles share it: four of normalised rows, whose parts are twice
+// the bytes (17 / 64 rows, 6144 columns 11.4 / 14.7, two tiles 13.4 / 17.9; 9728 columns and
+// SwiGLU 19.2 / 27.6, two 21.7 / 34.7, eight 21.2 / 30.3), otherwise two while those make one
+// workgroup a CU (2560 columns of 9728, 17 / 48 rows 10.1 / 11.2, four 13.0 / 13.6) and four
+// where they make more (64 rows 13.5, two 17.1).
 template <typename T, int IN, bool SWIGLU, int NV = SWIGLU || IN >= kNorm4 ? 2 : 1>
 int launch_group(const Int4Args& a, int group, hipStream_t s) {
   if (group == 128) return launch_tiles<T, IN, SWIGLU, 128, NV>(a, s);
@@ -435,23 +441,25 @@ int launch_group(const Int4Args& a, int group, hipStream_t s) {
 }
 
 // Rows that each workgroup normalises on their way in; more of them are normalised once, in a
-// launch of about 3 us (6144 columns of 2560: 16 rows 8.0 us, 17 rows 12.6; 64 rows 16.5 us, and
+// launch of about 3 us (6144 columns of 2560: 16 rows 8.0 us, 17 rows 11.4; 64 rows 14.7 us, and
 // 32.1 normalised by every workgroup's own row tiles of 8).
 constexpr int kFusedNormRows = 16;
 
 template <typename T, bool SWIGLU>
 int launch_in(const Int4Args& a, int group, hipStream_t s) {
+  constexpr int kRawPair = SWIGLU ? 16 : 32;  // columns of two W tiles
   if (a.norm_w == nullptr) {
     if (a.rows <= 4) return launch_group<T, kRaw4, SWIGLU>(a, group, s);
     if (a.rows <= 8) return launch_group<T, kRaw8, SWIGLU>(a, group, s);
     if (a.rows <= 16) return launch_group<T, kRaw16, SWIGLU>(a, group, s);
-    return launch_group<T, kRaw16, SWIGLU, 2>(a, group, s);
+    const int64_t wgs = (int64_t)((a.rows + 15) / 16) * ((a.cols + kRawPair - 1) / kRawPair);
+    return wgs <= 256 ? launch_group<T, kRaw16, SWIGLU, 2>(a, group, s) : launch_group<T, kRaw16, SWIGLU, 4>(a, group, s);
   }
   if (a.rows <= 4) return launch_group<T, kNorm4, SWIGLU>(a, group, s);
   if (a.rows <= 8) return launch_group<T, kNorm8, SWIGLU>(a, group, s);
   if (a.rows <= kFusedNormRows) return launch_group<T, kNorm16, SWIGLU>(a, group, s);
   hipLaunchKernelGGL(int4_norm_kernel<T>, dim3((unsigned)a.rows), dim3(256), 0, s, a, const_cast<uint16_t*>(a.h));
-  return launch_group<T, kParts16, SWIGLU>(a, group, s);
+  return launch_group<T, kParts16, SWIGLU, 4>(a, group, s);
 }
 
 bool bad_weight(const void* w, const void* steps, int32_t k, int32_t group) {
