@@ -491,8 +491,8 @@ def kv_block_bounds(k_cache: torch.Tensor, bounds: torch.Tensor, block_table: to
     ``bounds`` ``[pages, page_size // block_size, kv_heads, 2, head_dim]`` contiguous, of its
     dtype (a block is a power of two of 16 to 1024 tokens); ``block_table`` / ``cu_seq_q`` /
     ``seqused_k`` as for ``varlen_attn``. A block is read whole and its former bounds never,
-    so a page that was reused or truncated needs no clearing. A NaN key makes both bounds
-    NaN."""
+    so a page that was reused or truncated needs no clearing. ``max_q`` is at least the longest
+    sequence's new tokens. A NaN key makes both bounds NaN."""
     device = _require_gpu(k_cache, bounds, block_table, cu_seq_q, seqused_k)
     dtype, pages, page_size, n_kv, head_dim = _pool_layout("k_cache", k_cache)
     layout = bounds.shape
@@ -693,7 +693,7 @@ def int4_quantize(weight: torch.Tensor, group: int = 128) -> Int4Weight:
     if not bool(torch.isfinite(w).all()):
         raise ValueError("weight must be finite.")
     low, high = w.amin(dim=-1).clamp(max=0), w.amax(dim=-1).clamp(min=0)
-    scale = ((high - low) / 15).to(weight.dtype)
+    scale = (high / 15 - low / 15).to(weight.dtype)  # high - low may leave fp32
     step = scale.float().masked_fill(scale == 0, 1.0)[..., None]  # a group of zeros
     zero = (-low[..., None] / step).round().clamp(0, 15)
     values = ((w / step).round() + zero).clamp(0, 15).to(torch.uint8).view(rows, k)

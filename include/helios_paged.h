@@ -583,8 +583,8 @@ int hx_skinny_gemm(const void* x, int64_t x_row_stride, int64_t rows, const void
  * x and norm_weight 16-byte aligned, x_row_stride a multiple of 8. out must not overlap x or
  * the weights; it may be the residual. HX_E_UNSUPPORTED for more than 64 rows or another
  * group. The workspace is hx_int4_workspace_bytes(rows, k, norm_weight given) bytes (may be
- * 0), 16-byte aligned; calls that share one must be ordered. hx_int4_dequantize writes round(W), rows of k elements, out 16-byte aligned and
- * out_row_stride a multiple of 8. */
+ * 0), 16-byte aligned; calls that share one must be ordered. hx_int4_dequantize writes
+ * round(W), rows of k elements, out 16-byte aligned and out_row_stride a multiple of 8. */
 size_t hx_int4_workspace_bytes(int64_t rows, int32_t k, int32_t norm);
 int hx_int4_gemm(const void* x, int64_t x_row_stride, int64_t rows, const void* packed,
                  const void* steps, int32_t cols, int32_t k, int32_t group, int32_t dtype,
@@ -608,8 +608,8 @@ int hx_int4_dequantize(const void* packed, const void* steps, int32_t weight_row
  *   bounds[page][block of the page][h][0][d] = min, [1][d] = max of k[j][h][d]
  * over the block's tokens below seqused_k[b], both NaN where one of them is. Former bounds
  * are not read. bounds is [num_pages][page_size / block_size][n_kv_heads][2][head_dim],
- * contiguous like the pool, 16-byte aligned both. max_q sizes the grid only. Two sequences
- * that touch one block in one call write it in no particular order.
+ * contiguous like the pool, 16-byte aligned both. max_q, at least the largest n_b, sizes the
+ * grid only. Two sequences that touch one block in one call write it in no particular order.
  *
  * hx_select_blocks: entry i < n is query row rows[i] of q (i itself when rows is NULL; q_rows
  * rows in all) of sequence row_seq[i] (NULL: i), which sees its first key_counts[i] keys. For

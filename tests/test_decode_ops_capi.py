@@ -4,8 +4,9 @@ every call here returns an error or has no work."""
 from __future__ import annotations
 
 import pytest
+import torch
 
-from helios_amd import _capi
+from helios_amd import _capi, ops
 
 BAD, NO, WS = _capi.HX_E_INVALID_ARG, _capi.HX_E_UNSUPPORTED, _capi.HX_E_WORKSPACE
 P = 1 << 20  # an aligned address that no call here reads
@@ -54,7 +55,8 @@ RULES = dict(logits=P, row=64, rows=2, vocab=64, dtype=0, tokens=P, token_row=8,
     (dict(dtype=3), NO), (dict(rows=-1), BAD), (dict(vocab=0), BAD), (dict(row=63), BAD), (dict(logits=None), BAD),
     (dict(ids=None), BAD), (dict(out_row=63), BAD), (dict(lengths=None), BAD), (dict(token_row=7), BAD),
     (dict(bias_values=None), BAD), (dict(bias_row=3), BAD), (dict(n_bias=-1), BAD), (dict(allowed_row=1), BAD),
-    (dict(ws=None), WS), (dict(ws=P + 4), WS), (dict(ws_bytes=15), WS), (dict(rows=0), 0), (dict(logits=P + 1), BAD), (dict(dtype=2, out=P + 2), BAD),
+    (dict(ws=None), WS), (dict(ws=P + 4), WS), (dict(ws_bytes=15), WS), (dict(rows=0), 0),
+    (dict(logits=P + 1), BAD), (dict(dtype=2, out=P + 2), BAD),
     (dict(rows=1 << 31, ws_bytes=1 << 40), NO)])
 def test_logit_rules(change, code):
     assert _call("hx_logit_rules", RULES, **change) == code
@@ -99,7 +101,7 @@ SPARSE = dict(q=P, q_row=4096, q_head=128, q_rows=2, rows=None, row_seq=None, ke
     (dict(n=3), BAD), (dict(batch=1), BAD), (dict(k=None), BAD), (dict(v=P + 2), BAD), (dict(q=P + 8), BAD),
     (dict(q_row=4092), BAD), (dict(q_head=132), BAD), (dict(out=P + 2), BAD), (dict(out_row=4097), BAD),
     (dict(blocks=None), BAD), (dict(ws=None), WS), (dict(ws=P + 8), WS), (dict(ws_bytes=64), WS), (dict(n=0), 0),
-    (dict(hkv=1 << 18, hq=1 << 18), NO)])
+    (dict(hkv=1 << 18, hq=1 << 18), NO), (dict(budget=(1 << 24) + 1), BAD)])
 def test_block_sparse_attn(change, code):
     assert _call("hx_block_sparse_attn", SPARSE, **change) == code
 
@@ -118,3 +120,20 @@ def test_workspace_sizes():
     assert small > 0 and small % (32 * 130 * 4) == 0
     assert lib.hx_block_sparse_workspace_bytes(4096, 32, 8, 128, 2, 64) == 0  # one part each
     assert lib.hx_block_sparse_workspace_bytes(1, 31, 8, 128, 32, 64) == 0
+
+
+def test_int4_quantize_at_the_ends_of_the_range():
+    """A group from the type's lowest to its largest value, and one of its smallest: finite
+    steps, the ends within half a step of the outer values."""
+    for dtype in (torch.bfloat16, torch.float16):
+        most, least = torch.finfo(dtype).max, torch.finfo(dtype).smallest_normal
+        w = torch.zeros(2, 32, dtype=dtype)
+        w[0, :2] = torch.tensor([-most, most], dtype=dtype)
+        w[1, :2] = torch.tensor([-least, 64 * least], dtype=dtype)
+        q = ops.int4_quantize(w, 32)
+        scale = (q.steps & 0xffff).to(torch.int16).view(dtype)[0, :2].double()
+        zero = (q.steps >> 16).to(torch.int16).view(dtype)[0, :2].double() - 16
+        assert torch.isfinite(scale).all() and (scale > 0).all()
+        outer = torch.stack((-zero * scale, (15 - zero) * scale), dim=1)
+        step = scale[:, None] * (0.5 + 15 * torch.finfo(dtype).eps)
+        assert ((outer - w[:, :2].double()).abs() <= step).all()
