@@ -8,8 +8,8 @@
 // the G query heads that share the KV head the bound is linear in two vectors,
 //   s = sum_d (sum_g min(q_g[d], 0)) lower[d] + (sum_g max(q_g[d], 0)) upper[d],
 // and the blocks with the largest s, with the first `sink` and the last `recent` ones, are the
-// row's selection for that KV head (block_scores_kernel, select_blocks_kernel). The attention is the softmax over
-// the keys of those blocks alone (sparse_attn_kernel).
+// row's selection for that KV head (block_scores_kernel, select_blocks_kernel). The attention is
+// the softmax over the keys of those blocks alone (sparse_attn_kernel).
 
 #include "hx_common.h"
 

@@ -863,13 +863,13 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, *, out: torch.Ten
     _check_rules(rules, rows, vocab, device)
     if out is None:
         if return_logits:
-            out = torch.empty((rows, vocab), dtype=logits.dtype, device=device)
+            out = logits.new_empty((rows, vocab))
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != device \
             or (vocab > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < vocab):
         raise ValueError("out must have the logits' shape, dtype and device, and contiguous rows.")
     elif out.data_ptr() == logits.data_ptr() and rows > 1 and out.stride(0) != logits.stride(0):
         raise ValueError("out must be the logits or memory that does not overlap them.")
-    token_ids = torch.empty(rows, dtype=torch.int64, device=device)
+    token_ids = logits.new_empty(rows, dtype=torch.int64)
     if rows == 0:
         return RuledLogits(out, token_ids)
     lib = _capi.lib()
