@@ -7,6 +7,8 @@
  *   - KV append into a shared pool of pages           (hx_kv_append)
  *   - page-table-driven varlen GQA attention         (hx_varlen_attn*)
  *   - prefix block restore / page copy and gather    (hx_kv_copy_pages, hx_kv_gather)
+ * and the other steps of a tick: metadata, norms, RoPE, few-row products with 16-bit and
+ * 4-bit weights, logits and greedy ids, attention over selected blocks, logit rules.
  *
  * Conventions
  *   - Every pointer named *_pool, *_cache, q, k_new, v_new, out, lse, workspace,

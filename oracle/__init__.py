@@ -16,6 +16,9 @@ Modules
   kv_bytes    numpy restatements of the bit copies: KV append (index_copy_,
               paged_cache.py:335-345), page gather (_gather_cpu, :405-414) and block
               copy (cache.py:109-147).
+  decode_ops  float64 restatements of key bounds, block selection, attention over
+              selected blocks, 4-bit weights and logit rules, from their formulas (no
+              reference counterpart).
 
 How each function is pinned (tests/test_oracle.py): against closed forms
 (L = 1 gives V[0]; equal keys give the mean of V; a dominant key selects its V row;
