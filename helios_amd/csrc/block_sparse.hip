@@ -134,7 +134,7 @@ __global__ __launch_bounds__(kBdThreads) void block_bounds_kernel(BoundsArgs a) 
 //
 // 8 heads of 128: 64 rows of 256-640 blocks (113 MB of bounds) 31 us (3.6 TB/s; the loads alone,
 // in the same order, 24.5: what is left is 64-bit arithmetic that they do not hide) and 5.7 us
-// for the selection; one row of 2047 blocks 6.2 and 7.9 us, latency both. One workgroup a row and
+// for the selection; one row of 2047 blocks 6.2 and 6.2 us, latency both. One workgroup a row and
 // head for scores and selection: 71 and 137 us.
 
 constexpr int kScThreads = 256;
@@ -485,9 +485,13 @@ void launch_select(const SelectArgs& a, int64_t n, hipStream_t s) {
     else launch_scores<T, 32>(a, n, s);
   }
   const dim3 grid((unsigned)(n * a.n_heads));
-  // Few keys a thread: 512 rows of 448 blocks take 5.9 us with four waves, 7.1 with one.
+  // Few keys a thread, few waves to a barrier. One row / 64 rows, 8 heads, us: 900 blocks 5.2 /
+  // 6.3, 8 waves 5.6 / 8.2, 2 waves 5.9 / 7.2; 2000 blocks 6.2 / 8.4, 16 waves 8.1 / 12.2, 4 waves
+  // 8.7 / 10.3; 4000 blocks 7.1 / 14.1, 16 waves 8.0 / 19.3, 4 waves 8.2 / 13.6; 12000 blocks of 4
+  // rows 13.5, 8 waves 17.2.
   if (a.most <= 1024) hipLaunchKernelGGL((select_blocks_kernel<4, 4>), grid, dim3(256), 0, s, a);
-  else if (a.most <= 4096) hipLaunchKernelGGL((select_blocks_kernel<16, 4>), grid, dim3(1024), 0, s, a);
+  else if (a.most <= 2048) hipLaunchKernelGGL((select_blocks_kernel<8, 4>), grid, dim3(512), 0, s, a);
+  else if (a.most <= 4096) hipLaunchKernelGGL((select_blocks_kernel<8, 8>), grid, dim3(512), 0, s, a);
   else hipLaunchKernelGGL((select_blocks_kernel<16, 16>), grid, dim3(1024), 0, s, a);
 }
 

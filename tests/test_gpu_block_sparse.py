@@ -152,7 +152,7 @@ def test_select_blocks(device, hq, heads, d, block, keys, budget, sink, recent, 
     assert torch.equal(again.cpu(), want.flip(0))
 
 
-@pytest.mark.parametrize("blocks", [900, 2000, 5000, 16384])
+@pytest.mark.parametrize("blocks", [900, 2000, 3000, 5000, 16384])
 def test_select_blocks_of_long_sequences(device, blocks):
     """As many blocks as there may be, with scores that differ in few values: ties go to the
     earlier block."""
