@@ -43,7 +43,7 @@ struct Int4Args {
   const uint16_t* h;  // normalised rows (int4_norm_kernel)
   int64_t x_row;
   const uint8_t* w;       // [rows of W / 16][blocks][64][16]
-  const uint32_t* steps;  // [k_pad / group][w_pad]: the scale, and 16 + zero in the high half
+  const uint32_t* steps;  // [w_pad / 16][blocks][16][128 / group]: the scale, and 16 + zero in the high half
   int32_t rows, cols, k, blocks, w_pad;  // cols: of the output; w_pad: rows of W, padded to 16
   int32_t row_tiles, col_tiles;
   const float* norm_w;
@@ -149,6 +149,23 @@ __device__ __forceinline__ uint4 ld16(__amdgpu_buffer_rsrc_t r, uint32_t voff, u
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// A row's steps of a block: one load whatever the group.
+__device__ __forceinline__ void load_steps(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff, uint32_t (&st)[1]) {
+  st[0] = __builtin_amdgcn_raw_buffer_load_b32(r, (int)voff, (int)soff, 0);
+}
+__device__ __forceinline__ void load_steps(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff, uint32_t (&st)[2]) {
+  const auto u = __builtin_amdgcn_raw_buffer_load_b64(r, (int)voff, (int)soff, 0);
+  st[0] = u[0];
+  st[1] = u[1];
+}
+__device__ __forceinline__ void load_steps(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff, uint32_t (&st)[4]) {
+  const uint4 u = ld16(r, voff, soff);
+  st[0] = u.x;
+  st[1] = u.y;
+  st[2] = u.z;
+  st[3] = u.w;
+}
+
 // How x reaches the MFMA: as it is, up to 4, 8 or 16 rows a tile; normalised on the way, the same;
 // or as int4_norm_kernel's parts.
 enum : int { kRaw4, kRaw8, kRaw16, kNorm4, kNorm8, kNorm16, kParts16 };
@@ -198,7 +215,7 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
     const int row = min(first + lr, (part + 1) * a.cols - 1);
     wr[v] = hx::buffer_rsrc(a.w + (int64_t)(first >> 4) * a.blocks * 1024, wbytes);
     woff[v] = (uint32_t)((row >> 4) - (first >> 4)) * a.blocks * 1024 + ((row & 15) + 16 * lg) * 16;
-    soff[v] = 4u * row;
+    soff[v] = (uint32_t)((row >> 4) * a.blocks * 16 + (row & 15)) * 4 * kGroups;
   }
   // x is read in whole lines, 16 lanes to the 256 bytes of a row's block, and turned into the
   // MFMA's layout through the wave's part of LDS: lanes next to each other in that layout are
@@ -233,10 +250,7 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       wq[i][v] = hx::ld16_stream(wr[v], woff[v], in ? 1024u * b : wbytes);
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g)
-        st[i][v][g] = __builtin_amdgcn_raw_buffer_load_b32(
-            sr, (int)soff[v], (int)(in ? (uint32_t)(b * kGroups + g) * a.w_pad * 4 : sbytes), 0);
+      load_steps(sr, soff[v], in ? (uint32_t)b * 64 * kGroups : sbytes, st[i][v]);
     }
   };
 #pragma unroll
@@ -373,7 +387,7 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
 struct DequantArgs {
   const uint8_t* w;
   const uint32_t* steps;
-  int32_t w_rows, k, blocks, w_pad, group;
+  int32_t w_rows, k, blocks, group;
   uint16_t* out;
   int64_t out_row;
 };
@@ -394,8 +408,7 @@ __global__ __launch_bounds__(256) void int4_dequant_kernel(DequantArgs a, int64_
   for (int s = 0; s < 4; ++s) {
     const int k0 = b * kI4Block + 32 * s + 8 * lg;
     if (k0 >= a.k) return;
-    const int64_t at = (int64_t)(k0 / a.group) * a.w_pad + row;
-    const uint32_t step = a.steps[at];
+    const uint32_t step = a.steps[(blk * 16 + (lane & 15)) * (kI4Block / a.group) + 32 * s / a.group];
     const float sc = E::lo(step), zp = E::hi(step) - 16.f;
     const uint32_t turned = __builtin_amdgcn_alignbit(wd[s], wd[s], 3);
     uint32_t o[4];
@@ -463,7 +476,7 @@ int launch_in(const Int4Args& a, int group, hipStream_t s) {
 }
 
 bool bad_weight(const void* w, const void* steps, int32_t k, int32_t group) {
-  return !w || !steps || (reinterpret_cast<uintptr_t>(w) & 15) || (reinterpret_cast<uintptr_t>(steps) & 3) || k % group;
+  return !w || !steps || ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(steps)) & 15) || k % group;
 }
 
 }  // namespace
@@ -536,11 +549,10 @@ extern "C" int hx_int4_dequantize(const void* packed, const void* steps, int32_t
   a.w_rows = weight_rows;
   a.k = k;
   a.blocks = (k + kI4Block - 1) / kI4Block;
-  a.w_pad = (weight_rows + 15) / 16 * 16;
   a.group = group;
   a.out = static_cast<uint16_t*>(out);
   a.out_row = out_row_stride;
-  const int64_t units = (int64_t)(a.w_pad / 16) * a.blocks * 64;
+  const int64_t units = ((int64_t)weight_rows + 15) / 16 * a.blocks * 64;
   if ((units + 255) / 256 > 0x7fffffff) return HX_E_UNSUPPORTED;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)((units + 255) / 256));

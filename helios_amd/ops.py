@@ -632,10 +632,10 @@ def block_sparse_attn(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
 class Int4Weight(NamedTuple):
     """A weight matrix ``[rows, k]`` in 4 bits with a scale and a zero point per ``group``
     elements of k: ``W[n, k] = scale[k // group, n] * (q[n, k] - zero[k // group, n])``.
-    ``packed`` holds q in the order the kernel reads it (hx_int4_gemm), ``steps`` (int32
-    ``[groups, rows]``, rows rounded up to 16) a scale's bits in the low half and those of 16
-    + a zero point in the high one; ``dtype`` is the scales' and the products' type. Made by
-    ``int4_quantize`` or ``int4_pack``."""
+    ``packed`` holds q and ``steps`` (int32) a scale's bits in the low half and those of 16 + a
+    zero point in the high one, both in the order the kernel reads them (hx_int4_gemm);
+    ``dtype`` is the scales' and the products' type. Made by ``int4_quantize`` or
+    ``int4_pack``."""
 
     packed: torch.Tensor
     steps: torch.Tensor
@@ -675,7 +675,8 @@ def int4_pack(values: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor) -
     low, high = (t.contiguous().view(torch.int16).to(torch.int32) & 0xffff
                  for t in (scales, (zeros.to(torch.float32) + 16).to(scales.dtype)))
     steps = low | high << 16
-    steps = torch.nn.functional.pad(steps, (0, more_rows, 0, more_k // group)).contiguous()
+    steps = torch.nn.functional.pad(steps, (0, more_rows, 0, more_k // group))
+    steps = steps.view(-1, 128 // group, (rows + more_rows) // 16, 16).permute(2, 0, 3, 1).contiguous()
     return Int4Weight(packed.view(packed.shape[0], packed.shape[1], 64, 16), steps, rows, k, group, scales.dtype)
 
 
@@ -707,7 +708,7 @@ def _check_int4(weight: Int4Weight, device: torch.device) -> int:
         raise ValueError("the weight's group must be 32, 64 or 128 and divide its k.")
     blocks, tiles = -(-k // 128), -(-rows // 16)
     if packed.dtype != torch.uint8 or packed.shape != (tiles, blocks, 64, 16) or steps.dtype != torch.int32 \
-            or steps.shape != (blocks * 128 // group, tiles * 16) or dtype not in _SUPPORTED:
+            or steps.shape != (tiles, blocks, 16, 128 // group) or dtype not in _SUPPORTED:
         raise ValueError("an Int4Weight's tensors do not have the shapes and dtypes that int4_pack gives.")
     if packed.device != device or steps.device != device or not packed.is_contiguous() or not steps.is_contiguous():
         raise ValueError("an Int4Weight's tensors must be contiguous, on the product's device.")

@@ -580,8 +580,9 @@ int hx_skinny_gemm(const void* x, int64_t x_row_stride, int64_t rows, const void
  *           lane 16 c + r of a tile holds four words of row r; word s holds the k elements
  *           128 b + 32 s + 8 c + j, j = 0..7, element j at bits 3 + 4 (j / 2) + 16 (j % 2)
  *           modulo 32
- *   steps   uint32 [k_pad / group][w_pad]: in the element type, the scale in the low half and
- *           16 + zero in the high one; 0 where W has no row or k
+ *   steps   uint32 [w_pad / 16][k_pad / 128][16][128 / group], 16-byte aligned: a row's groups
+ *           of a block; in the element type, the scale in the low half and 16 + zero in the
+ *           high one; 0 where W has no row or k
  * x and norm_weight 16-byte aligned, x_row_stride a multiple of 8. out must not overlap x or
  * the weights; it may be the residual. HX_E_UNSUPPORTED for more than 64 rows or another
  * group. The workspace is hx_int4_workspace_bytes(rows, k, norm_weight given) bytes (may be

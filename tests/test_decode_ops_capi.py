@@ -26,7 +26,7 @@ INT4 = dict(x=P, x_row=256, rows=4, packed=P, steps=P, cols=16, k=256, group=64,
 @pytest.mark.parametrize("change,code", [
     (dict(dtype=2), NO), (dict(group=16), NO), (dict(group=48), NO), (dict(rows=65), NO), (dict(rows=-1), BAD),
     (dict(cols=0), BAD), (dict(k=0), BAD), (dict(k=96), BAD), (dict(x=None), BAD), (dict(packed=None), BAD),
-    (dict(steps=None), BAD), (dict(steps=P + 2), BAD), (dict(out=None), BAD), (dict(packed=P + 8), BAD),
+    (dict(steps=None), BAD), (dict(steps=P + 8), BAD), (dict(out=None), BAD), (dict(packed=P + 8), BAD),
     (dict(x=P + 2), BAD), (dict(x_row=255), BAD), (dict(x_row=252), BAD), (dict(norm=P, eps=-1.0), BAD),
     (dict(norm=P, eps=float("nan")), BAD), (dict(norm=P + 4), BAD), (dict(out=P + 1), BAD), (dict(out_row=15), BAD),
     (dict(residual=P, swiglu=1), BAD), (dict(residual=P, residual_row=15), BAD), (dict(rows=0), 0),
@@ -131,8 +131,8 @@ def test_int4_quantize_at_the_ends_of_the_range():
         w[0, :2] = torch.tensor([-most, most], dtype=dtype)
         w[1, :2] = torch.tensor([-least, 64 * least], dtype=dtype)
         q = ops.int4_quantize(w, 32)
-        scale = (q.steps & 0xffff).to(torch.int16).view(dtype)[0, :2].double()
-        zero = (q.steps >> 16).to(torch.int16).view(dtype)[0, :2].double() - 16
+        scale = (q.steps & 0xffff).to(torch.int16).view(dtype)[0, 0, :2, 0].double()
+        zero = (q.steps >> 16).to(torch.int16).view(dtype)[0, 0, :2, 0].double() - 16
         assert torch.isfinite(scale).all() and (scale > 0).all()
         outer = torch.stack((-zero * scale, (15 - zero) * scale), dim=1)
         step = scale[:, None] * (0.5 + 15 * torch.finfo(dtype).eps)

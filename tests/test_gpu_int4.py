@@ -134,7 +134,7 @@ def test_int4_quantize(device, group, dtype):
     q = ops.int4_quantize(w.to(device), group)
     assert (q.rows, q.k, q.group) == (33, 384, group)
     back = ops.int4_dequantize(q).cpu().double()
-    scales = (q.steps & 0xffff).to(torch.int16).view(dtype)
+    scales = (q.steps & 0xffff).to(torch.int16).view(dtype).permute(1, 3, 0, 2).reshape(-1, 48)
     step = scales.cpu().double()[:, :33].t().repeat_interleave(group, 1)[:, :384]
     # half a step; the scale's own rounding (half an eps of 15 steps) may push an end past the
     # last value; and the result's rounding
