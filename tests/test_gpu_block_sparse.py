@@ -264,6 +264,21 @@ def test_block_sparse_attn_many_rows(device, d):
     assert ((got.double().cpu() - ref).abs() <= _tolerance(q, v, ref, torch.bfloat16, d ** -0.5)).all()
 
 
+@pytest.mark.parametrize("d", [64, 160])
+def test_block_sparse_attn_many_splits(device, d):
+    """One row's list in more parts than a wave has lanes (88 of 128 keys: sums in 216 steps, 2^-16
+    of max |v|)."""
+    say("sparse many splits", d)
+    k, v, table = _pools([11190], 1, d, torch.bfloat16, seed=d)
+    g = torch.Generator().manual_seed(d)
+    q = torch.randn(1, 3, d, generator=g).to(torch.bfloat16)
+    blocks = torch.arange(700, dtype=torch.int32).view(1, 1, 700)
+    ref = oracle.sparse_attention(q, k, v, blocks, table, [11190], [0], 16, d ** -0.5)
+    got = ops.block_sparse_attn(q.to(device), k.to(device), v.to(device), blocks.to(device), table.to(device),
+                                torch.tensor([11190], dtype=torch.int32, device=device), block_size=16)
+    assert ((got.double().cpu() - ref).abs() <= _tolerance(q, v, ref, torch.bfloat16, d ** -0.5)).all()
+
+
 def test_block_sparse_attn_lists(device):
     """Lists in any order, with repeats (they count twice), ids past the keys, pages outside the
     pool, gaps of -1 in the middle, and nothing at all."""

@@ -142,6 +142,37 @@ def test_lengths_beyond_the_table(device):
     assert got[2].tolist() == [0.5] * 10 + [1.0] * 30
 
 
+@pytest.mark.parametrize("shift", [0, 1, 2, 3])
+def test_long_histories_and_bias_lists(device, shift):
+    """More tokens and biases than a workgroup takes at once, token rows at every offset from a
+    16-byte address."""
+    say("logit rules long", shift)
+    rules = _rules(3, 5000, 20001, 1300, True, seed=shift)
+    rules = rules._replace(lengths=torch.tensor([20001, 8193 + shift, 2047], dtype=torch.int32))
+    logits = torch.randn(3, 5000, generator=torch.Generator().manual_seed(shift)).to(torch.bfloat16)
+    on = _to(rules, device)
+    wide = torch.zeros(3, 20004 + shift, dtype=torch.int32, device=device)
+    wide[:, shift:shift + 20001] = on.tokens
+    on = on._replace(tokens=wide[:, shift:shift + 20001])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.apply_logit_rules(logits.to(device), on)
+    torch.cuda.current_stream().wait_stream(side)
+    _check(got, logits, rules)
+
+
+def test_rows_past_32_bits(device):
+    """A row that begins beyond 2^31 elements from the first."""
+    say("logit rules far rows")
+    wide = torch.empty(2 ** 31 + 8192, dtype=torch.bfloat16, device=device)
+    far = wide.as_strided((2, 3000), (2 ** 31 + 24, 1), 40)
+    rules = _rules(2, 3000, 40, 5, False, seed=9)
+    logits = torch.randn(2, 3000, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16)
+    far.copy_(logits)
+    _check(ops.apply_logit_rules(far, _to(rules, device), out=far), logits, rules)
+
+
 def test_logit_rules_in_two_graphs(device):
     """Two captured calls of one pool of memory, replayed in turn with eager calls between."""
     say("logit rules graphs")
