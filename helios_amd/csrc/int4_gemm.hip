@@ -25,7 +25,7 @@
 //
 // A layer of hidden 2560, 32/8 heads of 128 and ffn 9728, W from HBM, 1 / 8 / 16 rows (us): qkv
 // 5.5 / 6.0 / 8.0, o 4.0 / 4.5 / 5.3, gate_up 10.2 / 11.1 / 15.0, down 6.6 / 7.4 / 9.4, in all 26 /
-// 29 / 38 where the 16-bit products take 60 / 62 / 71; 17 / 64 rows 46 / 62. gate_up's 26 MB are
+// 29 / 38 where the 16-bit products take 60 / 62 / 71; 17 / 64 rows 47 / 62. gate_up's 26 MB are
 // 2.6 TB/s at one row: about 4 us of each launch are its start, the first loads' way and the
 // merge, as for the 16-bit products; the rest is bound by the address unit (x and W: 104 cycles a
 // block at 8 rows), at 64 rows by x's way from L2 (15 TB/s).
@@ -429,10 +429,10 @@ int launch_tiles(Int4Args a, hipStream_t s) {
   // columns of 2560 with SwiGLU, 4 waves and 1 block 10.2 / 11.1 / 15.0, 2 blocks 10.1 / 12.2 /
   // 15.2, 8 waves 9.9 / 11.7 / 21.8 (their LDS leaves one workgroup to a CU at 16 rows); 2560
   // columns of 9728, 8 waves and 2 blocks 6.6 / 7.4 / 9.4, 3 blocks 6.3 / 7.3 / 9.8, 4 waves
-  // 9.1 / 10.0 / 11.0. Four W tiles, or 16 loads of x and W a block, are enough in flight at one
-  // block: 64 rows of the columns of 9728 13.5, 2 blocks 14.5; 6144 columns of 2560, normalised, 4
+  // 9.1 / 10.0 / 11.0. Three W tiles and more are enough in flight at one block: 64 rows of the
+  // columns of 9728, three tiles, 12.0, 2 blocks 12.7, 16 waves 12.4; four tiles 13.5 and 14.5; 6144 columns of 2560, normalised, 4
   // waves and 1 block 14.7, 2 blocks 15.8, 8 waves 16.0.
-  constexpr int kWaves = SWIGLU || IN == kParts16 ? 4 : 8, kDepth = SWIGLU || NV == 4 ? 1 : 2;
+  constexpr int kWaves = SWIGLU || IN == kParts16 ? 4 : 8, kDepth = SWIGLU || NV >= 3 ? 1 : 2;
   const auto fn = int4_gemm_kernel<T, IN, SWIGLU, G, NV, kWaves, kDepth>;
   hipLaunchKernelGGL(fn, dim3((unsigned)((a.col_tiles + 7) / 8 * 8 * a.row_tiles)), dim3(64 * kWaves), 0, s, a);
   return hx::status_from_hip(hipGetLastError());
@@ -443,9 +443,9 @@ int launch_tiles(Int4Args a, hipStream_t s) {
 // columns of 9728: 6.4 / 7.3 / 9.3, two tiles 8.2 / 9.2 / 11.0). Past one row tile, x's way from
 // L2 bounds the kernel and more tiles share it: four of normalised rows, whose parts are twice
 // the bytes (17 / 64 rows, 6144 columns 11.4 / 14.7, two tiles 13.4 / 17.9; 9728 columns and
-// SwiGLU 19.2 / 27.6, two 21.7 / 34.7, eight 21.2 / 30.3), otherwise two while those make one
-// workgroup a CU (2560 columns of 9728, 17 / 48 rows 10.1 / 11.2, four 13.0 / 13.6) and four
-// where they make more (64 rows 13.5, two 17.1).
+// SwiGLU 19.2 / 27.6, two 21.7 / 34.7, eight 21.2 / 30.3), otherwise the fewest of two, three and
+// four that make at most one workgroup a CU (2560 columns of 9728, 17 / 48 rows two 10.1 / 11.2,
+// four 13.0 / 13.6; 64 rows two 17.1, three 12.0, four 13.5).
 template <typename T, int IN, bool SWIGLU, int NV = SWIGLU || IN >= kNorm4 ? 2 : 1>
 int launch_group(const Int4Args& a, int group, hipStream_t s) {
   if (group == 128) return launch_tiles<T, IN, SWIGLU, 128, NV>(a, s);
@@ -465,8 +465,11 @@ int launch_in(const Int4Args& a, int group, hipStream_t s) {
     if (a.rows <= 4) return launch_group<T, kRaw4, SWIGLU>(a, group, s);
     if (a.rows <= 8) return launch_group<T, kRaw8, SWIGLU>(a, group, s);
     if (a.rows <= 16) return launch_group<T, kRaw16, SWIGLU>(a, group, s);
-    const int64_t wgs = (int64_t)((a.rows + 15) / 16) * ((a.cols + kRawPair - 1) / kRawPair);
-    return wgs <= 256 ? launch_group<T, kRaw16, SWIGLU, 2>(a, group, s) : launch_group<T, kRaw16, SWIGLU, 4>(a, group, s);
+    const int tiles = (a.rows + 15) / 16;
+    if (tiles * (int64_t)((a.cols + kRawPair - 1) / kRawPair) <= 256) return launch_group<T, kRaw16, SWIGLU, 2>(a, group, s);
+    if constexpr (!SWIGLU)
+      if (tiles * (int64_t)((a.cols + 47) / 48) <= 256) return launch_group<T, kRaw16, SWIGLU, 3>(a, group, s);
+    return launch_group<T, kRaw16, SWIGLU, 4>(a, group, s);
   }
   if (a.rows <= 4) return launch_group<T, kNorm4, SWIGLU>(a, group, s);
   if (a.rows <= 8) return launch_group<T, kNorm8, SWIGLU>(a, group, s);

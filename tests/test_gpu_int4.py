@@ -59,7 +59,8 @@ def _check(got, x, values, scales, zeros, norm, residual, swiglu):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,cols,k,group", [(1, 16, 128, 128), (3, 1, 32, 32), (16, 40, 576, 64), (17, 33, 160, 32),
-                                               (32, 48, 1152, 128), (33, 17, 2560, 128), (64, 130, 1344, 64), (50, 2100, 160, 32)])
+                                               (32, 48, 1152, 128), (33, 17, 2560, 128), (64, 130, 1344, 64), (50, 2100, 160, 32),
+                                               (50, 4200, 96, 32)])
 def test_int4_linear(device, rows, cols, k, group, dtype):
     say("int4_linear", rows, cols, k, group, dtype)
     g = torch.Generator().manual_seed(rows + cols + k)
