@@ -811,24 +811,23 @@ class RuledLogits(NamedTuple):
     token_ids: torch.Tensor
 
 
-_PER_ROW_RULES = frozenset(("lengths", "prompt_lens", "repetition", "presence", "frequency"))
-_INT_RULES = frozenset(("tokens", "lengths", "prompt_lens", "bias_ids", "allowed"))
+_RULE_KINDS = ((torch.int32, 2), (torch.int32, 1), (torch.int32, 1), (torch.float32, 1), (torch.float32, 1),
+               (torch.float32, 1), (torch.int32, 2), (torch.float32, 2), (torch.int32, 2))  # of LogitRules' fields
 
 
 def _check_rules(rules: LogitRules, rows: int, vocab: int, device: torch.device) -> None:
-    for name, t in zip(LogitRules._fields, rules):
+    for i, (t, (dtype, ndim)) in enumerate(zip(rules, _RULE_KINDS)):
         if t is None:
             continue
-        dtype = torch.int32 if name in _INT_RULES else torch.float32
         shape = t.shape
-        if name in _PER_ROW_RULES:
+        if ndim == 1:
             if t.dtype != dtype or shape != (rows,) or not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous {dtype} [{rows}].")
-        elif t.dtype != dtype or len(shape) != 2 or shape[0] != rows or (shape[1] > 1 and t.stride(1) != 1) \
-                or (rows > 1 and t.stride(0) < shape[1]):
-            raise ValueError(f"{name} must be {dtype} [{rows}, n] with contiguous rows.")
+                raise ValueError(f"{rules._fields[i]} must be contiguous {dtype} [{rows}].")
+        elif t.dtype != dtype or len(shape) != 2 or shape[0] != rows or not t.is_contiguous() and (
+                (shape[1] > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < shape[1])):
+            raise ValueError(f"{rules._fields[i]} must be {dtype} [{rows}, n] with contiguous rows.")
         if t.device != device:
-            raise ValueError(f"{name} must be on the logits' device.")
+            raise ValueError(f"{rules._fields[i]} must be on the logits' device.")
     tokens, lengths, prompt_lens, repetition, presence, frequency, bias_ids, bias_values, allowed = rules
     if (tokens is None) != (lengths is None):
         raise ValueError("tokens and lengths go together.")
