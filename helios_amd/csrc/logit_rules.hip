@@ -20,7 +20,8 @@
 // atomics shows. The workgroups' best keys (value, then smaller index) meet in a second launch.
 //
 // 129 rows of 151936 bf16 logits (78 MB in and out): 22 us without rules, 24 with a mask, 36 with
-// histories of 5217 tokens in the mean too; both launches, as the time of calls one after another.
+// histories of 5217 tokens in the mean too (clearing the tables 3, looking through the tokens 5,
+// the touched logits 7); both launches, as the time of calls one after another.
 
 #include "hx_common.h"
 
