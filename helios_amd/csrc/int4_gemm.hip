@@ -27,8 +27,10 @@
 // 5.5 / 6.0 / 8.0, o 4.0 / 4.5 / 5.3, gate_up 10.2 / 11.1 / 15.0, down 6.6 / 7.4 / 9.4, in all 26 /
 // 29 / 38 where the 16-bit products take 60 / 62 / 71; 17 / 64 rows 47 / 62. gate_up's 26 MB are
 // 2.6 TB/s at one row: about 4 us of each launch are its start, the first loads' way and the
-// merge, as for the 16-bit products; the rest is bound by the address unit (x and W: 104 cycles a
-// block at 8 rows), at 64 rows by x's way from L2 (15 TB/s).
+// merge, as for the 16-bit products; the rest is the stream of W (25 MB at the copy rate: 5.4), with
+// the address unit close behind (x, W and norm weights: 104 cycles a block at 8 rows; 80 with the
+// norm weights loaded once and handed on through LDS take the same time), at 64 rows x's way
+// from L2 (15 TB/s).
 
 #include <type_traits>
 

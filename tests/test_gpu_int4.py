@@ -144,21 +144,26 @@ def test_int4_quantize(device, group, dtype):
     assert (back[3, :group] == 0).all()
 
 
-def test_int4_in_a_graph(device):
-    """Captured once, replayed with new inputs and eager calls between."""
-    say("int4 graph")
+def test_int4_in_two_graphs(device):
+    """Captured into two graphs that share their memory, one with normalised rows that go through
+    a workspace, replayed in turn with new inputs and eager calls between."""
+    say("int4 graphs")
     parts = _weight(64, 1024, 128, torch.bfloat16, seed=9)
     w = _packed(*parts, device)
-    x = torch.randn(5, 1024, device=device).to(torch.bfloat16)
+    x = torch.randn(40, 1024, device=device).to(torch.bfloat16)
     norm = torch.ones(1024, device=device)
     ops.int4_linear(x, w, norm_weight=norm, eps=1e-6)
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        got = ops.int4_linear(x, w, norm_weight=norm, eps=1e-6)
+    graphs, outs = [], []
+    for rows in (5, 40, 33):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            outs.append((ops.int4_linear(x[:rows], w, norm_weight=norm, eps=1e-6), rows))
+        graphs.append(graph)
     for seed in range(3):
-        x.copy_(torch.randn(5, 1024, generator=torch.Generator().manual_seed(seed)))
-        graph.replay()
-        assert torch.equal(got, ops.int4_linear(x, w, norm_weight=norm, eps=1e-6))
+        x.copy_(torch.randn(40, 1024, generator=torch.Generator().manual_seed(seed)))
+        for graph, (got, rows) in zip(graphs, outs):
+            graph.replay()
+            assert torch.equal(got, ops.int4_linear(x[:rows], w, norm_weight=norm, eps=1e-6))
 
 
 def test_int4_of_no_rows_and_on_a_side_stream(device):
