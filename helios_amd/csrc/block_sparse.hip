@@ -15,6 +15,9 @@
 
 namespace {
 
+// Work-items of a launch: a 32-bit number.
+constexpr int64_t kMostItems = 0xffffffff;
+
 // HIP's min and max go through double for some mixes of 64-bit types.
 template <typename I>
 __device__ __forceinline__ I least_of(I a, I b) { return b < a ? b : a; }
@@ -918,7 +921,7 @@ extern "C" int hx_kv_block_bounds(const void* k_pool, void* bounds, int32_t num_
   a.chunks = (a.pieces + kBdPieces - 1) / kBdPieces;
   a.inf = dtype == HX_DTYPE_BF16 ? 0x7f80 : 0x7c00;
   const int64_t wgs = (int64_t)batch * a.groups * a.chunks;
-  if (wgs > 0x7fffffff) return HX_E_UNSUPPORTED;
+  if (wgs > kMostItems / kBdThreads) return HX_E_UNSUPPORTED;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(block_bounds_kernel, dim3((unsigned)wgs), dim3(kBdThreads), 0, s, a);
   return hx::status_from_hip(hipGetLastError());
@@ -942,7 +945,9 @@ extern "C" int hx_select_blocks(const void* q, int64_t q_row_stride, int64_t q_h
       (int64_t)sink + recent > budget)
     return HX_E_INVALID_ARG;
   const int64_t most = (int64_t)block_table_width * (page_size / block_size);
-  if (most > kSelMaxBlocks || page_size / block_size > (1 << 16) || n > 0x7fffffff / n_kv_heads / (most + 1)) return HX_E_UNSUPPORTED;
+  if (most > kSelMaxBlocks || page_size / block_size > (1 << 16) || n > 0x7fffffff / n_kv_heads / (most + 1) ||
+      n > kMostItems / 1024 / n_kv_heads)
+    return HX_E_UNSUPPORTED;
   if (n == 0) return HX_OK;
   if (!q || !key_counts || !bounds || !block_table || !blocks ||
       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(bounds)) & 15) || q_row_stride % 8 ||
@@ -1057,7 +1062,7 @@ extern "C" int hx_block_sparse_attn(const void* q, int64_t q_row_stride, int64_t
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + parts * head_dim;
   }
-  if ((double)n * n_q_heads * a.splits > 2147483647.0) return HX_E_UNSUPPORTED;
+  if ((double)n * n_q_heads * a.splits > kMostItems / (64 * kSpWaves)) return HX_E_UNSUPPORTED;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == HX_DTYPE_BF16) launch_sparse_dims<__bf16>(a, n, s);
   else launch_sparse_dims<_Float16>(a, n, s);

@@ -558,7 +558,7 @@ extern "C" int hx_int4_dequantize(const void* packed, const void* steps, int32_t
   a.out = static_cast<uint16_t*>(out);
   a.out_row = out_row_stride;
   const int64_t units = ((int64_t)weight_rows + 15) / 16 * a.blocks * 64;
-  if ((units + 255) / 256 > 0x7fffffff) return HX_E_UNSUPPORTED;
+  if (units > 0xffffff00ll) return HX_E_UNSUPPORTED;  // work-items of a launch: 32 bits
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)((units + 255) / 256));
   if (dtype == HX_DTYPE_BF16) hipLaunchKernelGGL(int4_dequant_kernel<__bf16>, grid, dim3(256), 0, s, a, units);

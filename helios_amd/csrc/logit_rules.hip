@@ -413,7 +413,7 @@ extern "C" int hx_logit_rules(const void* logits, int64_t logits_row_stride, int
   a.allowed = allowed;
   a.allowed_stride = allowed_row_stride;
   a.keys = static_cast<uint64_t*>(workspace);
-  if (rows * a.slices > 0x7fffffff) return HX_E_UNSUPPORTED;
+  if (rows > 0xffffffffll / kLrThreads / a.slices) return HX_E_UNSUPPORTED;  // work-items of a launch: 32 bits
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == HX_DTYPE_FP32) launch_rules<float>(a, rows, s);
   else if (dtype == HX_DTYPE_BF16) launch_rules<__bf16>(a, rows, s);

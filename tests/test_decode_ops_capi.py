@@ -41,7 +41,8 @@ DEQUANT = dict(packed=P, steps=P, rows=20, k=256, group=64, dtype=0, out=P, out_
 
 @pytest.mark.parametrize("change,code", [
     (dict(dtype=7), NO), (dict(group=0), NO), (dict(rows=0), BAD), (dict(k=100), BAD), (dict(out=None), BAD),
-    (dict(out=P + 8), BAD), (dict(out_row=248), BAD), (dict(out_row=260), BAD), (dict(packed=P + 4), BAD)])
+    (dict(out=P + 8), BAD), (dict(out_row=248), BAD), (dict(out_row=260), BAD), (dict(packed=P + 4), BAD),
+    (dict(rows=1 << 30, k=4096, out_row=4096), NO)])
 def test_int4_dequantize(change, code):
     assert _call("hx_int4_dequantize", DEQUANT, **change) == code
 
@@ -57,7 +58,7 @@ RULES = dict(logits=P, row=64, rows=2, vocab=64, dtype=0, tokens=P, token_row=8,
     (dict(bias_values=None), BAD), (dict(bias_row=3), BAD), (dict(n_bias=-1), BAD), (dict(allowed_row=1), BAD),
     (dict(ws=None), WS), (dict(ws=P + 4), WS), (dict(ws_bytes=15), WS), (dict(rows=0), 0),
     (dict(logits=P + 1), BAD), (dict(dtype=2, out=P + 2), BAD),
-    (dict(rows=1 << 31, ws_bytes=1 << 40), NO)])
+    (dict(rows=1 << 31, ws_bytes=1 << 40), NO), (dict(rows=1 << 23, ws_bytes=1 << 40), NO)])
 def test_logit_rules(change, code):
     assert _call("hx_logit_rules", RULES, **change) == code
 
@@ -70,7 +71,7 @@ BOUNDS = dict(k=P, bounds=P, pages=4, page=256, block=64, heads=8, dim=128, dtyp
     (dict(dtype=2), NO), (dict(block=48), NO), (dict(block=8), NO), (dict(block=512), NO), (dict(dim=100), NO),
     (dict(dim=264), NO), (dict(pages=0), BAD), (dict(heads=0), BAD), (dict(k=None), BAD), (dict(bounds=P + 8), BAD),
     (dict(stride=3), BAD), (dict(width=0), BAD), (dict(cu=None), BAD), (dict(batch=-1), BAD), (dict(max_q=-1), BAD),
-    (dict(batch=0), 0), (dict(max_q=0), 0)])
+    (dict(batch=1 << 23), NO), (dict(batch=0), 0), (dict(max_q=0), 0)])
 def test_kv_block_bounds(change, code):
     assert _call("hx_kv_block_bounds", BOUNDS, **change) == code
 
@@ -86,7 +87,8 @@ SELECT = dict(q=P, q_row=4096, q_head=128, q_rows=2, rows=None, row_seq=None, ke
     (dict(dtype=2), NO), (dict(block=24), NO), (dict(hq=30), BAD), (dict(budget=0), BAD), (dict(sink=-1), BAD),
     (dict(recent=0), BAD), (dict(sink=7, recent=2), BAD), (dict(sink=2 ** 31 - 1, recent=2 ** 31 - 1), BAD),
     (dict(width=4097, stride=4097), NO), (dict(n=3), BAD), (dict(n=-1), BAD), (dict(q=None), BAD),
-    (dict(bounds=P + 4), BAD), (dict(blocks=None), BAD), (dict(batch=1), BAD), (dict(n=0), 0)])
+    (dict(bounds=P + 4), BAD), (dict(blocks=None), BAD), (dict(batch=1), BAD), (dict(n=0), 0),
+    (dict(n=1 << 20, q_rows=1 << 20, batch=1 << 20, ws_bytes=1 << 40), NO)])
 def test_select_blocks(change, code):
     assert _call("hx_select_blocks", SELECT, **change) == code
 
@@ -101,7 +103,8 @@ SPARSE = dict(q=P, q_row=4096, q_head=128, q_rows=2, rows=None, row_seq=None, ke
     (dict(n=3), BAD), (dict(batch=1), BAD), (dict(k=None), BAD), (dict(v=P + 2), BAD), (dict(q=P + 8), BAD),
     (dict(q_row=4092), BAD), (dict(q_head=132), BAD), (dict(out=P + 2), BAD), (dict(out_row=4097), BAD),
     (dict(blocks=None), BAD), (dict(ws=None), WS), (dict(ws=P + 8), WS), (dict(ws_bytes=64), WS), (dict(n=0), 0),
-    (dict(hkv=1 << 18, hq=1 << 18), NO), (dict(budget=(1 << 24) + 1), BAD)])
+    (dict(hkv=1 << 18, hq=1 << 18), NO), (dict(budget=(1 << 24) + 1), BAD),
+    (dict(n=1 << 20, q_rows=1 << 20, batch=1 << 20, ws_bytes=1 << 60), NO)])
 def test_block_sparse_attn(change, code):
     assert _call("hx_block_sparse_attn", SPARSE, **change) == code
 
