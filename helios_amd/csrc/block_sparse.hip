@@ -6,7 +6,8 @@
 //   lower[d] = min_j k_j[d],  upper[d] = max_j k_j[d]           (block_bounds_kernel)
 // bound the scores of its keys: q . k_j <= sum_d max(q[d] lower[d], q[d] upper[d]). Summed over
 // the G query heads that share the KV head the bound is linear in two vectors,
-//   s = sum_d (sum_g min(q_g[d], 0)) lower[d] + (sum_g max(q_g[d], 0)) upper[d],
+//   s = sum_d (sum_g min(q_g[d], 0)) lower[d] + (sum_g max(q_g[d], 0)) upper[d]
+// (an infinite bound whose vector is 0 there left out: no query takes it),
 // and the blocks with the largest s, with the first `sink` and the last `recent` ones, are the
 // row's selection for that KV head (block_scores_kernel, select_blocks_kernel). The attention is
 // the softmax over the keys of those blocks alone (sparse_attn_kernel).
@@ -169,7 +170,7 @@ struct SelectArgs {
 constexpr uint64_t kKeyTaken = 0, kKeyLast = 1;
 
 __device__ __forceinline__ uint64_t ordered_key(double s) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, s + 0.0);  // -0 like 0
+  const uint64_t u = hx::raw_bits(s + 0.0);  // -0 like 0
   if ((u & 0x7fffffffffffffffull) > 0x7ff0000000000000ull) return 0xfff0000000000000ull;  // NaN like +inf
   return (u >> 63) ? ~u : u | 0x8000000000000000ull;
 }
@@ -200,6 +201,10 @@ __device__ __forceinline__ double lanes_sum(double v) {
   return v;
 }
 
+// Bits of the type's infinity.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t inf_bits() { return __is_same(T, __bf16) ? 0x7f80u : 0x7c00u; }
+
 // A workgroup takes a stretch of a row's blocks for one KV head, kGroups x kScPer at a time.
 template <typename T, int LANES>
 __global__ __launch_bounds__(kScThreads) void block_scores_kernel(SelectArgs a) {
@@ -221,15 +226,16 @@ __global__ __launch_bounds__(kScThreads) void block_scores_kernel(SelectArgs a) 
   const uint16_t* const bounds = a.bounds + h * 2 * a.head_dim + d;
   uint4 low[kScPer], high[kScPer];
   uint32_t bad = 0;
+  auto page_of = [&](int at, int& in_page) __attribute__((always_inline)) {
+    const uint32_t j = min(at, count - 1);
+    const uint32_t k = per_page == 1 ? j : (uint32_t)((uint64_t)j * a.page_magic >> 32);  // j / per_page
+    in_page = j - k * per_page;
+    return table[k];
+  };
   auto load = [&](int j0) __attribute__((always_inline)) {
     int page[kScPer], in_page[kScPer];
 #pragma unroll
-    for (int p = 0; p < kScPer; ++p) {
-      const uint32_t j = min(j0 + g + p * kGroups, count - 1);
-      const uint32_t k = per_page == 1 ? j : (uint32_t)((uint64_t)j * a.page_magic >> 32);  // j / per_page
-      in_page[p] = j - k * per_page;
-      page[p] = table[k];
-    }
+    for (int p = 0; p < kScPer; ++p) page[p] = page_of(j0 + g + p * kGroups, in_page[p]);
     bad = 0;
 #pragma unroll
     for (int p = 0; p < kScPer; ++p) {
@@ -263,6 +269,10 @@ __global__ __launch_bounds__(kScThreads) void block_scores_kernel(SelectArgs a) 
     pos[e] = dims ? v.y : 0.0;
   }
   uint64_t* const order = a.order + ih * a.most;
+  auto key_at = [&](int j, bool off, double s) __attribute__((always_inline)) {
+    return j < a.sink || j >= count - a.recent ? kKeyTaken : off ? kKeyLast : ordered_key(s);
+  };
+  uint32_t most = 0;  // of the upper halves of the sums' magnitudes
   for (int j0 = begin;;) {
     double s[kScPer];
 #pragma unroll
@@ -282,12 +292,40 @@ __global__ __launch_bounds__(kScThreads) void block_scores_kernel(SelectArgs a) 
 #pragma unroll
     for (int p = 0; p < kScPer; ++p) {
       s[p] = lanes_sum<LANES>(s[p]);
+      most = max(most, (uint32_t)(hx::raw_bits(s[p]) >> 32) & 0x7fffffffu);
       const int j = j0 + g + p * kGroups;
-      if (li == 0 && j < end)
-        order[j] = j < a.sink || j >= count - a.recent ? kKeyTaken : was_bad >> p & 1 ? kKeyLast : ordered_key(s[p]);
+      if (li == 0 && j < end) order[j] = key_at(j, was_bad >> p & 1, s[p]);
     }
-    if (j1 >= end) return;
+    if (j1 >= end) break;
     j0 = j1;
+  }
+  // Of a wave with an infinite or NaN sum, all again: 0 * inf is a NaN in the two products of a
+  // dim, but not in max(q lower, q upper) unless a query is 0 itself. An infinite bound with a
+  // weight of 0 and no such query is left out.
+  if (__builtin_amdgcn_ballot_w64(most >= 0x7ff00000u) == 0) return;
+  uint32_t zero = 0;  // dims in which a query is 0
+  if (dims)
+    for (int k = 0; k < a.group; ++k)
+      for (int e = 0; e < 8; ++e)
+        zero |= (a.q[row * a.q_row + (int64_t)(h * a.group + k) * a.q_head + d + e] & 0x7fffu) == 0 ? 1u << e : 0u;
+  for (int j = begin + g; j - g < end; j += kGroups) {  // as many rounds for every group of lanes
+    int in_page;
+    const int page = page_of(j, in_page);
+    const bool off = page < 0 || page >= a.num_pages;
+    double s = 0.0;
+    if (!off && dims) {
+      const uint16_t* at = bounds + ((int64_t)page * per_page + in_page) * block_elems;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t lo = at[e], hi = at[a.head_dim + e], keep = zero >> e & 1;
+        const bool no_lo = !keep && (lo & 0x7fffu) == inf_bits<T>() && hx::raw_bits(neg[e]) << 1 == 0;
+        const bool no_hi = !keep && (hi & 0x7fffu) == inf_bits<T>() && hx::raw_bits(pos[e]) << 1 == 0;
+        s = fma((double)E::lo(no_lo ? 0 : lo), neg[e], s);
+        s = fma((double)E::lo(no_hi ? 0 : hi), pos[e], s);
+      }
+    }
+    s = lanes_sum<LANES>(s);
+    if (li == 0 && j < end) order[j] = key_at(j, off, s);
   }
 }
 

@@ -119,6 +119,15 @@ __device__ __forceinline__ uint32_t swiglu2(uint32_t g, uint32_t u) {
                             __fmul_rn(Elem<T>::hi(s), Elem<T>::hi(u)));
 }
 
+// The bits of a value that may be a NaN. The build assumes that no operand of a comparison is
+// one, and turns comparisons of a float's bits into those of the float; behind an empty asm
+// the compiler does not know that these are one's.
+__device__ __forceinline__ uint64_t raw_bits(double x) {
+  uint64_t b = __builtin_bit_cast(uint64_t, x);
+  asm("" : "+v"(b));
+  return b;
+}
+
 // Eight packed 1.0 values of element type T.
 template <typename T>
 __device__ __forceinline__ uint4 ones8();
