@@ -546,10 +546,14 @@ void launch_select(const SelectArgs& a, int64_t n, hipStream_t s) {
 // holds behind its last key never reaches the sums.
 //
 // S^T = K Q^T has the query heads as its columns, twice: of each key's weight p, columns 0-7
-// carry the leading bits of the element type into P V and columns 8-15 the remainder, so one
-// MFMA sums both, and P has 16 (fp16: 22) bits. S^T's registers are the P operand as they are.
-// bf16 weights are scaled down by 2^24, which their range has room for: values up to the
-// type's largest then cannot leave fp32 in the sums over a list's keys.
+// carry its rounding to the element type into P V and columns 8-15 that of the remainder, so one
+// MFMA sums both. S^T's registers are the P operand as they are. Two fp16 hold 23 bits of p, less
+// than exp2's error; bf16 takes a third part, in columns 8-15 of a second MFMA, and holds all 24.
+// (Two bf16 parts showed where values cancel: two keys with weights 2^-13 apart came out up to 6 %
+// off. The third takes 0.15 us of one row's 9.1, and nothing of 64 rows' 181.)
+// Weights are scaled by a power of two: bf16's by 2^-24, so that values up to the type's largest
+// cannot leave fp32 in the sums over a list's keys, fp16's by 2^14, so that small ones keep
+// their bits (unscaled, those below 2^-25 were lost: 940 of e^-18 are 1.4e-5 of a sum).
 //
 // 32/8 heads of 128, blocks of 64: 64 rows of 4096 keys (1.07 GB) 175 us, 6.1 TB/s, what this
 // card reads at most; one row of 2048 keys (8.4 MB) 6.9 us and 3.4 for the join of its 16 splits,
@@ -590,19 +594,9 @@ __device__ __forceinline__ int sp_piece(int r, int p) {
   return DP == 64 ? p ^ ((r >> 1) & 7) : p ^ (r & 15);
 }
 
-// The leading bits of p >= 0 in the element type, rounded down.
+// By which the weights are scaled.
 template <typename T>
-__device__ __forceinline__ float leading(float p);
-template <>
-__device__ __forceinline__ float leading<__bf16>(float p) { return __uint_as_float(__float_as_uint(p) & 0xffff0000u); }
-template <>
-__device__ __forceinline__ float leading<_Float16>(float p) {
-  return (float)__builtin_amdgcn_cvt_pkrtz(p, 0.f)[0];
-}
-
-// Powers of two by which the weights are scaled down (fp16 values never sum beyond fp32).
-template <typename T>
-__device__ __forceinline__ constexpr float weight_bias() { return __is_same(T, __bf16) ? 24.f : 0.f; }
+__device__ __forceinline__ constexpr float weight_scale() { return __is_same(T, __bf16) ? 0x1p-24f : 0x1p14f; }
 
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a) {
@@ -748,26 +742,28 @@ __global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a
       }
     mx = hx::max_xor32(hx::max_xor16(mx));
     const float alpha = mx == -INFINITY ? 1.f : hx::fast_exp2(m_run - mx);
-    const float neg = mx == -INFINITY ? 0.f : -mx - weight_bias<T>();
+    const float neg = mx == -INFINITY ? 0.f : -mx;
     m_run = mx;
     l_run *= alpha;
 #pragma unroll
     for (int d = 0; d < kDims; ++d) o[d] *= alpha;
-    uint32_t pw[4];
+    uint32_t pw[4], pl[4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      float x[4];
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p = hx::fast_exp2(sc[u][e] + neg);
-        l_run += p;
-        const float top = leading<T>(p);
-        x[e] = lr < 8 ? top : p - top;
+      for (int e = 0; e < 4; e += 2) {
+        const float p0 = hx::fast_exp2(sc[u][e] + neg) * weight_scale<T>();
+        const float p1 = hx::fast_exp2(sc[u][e + 1] + neg) * weight_scale<T>();
+        l_run += p0;
+        l_run += p1;
+        const uint32_t top = hx::pack2_round<T>(p0, p1);
+        const float r0 = p0 - E::lo(top), r1 = p1 - E::hi(top);
+        const uint32_t rest = hx::pack2_round<T>(r0, r1);
+        pw[2 * u + e / 2] = lr < 8 ? top : rest;
+        pl[2 * u + e / 2] = lr < 8 ? 0u : hx::pack2_round<T>(r0 - E::lo(rest), r1 - E::hi(rest));
       }
-      pw[2 * u] = hx::pack2_round<T>(x[0], x[1]);
-      pw[2 * u + 1] = hx::pack2_round<T>(x[2], x[3]);
-    }
     const v8 pf = hx::as_v8<T>(make_uint4(pw[0], pw[1], pw[2], pw[3]));
+    const v8 pf2 = hx::as_v8<T>(make_uint4(pl[0], pl[1], pl[2], pl[3]));
 #pragma unroll
     for (int d = 0; d < kDims; ++d) {
       uint2 f[2];
@@ -776,12 +772,14 @@ __global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a
         const int r = 16 * u + 4 * lg + (lr >> 2);
         f[u] = hx::ld8_lds_tr16(vt + r * kRowBytes + 16 * sp_piece<DP>(r, 2 * d + ((lr & 3) >> 1)) + 8 * (lr & 1));
       }
-      o[d] = E::mfma16x16x32(hx::as_v8<T>(make_uint4(f[0].x, f[0].y, f[1].x, f[1].y)), pf, o[d]);
+      const v8 vf = hx::as_v8<T>(make_uint4(f[0].x, f[0].y, f[1].x, f[1].y));
+      o[d] = E::mfma16x16x32(vf, pf, o[d]);
+      if constexpr (__is_same(T, __bf16)) o[d] = E::mfma16x16x32(vf, pf2, o[d]);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 
-  // Lane: dims 16 d + 4 lg .. + 3 of head lr % 8; both halves of P summed.
+  // Lane: dims 16 d + 4 lg .. + 3 of head lr % 8; the parts of P summed.
   l_run = hx::add_xor32(hx::add_xor16(l_run));
 #pragma unroll
   for (int d = 0; d < kDims; ++d)

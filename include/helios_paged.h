@@ -627,7 +627,7 @@ int hx_int4_dequantize(const void* packed, const void* steps, int32_t weight_row
  * aligned; calls that share one must be ordered.
  *
  * hx_block_sparse_attn: out[rows[i]][h] = softmax(scale q . k) V over the keys of blocks[i]
- * [h / group] below key_counts[i], in fp32 with weights of 16 (fp16: 22) bits, rounded once.
+ * [h / group] below key_counts[i], in fp32 (weights and sums), rounded once.
  * Entries of a list that are negative, past the keys or on a page outside the pool are
  * skipped; a block listed twice counts twice. Without any key the row is zeros. Entries whose
  * row is outside [0, q_rows) are skipped, and rows not listed are left as they were; a row

@@ -1,4 +1,5 @@
-"""Selection and attention over selected blocks where bounds, keys or values are infinite or NaN."""
+"""Selection and attention over selected blocks where bounds, keys or values are infinite or NaN,
+and the bits of the attention's weights."""
 
 from __future__ import annotations
 
@@ -62,3 +63,62 @@ def test_selection_by_bounds_with_one_infinity(device, rows, hq, heads, d, count
         want = torch.tensor([[oracle.select(s, count, budget, 1, 1) for s in row] for row in scores], dtype=torch.int32)
         got = ops.select_blocks(*args, keys, budget, block_size=16, sink=1, recent=1)
         assert torch.equal(got.cpu(), want), budget
+
+
+def _pool(ends, heads, d, dtype, seed):
+    """K and V pools [pages, 256, heads, d] and a page table; NaN behind the last keys."""
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-n // 256) for n in ends]
+    k, v = (torch.full((sum(need), 256, heads, d), NAN) for _ in range(2))
+    order = torch.randperm(sum(need), generator=g).tolist()
+    table = torch.zeros(len(ends), max(need), dtype=torch.int32)
+    for b, n in enumerate(ends):
+        for j in range(need[b]):
+            p, fill = order.pop(), min(256, n - 256 * j)
+            table[b, j] = p
+            k[p, :fill] = torch.randn(fill, heads, d, generator=g)
+            v[p, :fill] = torch.randn(fill, heads, d, generator=g)
+    return k.to(dtype), v.to(dtype), table
+
+
+def _attend(device, q, k, v, table, ends, block, budget, scale):
+    """The kernel's result (double, on the host) and the definition's, over all blocks."""
+    blocks = torch.arange(budget, dtype=torch.int32).view(1, 1, -1).repeat(len(ends), k.shape[2], 1)
+    got = ops.block_sparse_attn(*(t.to(device) for t in (q, k, v, blocks, table)),
+                                torch.tensor(ends, dtype=torch.int32, device=device), block_size=block, scale=scale)
+    ref = oracle.sparse_attention(q, k, v, blocks, table, ends, range(len(ends)), block, scale)
+    return got.double().cpu(), ref
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weights_keep_24_bits(device, dtype):
+    """Two keys whose weights 1 and 1 - 2^-13 .. 1 - 2^-12 nearly cancel in V. Scores are exact
+    in fp32 but for a rounding of 2^-24 of at most 2^-4; exp2 is within 2^-23 of a weight, the
+    sums and the quotient within 2^-23 of 1 each: 2^-21 in all beside the output's own half
+    step, which is 2^-21 at most. Weights of 16 bits are off by up to 2^-18."""
+    say("sparse 24 bits", dtype)
+    k, v = torch.zeros(1, 256, 1, 32), torch.zeros(1, 256, 1, 32)
+    k[0, 0, 0, 0], k[0, 1, 0, 0] = 1, 1 + 2.0 ** -7
+    v[0, 0], v[0, 1] = -1, 1
+    q = torch.zeros(16, 8, 32)
+    q[..., 0] = (2.0 ** -6 * (1 + torch.arange(128) / 128)).view(16, 8)
+    got, ref = _attend(device, q.to(dtype), k.to(dtype), v.to(dtype), torch.zeros(16, 1, dtype=torch.int32), [2] * 16,
+                       16, 1, 1.0)
+    off = torch.finfo(dtype).eps / 2 * ref.abs() * (1 + 2.0 ** -7) + 2.0 ** -21
+    assert ((got - ref).abs() <= off).all(), ((got - ref).abs() / off).max()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_small_weights(device, dtype):
+    """A key of weight 1 and V = 0 in every unit of 16, the others' weights e^-18 and V = 1024:
+    all of the result comes from weights of 2^-26. Their exponent 25.97 is rounded to 2^-20,
+    exp2 and up to 1000 sums in fp32 to 2^-23 + 1000 * 2^-24: within 2^-13 of the result."""
+    say("sparse small weights", dtype)
+    k, v = torch.full((4, 256, 1, 32), 0.0), torch.full((4, 256, 1, 32), 1024.0)
+    k[..., 0] = -18
+    k[:, ::16, 0, 0], v[:, ::16] = 0, 0
+    q = torch.zeros(3, 2, 32)
+    q[..., 0] = 1
+    got, ref = _attend(device, q.to(dtype), k.to(dtype), v.to(dtype), torch.arange(4, dtype=torch.int32).repeat(3, 1),
+                       [1000, 1024, 100], 64, 16, 1.0)
+    assert ((got - ref).abs() <= (torch.finfo(dtype).eps / 2 + 2.0 ** -13) * ref.abs()).all()
