@@ -781,10 +781,45 @@ __global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a
 
   // Lane: dims 16 d + 4 lg .. + 3 of head lr % 8; the parts of P summed.
   l_run = hx::add_xor32(hx::add_xor16(l_run));
+  float all = 0.f;
 #pragma unroll
   for (int d = 0; d < kDims; ++d)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[d][e] += hx::dpp<0x128>(o[d][e]);  // the lane 8 apart in its row of 16
+    for (int e = 0; e < 4; ++e) {
+      o[d][e] += hx::dpp<0x128>(o[d][e]);  // the lane 8 apart in its row of 16
+      all += o[d][e];
+    }
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(!hx::is_finite(all)) != 0, 0)) {
+    // An infinite or NaN sum. The parts of P made NaN of an infinite V too (0 * inf): what the
+    // wave's keys have in each dim is looked up again, and is the dim's result at any weight.
+    uint32_t has = 0;  // +inf, -inf, NaN: a bit for each of the piece's dims
+    for (int t = next(w); t < tiles; t = next(t + kSpWaves)) {
+      load(t);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q) {
+          const uint32_t wd[4] = {vb[u][q].x, vb[u][q].y, vb[u][q].z, vb[u][q].w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t x = wd[e / 2] >> (16 * (e % 2)) & 0xffffu, mag = x & 0x7fffu;
+            const uint32_t at = mag > inf_bits<T>() ? 16 : x >> 15 ? 8 : 0;
+            has |= mag >= inf_bits<T>() ? 1u << (at + e) : 0u;
+          }
+        }
+    }
+    for (int m = kPieces; m < 64; m <<= 1) has |= __shfl_xor(has, m);
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) {
+      const uint32_t of = __shfl(has, 2 * d + (lg >> 1)) >> (4 * (lg & 1));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool up = of >> e & 1, down = of >> (8 + e) & 1, nan = of >> (16 + e) & 1;
+        if (up || down || nan)
+          o[d][e] = __uint_as_float(nan || (up && down) ? 0x7fc00000u : up ? 0x7f800000u : 0xff800000u);
+      }
+    }
+  }
   __syncthreads();  // every wave is done with its stage
   float (*const s_o)[kSpHeads][DP] = reinterpret_cast<float (*)[kSpHeads][DP]>(smem);
   if (lr < kSpHeads) {
@@ -811,6 +846,14 @@ __global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a
       l = fmaf(f, s_l[ww][hd], l);
       x = fmaf(f, s_o[ww][hd][d], x);
       y = fmaf(f, s_o[ww][hd][d + 1], y);
+    }
+    if (__builtin_expect(!hx::is_finite(x + y), 0)) {  // an infinite part counts at any weight, 0 too
+      x = y = 0.f;
+      for (int ww = 0; ww < kSpWaves; ++ww) {
+        const float f = hx::fast_exp2(s_m[ww][hd] - ref);
+        x = hx::add_weighed<true>(f, s_o[ww][hd][d], x);
+        y = hx::add_weighed<true>(f, s_o[ww][hd][d + 1], y);
+      }
     }
     const int64_t head = head0 + hd;
     if (a.splits == 1) {
@@ -878,6 +921,16 @@ __global__ __launch_bounds__(64) void sparse_combine_kernel(SparseArgs a) {
     l += hx::dpp<hx::kDppHalfMirror>(l);
     l += hx::dpp<hx::kDppMirror>(l);
     l = hx::add_xor32(hx::add_xor16(l));
+    if (__builtin_expect(!hx::is_finite(x + y), 0)) {
+      // An infinite part counts at any weight, 0 too. (In the loop above this took 0.3 us of 3.)
+      x = y = 0.f;
+      for (int at = 0; at < a.splits; ++at) {
+        const float2 part = *reinterpret_cast<const float2*>(sums + (int64_t)at * a.head_dim + from);
+        const float f = hx::fast_exp2(ml[at].x - ref);
+        x = hx::add_weighed<true>(f, part.x, x);
+        y = hx::add_weighed<true>(f, part.y, y);
+      }
+    }
     const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
     if (d < a.head_dim)
       *reinterpret_cast<uint32_t*>(a.out + row * a.out_row + head * a.out_head + d) = hx::pack2_round<T>(x * inv, y * inv);

@@ -122,10 +122,25 @@ __device__ __forceinline__ uint32_t swiglu2(uint32_t g, uint32_t u) {
 // The bits of a value that may be a NaN. The build assumes that no operand of a comparison is
 // one, and turns comparisons of a float's bits into those of the float; behind an empty asm
 // the compiler does not know that these are one's.
+__device__ __forceinline__ uint32_t raw_bits(float x) {
+  uint32_t b = __float_as_uint(x);
+  asm("" : "+v"(b));
+  return b;
+}
 __device__ __forceinline__ uint64_t raw_bits(double x) {
   uint64_t b = __builtin_bit_cast(uint64_t, x);
   asm("" : "+v"(b));
   return b;
+}
+
+__device__ __forceinline__ bool is_inf(float x) { return (raw_bits(x) & 0x7fffffffu) == 0x7f800000u; }
+__device__ __forceinline__ bool is_finite(float x) { return (raw_bits(x) & 0x7fffffffu) < 0x7f800000u; }
+
+// x + w * y for partial results. With ODD an infinite y counts however small its weight: the
+// sum over the whole row would have it so.
+template <bool ODD>
+__device__ __forceinline__ float add_weighed(float w, float y, float x) {
+  return ODD && is_inf(y) ? x + y : fmaf(w, y, x);
 }
 
 // Eight packed 1.0 values of element type T.

@@ -2280,24 +2280,6 @@ struct WideLds {
   int odd[4];  // per wave: whether a sum of its is infinite or NaN
 };
 
-// The bits of a value that may be a NaN. The build assumes that no operand of a comparison is
-// one, and turns comparisons of a float's bits into those of the float; behind an empty asm
-// the compiler does not know that these are one's.
-__device__ __forceinline__ uint32_t raw_bits(float x) {
-  uint32_t b = __float_as_uint(x);
-  asm("" : "+v"(b));
-  return b;
-}
-__device__ __forceinline__ bool is_inf(float x) { return (raw_bits(x) & 0x7fffffffu) == 0x7f800000u; }
-__device__ __forceinline__ bool is_finite(float x) { return (raw_bits(x) & 0x7fffffffu) < 0x7f800000u; }
-
-// x + w * y for partial results. With ODD an infinite y counts however small its weight: the
-// sum over the whole row would have it so.
-template <bool ODD>
-__device__ __forceinline__ float add_weighed(float w, float y, float x) {
-  return ODD && is_inf(y) ? x + y : fmaf(w, y, x);
-}
-
 // Result (acc / l, four dims from d0) of one unit: output row piece, or partial.
 template <typename T>
 __device__ __forceinline__ void wide_store(const RunArgs& a, const WideShape& ws, const WideItem& it, int row, int head,
@@ -2334,10 +2316,10 @@ __device__ __forceinline__ void wide_merge_waves(const RunArgs& a, const WideSha
       const float alpha = mw == -INFINITY ? 0.f : hx::fast_exp2(mw - mm);
       const float4 o4 = *reinterpret_cast<const float4*>(&lds.o[ww][h][d0]);
       ll = fmaf(alpha, lds.l[ww][h], ll);
-      x[0] = add_weighed<ODD>(alpha, o4.x, x[0]);
-      x[1] = add_weighed<ODD>(alpha, o4.y, x[1]);
-      x[2] = add_weighed<ODD>(alpha, o4.z, x[2]);
-      x[3] = add_weighed<ODD>(alpha, o4.w, x[3]);
+      x[0] = hx::add_weighed<ODD>(alpha, o4.x, x[0]);
+      x[1] = hx::add_weighed<ODD>(alpha, o4.y, x[1]);
+      x[2] = hx::add_weighed<ODD>(alpha, o4.z, x[2]);
+      x[3] = hx::add_weighed<ODD>(alpha, o4.w, x[3]);
     }
     wide_store<T>(a, ws, it, 0, g * ws.group + it.h0 + h, d0, mm, ll, x);
   }
@@ -2404,7 +2386,7 @@ __device__ __forceinline__ void wide_odd_item(const RunArgs& a, const WideShape&
       s *= a.scale_log2;
       const float mt = seen ? fmaxf(m, s) : m;
       // A NaN score makes its row NaN (it is no maximum, also where it is the first).
-      const bool counts = seen && raw_bits(s) != 0xff800000u;
+      const bool counts = seen && hx::raw_bits(s) != 0xff800000u;
       const float p = counts ? hx::fast_exp2(s + (wide_p_shift<T>() - (mt != -INFINITY ? mt : 0.f))) : 0.f;
       const float alpha = m != -INFINITY ? hx::fast_exp2(m - mt) : 0.f;
       m = mt;
@@ -2638,7 +2620,7 @@ __device__ __forceinline__ bool wide_item(const RunArgs& a, const WideShape& ws,
 #pragma unroll
     for (int db = 0; db < NO; ++db)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = max(top, raw_bits(oacc[db][i]) & 0x7fffffffu);
+      for (int i = 0; i < 4; ++i) top = max(top, hx::raw_bits(oacc[db][i]) & 0x7fffffffu);
     const int odd = __any(top >= 0x7f800000u);
     if (lane == 0) lds.odd[w] = odd;
     __syncthreads();
@@ -2829,16 +2811,16 @@ __global__ __launch_bounds__(kWideThreads) void wide_combine_kernel(RunArgs a, W
         }
         m = mn;
       }
-      if (!(is_finite(x[0]) && is_finite(x[1]) && is_finite(x[2]) && is_finite(x[3]))) {
+      if (!(hx::is_finite(x[0]) && hx::is_finite(x[1]) && hx::is_finite(x[2]) && hx::is_finite(x[3]))) {
         x[0] = x[1] = x[2] = x[3] = 0.f;
         for (int sp = 0; sp < splits; ++sp) {
           const float ms = a.part_ml[base + (int64_t)sp * a.hq].x;
           const float wt = ms != -INFINITY ? hx::fast_exp2(ms - m) : 0.f;
           const float4 o4 = *reinterpret_cast<const float4*>(part_o + (base + (int64_t)sp * a.hq) * D + d0);
-          x[0] = add_weighed<true>(wt, o4.x, x[0]);
-          x[1] = add_weighed<true>(wt, o4.y, x[1]);
-          x[2] = add_weighed<true>(wt, o4.z, x[2]);
-          x[3] = add_weighed<true>(wt, o4.w, x[3]);
+          x[0] = hx::add_weighed<true>(wt, o4.x, x[0]);
+          x[1] = hx::add_weighed<true>(wt, o4.y, x[1]);
+          x[2] = hx::add_weighed<true>(wt, o4.z, x[2]);
+          x[3] = hx::add_weighed<true>(wt, o4.w, x[3]);
         }
       }
       const float inv = l > 0.f ? 1.f / l : 0.f;

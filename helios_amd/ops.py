@@ -585,8 +585,10 @@ def block_sparse_attn(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     past the keys are skipped, a block listed twice counts twice, a row without any key gets
     zeros. With ``rows`` (each at most once) only those rows of ``out`` are written: the
     others stay as they were (zeros when ``out`` is not given). Whatever the pool holds behind
-    a sequence's last key is not read; an infinite or NaN element of a key or value that a
-    row does see makes that row's result infinite or NaN."""
+    a sequence's last key is not read. An infinite or NaN element of a value that a row sees
+    makes that element of its result infinite or NaN, at any weight. Of a key, a score of -inf
+    is a weight of 0 (zeros for a row whose scores all are), one of +inf or NaN makes the row
+    NaN, as in ``varlen_attn``."""
     device = _require_gpu(query, k_cache, v_cache, blocks, block_table, key_counts)
     dtype, pages, page_size, n_kv, head_dim = _pool_layout("k_cache", k_cache)
     _check_block_size(block_size, page_size)

@@ -629,7 +629,9 @@ int hx_int4_dequantize(const void* packed, const void* steps, int32_t weight_row
  * hx_block_sparse_attn: out[rows[i]][h] = softmax(scale q . k) V over the keys of blocks[i]
  * [h / group] below key_counts[i], in fp32 (weights and sums), rounded once.
  * Entries of a list that are negative, past the keys or on a page outside the pool are
- * skipped; a block listed twice counts twice. Without any key the row is zeros. Entries whose
+ * skipped; a block listed twice counts twice. Without any key, or with scores of -inf alone,
+ * the row is zeros. An infinite or NaN element of a listed V is its dim's result at any
+ * weight; a score of +inf or NaN makes the row NaN. Entries whose
  * row is outside [0, q_rows) are skipped, and rows not listed are left as they were; a row
  * must not be listed twice. q and the pools 16-byte aligned, q's strides multiples of 8; out
  * 4-byte aligned, its strides even. The workspace is hx_block_sparse_workspace_bytes bytes

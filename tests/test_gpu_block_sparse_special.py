@@ -122,3 +122,64 @@ def test_many_small_weights(device, dtype):
     got, ref = _attend(device, q.to(dtype), k.to(dtype), v.to(dtype), torch.arange(4, dtype=torch.int32).repeat(3, 1),
                        [1000, 1024, 100], 64, 16, 1.0)
     assert ((got - ref).abs() <= (torch.finfo(dtype).eps / 2 + 2.0 ** -13) * ref.abs()).all()
+
+
+def _expect(got, ref, dtype, most):
+    """NaN and infinities where the definition has them; elsewhere its values to the output's half
+    step, and 2^-16 of the values weighed (weights, exp and sums in fp32)."""
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    inf = torch.isinf(ref)
+    assert torch.equal(got[inf], ref[inf])
+    fine = torch.isfinite(ref)
+    off = torch.finfo(dtype).eps / 2 * ref.abs() * (1 + 2.0 ** -8) + 2.0 ** -16 * most
+    assert ((got - ref).abs()[fine] <= off[fine]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,heads,d,ends", [
+    (4, 1, 64, [256, 40, 1000]), (16, 2, 128, [300] * 3), (3, 1, 200, [17, 900]), (8, 8, 128, [1000] * 40)])
+def test_infinite_and_nan_values(device, hq, heads, d, ends, dtype):
+    """An infinite or NaN element of V that a row sees makes that element of its result infinite or
+    NaN, for every head of the group and at any weight, and no other element."""
+    say("sparse infinite values", hq, heads, d, dtype)
+    k, v, table = _pool(ends, heads, d, dtype, seed=d + hq)
+    q = torch.randn(len(ends), hq, d, generator=torch.Generator().manual_seed(1)).to(dtype)
+    for b, n in enumerate(ends):
+        at = lambda t: (int(table[b, t // 256]), t % 256, b % heads)  # noqa: E731
+        v[at(n - 1)][5] = INF
+        v[at(0)][9] = -INF
+        v[at(n // 2)][12], v[at(n // 3)][12] = INF, -INF
+        v[at(n // 2)][d - 1] = NAN
+        v[at(n // 3)][13] = v[at(n - 2)][13] = -INF
+        # This key's weight is e^-60 or less of the largest for every query.
+        far = at(n // 4)
+        k[far] = 0
+        v[far][20] = INF
+    k[..., 0] += 60
+    q[..., 0] = 9 * (d / 64) ** 0.5
+    for b, n in enumerate(ends):
+        k[int(table[b, n // 4 // 256]), n // 4 % 256, b % heads, 0] = 0
+    got, ref = _attend(device, q, k, v, table, ends, 64, 16, d ** -0.5)
+    _expect(got, ref, dtype, 6.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ends", [[100, 40, 256, 17], [1000] * 4])
+def test_infinite_and_nan_keys(device, ends, dtype):
+    """A score of -inf is a weight of 0, one of +inf or NaN makes the row NaN, for the heads that
+    have it alone; a row whose scores are all -inf gets zeros."""
+    say("sparse infinite keys", dtype)
+    k, v, table = _pool(ends, 1, 64, dtype, seed=11)
+    q = torch.randn(4, 4, 64, generator=torch.Generator().manual_seed(2)).to(dtype)
+    q[:, :, 0] = torch.tensor([1.0, -1.0, 2.0, 0.0])
+    first = table[:, 0].tolist()
+    k[first[0], 7, 0, 0] = -INF      # head 0, 2: no weight; 1: NaN (+inf); 3: NaN (0 * inf)
+    k[first[1], 16, 0, 3] = NAN      # all of the row
+    k[first[2], :, 0, 0] = -INF      # every key of the sequence
+    for p in table[2].tolist():
+        k[p, :, 0, 0] = torch.where(torch.isnan(k[p, :, 0, 0]), k[p, :, 0, 0], torch.tensor(-INF, dtype=dtype))
+    got, ref = _attend(device, q, k, v, table, ends, 64, 16, 0.125)
+    assert torch.isnan(ref[0, [1, 3]]).all() and torch.isfinite(ref[0, [0, 2]]).all() and torch.isnan(ref[1]).all()
+    assert torch.isnan(ref[2]).all() and (got[2, [0, 2]] == 0).all() and torch.isnan(got[2, [1, 3]]).all()
+    keep = [0, 1, 3]
+    _expect(got[keep], ref[keep], dtype, 6.0)
