@@ -9,7 +9,9 @@
 //   sum_k h_k s (q_k - z) = s (sum_k h_k (16 + q_k) - (16 + z) sum_k h_k):
 // 16 + q is a bf16 (fp16) number with q in its upper mantissa bits, so a pair of weights costs
 // a rotation and one and-or, and the sums of h come from one more MFMA against ones. Both sums
-// are fp32; the offset 16 makes the terms at most 31 / 15 times as large as they have to be.
+// are fp32; the offset 16 makes the terms at most 31 / 15 times as large as they have to be. Where
+// they are infinite (an infinite h, or one near the type's largest), the two sums cancel to a NaN:
+// such a result is summed again term by term.
 //
 // Weights are packed in the order in which the MFMA takes them: 1 KiB holds 16 rows x 128 k,
 // lane l = 16 c + r of a wave reads 16 bytes, the k elements 32 s + 8 c .. + 7 of row r in its
@@ -174,6 +176,45 @@ enum : int { kRaw4, kRaw8, kRaw16, kNorm4, kNorm8, kNorm16, kParts16 };
 
 // LDS slot of 16-byte piece p of row r: the 16 rows of a fragment read spread over the banks.
 __device__ __forceinline__ int turn_piece(int r, int p) { return p ^ (r & 15); }
+
+// Whether one of eight elements is a NaN.
+template <typename T>
+__device__ __forceinline__ bool has_nan(uint4 u) {
+  constexpr uint32_t kInf = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
+  const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) nan |= (wd[i] & 0x7fffu) > kInf || (wd[i] >> 16 & 0x7fffu) > kInf;
+  return nan;
+}
+
+// sum_k x[k] W[n][k] by one lane: scale (q - zero) is exact in fp32. About a microsecond for every
+// 30 elements of k, for rows that have an infinity or leave fp32; a row with a NaN costs one in all.
+template <typename T, int G>
+__device__ __forceinline__ float sum_of_terms(const Int4Args& a, const uint16_t* x, int n) {
+  typedef hx::Elem<T> E;
+  constexpr int kGroups = kI4Block / G;
+  const int64_t tile = (int64_t)(n >> 4) * a.blocks;
+  const uint8_t* const w = a.w + tile * 1024 + (n & 15) * 16;
+  const uint32_t* const steps = a.steps + (tile * 16 + (n & 15)) * kGroups;
+  float y = 0.f;
+#pragma unroll 1
+  for (int k0 = 0; k0 < a.k; k0 += 8) {
+    const int b = k0 / kI4Block, s = k0 / 32 % 4, c = k0 / 8 % 4;
+    const uint32_t step = steps[(int64_t)b * 16 * kGroups + 32 * s / G];
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(w + (int64_t)b * 1024 + c * 256 + 4 * s);
+    const uint32_t turned = __builtin_amdgcn_alignbit(word, word, 3);
+    const uint4 u = *reinterpret_cast<const uint4*>(x + k0);
+    const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
+    const float sc = E::lo(step), zp = E::hi(step) - 16.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y = fmaf(E::lo(wd[i]), sc * ((float)(turned >> (4 * i) & 15u) - zp), y);
+      y = fmaf(E::hi(wd[i]), sc * ((float)(turned >> (4 * i + 16) & 15u) - zp), y);
+    }
+  }
+  return y;
+}
 
 // G: k elements per group (32, 64 or 128). NV: W tiles of a wave (SWIGLU: gate tiles, then the up
 // tiles they multiply). D: packed blocks in flight per wave.
@@ -359,7 +400,6 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
   for (int e = tid; e < kTiles * kRows * 16; e += 64 * WAVES) {
     const int v0 = e / (kRows * 16), at = e % (kRows * 16);
     const int row = rt * kRows + at / 16, n = n0 + 16 * v0 + at % 16;
-    if (row >= a.rows || n >= a.cols) continue;
     constexpr int kSums = SWIGLU ? 2 : 1;
     float y[kSums];
 #pragma unroll
@@ -371,6 +411,30 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
         if constexpr (kPaired) y[v] += red[ww][v0 + v * kTiles][at + 128];  // the other part
       }
     }
+    const bool there = row < a.rows && n < a.cols;
+    if constexpr (kRaw) {
+      bool odd = false;
+#pragma unroll
+      for (int v = 0; v < kSums; ++v) odd |= there && !hx::is_finite(y[v]);
+      const uint64_t odds = __builtin_amdgcn_ballot_w64(odd);
+      if (__builtin_expect(odds != 0, 0)) {
+        // Sixteen lanes share a row of x. One with a NaN in it, which garbage may hold, stays NaN.
+        const uint16_t* const x = a.x + (int64_t)row * a.x_row;
+        bool nan = false;
+        if ((odds >> (lane & 48) & 0xffff) != 0)
+          for (int p = lr; p < a.k / 8 && !nan; p += 64)
+#pragma unroll
+            for (int i = 0; i < 64; i += 16)
+              if (p + i < a.k / 8) nan |= has_nan<T>(reinterpret_cast<const uint4*>(x)[p + i]);
+        const uint64_t nans = __builtin_amdgcn_ballot_w64(nan);
+        if ((nans >> (lane & 48) & 0xffff) == 0) {
+#pragma unroll
+          for (int v = 0; v < kSums; ++v)
+            if (odd && !hx::is_finite(y[v])) y[v] = sum_of_terms<T, G>(a, x, n + v * a.cols);
+        }
+      }
+    }
+    if (!there) continue;
     if constexpr (kNorm) {
       float sum = 0.f;
 #pragma unroll

@@ -1,0 +1,73 @@
+"""Products with 4-bit weights of rows with infinite and NaN elements."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from helios_amd import ops
+from oracle import decode_ops as oracle
+from tests.gpu_cases import say
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16]
+NAN, INF = float("nan"), float("inf")
+
+
+def _weight(rows, k, group, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    values = torch.randint(0, 16, (rows, k), generator=g, dtype=torch.uint8)
+    scales = ((0.5 + torch.rand(k // group, rows, generator=g)) * 0.3 * k ** -0.5).to(dtype)
+    zeros = torch.randint(0, 16, (k // group, rows), generator=g, dtype=torch.uint8)
+    return values, scales, zeros
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,k,group", [(2, 40, 160, 32), (7, 33, 512, 128), (16, 100, 576, 64), (20, 2100, 160, 32),
+                                               (64, 50, 2560, 128)])
+def test_infinite_elements_of_x(device, rows, cols, k, group, dtype):
+    """y has the infinities and NaN of sum_k x[k] W[k]: an infinity times a weight, NaN where that
+    weight is 0 or infinities of both signs meet. Finite rows are the same bit for bit."""
+    say("int4 infinite x", rows, cols, k, group, dtype)
+    parts = _weight(cols, k, group, dtype, seed=rows)
+    w = oracle.int4_matrix(*parts)
+    packed = ops.int4_pack(*(p.to(device) for p in parts))
+    x = torch.randn(rows, k, generator=torch.Generator().manual_seed(k)).to(dtype)
+    residual = torch.randn(rows, cols, generator=torch.Generator().manual_seed(1)).to(dtype).to(device)
+    clean = ops.int4_linear(x.to(device), packed, residual=residual)
+    bad = x.clone()
+    bad[0, k - 1] = INF
+    bad[1, 3] = -INF
+    spoiled = [0, 1]
+    if rows > 5:
+        bad[4, 5], bad[4, k // 2] = INF, -INF
+        bad[5, 9] = NAN
+        bad[rows - 1, k // 3], bad[rows - 1, 2] = INF, INF
+        spoiled += [4, 5, rows - 1]
+    got = ops.int4_linear(bad.to(device), packed, residual=residual)
+    keep = [r for r in range(rows) if r not in spoiled]
+    assert torch.equal(got[keep], clean[keep])
+    y = torch.stack([(bad[r].double() * w).sum(1) for r in spoiled])
+    got = got[spoiled].double().cpu()
+    assert not torch.isfinite(y).any() and torch.isinf(y).any() and torch.isnan(y).any()
+    assert torch.equal(torch.isnan(got), torch.isnan(y))
+    assert torch.equal(got[torch.isinf(y)], y[torch.isinf(y)])
+
+
+def test_elements_near_the_end_of_the_range(device):
+    """bfloat16 elements whose products with 16 + q leave fp32 where the result does not: fp32 sums
+    of k terms of at most |x W|, k + 16 roundings."""
+    say("int4 near the end of the range")
+    parts = _weight(70, 256, 64, torch.bfloat16, seed=4)
+    parts = (parts[0], parts[1] * 2.0 ** -8, parts[2])
+    w = oracle.int4_matrix(*parts)
+    x = torch.randn(18, 256, generator=torch.Generator().manual_seed(3))
+    x[5] = 3e37 + 1e36 * x[5]
+    x[17] *= 1e37
+    x = x.to(torch.bfloat16)
+    got = ops.int4_linear(x.to(device), ops.int4_pack(*(p.to(device) for p in parts))).double().cpu()
+    y = x.double() @ w.t()
+    most = x.double().abs() @ w.abs().t()
+    off = 2.0 ** -8 * y.abs() + 2.0 ** -24 * (256 + 16) * 31 * most
+    assert ((got - y).abs() <= off).all()
