@@ -18,21 +18,23 @@
 // word s. Element j of a word sits at bits 3 + 4 (j / 2) + 16 (j % 2), modulo 32: turned by 4 i,
 // elements 2 i and 2 i + 1 lie in the upper mantissa bits of a bf16 pair.
 //
-// The norm's row factor 1 / rms multiplies y at the end; x * norm_weight is split into two
-// bf16 (their sum has 16 bits), each an operand row of its own: of up to eight rows the leading
-// parts are rows 0-7 of one MFMA operand and the rest rows 8-15, at no further cost.
+// The norm's row factor 1 / rms multiplies y at the end; x * norm_weight is split into three
+// bf16, which hold fp32's 24 bits. Of up to four rows they are rows 0-3, 4-7 and 8-11 of one MFMA
+// operand, at no further cost; of up to eight, rows 0-7 and 8-15 of one and 0-7 of another; of
+// up to sixteen, three operands. More rows are normalised by a launch of their own, which knows
+// how large they can get, and scaled so that two fp16 hold 23 bits of them.
 //
 // A workgroup owns 16 to 64 columns of y (SwiGLU: gate and the up columns they multiply) and 16
 // (8) rows; its waves split K and merge through LDS in wave order.
 //
 // A layer of hidden 2560, 32/8 heads of 128 and ffn 9728, W from HBM, 1 / 8 / 16 rows (us): qkv
-// 5.5 / 6.0 / 8.0, o 4.0 / 4.5 / 5.3, gate_up 10.2 / 11.1 / 15.0, down 6.6 / 7.4 / 9.4, in all 26 /
-// 29 / 38 where the 16-bit products take 60 / 62 / 71; 17 / 64 rows 47 / 62. gate_up's 26 MB are
-// 2.6 TB/s at one row: about 4 us of each launch are its start, the first loads' way and the
-// merge, as for the 16-bit products; the rest is the stream of W (25 MB at the copy rate: 5.4), with
-// the address unit close behind (x, W and norm weights: 104 cycles a block at 8 rows; 80 with the
-// norm weights loaded once and handed on through LDS take the same time), at 64 rows x's way
-// from L2 (15 TB/s).
+// 5.5 / 6.8 / 9.0, o 4.0 / 4.5 / 5.3, gate_up 10.3 / 12.1 / 17.1, down 6.7 / 7.4 / 9.4, in all 26 /
+// 31 / 41 where the 16-bit products take 60 / 62 / 71; 17 / 64 rows 48 / 64. (Normalised rows in two
+// bf16 parts, 16 bits: 26 / 28 / 38, 47 / 61.) gate_up's 26 MB are 2.5 TB/s at one row: about 4 us
+// of each launch are its start, the first loads' way and the merge, as for the 16-bit products; the
+// rest is the stream of W (25 MB at the copy rate: 5.4), with the address unit close behind (x, W and
+// norm weights: 104 cycles a block at 8 rows; 80 with the norm weights loaded once and handed on
+// through LDS take the same time), at 64 rows x's way from L2.
 
 #include <type_traits>
 
@@ -81,69 +83,121 @@ __device__ __forceinline__ uint4 widen(uint32_t w, const WidenBits<T>& c) {
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// Eight elements of x times norm_weight times r, each as two bf16 numbers: their sum has 16 bits.
-template <typename T>
-__device__ __forceinline__ void split_pair(uint4 u, const float (&nw)[8], float r, uint4& high, uint4& low) {
-  typedef hx::Elem<T> E;
+// Eight fp32 numbers, each as three bf16 ones that add up to it.
+__device__ __forceinline__ void split8(const float (&p)[8], uint4 (&part)[3]) {
   typedef hx::Elem<__bf16> B;
-  const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
-  uint32_t h[4], l[4];
+  uint32_t w[3][4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const float p0 = E::lo(wd[q]) * r * nw[2 * q], p1 = E::hi(wd[q]) * r * nw[2 * q + 1];
-    h[q] = hx::pack2_round<__bf16>(p0, p1);
-    l[q] = hx::pack2_round<__bf16>(p0 - B::lo(h[q]), p1 - B::hi(h[q]));
+    float x = p[2 * q], y = p[2 * q + 1];
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+      w[n][q] = hx::pack2_round<__bf16>(x, y);
+      x -= B::lo(w[n][q]);
+      y -= B::hi(w[n][q]);
+    }
   }
-  high = make_uint4(h[0], h[1], h[2], h[3]);
-  low = make_uint4(l[0], l[1], l[2], l[3]);
+#pragma unroll
+  for (int n = 0; n < 3; ++n) part[n] = make_uint4(w[n][0], w[n][1], w[n][2], w[n][3]);
 }
 
-// RMSNorm of row r as two bf16 parts, for more rows than one tile: h holds, per row tile, block of
-// 128 k, part and step, the MFMA's operand [lane][8]. The first kHold x 256 pieces of a row stay
-// in registers.
+// Eight elements of x times r times norm_weight.
+template <typename T>
+__device__ __forceinline__ void times8(uint4 u, float r, uint4 na, uint4 nb, float (&p)[8]) {
+  typedef hx::Elem<T> E;
+  const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
+  const uint32_t n[8] = {na.x, na.y, na.z, na.w, nb.x, nb.y, nb.z, nb.w};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    p[2 * q] = E::lo(wd[q]) * r * __uint_as_float(n[2 * q]);
+    p[2 * q + 1] = E::hi(wd[q]) * r * __uint_as_float(n[2 * q + 1]);
+  }
+}
+
+// More rows than one tile: RMSNorm's results are below sqrt(k) `most`, the largest |norm_weight|.
+// Scaled by 2^scale_of they are below 2^15 and go into two fp16, which hold 23 bits of them,
+// or of small ones 2^-40 of that bound (fp16's smallest step is 2^-24).
+__device__ __forceinline__ int scale_of(float most, int k) {
+  const int root = (33 - __builtin_clz(k)) / 2;  // 2^root >= sqrt(k)
+  return min(14 + 127 - (int)(__float_as_uint(most) >> 23) - root, 126);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+__device__ __forceinline__ float most_of(float most, uint4 u) {
+  most = fmaxf(fmaxf(most, fabsf(__uint_as_float(u.x))), fabsf(__uint_as_float(u.y)));
+  return fmaxf(fmaxf(most, fabsf(__uint_as_float(u.z))), fabsf(__uint_as_float(u.w)));
+}
+__device__ __forceinline__ float wave_most(float v) {
+  v = fmaxf(v, hx::dpp<hx::kDppXor1>(v));
+  v = fmaxf(v, hx::dpp<hx::kDppXor2>(v));
+  v = fmaxf(v, hx::dpp<hx::kDppHalfMirror>(v));
+  v = fmaxf(v, hx::dpp<hx::kDppMirror>(v));
+  return hx::max_xor32(hx::max_xor16(v));
+}
+
+// RMSNorm of row r as two fp16 parts: h holds, per row tile, block of 128 k, part and step, the
+// MFMA's operand [lane][8]. The first kHold x 256 pieces of a row stay in registers.
 template <typename T>
 __global__ __launch_bounds__(256) void int4_norm_kernel(Int4Args a, uint16_t* h) {
   constexpr int kHold = 2;
   __shared__ float s_part[4];
+  __shared__ float s_most[4];
   const int row = hx::wg_x(), tid = hx::tid_x(), pieces = a.k / 8, padded = a.blocks * (kI4Block / 8);
   const uint4* x = reinterpret_cast<const uint4*>(a.x + (int64_t)row * a.x_row);
-  const float4* n = reinterpret_cast<const float4*>(a.norm_w);
-  uint4 held[kHold];
-  float4 nw[kHold][2];
+  const uint4* n = reinterpret_cast<const uint4*>(a.norm_w);
+  uint4 held[kHold], nw[kHold][2];
 #pragma unroll
   for (int i = 0; i < kHold; ++i) {
     const int p = tid + 256 * i;
-    held[i] = hx::zero4();
-    nw[i][0] = nw[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    held[i] = nw[i][0] = nw[i][1] = hx::zero4();
     if (p >= pieces) continue;
     held[i] = x[p];
     nw[i][0] = n[2 * p];
     nw[i][1] = n[2 * p + 1];
   }
-  float ss = 0.f;
+  float ss = 0.f, most = 0.f;
 #pragma unroll
-  for (int i = 0; i < kHold; ++i) ss = hx::dot8<T>(held[i], held[i], ss);
+  for (int i = 0; i < kHold; ++i) {
+    ss = hx::dot8<T>(held[i], held[i], ss);
+    most = most_of(most_of(most, nw[i][0]), nw[i][1]);
+  }
   for (int p = tid + 256 * kHold; p < pieces; p += 256) {
     const uint4 u = x[p];
     ss = hx::dot8<T>(u, u, ss);
+    most = most_of(most_of(most, n[2 * p]), n[2 * p + 1]);
   }
   ss = hx::wave_sum_xor(ss, 1, 32);
-  if ((tid & 63) == 0) s_part[tid >> 6] = ss;
+  most = wave_most(most);
+  if ((tid & 63) == 0) {
+    s_part[tid >> 6] = ss;
+    s_most[tid >> 6] = most;
+  }
   __syncthreads();
   ss = (s_part[0] + s_part[1]) + (s_part[2] + s_part[3]);
+  most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
   const float r = __builtin_amdgcn_rsqf(__fadd_rn(__fdiv_rn(ss, (float)a.k), a.eps));
-  uint4* tile = reinterpret_cast<uint4*>(h) + (int64_t)(row >> 4) * 2 * padded * 16 + (row & 15);
-  auto put = [&](int p, uint4 u, float4 na, float4 nb) __attribute__((always_inline)) {
-    const float w[8] = {na.x, na.y, na.z, na.w, nb.x, nb.y, nb.z, nb.w};
+  const float scale = power_of_two(scale_of(most, a.k));
+  uint4* tile = reinterpret_cast<uint4*>(h) + (int64_t)(row >> 4) * a.blocks * 512 + (row & 15);
+  auto put = [&](int p, uint4 u, uint4 na, uint4 nb) __attribute__((always_inline)) {
+    typedef hx::Elem<_Float16> H;
+    float v[8];
+    times8<T>(u, r, na, nb, v);
+    uint32_t high[4], low[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float v0 = v[2 * q] * scale, v1 = v[2 * q + 1] * scale;
+      high[q] = hx::pack2_round<_Float16>(v0, v1);
+      low[q] = hx::pack2_round<_Float16>(v0 - H::lo(high[q]), v1 - H::hi(high[q]));
+    }
     uint4* to = tile + (p / 16 * 8 + p / 4 % 4) * 64 + 16 * (p % 4);
-    split_pair<T>(u, w, r, to[0], to[256]);
+    to[0] = make_uint4(high[0], high[1], high[2], high[3]);
+    to[256] = make_uint4(low[0], low[1], low[2], low[3]);
   };
 #pragma unroll
   for (int i = 0; i < kHold; ++i)
     if (tid + 256 * i < padded) put(tid + 256 * i, held[i], nw[i][0], nw[i][1]);
-  const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int p = tid + 256 * kHold; p < padded; p += 256)
-    put(p, p < pieces ? x[p] : hx::zero4(), p < pieces ? n[2 * p] : none, p < pieces ? n[2 * p + 1] : none);
+    put(p, p < pieces ? x[p] : hx::zero4(), p < pieces ? n[2 * p] : hx::zero4(), p < pieces ? n[2 * p + 1] : hx::zero4());
 }
 
 // 16-byte buffer load at byte offset voff + soff.
@@ -173,6 +227,8 @@ __device__ __forceinline__ void load_steps(__amdgpu_buffer_rsrc_t r, uint32_t vo
 // How x reaches the MFMA: as it is, up to 4, 8 or 16 rows a tile; normalised on the way, the same;
 // or as int4_norm_kernel's parts.
 enum : int { kRaw4, kRaw8, kRaw16, kNorm4, kNorm8, kNorm16, kParts16 };
+
+__host__ __device__ constexpr int rows_of(int in) { return in == kNorm4 ? 4 : in == kNorm8 ? 8 : 16; }
 
 // LDS slot of 16-byte piece p of row r: the 16 rows of a fragment read spread over the banks.
 __device__ __forceinline__ int turn_piece(int r, int p) { return p ^ (r & 15); }
@@ -221,20 +277,25 @@ __device__ __forceinline__ float sum_of_terms(const Int4Args& a, const uint16_t*
 template <typename T, int IN, bool SWIGLU, int G, int NV, int WAVES, int D>
 __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
   constexpr bool kRaw = IN <= kRaw16, kNorm = IN >= kNorm4 && IN <= kNorm16, kTurn = kRaw || kNorm;
-  // Normalised rows are bf16 parts whatever the element type: 16 + q is exact in either.
-  typedef typename std::conditional<kRaw, T, __bf16>::type M;
+  // The parts' type, whatever the element type: 16 + q is exact in either.
+  typedef typename std::conditional<kRaw, T, typename std::conditional<kNorm, __bf16, _Float16>::type>::type M;
   typedef hx::Elem<T> E;
   typedef hx::Elem<M> EM;
   typedef typename EM::v8 v8;
   constexpr int kSteps = kI4Block / 32, kGroups = kI4Block / G;
   constexpr int kTiles = SWIGLU ? NV / 2 : NV, kCols = 16 * kTiles;  // of the output
-  constexpr int kRows = IN == kNorm4 || IN == kNorm8 ? 8 : 16;  // of a row tile
-  constexpr int kOps = IN == kNorm16 || IN == kParts16 ? 2 : 1;  // MFMA operands of a tile's rows
-  // Up to eight normalised rows share one operand: leading parts in rows 0-7, the rest in 8-15.
-  constexpr bool kPaired = IN == kNorm4 || IN == kNorm8;
+  constexpr int kRows = rows_of(IN);  // of a row tile
+  constexpr int kOps = kRaw || IN == kNorm4 ? 1 : IN == kNorm16 ? 3 : 2;  // MFMA operands of a tile's rows
+  // Where the parts of up to eight normalised rows lie: operand and first row.
+  constexpr bool kFew = IN == kNorm4 || IN == kNorm8;
+  constexpr int kAt[3][2] = {{0, 0}, {0, kRows}, {IN == kNorm8 ? 1 : 0, IN == kNorm8 ? 0 : 2 * kRows}};
+  // Rows 8-15 of the second operand are one row of zeros.
+  constexpr int kSecond = 4096, kZeros = kSecond + 8 * 256;
+  constexpr int kTurnBytes = IN == kNorm8 ? kZeros + 256 : IN == kNorm16 ? 8192 : 4096;
+  constexpr bool kSplit = IN == kNorm16;  // kept in fp32, split where the MFMA takes them
   constexpr int kLoads = IN == kParts16 ? 2 * kSteps : IN == kRaw4 || IN == kNorm4 ? 1 : IN == kRaw8 || IN == kNorm8 ? 2 : 4;
   __shared__ __attribute__((aligned(16))) float red[WAVES][NV][256];
-  __shared__ __attribute__((aligned(16))) uint8_t turn[kTurn ? WAVES : 1][kTurn ? 4096 * kOps : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t turn[kTurn ? WAVES : 1][kTurn ? kTurnBytes : 16];
   __shared__ float s_ss[WAVES][16];
   const int tid = hx::tid_x(), lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -306,12 +367,29 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
     if (a.res != nullptr && tid < kRows * 16 && r_row < a.rows && r_col < a.cols)
       r_first = a.res[(int64_t)r_row * a.res_row + r_col];
 
+  // The norm weights that give the scale of the normalised rows' parts, in flight with the weights
+  // too. (Kept in registers and looked at after the loop they cost occupancy: SwiGLU of 64 rows
+  // took 1.2 us longer.)
+  float most = 0.f;
+  if constexpr (IN == kParts16) {
+    const uint4* const n = reinterpret_cast<const uint4*>(a.norm_w);
+    for (int p = tid; p < a.k / 4; p += 256 * WAVES) {
+      uint4 u[4];  // past the end the last piece again
+#pragma unroll
+      for (int q = 0; q < 4; ++q) u[q] = n[min(p + 64 * WAVES * q, a.k / 4 - 1)];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) most = most_of(most, u[q]);
+    }
+  }
+
   hx::f32x4_t acc[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) acc[v] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
   float ss[kLoads];
 #pragma unroll
   for (int q = 0; q < kLoads; ++q) ss[q] = 0.f;
+  if constexpr (IN == kNorm8)
+    if (lane < 16) reinterpret_cast<uint4*>(turn[w] + kZeros)[lane] = hx::zero4();
   const v8 ones = hx::as_v8<M>(hx::ones8<M>());
   const WidenBits<M> bits;
   auto consume = [&](int i, int b) __attribute__((always_inline)) {
@@ -324,18 +402,23 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
         const int r = 4 * q + lg;
         uint8_t* to = turn[w] + 256 * r + 16 * turn_piece(r, lr);
         if constexpr (kNorm) {
-          // x * norm_weight in two parts; 1 / rms multiplies the sums at the end.
-          const uint32_t nw4[8] = {nb[i][0].x, nb[i][0].y, nb[i][0].z, nb[i][0].w,
-                                   nb[i][kNorm].x, nb[i][kNorm].y, nb[i][kNorm].z, nb[i][kNorm].w};
-          float nw[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) nw[e] = __uint_as_float(nw4[e]);
-          uint4 h, l;
-          split_pair<T>(u, nw, 1.f, h, l);
+          // x * norm_weight; 1 / rms multiplies the sums at the end.
+          float p[8];
+          times8<T>(u, 1.f, nb[i][0], nb[i][kNorm], p);
           ss[q] = hx::dot8<T>(u, u, ss[q]);
-          *reinterpret_cast<uint4*>(to) = h;
-          const int r2 = kPaired ? r + 8 : r;  // the same slot of another row, or another operand
-          *reinterpret_cast<uint4*>(turn[w] + 256 * r2 + 16 * turn_piece(r2, lr) + (kPaired ? 0 : 4096)) = l;
+          if constexpr (kFew) {
+            uint4 part[3];
+            split8(p, part);
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+              const int r2 = r + kAt[n][1];
+              *reinterpret_cast<uint4*>(turn[w] + kSecond * kAt[n][0] + 256 * r2 + 16 * turn_piece(r2, lr)) = part[n];
+            }
+          } else {  // a row's first halves of its pieces of eight, then the second ones
+            float4* const to4 = reinterpret_cast<float4*>(turn[w] + 512 * r) + turn_piece(r, lr);
+            to4[0] = make_float4(p[0], p[1], p[2], p[3]);
+            to4[16] = make_float4(p[4], p[5], p[6], p[7]);
+          }
         } else {
           *reinterpret_cast<uint4*>(to) = u;
         }
@@ -345,11 +428,20 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
+    for (int s = 0; s < kSteps; ++s) {
+      if constexpr (kSplit) {
+        const float4* const from = reinterpret_cast<const float4*>(turn[w] + 512 * lr) + turn_piece(lr, 4 * s + lg);
+        const float4 a4 = from[0], b4 = from[16];
+        const float p[8] = {a4.x, a4.y, a4.z, a4.w, b4.x, b4.y, b4.z, b4.w};
+        split8(p, xf[s]);
+      } else {
 #pragma unroll
-      for (int o = 0; o < kOps; ++o)
-        xf[s][o] = kTurn ? *reinterpret_cast<const uint4*>(turn[w] + 4096 * o + 256 * lr + 16 * turn_piece(lr, 4 * s + lg))
-                         : xb[i][(kSteps * o + s) % kLoads];
+        for (int o = 0; o < kOps; ++o)
+          xf[s][o] = kTurn ? *reinterpret_cast<const uint4*>(turn[w] + kSecond * o + 256 * (o == 0 ? lr : min(lr, 8)) +
+                                                             16 * turn_piece(lr, 4 * s + lg))
+                           : xb[i][(kSteps * o + s) % kLoads];
+      }
+    }
     if constexpr (kTurn) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
@@ -396,6 +488,10 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
       if (lr == 0) s_ss[w][4 * q + lg] = sum;
     }
   }
+  if constexpr (IN == kParts16) {
+    most = wave_most(most);
+    if (lane == 0) s_ss[w][0] = most;
+  }
   __syncthreads();
   for (int e = tid; e < kTiles * kRows * 16; e += 64 * WAVES) {
     const int v0 = e / (kRows * 16), at = e % (kRows * 16);
@@ -408,7 +504,8 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
 #pragma unroll
       for (int ww = 0; ww < WAVES; ++ww) {
         y[v] += red[ww][v0 + v * kTiles][at];
-        if constexpr (kPaired) y[v] += red[ww][v0 + v * kTiles][at + 128];  // the other part
+        if constexpr (kFew) y[v] += red[ww][v0 + v * kTiles][at + 16 * kRows];  // the second parts
+        if constexpr (IN == kNorm4) y[v] += red[ww][v0 + v * kTiles][at + 32 * kRows];  // the third
       }
     }
     const bool there = row < a.rows && n < a.cols;
@@ -442,6 +539,14 @@ __global__ __launch_bounds__(64 * WAVES) void int4_gemm_kernel(Int4Args a) {
       const float r = __builtin_amdgcn_rsqf(__fadd_rn(__fdiv_rn(sum, (float)a.k), a.eps));
 #pragma unroll
       for (int v = 0; v < kSums; ++v) y[v] *= r;
+    }
+    if constexpr (IN == kParts16) {
+      float top = 0.f;
+#pragma unroll
+      for (int ww = 0; ww < WAVES; ++ww) top = fmaxf(top, s_ss[ww][0]);
+      const float unscale = power_of_two(-scale_of(top, a.k));
+#pragma unroll
+      for (int v = 0; v < kSums; ++v) y[v] *= unscale;
     }
     float o = y[0];
     if constexpr (SWIGLU) o = hx::silu(o) * y[kSums - 1];
@@ -488,30 +593,31 @@ __global__ __launch_bounds__(256) void int4_dequant_kernel(DequantArgs a, int64_
 
 template <typename T, int IN, bool SWIGLU, int G, int NV>
 int launch_tiles(Int4Args a, hipStream_t s) {
-  constexpr int kCols = SWIGLU ? 8 * NV : 16 * NV, kRows = IN == kNorm4 || IN == kNorm8 ? 8 : 16;
+  constexpr int kCols = SWIGLU ? 8 * NV : 16 * NV, kRows = rows_of(IN);
   a.row_tiles = (a.rows + kRows - 1) / kRows;
   a.col_tiles = (a.cols + kCols - 1) / kCols;
   // Waves that split K, and blocks in flight. bf16, 1 / 8 / 16 rows, W from HBM (us): 9728 + 9728
-  // columns of 2560 with SwiGLU, 4 waves and 1 block 10.2 / 11.1 / 15.0, 2 blocks 10.1 / 12.2 /
-  // 15.2, 8 waves 9.9 / 11.7 / 21.8 (their LDS leaves one workgroup to a CU at 16 rows); 2560
-  // columns of 9728, 8 waves and 2 blocks 6.6 / 7.4 / 9.4, 3 blocks 6.3 / 7.3 / 9.8, 4 waves
+  // columns of 2560 with SwiGLU, 4 waves and 1 block 10.3 / 12.1 / 17.1, 2 blocks 10.3 / 12.4 /
+  // 17.4, 8 waves 10.2 / 13.3 / 25.4 (their LDS leaves one workgroup to a CU at 16 rows); 2560
+  // columns of 9728, 8 waves and 2 blocks 6.6 / 7.4 / 9.4, 3 blocks 6.3 / 7.5 / 9.8, 4 waves
   // 9.1 / 10.0 / 11.0. Three W tiles and more are enough in flight at one block: 64 rows of the
-  // columns of 9728, three tiles, 12.0, 2 blocks 12.7, 16 waves 12.4; four tiles 13.5 and 14.5; 6144 columns of 2560, normalised, 4
-  // waves and 1 block 14.7, 2 blocks 15.8, 8 waves 16.0.
-  constexpr int kWaves = SWIGLU || IN == kParts16 ? 4 : 8, kDepth = SWIGLU || NV >= 3 ? 1 : 2;
+  // columns of 9728, three tiles, 11.9, 2 blocks 12.7; 6144 columns of 2560, normalised, four tiles,
+  // 17 / 64 rows, 8 waves and 1 block 11.6 / 16.2, 4 waves 13.2 / 16.5, 4 waves and 2 blocks 11.8 /
+  // 16.0 (SwiGLU's 9728 20.2 / 29.0, 2 blocks 21.9 / 31.9).
+  constexpr int kWaves = SWIGLU ? 4 : 8, kDepth = SWIGLU || NV >= 3 ? 1 : 2;
   const auto fn = int4_gemm_kernel<T, IN, SWIGLU, G, NV, kWaves, kDepth>;
   hipLaunchKernelGGL(fn, dim3((unsigned)((a.col_tiles + 7) / 8 * 8 * a.row_tiles)), dim3(64 * kWaves), 0, s, a);
   return hx::status_from_hip(hipGetLastError());
 }
 
 // W tiles of a workgroup. Two where x costs more than a load (6144 columns of 2560, normalised,
-// 1 / 8 / 16 rows: 5.5 / 6.0 / 8.0 us, one tile 6.2 / 7.6 / 10.6), one where it does not (2560
-// columns of 9728: 6.4 / 7.3 / 9.3, two tiles 8.2 / 9.2 / 11.0). Past one row tile, x's way from
+// 1 / 8 / 16 rows: 5.5 / 6.8 / 9.0 us, one tile 5.9 / 7.6 / 14.1), one where it does not (2560
+// columns of 9728: 6.6 / 7.4 / 9.4, two tiles 8.2 / 9.2 / 11.0). Past one row tile, x's way from
 // L2 bounds the kernel and more tiles share it: four of normalised rows, whose parts are twice
-// the bytes (17 / 64 rows, 6144 columns 11.4 / 14.7, two tiles 13.4 / 17.9; 9728 columns and
-// SwiGLU 19.2 / 27.6, two 21.7 / 34.7, eight 21.2 / 30.3), otherwise the fewest of two, three and
-// four that make at most one workgroup a CU (2560 columns of 9728, 17 / 48 rows two 10.1 / 11.2,
-// four 13.0 / 13.6; 64 rows two 17.1, three 12.0, four 13.5).
+// the bytes (17 / 64 rows, 6144 columns 11.6 / 16.2, two tiles 14.0 / 18.9, eight 14.8 / 15.6; 9728
+// columns and SwiGLU 20.0 / 29.0, two 24.0 / 36.6, eight 25.5 / 36.3), otherwise the fewest of two,
+// three and four that make at most one workgroup a CU (2560 columns of 9728, 17 / 48 rows two 10.1 /
+// 10.7, four 13.0 / 13.6; 64 rows two 17.1, three 11.9, four 13.5).
 template <typename T, int IN, bool SWIGLU, int NV = SWIGLU || IN >= kNorm4 ? 2 : 1>
 int launch_group(const Int4Args& a, int group, hipStream_t s) {
   if (group == 128) return launch_tiles<T, IN, SWIGLU, 128, NV>(a, s);
@@ -520,8 +626,8 @@ int launch_group(const Int4Args& a, int group, hipStream_t s) {
 }
 
 // Rows that each workgroup normalises on their way in; more of them are normalised once, in a
-// launch of about 3 us (6144 columns of 2560: 16 rows 8.0 us, 17 rows 11.4; 64 rows 14.7 us, and
-// 32.1 normalised by every workgroup's own row tiles of 8).
+// launch of about 3 us (6144 columns of 2560: 16 rows 9.0 us, 17 rows 11.6, 64 rows 16.2; normalised
+// by every workgroup 17 rows 16.6, 64 rows 24.7).
 constexpr int kFusedNormRows = 16;
 
 template <typename T, bool SWIGLU>

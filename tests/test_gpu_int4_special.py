@@ -1,4 +1,5 @@
-"""Products with 4-bit weights of rows with infinite and NaN elements."""
+"""Products with 4-bit weights of rows with infinite and NaN elements, and the bits of normalised
+rows."""
 
 from __future__ import annotations
 
@@ -71,3 +72,38 @@ def test_elements_near_the_end_of_the_range(device):
     most = x.double().abs() @ w.abs().t()
     off = 2.0 ** -8 * y.abs() + 2.0 ** -24 * (256 + 16) * 31 * most
     assert ((got - y).abs() <= off).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 4, 5, 8, 11, 16, 17, 40, 64])
+def test_normalised_rows_keep_24_bits(device, rows, dtype):
+    """Two elements, in groups of their own with weights of 15 s and -15 s, that normalise to values
+    2^-12 of themselves apart. h = x r norm is rounded in fp32 (and r cancels but for 2^-20 of
+    the small y); a group's sums are of 31 h, 16 h and 15 h with a rounding of 2^-24 each for every
+    of three parts, so 220 h 2^-24 covers both. An h of 16 bits is off by up to 2^-17. Norm weights of
+    2^-24 to 2^18, one of them 2^10 times the others where x is 0."""
+    say("int4 24 bits", rows, dtype)
+    g = torch.Generator().manual_seed(rows)
+    values = torch.zeros(24, 64, dtype=torch.uint8)
+    zeros = torch.zeros(2, 24, dtype=torch.uint8)
+    values[:, 7], zeros[1] = 15, 15
+    values[:, 32:] = 15
+    values[:, 50] = 0
+    scales = torch.ones(2, 24).to(dtype)
+    x = torch.zeros(rows, 64)
+    x[:, 7] = x[:, 50] = 1 + torch.rand(rows, generator=g)
+    x = x.to(dtype)
+    for seed in range(8):
+        g = torch.Generator().manual_seed(seed)
+        norm = torch.ones(64)
+        norm[7] = 1 + torch.rand(1, generator=g)
+        norm[50] = norm[7] * (1 + 2.0 ** -12 * (0.5 + torch.rand(1, generator=g)))
+        norm[20] = 2.0 ** 10
+        norm *= 2.0 ** (6 * (seed - 4))
+        packed = ops.int4_pack(*(t.to(device) for t in (values, scales, zeros)))
+        got = ops.int4_linear(x.to(device), packed, norm_weight=norm.to(device), eps=1e-6).double().cpu()
+        h = x.double() / torch.sqrt((x.double() ** 2).mean(1, keepdim=True) + 1e-6) * norm.double()
+        y = h @ oracle.int4_matrix(values, scales, zeros).t()
+        off = (torch.finfo(dtype).eps / 2 + 2.0 ** -19) * y.abs() + 2.0 ** -24 * 220 * h[:, 50:51].abs() \
+            + torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2  # half of the smallest step
+        assert ((got - y).abs() <= off).all(), ((got - y).abs() / off).max()
