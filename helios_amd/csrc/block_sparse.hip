@@ -677,7 +677,7 @@ __global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a
       const __amdgpu_buffer_rsrc_t kr = hx::buffer_rsrc(a.k + base, bytes), vr = hx::buffer_rsrc(a.v + base, bytes);
 #pragma unroll
       for (int q = 0; q < kLoads; ++q) {
-        // All of the offset in the vector part: the range check is on it alone.
+        // A piece past the head's dims stays past the buffer's end: 0x7ffffff0 + 2^29 at most.
         kb[u][q] = hx::ld16_stream(kr, voff + q * kPerLoad * row_bytes, 0);
         vb[u][q] = hx::ld16_stream(vr, voff + q * kPerLoad * row_bytes, 0);
       }

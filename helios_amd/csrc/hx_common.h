@@ -167,7 +167,10 @@ __device__ __forceinline__ uint4 ld16_stream(const void* p) {
 
 // Raw buffer resource over `bytes` bytes from `base` (stride 0: byte addressing, reads
 // past `bytes` return zeros), for loads whose per-lane part is a 32-bit offset and whose
-// per-load part is a scalar offset: no per-load vector address arithmetic.
+// per-load part is a scalar offset: no per-load vector address arithmetic. The range check is on
+// the sum of both offsets, also where the scalar one alone passes `bytes` (measured over 7 sizes
+// and 11 scalar offsets inside one allocation): a scalar offset of `bytes` reads zeros in every lane.
+// The sum must stay below 2^32.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_rsrc(const void* base, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
 }

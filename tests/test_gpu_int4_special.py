@@ -1,5 +1,5 @@
-"""Products with 4-bit weights of rows with infinite and NaN elements, and the bits of normalised
-rows."""
+"""Products with 4-bit weights of rows with infinite and NaN elements, the bits of normalised rows,
+and memory behind the operands."""
 
 from __future__ import annotations
 
@@ -107,3 +107,26 @@ def test_normalised_rows_keep_24_bits(device, rows, dtype):
         off = (torch.finfo(dtype).eps / 2 + 2.0 ** -19) * y.abs() + 2.0 ** -24 * 220 * h[:, 50:51].abs() \
             + torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2  # half of the smallest step
         assert ((got - y).abs() <= off).all(), ((got - y).abs() / off).max()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,group", [(1, 160, 32), (4, 32, 32), (7, 192, 64), (16, 96, 32), (33, 160, 32)])
+def test_memory_behind_the_operands(device, rows, k, group, dtype):
+    """K that ends inside a packed block of 128: what lies in memory behind x, the norm's weights,
+    the packed weights and their steps does not show."""
+    say("int4 memory behind", rows, k, group, dtype)
+    parts = _weight(33, k, group, dtype, seed=k)
+    w = ops.int4_pack(*(p.to(device) for p in parts))
+    x = torch.randn(rows, k, generator=torch.Generator().manual_seed(1)).to(dtype).to(device)
+    norm = 1 + 0.1 * torch.rand(k, generator=torch.Generator().manual_seed(2)).to(device)
+
+    def inside(t, fill):
+        flat = torch.full((t.numel() + 8192,), fill, dtype=t.dtype, device=device)
+        flat[:t.numel()] = t.flatten()
+        return flat[:t.numel()].view(t.shape)
+
+    far = w._replace(packed=inside(w.packed, 255), steps=inside(w.steps, -1))  # steps of NaN
+    for n in (None, norm):
+        want = ops.int4_linear(x, w, norm_weight=n, eps=1e-6)
+        got = ops.int4_linear(inside(x, NAN), far, norm_weight=None if n is None else inside(n, NAN), eps=1e-6)
+        assert torch.isfinite(want).all() and torch.equal(got, want)
