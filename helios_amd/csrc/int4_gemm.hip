@@ -25,12 +25,12 @@
 // how large they can get, and scaled so that two fp16 hold 23 bits of them.
 //
 // A workgroup owns 16 to 64 columns of y (SwiGLU: gate and the up columns they multiply) and 16
-// (8) rows; its waves split K and merge through LDS in wave order.
+// (8, 4) rows; its waves split K and merge through LDS in wave order.
 //
 // A layer of hidden 2560, 32/8 heads of 128 and ffn 9728, W from HBM, 1 / 8 / 16 rows (us): qkv
-// 5.5 / 6.8 / 9.0, o 4.0 / 4.5 / 5.3, gate_up 10.3 / 12.1 / 17.1, down 6.7 / 7.4 / 9.4, in all 26 /
-// 31 / 41 where the 16-bit products take 60 / 62 / 71; 17 / 64 rows 48 / 64. (Normalised rows in two
-// bf16 parts, 16 bits: 26 / 28 / 38, 47 / 61.) gate_up's 26 MB are 2.5 TB/s at one row: about 4 us
+// 5.7 / 6.9 / 9.2, o 4.2 / 4.6 / 5.4, gate_up 10.3 / 12.0 / 17.2, down 6.9 / 7.6 / 9.5, in all 27 /
+// 31 / 41 where the 16-bit products take 60 / 62 / 71; 17 / 64 rows 48 / 65. (Normalised rows in two
+// bf16 parts, 16 bits: 27 / 29 / 38, 47 / 61.) gate_up's 26 MB are 2.5 TB/s at one row: about 4 us
 // of each launch are its start, the first loads' way and the merge, as for the 16-bit products; the
 // rest is the stream of W (25 MB at the copy rate: 5.4), with the address unit close behind (x, W and
 // norm weights: 104 cycles a block at 8 rows; 80 with the norm weights loaded once and handed on

@@ -16,7 +16,8 @@ the arithmetic is otherwise the reference's.
 
 With ``weight_bits=4`` the four products' weights are ``ops.Int4Weight``s: ticks of up to
 ``ops.INT4_MAX_ROWS`` rows run them through ``ops.int4_linear`` with the steps between them
-fused in, longer ones dequantise a weight and take the library's product. ``rules`` puts the
+fused in, longer ones dequantise a weight, to its type, and take the library's product (slower
+there than 16-bit weights). ``rules`` puts the
 requests' penalties, biases and allowed tokens on the logits (``ops.apply_logit_rules``).
 """
 

@@ -735,7 +735,8 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, *, norm_weight: torch.Tenso
     RMSNormed first by ``norm_weight``, ``residual`` added, or, with ``swiglu`` (``W`` holds
     gate, then up rows), ``silu(gate) * up``, in one launch. In fp32 and rounded once, at the
     end. ``x`` ``[..., k]`` and ``residual`` ``[..., n]`` contiguous, in the weight's dtype, ``x``
-    16-byte aligned. More rows: ``int4_dequantize`` and a library product."""
+    16-byte aligned. More rows: ``int4_dequantize``, which rounds W to its type, and a library
+    product."""
     device = _require_gpu(x)
     dtype = _check_int4(weight, device)
     cols, k = weight.rows, weight.k
@@ -789,10 +790,10 @@ class LogitRules(NamedTuple):
     are ``tokens[r, :lengths[r]]`` (a server appends a column a tick), the first
     ``prompt_lens[r]`` (int32, None: 0) its prompt, the others said. ``repetition`` (of
     known tokens), ``presence`` and ``frequency`` (of said ones): float32 ``[rows]``.
-    ``bias_ids`` int32 and ``bias_values`` float32 ``[rows, n]``: added to those tokens; of an
-    id listed twice in a row the last counts. ``allowed`` int32 ``[rows, ceil(vocab / 32)]``:
+    ``bias_ids`` int32 and ``bias_values`` float32 ``[rows, n]``, of one row stride: added to
+    those tokens; of an id listed twice in a row the last counts. ``allowed`` int32 ``[rows, ceil(vocab / 32)]``:
     bit ``v % 32`` of word ``v // 32`` allows token v. Token and bias ids outside the
-    vocabulary (-1: padding) are skipped."""
+    vocabulary (-1: padding) are skipped. Rows of a table are contiguous and do not overlap."""
 
     tokens: torch.Tensor | None = None
     lengths: torch.Tensor | None = None
