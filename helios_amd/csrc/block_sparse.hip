@@ -555,8 +555,8 @@ void launch_select(const SelectArgs& a, int64_t n, hipStream_t s) {
 // cannot leave fp32 in the sums over a list's keys, fp16's by 2^14, so that small ones keep
 // their bits (unscaled, those below 2^-25 were lost: 940 of e^-18 are 1.4e-5 of a sum).
 //
-// 32/8 heads of 128, blocks of 64: 64 rows of 4096 keys (1.07 GB) 175 us, 6.1 TB/s, what this
-// card reads at most; one row of 2048 keys (8.4 MB) 6.9 us and 3.4 for the join of its 16 splits,
+// 32/8 heads of 128, blocks of 64: 64 rows of 4096 keys (1.07 GB) 177 us, 6.1 TB/s, what this
+// card reads at most; one row of 2048 keys (8.4 MB) 7.1 us and 3.2 for the join of its 16 splits,
 // the launches' and dependent loads' latency.
 
 constexpr int kSpWaves = 4;
