@@ -25,6 +25,12 @@ HX_DTYPE_BF16 = 0
 HX_DTYPE_FP16 = 1
 HX_DTYPE_FP32 = 2
 
+HX_CODE_E4M3 = 0
+HX_CODE_INT8 = 1
+
+HX_KV8_FEW_ROWS = 1
+HX_KV8_CHUNK_ROWS = 2
+
 HX_WERR_BAD_PAGE = 1
 HX_WERR_CLAMPED_LEN = 2
 HX_WERR_BAD_CU_SEQ = 4
@@ -240,6 +246,35 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _c_void_p, _c_void_p, _i32, _i32, _i32, _c_void_p, _i32,
          _c_void_p, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _i32,
          _c_void_p, _i64, _i64, _c_void_p, _size, _c_void_p],
+    ),
+    "hx_kv8_append": (
+        ctypes.c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _i32, _i32, _i32,
+         _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p],
+    ),
+    "hx_kv8_norm_rope_append": (
+        ctypes.c_int,
+        [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64,
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i64,
+         _i32, _i32, _i32, _f32, _i32, _c_void_p, _i64, _i64,
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _i32, _c_void_p, _c_void_p],
+    ),
+    "hx_kv8_gather": (
+        ctypes.c_int,
+        [_c_void_p, _c_void_p, _i32, _i32, _i32, _i32, _i32, _c_void_p, _i32, _i64, _i32, _c_void_p, _c_void_p],
+    ),
+    "hx_kv8_attn_workspace_bytes": (_size, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "hx_kv8_attn_error_word_offset": (_size, []),
+    "hx_kv8_attn_plan": (
+        ctypes.c_int,
+        [_c_void_p, _c_void_p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+         _c_void_p, _size, _c_void_p],
+    ),
+    "hx_kv8_attn_run": (
+        ctypes.c_int,
+        [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _i32,
+         _c_void_p, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _i32,
+         _c_void_p, _i64, _i64, _i32, _c_void_p, _size, _c_void_p],
     ),
     "hx_logit_rules_workspace_bytes": (_size, [_i64, _i64]),
     "hx_logit_rules": (

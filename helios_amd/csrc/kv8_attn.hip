@@ -1,0 +1,1228 @@
+// Varlen GQA attention over the paged 8-bit KV cache (gfx950).
+//
+// With key codes c, value codes v, scales s_k and s_v per token and KV head:
+//   u_j = log2(e) scale (q . c_j) s_kj + log2 s_vj,   w_j = 2^(u_j - M),   M = max_j u_j
+//   out = sum_j w_j v_j / sum_j (w_j / s_vj)
+// The value's scale rides on the softmax's exponent: the weights that meet the codes have their
+// maximum at 1 whatever the scales of the values are, and fit fp16 together with the codes, which
+// fp16 holds exactly. q goes into the products as fp16 too, after a power of two that puts its
+// largest element at 2^14: exact for fp16, and for bf16 down to 2^-28 of the largest element
+// (smaller ones within 2^-40 of it). Sums are fp32.
+//
+// Two kernels over a plan's work lists, and one that joins splits:
+//   few_kernel    sequences whose (row, query head) pairs of a KV head fit one MFMA's 16 columns
+//                 (decode rows, a few drafted ones), split over their keys. Bound by HBM.
+//   chunk_kernel  the others: blocks of rows over 64-key tiles, split over their tiles where the
+//                 blocks alone leave CUs without work. Bound by MFMA and the softmax.
+
+#include "kv8_common.h"
+
+#include <math.h>
+
+namespace {
+
+constexpr int64_t kMostItems = (int64_t)1 << 32;  // work-items of a launch
+constexpr float kLog2e = 1.44269504088896340736f;
+
+constexpr int kFewUnits = 16;     // (row, head) pairs of a few_kernel item
+constexpr int kFewThreads = 256;  // 4 waves, each on its own 32-key tiles
+constexpr int kFewTile = 32;
+constexpr int kFewWGs = 2048;     // workgroups that the split size aims at: 8 a CU
+constexpr int kFewLeast = 8;      // tiles of a split, at least (two a wave)
+constexpr int kFewMost = 256;     // and at most
+constexpr int kChunkThreads = 512;
+constexpr int kChunkTile = 64;
+constexpr int kChunkWGs = 512;    // workgroups below which row blocks are split
+constexpr int kChunkLeast = 4;    // tiles of a split, at least
+constexpr int kPlanThreads = 1024;
+
+// Plan header words.
+enum { H_FEW = 0, H_CHUNK = 1, H_JOIN = 2, H_ERR = 3, H_STAMP = 4, H_WORDS = 16 };
+
+__host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// What a plan is built for; its runs must agree (the first 8 words are checked on the device).
+struct Shape {
+  int32_t batch, total_q, max_q, max_k, hq, hkv, head_dim, page;
+  int32_t left, right, width;
+};
+
+struct Sizes {
+  int32_t group;
+  int32_t few_heads, head_blocks;  // query heads of a few item, and items over a group's heads
+  int32_t few_rows;                // rows of a sequence that few_kernel takes
+  int32_t few_cap;                 // most tiles of a few split
+  int32_t chunk_rows;              // rows of a chunk block
+};
+
+__host__ __device__ inline int chunk_units(int head_dim) { return head_dim > 128 ? 128 : 256; }
+
+inline Sizes sizes_of(const Shape& s) {
+  Sizes z;
+  z.group = s.hq / s.hkv;
+  z.few_heads = z.group < kFewUnits ? z.group : kFewUnits;
+  z.head_blocks = ceil_div(z.group, kFewUnits);
+  z.few_rows = z.group <= kFewUnits ? kFewUnits / z.group : 1;
+  const int pages = 62 * (s.page / kFewTile);  // a wave holds a split's page ids, one a lane
+  z.few_cap = pages < kFewMost ? pages / 4 * 4 : kFewMost;
+  z.chunk_rows = chunk_units(s.head_dim) / z.group;
+  return z;
+}
+
+struct Layout {
+  size_t seq, few, chunk, join, ml, o, total;
+  int64_t most_few, most_chunk, most_join, slots;
+};
+
+inline Layout layout_of(const Shape& s) {
+  const Sizes z = sizes_of(s);
+  Layout l;
+  const int64_t few_rows = s.max_q < z.few_rows ? s.max_q : z.few_rows;
+  l.most_few = ceil_div64(kFewWGs, (int64_t)s.hkv * z.head_blocks) +
+               (int64_t)s.batch * (2 + ceil_div64(s.max_k / kFewTile + 2, z.few_cap));
+  l.slots = l.most_few * few_rows;
+  l.most_join = (int64_t)s.batch * few_rows;
+  l.most_chunk = 0;
+  if (s.max_q > z.few_rows) {
+    const int64_t rows = s.max_q < z.chunk_rows ? s.max_q : z.chunk_rows;
+    const int64_t unsplit = ceil_div64(kChunkWGs, s.hkv);  // splits exist below this many blocks
+    int64_t blocks = (int64_t)s.batch * ceil_div64(s.max_q, z.chunk_rows);
+    const int64_t by_rows = s.total_q / z.chunk_rows + s.batch;
+    blocks = blocks < by_rows ? blocks : by_rows;
+    l.most_chunk = blocks + unsplit + 1;
+    l.slots += (2 * unsplit + 1) * rows;
+    l.most_join += unsplit * rows;
+  }
+  size_t off = align256(H_WORDS * sizeof(int32_t));
+  l.seq = off;    off = align256(off + (size_t)s.batch * sizeof(int4));
+  l.few = off;    off = align256(off + (size_t)l.most_few * 2 * sizeof(int4));
+  l.chunk = off;  off = align256(off + (size_t)l.most_chunk * 2 * sizeof(int4));
+  l.join = off;   off = align256(off + (size_t)l.most_join * sizeof(int4));
+  l.ml = off;     off = align256(off + (size_t)l.slots * s.hq * sizeof(float2));
+  l.o = off;      off = align256(off + (size_t)l.slots * s.hq * s.head_dim * sizeof(float));
+  l.total = off;
+  return l;
+}
+
+// -------------------------------------------------------------------------------- plan
+//
+// Work lists, two int4 an entry:
+//   few:   {sequence, first key, key end, slot or -1} {first query row, rows, keys, -}
+//   chunk: {sequence, first row, first tile, tile end} {first query row, rows, keys, slot or -1}
+//   join:  {output row, first slot, slots from one split to the next, splits}
+// A slot holds the partial result of one query row, all heads.
+struct PlanArgs {
+  const int32_t* cu_q;
+  const int32_t* used;
+  int32_t* hdr;
+  int4* seq;
+  int4* few;
+  int4* chunk;
+  int4* join;
+  int64_t most_few, most_chunk, most_join, slots;
+  Shape s;
+  Sizes z;
+};
+
+// Keys [lo, hi) that rows [row0, row0 + rows) of a sequence with n rows and L keys see.
+__device__ __forceinline__ void keys_of(const Shape& s, int n, int L, int row0, int rows, int* lo, int* hi) {
+  const int64_t first = (int64_t)L - n + row0;
+  int64_t a = s.left >= 0 ? first - s.left : 0, b = s.right >= 0 ? first + rows + s.right : L;
+  a = a < 0 ? 0 : a;
+  b = b > L ? L : b;
+  *lo = (int)(a < L ? a : L);
+  *hi = (int)(b > *lo ? b : *lo);
+}
+
+// Exclusive prefix sum over the workgroup of three values; their totals.
+__device__ int3 plan_scan(int3 v, int3* total, int3 (*waves)) {
+  const int lane = hx::tid_x() & 63, w = hx::tid_x() >> 6;
+  int3 x = v;
+  for (int m = 1; m < 64; m <<= 1) {
+    const int a = __shfl_up(x.x, m), b = __shfl_up(x.y, m), c = __shfl_up(x.z, m);
+    if (lane >= m) {
+      x.x += a;
+      x.y += b;
+      x.z += c;
+    }
+  }
+  __syncthreads();
+  if (lane == 63) waves[w] = x;
+  __syncthreads();
+  int3 before = make_int3(0, 0, 0), all = make_int3(0, 0, 0);
+  for (int i = 0; i < kPlanThreads / 64; ++i) {
+    if (i < w) {
+      before.x += waves[i].x;
+      before.y += waves[i].y;
+      before.z += waves[i].z;
+    }
+    all.x += waves[i].x;
+    all.y += waves[i].y;
+    all.z += waves[i].z;
+  }
+  *total = all;
+  return make_int3(before.x + x.x - v.x, before.y + x.y - v.y, before.z + x.z - v.z);
+}
+
+// Which of the prefix sums p[0 .. n] (n of them and the total) holds i: the last at or below it.
+__device__ __forceinline__ int plan_find(const int* p, int n, int i) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p[mid] <= i) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int block_tiles(const PlanArgs& a, int n, int L, int row0, int* first) {
+  int lo, hi;
+  keys_of(a.s, n, L, row0, n - row0 < a.z.chunk_rows ? n - row0 : a.z.chunk_rows, &lo, &hi);
+  *first = lo / kChunkTile;
+  return hi > lo ? ceil_div(hi, kChunkTile) - *first : 0;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanArgs a) {
+  __shared__ int3 s_waves[kPlanThreads / 64];
+  __shared__ int s_items[kPlanThreads + 1], s_slots[kPlanThreads + 1], s_blocks[kPlanThreads + 1];
+  __shared__ unsigned long long s_few, s_tiles;
+  __shared__ int s_err, s_nblocks;
+  const int tid = hx::tid_x(), batch = a.s.batch;
+  if (tid == 0) {
+    s_few = s_tiles = 0;
+    s_err = s_nblocks = 0;
+  }
+  __syncthreads();
+  const int64_t room = (int64_t)a.s.width * a.s.page;
+  // Every sequence's rows and keys, checked, and the tick's tiles.
+  for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int n = 0, L = 0, blocks = 0;
+    if (b < batch) {
+      const int q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
+      int err = 0;
+      L = a.used[b];
+      if (q0 < 0 || q1 < q0 || q1 > a.s.total_q) {
+        err |= HX_WERR_BAD_CU_SEQ;
+      } else {
+        n = q1 - q0;
+        if (n > a.s.max_q) {
+          n = a.s.max_q;
+          err |= HX_WERR_CLAMPED_LEN;
+        }
+      }
+      const int64_t most = a.s.max_k < room ? a.s.max_k : room;
+      if (L < 0 || L > most) {
+        L = L < 0 ? 0 : (int)most;
+        err |= HX_WERR_CLAMPED_LEN;
+      }
+      if (err) atomicOr(&s_err, err);
+      a.seq[b] = make_int4(q0, n, L, 0);
+      if (n > 0 && n <= a.z.few_rows) {
+        int lo, hi;
+        keys_of(a.s, n, L, 0, n, &lo, &hi);
+        if (hi > lo) atomicAdd(&s_few, (unsigned long long)(ceil_div(hi, kFewTile) - lo / kFewTile));
+      } else if (n > 0) {
+        blocks = ceil_div(n, a.z.chunk_rows);
+      }
+    }
+    int3 total;
+    const int3 at = plan_scan(make_int3(blocks, 0, 0), &total, s_waves);
+    __syncthreads();
+    s_blocks[tid] = at.x;
+    if (tid == 0) s_nblocks += total.x;
+    __syncthreads();
+    unsigned long long tiles = 0;
+    for (int i = tid; i < total.x; i += kPlanThreads) {
+      const int j = plan_find(s_blocks, kPlanThreads, i);
+      const int4 si = a.seq[b0 + j];
+      int first;
+      tiles += (unsigned long long)block_tiles(a, si.y, si.z, (i - s_blocks[j]) * a.z.chunk_rows, &first);
+    }
+    if (tiles) atomicAdd(&s_tiles, tiles);
+    __syncthreads();
+  }
+  // Split sizes: for few rows, so that about kFewWGs workgroups run; blocks of chunk rows only
+  // when they are fewer than kChunkWGs.
+  const int64_t few_wgs = kFewWGs / (a.s.hkv * a.z.head_blocks) > 0 ? kFewWGs / (a.s.hkv * a.z.head_blocks) : 1;
+  int64_t fs = ((int64_t)s_few + few_wgs - 1) / few_wgs;
+  fs = (fs + 3) / 4 * 4;
+  const int few_split = (int)(fs < kFewLeast ? kFewLeast : fs > a.z.few_cap ? a.z.few_cap : fs);
+  int chunk_split = 1 << 30;
+  if ((int64_t)s_nblocks * a.s.hkv < kChunkWGs) {
+    const int64_t t = ((int64_t)s_tiles * a.s.hkv + kChunkWGs - 1) / kChunkWGs;
+    chunk_split = (int)(t < kChunkLeast ? kChunkLeast : t);
+  }
+  int few_base = 0, chunk_base = 0, slot_base = 0, join_base = 0;
+  for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int4 si = make_int4(0, 0, 0, 0);
+    int splits = 0, blocks = 0, rows = 0;
+    if (b < batch) {
+      si = a.seq[b];
+      if (si.y > 0 && si.y <= a.z.few_rows) {
+        int lo, hi;
+        keys_of(a.s, si.y, si.z, 0, si.y, &lo, &hi);
+        splits = hi > lo ? ceil_div(ceil_div(hi, kFewTile) - lo / kFewTile, few_split) : 1;
+        rows = si.y;
+      } else if (si.y > 0) {
+        blocks = ceil_div(si.y, a.z.chunk_rows);
+      }
+    }
+    const int joined = splits > 1 ? rows : 0;
+    int3 total, total2;
+    const int3 at = plan_scan(make_int3(splits, joined * splits, joined), &total, s_waves);
+    const int3 at2 = plan_scan(make_int3(blocks, 0, 0), &total2, s_waves);
+    __syncthreads();
+    s_items[tid] = at.x;
+    s_slots[tid] = at.y;
+    s_blocks[tid] = at2.x;
+    __syncthreads();
+    for (int r = 0; r < joined; ++r) {
+      const int64_t to = join_base + at.z + r;
+      if (to < a.most_join) a.join[to] = make_int4(si.x + r, slot_base + at.y + r, rows, splits);
+    }
+    for (int i = tid; i < total.x; i += kPlanThreads) {
+      const int j = plan_find(s_items, kPlanThreads, i);
+      const int4 of = a.seq[b0 + j];
+      int lo, hi;
+      keys_of(a.s, of.y, of.z, 0, of.y, &lo, &hi);
+      const int t0 = lo / kFewTile, tiles = hi > lo ? ceil_div(hi, kFewTile) - t0 : 0;
+      const int n = tiles > 0 ? ceil_div(tiles, few_split) : 1, sp = i - s_items[j];
+      // Shares of whole rounds of the waves, as even as they come.
+      const int share = ceil_div(ceil_div(tiles, n), 4) * 4;
+      const int from = t0 + (sp * share < tiles ? sp * share : tiles), to = from + share < t0 + tiles ? from + share : t0 + tiles;
+      const int64_t entry = few_base + i;
+      if (entry < a.most_few) {
+        a.few[2 * entry] = make_int4(b0 + j, from * kFewTile > lo ? from * kFewTile : lo, to * kFewTile < hi ? to * kFewTile : hi,
+                                     n > 1 ? slot_base + s_slots[j] + sp * of.y : -1);
+        a.few[2 * entry + 1] = make_int4(of.x, of.y, of.z, 0);
+      }
+    }
+    few_base += total.x;
+    slot_base += total.y;
+    join_base += total.z;
+    // Chunk blocks, a round of the threads at a time: their items, slots and joined rows follow
+    // those of the blocks before them. Later blocks of a sequence first: they see more keys.
+    for (int i0 = 0; i0 < total2.x; i0 += kPlanThreads) {
+      const int i = i0 + tid;
+      int n = 0, tiles = 0, first = 0, row0 = 0, rows_here = 0, j = 0;
+      int4 of = make_int4(0, 0, 0, 0);
+      if (i < total2.x) {
+        j = plan_find(s_blocks, kPlanThreads, i);
+        of = a.seq[b0 + j];
+        row0 = (ceil_div(of.y, a.z.chunk_rows) - 1 - (i - s_blocks[j])) * a.z.chunk_rows;
+        rows_here = of.y - row0 < a.z.chunk_rows ? of.y - row0 : a.z.chunk_rows;
+        tiles = block_tiles(a, of.y, of.z, row0, &first);
+        n = tiles > 0 ? ceil_div(tiles, chunk_split) : 1;
+      }
+      const int joins = n > 1 ? rows_here : 0;
+      int3 all;
+      const int3 to = plan_scan(make_int3(n, joins * n, joins), &all, s_waves);
+      const int share = n > 0 ? ceil_div(tiles, n) : 0;
+      for (int sp = 0; sp < n; ++sp) {
+        const int64_t entry = (int64_t)chunk_base + to.x + sp;
+        if (entry >= a.most_chunk) break;
+        const int from = first + (sp * share < tiles ? sp * share : tiles);
+        const int end = from + share < first + tiles ? from + share : first + tiles;
+        a.chunk[2 * entry] = make_int4(b0 + j, row0, from, end);
+        a.chunk[2 * entry + 1] = make_int4(of.x, of.y, of.z, n > 1 ? slot_base + to.y + sp * rows_here : -1);
+      }
+      for (int r = 0; r < joins; ++r) {
+        const int64_t entry = (int64_t)join_base + to.z + r;
+        if (entry < a.most_join) a.join[entry] = make_int4(of.x + row0 + r, slot_base + to.y + r, rows_here, n);
+      }
+      chunk_base += all.x;
+      slot_base += all.y;
+      join_base += all.z;
+    }
+    __syncthreads();
+  }
+  if (tid == 0) {
+    int err = s_err;
+    // By the bounds that the workspace was sized with none of these can happen.
+    if (few_base > a.most_few || chunk_base > a.most_chunk || join_base > a.most_join || slot_base > a.slots) err |= HX_WERR_GRID;
+    a.hdr[H_FEW] = few_base < a.most_few ? few_base : (int)a.most_few;
+    a.hdr[H_CHUNK] = chunk_base < a.most_chunk ? chunk_base : (int)a.most_chunk;
+    a.hdr[H_JOIN] = join_base < a.most_join ? join_base : (int)a.most_join;
+    a.hdr[H_ERR] = err;
+    const int32_t stamp[8] = {a.s.batch, a.s.total_q, a.s.max_q, a.s.max_k, a.s.hq, a.s.hkv, a.s.head_dim, a.s.page};
+    for (int i = 0; i < 8; ++i) a.hdr[H_STAMP + i] = stamp[i];
+  }
+}
+
+// --------------------------------------------------------------------------------- run
+struct RunArgs {
+  const uint16_t* q;
+  int64_t q_row, q_head;
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* k_scale;
+  const float* v_scale;
+  int32_t num_pages;
+  const int32_t* table;
+  int64_t table_stride;
+  float scale_log2;
+  uint16_t* out;
+  int64_t out_row, out_head;
+  int32_t* hdr;
+  const int4* few;
+  const int4* chunk;
+  const int4* join;
+  float2* part_ml;
+  float* part_o;
+  int64_t slots;
+  Shape s;
+  Sizes z;
+};
+
+// The plan's counts, if it was built for this shape.
+__device__ __forceinline__ bool plan_ok(const RunArgs& a, int4* counts) {
+  const int4 h0 = *reinterpret_cast<const int4*>(a.hdr), h1 = *reinterpret_cast<const int4*>(a.hdr + H_STAMP),
+             h2 = *reinterpret_cast<const int4*>(a.hdr + H_STAMP + 4);
+  *counts = h0;
+  const bool ok = h1.x == a.s.batch && h1.y == a.s.total_q && h1.z == a.s.max_q && h1.w == a.s.max_k && h2.x == a.s.hq &&
+                  h2.y == a.s.hkv && h2.z == a.s.head_dim && h2.w == a.s.page;
+  if (!ok && hx::wg_x() == 0 && hx::tid_x() == 0) atomicOr(&a.hdr[H_ERR], HX_WERR_PLAN_MISMATCH);
+  return ok;
+}
+
+__device__ __forceinline__ int4 uniform4(const int4* p) {
+  const int4 v = *p;
+  return make_int4(__builtin_amdgcn_readfirstlane(v.x), __builtin_amdgcn_readfirstlane(v.y),
+                   __builtin_amdgcn_readfirstlane(v.z), __builtin_amdgcn_readfirstlane(v.w));
+}
+
+// The power of two that takes magnitudes up to `top` (bits) to [2^14, 2^15), and its inverse.
+// Below 2^-107 magnitudes stay smaller than that: what they lose is nothing to a score.
+__device__ __forceinline__ float fit_up(uint32_t top) { return __uint_as_float((268u - max(top >> 23, 20u)) << 23); }
+__device__ __forceinline__ float fit_down(uint32_t top) { return __uint_as_float((max(top >> 23, 20u) - 14u) << 23); }
+
+// The largest finite magnitude's bits. (An infinite or NaN element passes through any power of two.)
+__device__ __forceinline__ uint32_t largest(const float (&x)[8], uint32_t top) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t b = hx::raw_bits(x[e]) & 0x7fffffffu;
+    top = max(top, b < 0x7f800000u ? b : 0u);
+  }
+  return top;
+}
+
+// Key positions `at + more`, which may lie far past the last key.
+__device__ __forceinline__ int beyond(int at, int more) {
+  const int64_t x = (int64_t)at + more;
+  return x < 0x7fffffff ? (int)x : 0x7fffffff;
+}
+
+template <typename T>
+__device__ __forceinline__ void widen8(uint4 u, float (&x)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[2 * e] = hx::Elem<T>::lo(w[e]);
+    x[2 * e + 1] = hx::Elem<T>::hi(w[e]);
+  }
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&x)[8], float by) {
+  return make_uint4(hx::pack2_round<_Float16>(x[0] * by, x[1] * by), hx::pack2_round<_Float16>(x[2] * by, x[3] * by),
+                    hx::pack2_round<_Float16>(x[4] * by, x[5] * by), hx::pack2_round<_Float16>(x[6] * by, x[7] * by));
+}
+
+template <typename C>
+__device__ __forceinline__ hx::f16x8_t codes8(uint2 w) {
+  const uint2 a = hx8::to_f16<C>(w.x), b = hx8::to_f16<C>(w.y);
+  return hx::as_v8<_Float16>(make_uint4(a.x, a.y, b.x, b.y));
+}
+
+__device__ __forceinline__ uint2 ld8_lds_tr8(const void* p) {
+  typedef int v2i __attribute__((ext_vector_type(2)));
+  const v2i r = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(p));
+  return __builtin_bit_cast(uint2, r);
+}
+
+// LDS position of 16-byte piece p of value row r, of DP bytes: 16 rows' pieces of one dim block
+// then cover all banks once.
+template <int DP>
+__device__ __forceinline__ int v8_piece(int r, int p) {
+  return DP == 64 ? p ^ ((r >> 2) & 3) : DP == 128 ? p ^ ((r >> 1) & 7) : p ^ (r & 15);
+}
+
+constexpr float kFewShift = 14.f;  // weights are scaled by 2^14 into fp16, and their remainders stay normal
+
+// One item and KV head (and block of 16 query heads) to a workgroup. The units, (row, head) pairs,
+// are the columns of S^T = K Q^T. A wave walks every fourth 32-key tile on its own, the next one's
+// codes in flight in registers: key codes are the MFMA's operand as they are loaded (lane r of a
+// 16-lane group takes key 8 (r / 4) + 4 u + r % 4 for block u, so that a lane's 8 scores belong to 8
+// consecutive keys), value codes pass through LDS to be read transposed. Up to 8 units have a
+// second set of columns, which carries the weights' remainders; more take a second MFMA: 22 bits.
+template <typename T, typename C, int DP>
+__global__ __launch_bounds__(kFewThreads) void kv8_few_kernel(RunArgs a, int n_wg) {
+  typedef hx::f16x8_t v8;
+  typedef hx::Elem<_Float16> E;
+  constexpr int kLoads = DP / 64, kSteps = DP / 32, kDims = DP / 16, kPieces = DP / 16, kVLoads = DP / 32;
+  constexpr int kStage = kFewTile * DP;
+  constexpr int kLdsBytes = 4 * kStage > 4 * kFewUnits * DP * 4 ? 4 * kStage : 4 * kFewUnits * DP * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kLdsBytes];
+  __shared__ float s_m[4][kFewUnits], s_l[4][kFewUnits];
+  const int tid = hx::tid_x(), lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int4 counts;
+  if (!plan_ok(a, &counts)) return;
+  const int per_item = a.s.hkv * a.z.head_blocks, D = a.s.head_dim, page = a.s.page;
+  const int64_t work = (int64_t)counts.x * per_item;
+  const uint32_t row_bytes = (uint32_t)a.s.hkv * (uint32_t)D;
+  uint8_t* const vt = smem + w * kStage;
+
+  for (int64_t i = hx::wg_x(); i < work; i += n_wg) {
+    const int item = (int)((uint32_t)i / (uint32_t)per_item), sub = (int)((uint32_t)i % (uint32_t)per_item);
+    const int hb = sub / a.s.hkv, h = sub - hb * a.s.hkv;
+    const int4 it = uniform4(a.few + 2 * (int64_t)item), si = uniform4(a.few + 2 * (int64_t)item + 1);
+    const int k0 = it.y, k1 = it.z, n = si.y, L = si.z;
+    const int heads = min(a.z.few_heads, a.z.group - hb * kFewUnits), units = n * heads;
+    const int head0 = h * a.z.group + hb * kFewUnits;
+    const bool twice = units <= 8;
+    const int unit = twice ? lr & 7 : lr;
+    const bool live = unit < units;
+    const int urow = live ? unit / heads : 0, uhead = head0 + (live ? unit - urow * heads : 0);
+
+    v8 qf[kSteps];
+    float qc;  // of this lane's unit: log2(e) scale, and what undoes q's power of two
+    {
+      float x[kSteps][8];
+      uint32_t top = 0;
+      const uint16_t* const qp = a.q + (int64_t)(si.x + urow) * a.q_row + (int64_t)uhead * a.q_head;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int d = 64 * (s >> 1) + 16 * lg + 8 * (s & 1);
+        widen8<T>(live && d < D ? *reinterpret_cast<const uint4*>(qp + d) : hx::zero4(), x[s]);
+        top = largest(x[s], top);
+      }
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+      const float up = fit_up(top);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) qf[s] = hx::as_v8<_Float16>(pack8(x[s], up));
+      qc = a.scale_log2 * fit_down(top);
+    }
+    // Keys this lane's unit sees of the item's. (Columns without a unit have q = 0 and go nowhere.)
+    int klo = k0, khi = k1 - 1;
+    {
+      const int at = L - n + urow;
+      if (a.s.left >= 0) klo = max(klo, at > a.s.left ? at - a.s.left : 0);
+      if (a.s.right >= 0) khi = min(khi, beyond(at, a.s.right));
+    }
+
+    const int t0 = k0 / kFewTile, t1 = k1 > k0 ? (k1 + kFewTile - 1) / kFewTile : t0;
+    // Page ids of the item's keys: lane j holds that of page pg0 + j.
+    const int pg0 = t0 * kFewTile / page;
+    int ids = -1;
+    if (t1 > t0 && pg0 + lane <= (k1 - 1) / page) ids = a.table[(int64_t)it.x * a.table_stride + pg0 + lane];
+
+    uint4 kb[2][kLoads], vb[kVLoads];
+    float4 ks[2], vs[2];
+    int next_cnt = 0;
+    bool bad = false;
+    auto load = [&](int t) __attribute__((always_inline)) {
+      const int key0 = t * kFewTile, j = key0 / page;
+      int id = __builtin_amdgcn_readlane(ids, j - pg0);
+      const bool off = (unsigned)id >= (unsigned)a.num_pages;
+      bad |= off;
+      id = off ? 0 : id;
+      const int cnt = off ? 0 : min(kFewTile, k1 - key0);
+      next_cnt = cnt;
+      const int64_t in = key0 - j * page;
+      const int64_t base = (((int64_t)id * page + in) * a.s.hkv + h) * D;
+      const uint32_t bytes = cnt > 0 ? (uint32_t)(cnt - 1) * row_bytes + (uint32_t)D : 0u;
+      const __amdgpu_buffer_rsrc_t kr = hx::buffer_rsrc(a.k + base, bytes), vr = hx::buffer_rsrc(a.v + base, bytes);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q) {
+          const int d = 64 * q + 16 * lg;
+          const uint32_t at = (uint32_t)(8 * (lr >> 2) + 4 * u + (lr & 3)) * row_bytes + (uint32_t)d;
+          kb[u][q] = hx::ld16_stream(kr, d < D ? at : 0x7ffffff0u, 0);
+        }
+      const int piece = lane % kPieces, tok = lane / kPieces;
+#pragma unroll
+      for (int q = 0; q < kVLoads; ++q)
+        vb[q] = hx::ld16_stream(vr, 16 * piece < D ? (uint32_t)(tok + q * (64 / kPieces)) * row_bytes + 16u * piece : 0x7ffffff0u, 0);
+      const int64_t st = ((int64_t)id * a.s.hkv + h) * page + in + 8 * lg;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        ks[e] = *reinterpret_cast<const float4*>(a.k_scale + st + 4 * e);
+        vs[e] = *reinterpret_cast<const float4*>(a.v_scale + st + 4 * e);
+      }
+    };
+
+    float m_run = -INFINITY, l_run = 0.f;
+    hx::f32x4_t o[kDims];
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) o[d] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+    int t = t0 + w;
+    if (t < t1) load(t);
+    while (t < t1) {
+      const int key0 = t * kFewTile, cnt = next_cnt;
+#pragma unroll
+      for (int q = 0; q < kVLoads; ++q) {
+        const int r = lane / kPieces + q * (64 / kPieces);
+        *reinterpret_cast<uint4*>(vt + r * DP + 16 * v8_piece<DP>(r, lane % kPieces)) = vb[q];
+      }
+      // Lanes read what others of the wave stored: a wave's LDS accesses complete in order, the
+      // fences hold the compiler to it.
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      hx::f32x4_t sc[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        sc[u] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q) {
+          sc[u] = E::mfma16x16x32(codes8<C>(make_uint2(kb[u][q].x, kb[u][q].y)), qf[2 * q], sc[u]);
+          sc[u] = E::mfma16x16x32(codes8<C>(make_uint2(kb[u][q].z, kb[u][q].w)), qf[2 * q + 1], sc[u]);
+        }
+      }
+      const float kf[8] = {ks[0].x, ks[0].y, ks[0].z, ks[0].w, ks[1].x, ks[1].y, ks[1].z, ks[1].w};
+      const float vf[8] = {vs[0].x, vs[0].y, vs[0].z, vs[0].w, vs[1].x, vs[1].y, vs[1].z, vs[1].w};
+      float u[8], inv[8];
+      t += 4;
+      const int next = t;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        u[e] = fmaf(sc[e >> 2][e & 3], kf[e] * qc, __builtin_amdgcn_logf(vf[e]));
+        inv[e] = __builtin_amdgcn_rcpf(vf[e]);
+      }
+      if (next < t1) load(next);
+      const int from = key0 + 8 * lg, last = min(khi, key0 + cnt - 1);
+      if (__any(from < klo || from + 7 > last)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool seen = from + e >= klo && from + e <= last;
+          u[e] = seen ? u[e] : -INFINITY;
+          inv[e] = seen ? inv[e] : 0.f;
+        }
+      }
+      float mx = m_run;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, u[e]);
+      mx = hx::max_xor32(hx::max_xor16(mx));
+      const float alpha = mx == -INFINITY ? 1.f : hx::fast_exp2(m_run - mx);
+      const float neg = mx == -INFINITY ? 0.f : kFewShift - mx;
+      m_run = mx;
+      l_run *= alpha;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) o[d] *= alpha;
+      uint32_t pw[4], pr[4];
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float p0 = hx::fast_exp2(u[e] + neg), p1 = hx::fast_exp2(u[e + 1] + neg);
+        l_run = fmaf(p0, inv[e], l_run);
+        l_run = fmaf(p1, inv[e + 1], l_run);
+        const uint32_t top = hx::pack2_round<_Float16>(p0, p1);
+        pr[e / 2] = hx::pack2_round<_Float16>(p0 - E::lo(top), p1 - E::hi(top));
+        pw[e / 2] = twice && lr >= 8 ? pr[e / 2] : top;
+      }
+      const v8 pf = hx::as_v8<_Float16>(make_uint4(pw[0], pw[1], pw[2], pw[3]));
+      const v8 pf2 = hx::as_v8<_Float16>(make_uint4(pr[0], pr[1], pr[2], pr[3]));
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) {
+        const int r = 8 * lg + (lr >> 1);
+        const v8 vv = codes8<C>(ld8_lds_tr8(vt + r * DP + 16 * v8_piece<DP>(r, d) + 8 * (lr & 1)));
+        o[d] = E::mfma16x16x32(vv, pf, o[d]);
+        if (!twice) o[d] = E::mfma16x16x32(vv, pf2, o[d]);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    if (bad && lane == 0) atomicOr(&a.hdr[H_ERR], HX_WERR_BAD_PAGE);
+
+    // Lane: dims 16 d + 4 lg .. + 3 of its unit; remainders' columns added.
+    l_run = hx::add_xor32(hx::add_xor16(l_run));
+    if (twice) {
+#pragma unroll
+      for (int d = 0; d < kDims; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] += hx::dpp<0x128>(o[d][e]);  // the lane 8 apart in its row of 16
+    }
+    __syncthreads();  // every wave is done with its stage
+    float (*const s_o)[kFewUnits][DP] = reinterpret_cast<float (*)[kFewUnits][DP]>(smem);
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+      *reinterpret_cast<float4*>(&s_o[w][lr][16 * d + 4 * lg]) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+    if (lg == 0) {
+      s_m[w][lr] = m_run;
+      s_l[w][lr] = l_run;
+    }
+    __syncthreads();
+    const int half = D / 2;
+    for (int e = tid; e < units * half; e += kFewThreads) {
+      const int un = e / half, d = 2 * (e % half);
+      float m = s_m[0][un];
+#pragma unroll
+      for (int ww = 1; ww < 4; ++ww) m = fmaxf(m, s_m[ww][un]);
+      const float ref = m == -INFINITY ? 0.f : m;
+      float l = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+      for (int ww = 0; ww < 4; ++ww) {
+        const float f = hx::fast_exp2(s_m[ww][un] - ref);
+        l = fmaf(f, s_l[ww][un], l);
+        x = fmaf(f, s_o[ww][un][d], x);
+        y = fmaf(f, s_o[ww][un][d + 1], y);
+      }
+      const int row = un / heads, head = head0 + un - row * heads;
+      if (it.w < 0) {
+        const float r = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+        *reinterpret_cast<uint32_t*>(a.out + (int64_t)(si.x + row) * a.out_row + (int64_t)head * a.out_head + d) =
+            hx::pack2_round<T>(x * r, y * r);
+      } else if ((int64_t)it.w + row < a.slots) {
+        const int64_t p = ((int64_t)it.w + row) * a.s.hq + head;
+        *reinterpret_cast<float2*>(a.part_o + p * D + d) = make_float2(x, y);
+        if (d == 0) a.part_ml[p] = make_float2(m, l);
+      }
+    }
+    __syncthreads();  // the next item's stages take the place of s_o
+  }
+}
+
+// ------------------------------------------------------------------------------- chunks
+constexpr float kChunkShift = 7.f;  // 2^7 times weights of up to 2^8 fits fp16
+constexpr float kLazy = 8.f;        // the reference maximum moves when exceeded by this, in log2
+
+template <int DP>
+__device__ __forceinline__ int k16_piece(int r, int c) { return DP == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15); }
+template <int DP>
+__device__ __forceinline__ int v16_piece(int r, int c) { return DP == 64 ? c ^ (2 * ((r >> 1) & 3)) : c ^ (2 * (r & 7)); }
+
+// One item and KV head to a workgroup of 8 waves: wave w owns units 16 RB w .. + 16 RB - 1, (row,
+// head) pairs with the group's heads fastest. 64-key tiles of K and V go from HBM through registers,
+// where the workgroup widens their codes to fp16 once for all waves, into two LDS buffers in turn:
+// a tile's loads are in flight for a whole tile, and one barrier a tile suffices.
+// The weights go into P V as one fp16 (11 bits, an eighth of a bf16 output's rounding), or with
+// fp16 outputs as two.
+template <typename T, typename C, int DP>
+__global__ __launch_bounds__(kChunkThreads, 2) void kv8_chunk_kernel(RunArgs a, int n_wg) {
+  typedef hx::f16x8_t v8;
+  typedef hx::Elem<_Float16> E;
+  constexpr bool kTwo = __is_same(T, _Float16);
+  constexpr int RB = DP == 256 ? 1 : 2, kSteps = DP / 32, kDims = DP / 16, kPieces = DP / 16;
+  constexpr int kRow = 2 * DP, kTileBytes = kChunkTile * kRow, kMine = DP / 64;  // pieces a thread moves
+  __shared__ __attribute__((aligned(16))) uint8_t s_k[2][kTileBytes];
+  __shared__ __attribute__((aligned(16))) uint8_t s_v[2][kTileBytes];
+  __shared__ __attribute__((aligned(16))) float s_ks[2][kChunkTile], s_lv[2][kChunkTile], s_iv[2][kChunkTile];
+  const int tid = hx::tid_x(), lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int4 counts;
+  if (!plan_ok(a, &counts)) return;
+  const int D = a.s.head_dim, page = a.s.page, G = a.z.group;
+  const int64_t work = (int64_t)counts.y * a.s.hkv;
+  const uint32_t row_bytes = (uint32_t)a.s.hkv * (uint32_t)D;
+
+  for (int64_t i = hx::wg_x(); i < work; i += n_wg) {
+    const int item = (int)((uint32_t)i / (uint32_t)a.s.hkv), h = (int)((uint32_t)i % (uint32_t)a.s.hkv);
+    const int4 it = uniform4(a.chunk + 2 * (int64_t)item), si = uniform4(a.chunk + 2 * (int64_t)item + 1);
+    const int row0 = it.y, t_begin = it.z, t_end = it.w, n = si.y, L = si.z;
+    const int rows = min(a.z.chunk_rows, n - row0), units = rows * G;
+
+    // Q^T as the MFMA's B operand, and the keys each of this lane's units sees.
+    v8 qf[RB][kSteps];
+    float qc;
+    int klo[RB], khi[RB], urow[RB], uhead[RB];
+    bool live[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const int u = 16 * (RB * w + rb) + lr;
+      live[rb] = u < units;
+      urow[rb] = live[rb] ? u / G : 0;
+      uhead[rb] = h * G + (live[rb] ? u - urow[rb] * G : 0);
+      const int at = L - n + row0 + urow[rb];
+      klo[rb] = a.s.left >= 0 && at > a.s.left ? at - a.s.left : 0;
+      khi[rb] = a.s.right >= 0 ? min(L - 1, beyond(at, a.s.right)) : L - 1;
+    }
+    {
+      uint32_t top = 0;
+      uint4 raw[RB][kSteps];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        const uint16_t* const qp = a.q + (int64_t)(si.x + row0 + urow[rb]) * a.q_row + (int64_t)uhead[rb] * a.q_head;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const int d = 32 * s + 8 * lg;
+          raw[rb][s] = live[rb] && d < D ? *reinterpret_cast<const uint4*>(qp + d) : hx::zero4();
+          float x[8];
+          widen8<T>(raw[rb][s], x);
+          top = largest(x, top);
+        }
+      }
+      // One power of two for the wave's units.
+      for (int m = 1; m < 64; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m));
+      top = __builtin_amdgcn_readfirstlane((int)top);
+      const float up = fit_up(top);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          float x[8];
+          widen8<T>(raw[rb][s], x);
+          qf[rb][s] = hx::as_v8<_Float16>(pack8(x, up));
+        }
+      qc = a.scale_log2 * fit_down(top);
+    }
+    // Keys that any unit of the wave sees, and those that all of them do.
+    int any_lo = 0x7fffffff, any_hi = -1, all_lo = 0, all_hi = 0x7fffffff;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      any_lo = live[rb] ? min(any_lo, klo[rb]) : any_lo;
+      any_hi = live[rb] ? max(any_hi, khi[rb]) : any_hi;
+      all_lo = live[rb] ? max(all_lo, klo[rb]) : all_lo;
+      all_hi = live[rb] ? min(all_hi, khi[rb]) : all_hi;
+    }
+    for (int m = 1; m < 16; m <<= 1) {
+      any_lo = min(any_lo, __shfl_xor(any_lo, m));
+      any_hi = max(any_hi, __shfl_xor(any_hi, m));
+      all_lo = max(all_lo, __shfl_xor(all_lo, m));
+      all_hi = min(all_hi, __shfl_xor(all_hi, m));
+    }
+    any_lo = __builtin_amdgcn_readfirstlane(any_lo);
+    any_hi = __builtin_amdgcn_readfirstlane(any_hi);
+    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+
+    // Page ids, 64 at a time: lane j holds that of page pg0 + j.
+    const int last_pg = t_end > t_begin ? (min(L, t_end * kChunkTile) - 1) / page : -1;
+    int pg0 = t_begin * kChunkTile / page, ids = -1;
+    auto fetch = [&]() {
+      ids = pg0 + lane <= last_pg ? a.table[(int64_t)it.x * a.table_stride + pg0 + lane] : -1;
+    };
+    fetch();
+    bool bad = false;
+    uint4 reg[kMine];
+    float sreg = 0.f;
+    int cnt_next = 0;
+    auto load = [&](int t) __attribute__((always_inline)) {
+      const int key0 = t * kChunkTile, j = key0 / page;
+      if (j - pg0 >= 64) {
+        pg0 = j;
+        fetch();
+      }
+      int id = __builtin_amdgcn_readlane(ids, j - pg0);
+      const bool off = (unsigned)id >= (unsigned)a.num_pages;
+      bad |= off;
+      id = off ? 0 : id;
+      cnt_next = off ? 0 : min(kChunkTile, L - key0);
+      const int64_t in = key0 - j * page;
+      const int64_t base = (((int64_t)id * page + in) * a.s.hkv + h) * D;
+      const uint32_t bytes = cnt_next > 0 ? (uint32_t)(cnt_next - 1) * row_bytes + (uint32_t)D : 0u;
+      const __amdgpu_buffer_rsrc_t kr = hx::buffer_rsrc(a.k + base, bytes), vr = hx::buffer_rsrc(a.v + base, bytes);
+#pragma unroll
+      for (int e = 0; e < kMine; ++e) {
+        // The first half of the pieces are K's (DP = 64: of the threads).
+        const bool of_v = DP == 64 ? w >= 4 : 2 * e >= kMine;
+        const int p = DP == 64 ? tid & 255 : tid + (2 * e >= kMine ? e - kMine / 2 : e) * kChunkThreads;
+        const int r = p / kPieces, c = p % kPieces;
+        reg[e] = hx::ld16_buf(of_v ? vr : kr, 16 * c < D ? (uint32_t)r * row_bytes + 16u * c : 0x7ffffff0u);
+      }
+      if (w < 2) sreg = (w ? a.v_scale : a.k_scale)[((int64_t)id * a.s.hkv + h) * page + in + lane];
+    };
+    // Into buffer b: codes as fp16, scales as the softmax takes them.
+    auto store = [&](int b, int cnt) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < kMine; ++e) {
+        const bool of_v = DP == 64 ? w >= 4 : 2 * e >= kMine;
+        const int p = DP == 64 ? tid & 255 : tid + (2 * e >= kMine ? e - kMine / 2 : e) * kChunkThreads;
+        const int r = p / kPieces, c = p % kPieces;
+        const uint2 x0 = hx8::to_f16<C>(reg[e].x), x1 = hx8::to_f16<C>(reg[e].y), x2 = hx8::to_f16<C>(reg[e].z),
+                    x3 = hx8::to_f16<C>(reg[e].w);
+        uint8_t* const to = (of_v ? s_v[b] : s_k[b]) + r * kRow;
+        const int c0 = of_v ? v16_piece<DP>(r, 2 * c) : k16_piece<DP>(r, 2 * c);
+        const int c1 = of_v ? v16_piece<DP>(r, 2 * c + 1) : k16_piece<DP>(r, 2 * c + 1);
+        *reinterpret_cast<uint4*>(to + 16 * c0) = make_uint4(x0.x, x0.y, x1.x, x1.y);
+        *reinterpret_cast<uint4*>(to + 16 * c1) = make_uint4(x2.x, x2.y, x3.x, x3.y);
+      }
+      if (w == 0) {
+        s_ks[b][lane] = lane < cnt ? sreg : 0.f;
+      } else if (w == 1) {
+        s_lv[b][lane] = lane < cnt ? __builtin_amdgcn_logf(sreg) : 0.f;
+        s_iv[b][lane] = lane < cnt ? __builtin_amdgcn_rcpf(sreg) : 0.f;
+      }
+    };
+
+    hx::f32x4_t o[kDims][RB];
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) o[d][rb] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m_run[RB], l_run[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      m_run[rb] = -INFINITY;
+      l_run[rb] = 0.f;
+    }
+
+    int cnt = 0;
+    if (t_begin < t_end) {
+      load(t_begin);
+      cnt = cnt_next;
+      store(t_begin & 1, cnt);
+      if (t_begin + 1 < t_end) load(t_begin + 1);
+    }
+    for (int t = t_begin; t < t_end; ++t) {
+      const int b = t & 1, key0 = t * kChunkTile, here = cnt;
+      __syncthreads();  // tile t is stored, and every wave is done with tile t - 1
+      if (t + 1 < t_end) {
+        cnt = cnt_next;
+        store(b ^ 1, cnt);
+        if (t + 2 < t_end) load(t + 2);
+      }
+      if (key0 > any_hi || key0 + kChunkTile - 1 < any_lo) continue;
+
+      hx::f32x4_t sc[4][RB];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) sc[kb][rb] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+          const int r = 16 * kb + lr;
+          const v8 kf = hx::as_v8<_Float16>(*reinterpret_cast<const uint4*>(s_k[b] + r * kRow + 16 * k16_piece<DP>(r, 4 * s + lg)));
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) sc[kb][rb] = E::mfma16x16x32(kf, qf[rb][s], sc[kb][rb]);
+        }
+      // Lane: keys 16 kb + 4 lg + e of its units.
+      float4 iv[4];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+        const float4 ks = *reinterpret_cast<const float4*>(&s_ks[b][16 * kb + 4 * lg]);
+        const float4 lv = *reinterpret_cast<const float4*>(&s_lv[b][16 * kb + 4 * lg]);
+        iv[kb] = *reinterpret_cast<const float4*>(&s_iv[b][16 * kb + 4 * lg]);
+        const float k4[4] = {ks.x * qc, ks.y * qc, ks.z * qc, ks.w * qc}, l4[4] = {lv.x, lv.y, lv.z, lv.w};
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[kb][rb][e] = fmaf(sc[kb][rb][e], k4[e], l4[e]);
+      }
+      const bool whole = here == kChunkTile && key0 >= all_lo && key0 + kChunkTile - 1 <= all_hi;
+      float mx[RB];
+      bool move[RB];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        if (!whole) {
+          const int from = key0 + 4 * lg, lo = klo[rb] - from, hi = min(khi[rb], key0 + here - 1) - from;
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint64_t hidden =
+                  __builtin_amdgcn_ballot_w64(16 * kb + e < lo) | __builtin_amdgcn_ballot_w64(16 * kb + e > hi);
+              sc[kb][rb][e] = hx::lane_sel(hidden, -INFINITY, sc[kb][rb][e]);
+            }
+        }
+        float m = fmaxf(fmaxf(sc[0][rb][0], sc[0][rb][1]), fmaxf(sc[0][rb][2], sc[0][rb][3]));
+#pragma unroll
+        for (int kb = 1; kb < 4; ++kb)
+          m = fmaxf(m, fmaxf(fmaxf(sc[kb][rb][0], sc[kb][rb][1]), fmaxf(sc[kb][rb][2], sc[kb][rb][3])));
+        mx[rb] = hx::max_xor32(hx::max_xor16(m));
+        move[rb] = mx[rb] > m_run[rb] + kLazy;
+      }
+      bool moved = move[0];
+#pragma unroll
+      for (int rb = 1; rb < RB; ++rb) moved = moved || move[rb];
+      if (__any(moved)) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          const float alpha = move[rb] ? hx::fast_exp2(m_run[rb] - mx[rb]) : 1.f;
+          m_run[rb] = move[rb] ? mx[rb] : m_run[rb];
+          l_run[rb] *= alpha;
+#pragma unroll
+          for (int d = 0; d < kDims; ++d) o[d][rb] *= alpha;
+        }
+      }
+      v8 pf[2][RB], pf2[2][RB];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        const float neg = m_run[rb] == -INFINITY ? 0.f : kChunkShift - m_run[rb];
+        float sum = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+          const float i4[4] = {iv[kb].x, iv[kb].y, iv[kb].z, iv[kb].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sc[kb][rb][e] = hx::fast_exp2(sc[kb][rb][e] + neg);
+            // A key that is hidden has the weight 0 under any scale, a NaN too.
+            if (whole) sum = fmaf(sc[kb][rb][e], i4[e], sum);
+            else sum += sc[kb][rb][e] == 0.f ? 0.f : sc[kb][rb][e] * i4[e];
+          }
+        }
+        l_run[rb] += sum;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          const hx::f32x4_t &x = sc[2 * ks][rb], &y = sc[2 * ks + 1][rb];
+          const uint32_t p[4] = {hx::pack2_round<_Float16>(x[0], x[1]), hx::pack2_round<_Float16>(x[2], x[3]),
+                                 hx::pack2_round<_Float16>(y[0], y[1]), hx::pack2_round<_Float16>(y[2], y[3])};
+          pf[ks][rb] = hx::as_v8<_Float16>(make_uint4(p[0], p[1], p[2], p[3]));
+          if constexpr (kTwo)
+            pf2[ks][rb] = hx::as_v8<_Float16>(
+                make_uint4(hx::pack2_round<_Float16>(x[0] - E::lo(p[0]), x[1] - E::hi(p[0])),
+                           hx::pack2_round<_Float16>(x[2] - E::lo(p[1]), x[3] - E::hi(p[1])),
+                           hx::pack2_round<_Float16>(y[0] - E::lo(p[2]), y[1] - E::hi(p[2])),
+                           hx::pack2_round<_Float16>(y[2] - E::lo(p[3]), y[3] - E::hi(p[3]))));
+        }
+      }
+      // O^T += V^T P^T, V^T read transposed: keys 32 ks + 4 lg + 0..3 and 16 further of dim 16 d + lr.
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const int r0 = 32 * ks + 4 * lg + (lr >> 2), r1 = r0 + 16;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) {
+          const int c = 2 * d + ((lr >> 1) & 1);
+          const uint2 lo = hx::ld8_lds_tr16(s_v[b] + r0 * kRow + 16 * v16_piece<DP>(r0, c) + 8 * (lr & 1));
+          const uint2 hi = hx::ld8_lds_tr16(s_v[b] + r1 * kRow + 16 * v16_piece<DP>(r1, c) + 8 * (lr & 1));
+          const v8 vv = hx::as_v8<_Float16>(make_uint4(lo.x, lo.y, hi.x, hi.y));
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) {
+            o[d][rb] = E::mfma16x16x32(vv, pf[ks][rb], o[d][rb]);
+            if constexpr (kTwo) o[d][rb] = E::mfma16x16x32(vv, pf2[ks][rb], o[d][rb]);
+          }
+        }
+      }
+    }
+    if (bad && tid == 0) atomicOr(&a.hdr[H_ERR], HX_WERR_BAD_PAGE);
+
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const float l = hx::add_xor32(hx::add_xor16(l_run[rb]));
+      if (!live[rb]) continue;
+      if (si.w < 0) {
+        const float r = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+        uint16_t* const to = a.out + (int64_t)(si.x + row0 + urow[rb]) * a.out_row + (int64_t)uhead[rb] * a.out_head;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+          if (16 * d < D) {
+            uint32_t* const p = reinterpret_cast<uint32_t*>(to + 16 * d + 4 * lg);
+            p[0] = hx::pack2_round<T>(o[d][rb][0] * r, o[d][rb][1] * r);
+            p[1] = hx::pack2_round<T>(o[d][rb][2] * r, o[d][rb][3] * r);
+          }
+      } else if ((int64_t)si.w + urow[rb] < a.slots) {
+        const int64_t p = ((int64_t)si.w + urow[rb]) * a.s.hq + uhead[rb];
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+          if (16 * d < D)
+            *reinterpret_cast<float4*>(a.part_o + p * D + 16 * d + 4 * lg) = make_float4(o[d][rb][0], o[d][rb][1], o[d][rb][2], o[d][rb][3]);
+        if (lg == 0) a.part_ml[p] = make_float2(m_run[rb], l);
+      }
+    }
+    __syncthreads();  // every wave is done with the last tile before the next item's first is stored
+  }
+}
+
+// -------------------------------------------------------------------------------- join
+// The splits of an output row and query head: a thread takes four dims of every n-th split, in
+// order, then the groups of threads are summed in order.
+constexpr int kJoinThreads = 256;
+
+template <typename T>
+__global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(RunArgs a, int n_wg) {
+  __shared__ float s_max[4];
+  __shared__ float4 s_o[kJoinThreads];
+  __shared__ float s_l[kJoinThreads];
+  int4 counts;
+  if (!plan_ok(a, &counts)) return;
+  const int tid = hx::tid_x(), D = a.s.head_dim, quads = D / 4, groups = kJoinThreads / quads;
+  const int g = tid / quads, d = 4 * (tid % quads);
+  const int64_t work = (int64_t)counts.z * a.s.hq;
+  for (int64_t i = hx::wg_x(); i < work; i += n_wg) {
+    const int rec = (int)((uint32_t)i / (uint32_t)a.s.hq), head = (int)((uint32_t)i % (uint32_t)a.s.hq);
+    const int4 r = uniform4(a.join + rec);
+    const int splits = r.w;
+    if (r.x < 0 || r.x >= a.s.total_q || r.y < 0 || splits < 1 || (int64_t)r.y + (int64_t)(splits - 1) * r.z >= a.slots) continue;
+    float m = -INFINITY;
+    for (int s = tid; s < splits; s += kJoinThreads) m = fmaxf(m, a.part_ml[((int64_t)r.y + (int64_t)s * r.z) * a.s.hq + head].x);
+    for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+    if ((tid & 63) == 0) s_max[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (g < groups) {
+      for (int s = g; s < splits; s += groups) {
+        const int64_t p = ((int64_t)r.y + (int64_t)s * r.z) * a.s.hq + head;
+        const float2 ml = a.part_ml[p];
+        const float4 o = *reinterpret_cast<const float4*>(a.part_o + p * D + d);
+        const float f = hx::fast_exp2(ml.x - ref);
+        l = fmaf(f, ml.y, l);
+        x.x = fmaf(f, o.x, x.x);
+        x.y = fmaf(f, o.y, x.y);
+        x.z = fmaf(f, o.z, x.z);
+        x.w = fmaf(f, o.w, x.w);
+      }
+    }
+    s_o[tid] = x;
+    s_l[tid] = l;
+    __syncthreads();
+    if (tid < quads) {
+      for (int k = 1; k < groups; ++k) {
+        const float4 o = s_o[tid + k * quads];
+        l += s_l[tid + k * quads];
+        x.x += o.x;
+        x.y += o.y;
+        x.z += o.z;
+        x.w += o.w;
+      }
+      const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+      uint32_t* const to = reinterpret_cast<uint32_t*>(a.out + (int64_t)r.x * a.out_row + (int64_t)head * a.out_head + d);
+      to[0] = hx::pack2_round<T>(x.x * inv, x.y * inv);
+      to[1] = hx::pack2_round<T>(x.z * inv, x.w * inv);
+    }
+    __syncthreads();
+  }
+}
+
+// -------------------------------------------------------------------------------- host
+int check_shape(const Shape& s) {
+  if (s.batch < 0 || s.total_q < 0 || s.max_q < 0 || s.max_k < 0 || s.hq < 1 || s.hkv < 1 || s.hq % s.hkv || s.width < 1 ||
+      s.head_dim < 1 || s.page < 1)
+    return HX_E_INVALID_ARG;
+  if (s.head_dim % 16 || s.head_dim > 256 || s.page % 64 || s.hq / s.hkv > 128 || s.max_k > 0x7fffff00 - s.page ||
+      (int64_t)s.hkv * s.head_dim > (1 << 22) || s.hkv > 1024)
+    return HX_E_UNSUPPORTED;  // a tile must fit a buffer resource, item indexes 32 bits
+  return HX_OK;
+}
+
+struct Run {
+  RunArgs a;
+  Layout l;
+  hipStream_t s;
+};
+
+template <typename T, typename C, int DP>
+void launch_run(const Run& r, bool few, bool chunk) {
+  const RunArgs& a = r.a;
+  if (few) {
+    const int64_t most = r.l.most_few * a.s.hkv * a.z.head_blocks;
+    const int n = (int)(most < 8192 ? most : 8192);
+    hipLaunchKernelGGL((kv8_few_kernel<T, C, DP>), dim3(n), dim3(kFewThreads), 0, r.s, a, n);
+  }
+  if (chunk) {
+    const int64_t most = r.l.most_chunk * a.s.hkv;
+    const int n = (int)(most < 8192 ? most : 8192);
+    hipLaunchKernelGGL((kv8_chunk_kernel<T, C, DP>), dim3(n), dim3(kChunkThreads), 0, r.s, a, n);
+  }
+}
+
+template <typename T, typename C>
+void launch_run(const Run& r, bool few, bool chunk) {
+  if (r.a.s.head_dim <= 64) launch_run<T, C, 64>(r, few, chunk);
+  else if (r.a.s.head_dim <= 128) launch_run<T, C, 128>(r, few, chunk);
+  else launch_run<T, C, 256>(r, few, chunk);
+}
+
+template <typename T>
+int launch_run(const Run& r, int32_t code, bool few, bool chunk) {
+  if (code == HX_CODE_E4M3) launch_run<T, hx8::E4m3>(r, few, chunk);
+  else launch_run<T, hx8::Int8>(r, few, chunk);
+  // Splits exist past the least split of a few item, and among few chunk blocks.
+  if ((few && r.a.s.max_k > kFewLeast * kFewTile - kFewTile) || (chunk && r.a.s.max_k > kChunkLeast * kChunkTile - kChunkTile)) {
+    const int64_t most = r.l.most_join * r.a.s.hq;
+    const int n = (int)(most < 4096 ? most : 4096);
+    hipLaunchKernelGGL(kv8_join_kernel<T>, dim3(n), dim3(kJoinThreads), 0, r.s, r.a, n);
+  }
+  return hx::status_from_hip(hipGetLastError());
+}
+
+bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
+
+}  // namespace
+
+extern "C" size_t hx_kv8_attn_workspace_bytes(int32_t batch, int32_t total_q, int32_t max_q, int32_t max_k,
+                                              int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t page_size) {
+  const Shape s{batch, total_q, max_q, max_k, n_q_heads, n_kv_heads, head_dim, page_size, -1, -1, 1};
+  return check_shape(s) == HX_OK ? layout_of(s).total : 0;
+}
+
+extern "C" size_t hx_kv8_attn_error_word_offset(void) { return H_ERR * sizeof(int32_t); }
+
+extern "C" int hx_kv8_attn_plan(const int32_t* cu_seq_q, const int32_t* seqused_k, int32_t batch, int32_t total_q,
+                                int32_t max_q, int32_t max_k, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                int32_t page_size, int32_t block_table_width, int32_t window_left, int32_t window_right,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  const Shape s{batch,     total_q,     max_q,        max_k,            n_q_heads, n_kv_heads, head_dim,
+                page_size, window_left, window_right, block_table_width};
+  const int bad = check_shape(s);
+  if (bad != HX_OK) return bad;
+  if (batch == 0 || total_q == 0 || max_q == 0) return HX_OK;
+  if (!cu_seq_q || !seqused_k) return HX_E_INVALID_ARG;
+  const Layout l = layout_of(s);
+  if (!workspace || misaligned(workspace, 256) || workspace_bytes < l.total) return HX_E_WORKSPACE;
+  if (l.slots > 0x7fffffff || l.most_chunk > 0x7fffffff / n_kv_heads || l.most_few > 0x7fffffff / n_q_heads) return HX_E_UNSUPPORTED;
+  uint8_t* const base = static_cast<uint8_t*>(workspace);
+  PlanArgs a;
+  a.cu_q = cu_seq_q;
+  a.used = seqused_k;
+  a.hdr = reinterpret_cast<int32_t*>(base);
+  a.seq = reinterpret_cast<int4*>(base + l.seq);
+  a.few = reinterpret_cast<int4*>(base + l.few);
+  a.chunk = reinterpret_cast<int4*>(base + l.chunk);
+  a.join = reinterpret_cast<int4*>(base + l.join);
+  a.most_few = l.most_few;
+  a.most_chunk = l.most_chunk;
+  a.most_join = l.most_join;
+  a.slots = l.slots;
+  a.s = s;
+  a.z = sizes_of(s);
+  hipLaunchKernelGGL(kv8_plan_kernel, dim3(1), dim3(kPlanThreads), 0, reinterpret_cast<hipStream_t>(stream), a);
+  return hx::status_from_hip(hipGetLastError());
+}
+
+extern "C" int hx_kv8_attn_run(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k_codes,
+                               const void* v_codes, const float* k_scales, const float* v_scales, int32_t num_pages,
+                               int32_t page_size, int32_t code, const int32_t* block_table, int64_t block_table_stride,
+                               int32_t block_table_width, int32_t batch, int32_t total_q, int32_t max_q, int32_t max_k,
+                               int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, float scale, int32_t window_left,
+                               int32_t window_right, int32_t dtype, void* out, int64_t out_row_stride,
+                               int64_t out_head_stride, int32_t kinds, void* workspace, size_t workspace_bytes, void* stream) {
+  const Shape s{batch,     total_q,     max_q,        max_k,            n_q_heads, n_kv_heads, head_dim,
+                page_size, window_left, window_right, block_table_width};
+  const int bad = check_shape(s);
+  if (bad != HX_OK) return bad;
+  if ((dtype != HX_DTYPE_BF16 && dtype != HX_DTYPE_FP16) || (code != HX_CODE_E4M3 && code != HX_CODE_INT8)) return HX_E_UNSUPPORTED;
+  if (num_pages < 1 || block_table_stride < block_table_width || !(scale > 0.f) || !isfinite(scale)) return HX_E_INVALID_ARG;
+  if (batch == 0 || total_q == 0 || max_q == 0) return HX_OK;
+  if (!q || !k_codes || !v_codes || !k_scales || !v_scales || !block_table || !out || misaligned(q, 16) ||
+      misaligned(k_codes, 16) || misaligned(v_codes, 16) || misaligned(k_scales, 16) || misaligned(v_scales, 16) ||
+      q_row_stride % 8 || q_head_stride % 8 || misaligned(out, 4) || out_row_stride % 2 || out_head_stride % 2)
+    return HX_E_INVALID_ARG;
+  Run r;
+  r.l = layout_of(s);
+  r.s = reinterpret_cast<hipStream_t>(stream);
+  if (!workspace || misaligned(workspace, 256) || workspace_bytes < r.l.total) return HX_E_WORKSPACE;
+  uint8_t* const base = static_cast<uint8_t*>(workspace);
+  RunArgs& a = r.a;
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_row = q_row_stride;
+  a.q_head = q_head_stride;
+  a.k = static_cast<const uint8_t*>(k_codes);
+  a.v = static_cast<const uint8_t*>(v_codes);
+  a.k_scale = k_scales;
+  a.v_scale = v_scales;
+  a.num_pages = num_pages;
+  a.table = block_table;
+  a.table_stride = block_table_stride;
+  a.scale_log2 = scale * kLog2e;
+  a.out = static_cast<uint16_t*>(out);
+  a.out_row = out_row_stride;
+  a.out_head = out_head_stride;
+  a.hdr = reinterpret_cast<int32_t*>(base);
+  a.few = reinterpret_cast<const int4*>(base + r.l.few);
+  a.chunk = reinterpret_cast<const int4*>(base + r.l.chunk);
+  a.join = reinterpret_cast<const int4*>(base + r.l.join);
+  a.part_ml = reinterpret_cast<float2*>(base + r.l.ml);
+  a.part_o = reinterpret_cast<float*>(base + r.l.o);
+  a.slots = r.l.slots;
+  a.s = s;
+  a.z = sizes_of(s);
+  const bool chunk = max_q > a.z.few_rows && (kinds & HX_KV8_CHUNK_ROWS), few = (kinds & HX_KV8_FEW_ROWS) != 0;
+  return dtype == HX_DTYPE_BF16 ? launch_run<__bf16>(r, code, few, chunk) : launch_run<_Float16>(r, code, few, chunk);
+}

@@ -782,6 +782,273 @@ def int4_dequantize(weight: Int4Weight) -> torch.Tensor:
     return out
 
 
+# --------------------------------------------------------------------- 8-bit KV cache
+_CODES = {torch.float8_e4m3fn: _capi.HX_CODE_E4M3, torch.int8: _capi.HX_CODE_INT8}
+
+
+class Kv8Cache(NamedTuple):
+    """One layer of a paged cache in 8 bits: ``keys`` and ``values`` ``[pages, page_size,
+    kv_heads, head_dim]`` float8_e4m3fn or int8, ``key_scales`` and ``value_scales`` float32
+    ``[pages, kv_heads, page_size]``, all contiguous. An element stands for its code times the
+    scale of its token and head; ``kv8_append`` and ``kv8_norm_rope_append`` write them.
+    head_dim is a multiple of 16 up to 256."""
+
+    keys: torch.Tensor
+    values: torch.Tensor
+    key_scales: torch.Tensor
+    value_scales: torch.Tensor
+
+
+def _check_codes(codes: torch.Tensor, scales: torch.Tensor) -> tuple[int, int, int, int, int]:
+    """A code of codes and scales checked: its type's code, pages, page size, KV heads, head dim."""
+    code, shape = _CODES.get(codes.dtype), codes.shape
+    if code is None:
+        raise ValueError("8-bit codes must be float8_e4m3fn or int8.")
+    if len(shape) != 4 or 0 in shape or not codes.is_contiguous():
+        raise ValueError("8-bit codes must be a contiguous [pages, page_size, kv_heads, head_dim] pool.")
+    pages, page_size, n_kv, head_dim = shape
+    if head_dim % 16 or head_dim > 256:
+        raise ValueError("head_dim of an 8-bit cache must be a multiple of 16 from 16 to 256.")
+    if scales.dtype != torch.float32 or scales.shape != (pages, n_kv, page_size) or not scales.is_contiguous():
+        raise ValueError("scales must be contiguous float32 [pages, kv_heads, page_size].")
+    return code, pages, page_size, n_kv, head_dim
+
+
+def _check_kv8(cache: Kv8Cache) -> tuple[int, int, int, int, int]:
+    keys, values, key_scales, value_scales = cache
+    layout = _check_codes(keys, key_scales)
+    if values.dtype != keys.dtype or values.shape != keys.shape or not values.is_contiguous() \
+            or value_scales.dtype != torch.float32 or value_scales.shape != key_scales.shape \
+            or not value_scales.is_contiguous():
+        raise ValueError("keys and values of an 8-bit cache must have the same dtypes, shapes and layout.")
+    return layout
+
+
+def _check_kv8_rows(keys: torch.Tensor, values: torch.Tensor, write_slots: torch.Tensor, n_kv: int,
+                    head_dim: int) -> int:
+    """Checks of new keys and values for an 8-bit cache; their dtype code."""
+    dtype = _SUPPORTED.get(keys.dtype)
+    if dtype is None or values.dtype != keys.dtype:
+        raise ValueError("Appended K/V must be bfloat16 or float16, of one dtype.")
+    if keys.ndim != 3 or values.shape != keys.shape:
+        raise ValueError("Appended keys and values must be [tokens, kv_heads, head_dim].")
+    if tuple(keys.shape[1:]) != (n_kv, head_dim):
+        raise ValueError("Appended K/V heads do not match the pool layout.")
+    if write_slots.dtype != torch.int64 or write_slots.shape != (keys.shape[0],):
+        raise ValueError("write_slots must be int64 [tokens].")
+    if keys.stride(2) != 1 or values.stride(2) != 1:
+        raise ValueError("Appended K/V must have a contiguous head_dim.")
+    return dtype
+
+
+def kv8_append(cache: Kv8Cache, write_slots: torch.Tensor, keys: torch.Tensor, values: torch.Tensor) -> None:
+    """``kv_append`` into an 8-bit cache: token t's rows, each with the scale ``max(max |x| * (1 / Q),
+    2^-100)`` (Q: 448 for float8_e4m3fn, 127 for int8) and the codes ``x / scale`` rounded to
+    nearest even, in fp32 with 1 / Q rounded to it, at slot ``write_slots[t]`` (``page * page_size + offset``; outside the pool:
+    skipped; listed twice: one of its tokens, or parts of several). ``keys`` / ``values``
+    ``[T, kv_heads, head_dim]`` bfloat16 or float16, any row and head strides. A row with an
+    infinite or NaN element is stored as NaN: under a NaN scale."""
+    device = _require_gpu(*cache, write_slots, keys, values)
+    code, pages, page_size, n_kv, head_dim = _check_kv8(cache)
+    dtype = _check_kv8_rows(keys, values, write_slots, n_kv, head_dim)
+    write_slots = write_slots.contiguous()
+    status = _launch(
+        device, _capi.lib().hx_kv8_append, cache.keys.data_ptr(), cache.values.data_ptr(),
+        cache.key_scales.data_ptr(), cache.value_scales.data_ptr(), pages, page_size, n_kv, head_dim, code,
+        keys.data_ptr(), keys.stride(0), keys.stride(1), values.data_ptr(), values.stride(0), values.stride(1),
+        write_slots.data_ptr(), keys.shape[0], dtype)
+    _capi.check(status, "hx_kv8_append")
+
+
+def kv8_norm_rope_append(
+    queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, q_norm_weight: torch.Tensor,
+    k_norm_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, cache: Kv8Cache,
+    write_slots: torch.Tensor, eps: float, out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``qk_norm_rope_append`` into an 8-bit cache, at any head_dim it holds: RMSNorm and position
+    rotation of queries and keys, and the quantised append, in one launch. Returns the
+    normalised, rotated queries (``out`` if given). In fp32 and rounded once, to the queries'
+    dtype or to the codes (``qk_norm_rope_append`` rounds between the norm and the rotation, as
+    its reference does). Arguments as there, ``write_slots`` as for ``kv8_append``."""
+    device = _require_gpu(queries, keys, values, q_norm_weight, k_norm_weight, cos, sin, positions, *cache,
+                          write_slots)
+    code, pages, page_size, n_kv, head_dim = _check_kv8(cache)
+    dtype = _check_kv8_rows(keys, values, write_slots, n_kv, head_dim)
+    if queries.ndim != 3 or queries.shape[0] != keys.shape[0] or queries.shape[2] != head_dim or queries.shape[1] < 1:
+        raise ValueError("queries must be [tokens, q_heads, head_dim] matching the keys.")
+    if queries.dtype != keys.dtype or queries.stride(2) != 1:
+        raise ValueError("queries must share the K/V dtype and have a contiguous head_dim.")
+    _check_rope(q_norm_weight, k_norm_weight, cos, sin, head_dim)
+    if cos.shape[0] < 1:
+        raise ValueError("cos/sin need at least one row.")
+    positions = positions.reshape(-1)
+    if positions.dtype != torch.int64 or positions.numel() != queries.shape[0]:
+        raise ValueError("positions must be int64 with one entry per row.")
+    positions, write_slots = positions.contiguous(), write_slots.contiguous()
+    if out is None:
+        out = torch.empty(queries.shape, dtype=queries.dtype, device=device)
+    elif out.shape != queries.shape or out.dtype != queries.dtype or out.device != device or out.stride(2) != 1:
+        raise ValueError("out must match the queries' shape, dtype and device.")
+    q_norm_weight, k_norm_weight, cos, sin = (
+        t if t.data_ptr() % 16 == 0 else t.clone() for t in (q_norm_weight, k_norm_weight, cos, sin))
+    status = _launch(
+        device, _capi.lib().hx_kv8_norm_rope_append, queries.data_ptr(), queries.stride(0), queries.stride(1),
+        keys.data_ptr(), keys.stride(0), keys.stride(1), values.data_ptr(), values.stride(0), values.stride(1),
+        q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+        positions.data_ptr(), queries.shape[0], queries.shape[1], n_kv, head_dim, eps, dtype,
+        out.data_ptr(), out.stride(0), out.stride(1), cache.keys.data_ptr(), cache.values.data_ptr(),
+        cache.key_scales.data_ptr(), cache.value_scales.data_ptr(), pages, page_size, code, write_slots.data_ptr())
+    _capi.check(status, "hx_kv8_norm_rope_append")
+    return out
+
+
+def kv8_gather(codes: torch.Tensor, scales: torch.Tensor, pages: torch.Tensor | Sequence[int], length: int,
+               dtype: torch.dtype) -> torch.Tensor:
+    """``kv_gather`` of an 8-bit pool's keys or values: paged -> dense ``[1, Hkv, length, d]`` in
+    ``dtype`` (bfloat16, float16 or float32), ``code * scale`` rounded once."""
+    device = _require_gpu(codes, scales)
+    code, num_pages, page_size, n_kv, head_dim = _check_codes(codes, scales)
+    out_type = _capi.HX_DTYPE_FP32 if dtype == torch.float32 else _SUPPORTED.get(dtype)
+    if out_type is None:
+        raise ValueError("kv8_gather gives bfloat16, float16 or float32.")
+    if not isinstance(pages, torch.Tensor):
+        pages = torch.tensor(list(pages), dtype=torch.int32, device=device)
+    if pages.ndim != 1 or pages.dtype != torch.int32 or pages.device != device:
+        raise ValueError("pages must be an int32 vector on the cache's device.")
+    pages = pages.contiguous()
+    if length < 0 or length > pages.shape[0] * page_size:
+        raise ValueError("length exceeds the listed pages.")
+    out = torch.empty((1, n_kv, length, head_dim), dtype=dtype, device=device)
+    status = _launch(device, _capi.lib().hx_kv8_gather, codes.data_ptr(), scales.data_ptr(), num_pages, page_size,
+                     n_kv, head_dim, code, pages.data_ptr(), pages.shape[0], length, out_type, out.data_ptr())
+    _capi.check(status, "hx_kv8_gather")
+    return out
+
+
+class Kv8AttnPlan:
+    """``VarlenAttnPlan`` for an 8-bit cache: the work lists of one set of varlen metadata, built
+    once per tick, then ``run`` per layer. Query heads that share a KV head: at most 128;
+    page_size a multiple of 64. ``q_lens`` (the sequences' new tokens, a host list), when given,
+    leaves out launches for kinds of rows that the tick does not have. Runs of one plan share its
+    workspace: on several streams, or captured into graphs that may run at once, they need an
+    order."""
+
+    def __init__(self, cu_seq_q: torch.Tensor, seqused_k: torch.Tensor, *, total_q: int, max_q: int, max_k: int,
+                 n_q_heads: int, n_kv_heads: int, head_dim: int, page_size: int, window: tuple[int, int] = (-1, 0),
+                 q_lens: Sequence[int] | None = None, block_table_width: int | None = None) -> None:
+        device = _require_gpu(cu_seq_q, seqused_k)
+        batch = seqused_k.shape[0] if seqused_k.ndim == 1 else -1
+        for name, t, count in (("cu_seq_q", cu_seq_q, batch + 1), ("seqused_k", seqused_k, batch)):
+            if t.dtype != torch.int32 or t.shape != (count,):
+                raise ValueError(f"{name} must be an int32 vector: batch + 1 and batch entries.")
+        if total_q < 0 or max_q < 0 or max_k < 0:
+            raise ValueError("total_q, max_q and max_k must be non-negative.")
+        if n_kv_heads < 1 or n_q_heads < 1 or n_q_heads % n_kv_heads:
+            raise ValueError(f"GQA needs n_q_heads ({n_q_heads}) to be a multiple of n_kv_heads ({n_kv_heads}).")
+        if page_size < 1:
+            raise ValueError("page_size must be positive.")
+        left, right = (max(-1, min(int(x), 2 ** 31 - 1)) for x in window)
+        # Without a width the table of every run must cover max_k.
+        width = max(1, -(-max_k // page_size)) if block_table_width is None else block_table_width
+        lib = _capi.lib()
+        self.ws_bytes = lib.hx_kv8_attn_workspace_bytes(batch, total_q, max_q, max_k, n_q_heads, n_kv_heads, head_dim,
+                                                        page_size)
+        if not self.ws_bytes:
+            raise ValueError("Unsupported attention shape: head_dim must be a multiple of 16 from 16 to 256, page_size "
+                             "of 64, and at most 128 query heads may share a KV head.")
+        self.device, self.width = device, width
+        self._shape = (batch, total_q, max_q, max_k, n_q_heads, n_kv_heads, head_dim)
+        self.page_size, self.window = page_size, (left, right)
+        group = n_q_heads // n_kv_heads
+        few = max(1, 16 // group)  # rows of a sequence that share one pass over its keys
+        self._kinds = _capi.HX_KV8_FEW_ROWS | _capi.HX_KV8_CHUNK_ROWS
+        if q_lens is not None:
+            kinds = {_capi.HX_KV8_CHUNK_ROWS if n > few else _capi.HX_KV8_FEW_ROWS for n in q_lens if n > 0}
+            self._kinds = sum(kinds)
+        self._scale = 1.0 / math.sqrt(head_dim)
+        self._q_shape = torch.Size((total_q, n_q_heads, head_dim))
+        self.workspace = torch.empty(self.ws_bytes + 256, dtype=torch.uint8, device=device)
+        self._offset = -self.workspace.data_ptr() % 256
+        self._ws_ptr = self.workspace.data_ptr() + self._offset
+        cu_seq_q, seqused_k = cu_seq_q.contiguous(), seqused_k.contiguous()
+        status = _launch(device, lib.hx_kv8_attn_plan, cu_seq_q.data_ptr(), seqused_k.data_ptr(), *self._shape,
+                         page_size, width, left, right, self._ws_ptr, self.ws_bytes)
+        _capi.check(status, "hx_kv8_attn_plan")
+
+    def error_word(self) -> int:
+        """HX_WERR_* bits raised so far (synchronises the device to read them)."""
+        if 0 in self._shape[:3]:
+            return 0  # nothing to plan, nothing written
+        at = self._offset + _capi.lib().hx_kv8_attn_error_word_offset()
+        return int(self.workspace[at:at + 4].view(torch.int32).item())
+
+    def check_errors(self) -> None:
+        """Raise RuntimeError if the plan or a run flagged bad metadata (synchronises)."""
+        word = self.error_word()
+        if word:
+            raise RuntimeError(f"8-bit paged attention metadata error {word:#x}: {describe_error_word(word)}")
+
+    def run(self, query: torch.Tensor, cache: Kv8Cache, block_table: torch.Tensor, *, scale: float | None = None,
+            out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention for one layer: ``query`` ``[total_q, Hq, d]`` bfloat16 or float16, packed, over
+        the pages of ``cache`` that ``block_table`` (int32 ``[batch, width]``) lists. Returns
+        ``[total_q, Hq, d]`` like ``query``: in fp32, rounded once. A row without a key gets zeros;
+        output rows behind the last sequence stay as they were. A key or value that was stored as
+        NaN makes the rows that see it NaN."""
+        keys, values, key_scales, value_scales = cache
+        device, index = self.device, self.device.index
+        for t in (query, keys, values, key_scales, value_scales, block_table):
+            if t.get_device() != index:
+                _require_gpu(query, *cache, block_table)
+                raise ValueError("Query and cache must be on the plan's device.")
+        code, pages, page_size, n_kv, head_dim = _check_kv8(cache)
+        dtype = _SUPPORTED.get(query.dtype)
+        if dtype is None or query.shape != self._q_shape:
+            raise ValueError("query must be bfloat16 or float16 [total_q, n_q_heads, head_dim] as planned.")
+        if page_size != self.page_size or n_kv != self._shape[5] or head_dim != self._shape[6]:
+            raise ValueError("the cache's page size, heads and head_dim must be the planned ones.")
+        batch, width, table_stride = _table_layout(block_table)
+        if batch != self._shape[0] or width < self.width:
+            raise ValueError(f"block_table must be int32 [{self._shape[0]}, {self.width}] or wider, as planned.")
+        scale = self._scale if scale is None else float(scale)
+        if not 0.0 < scale < math.inf:
+            raise ValueError("scale must be positive.")
+        if out is None:
+            out = torch.empty(self._q_shape, dtype=query.dtype, device=device)
+        elif out.shape != query.shape or out.dtype != query.dtype or out.get_device() != index or out.stride(2) != 1 \
+                or out.data_ptr() % 4 or out.stride(0) % 2 or out.stride(1) % 2:
+            raise ValueError("out must have the query's shape, dtype and device, a contiguous head_dim and even strides.")
+        query = _vector_rows(query)
+        q_row, q_head, _ = query.stride()
+        out_row, out_head, _ = out.stride()
+        status = _launch(
+            device, _capi.lib().hx_kv8_attn_run, query.data_ptr(), q_row, q_head, keys.data_ptr(), values.data_ptr(),
+            key_scales.data_ptr(), value_scales.data_ptr(), pages, page_size, code, block_table.data_ptr(),
+            table_stride, self.width, *self._shape, scale, *self.window, dtype, out.data_ptr(), out_row, out_head,
+            self._kinds, self._ws_ptr, self.ws_bytes)
+        _capi.check(status, "hx_kv8_attn_run")
+        if CHECK_ERRORS:
+            self.check_errors()
+        return out
+
+
+def kv8_attn(query: torch.Tensor, cache: Kv8Cache, cu_seq_q: torch.Tensor, seqused_k: torch.Tensor,
+             block_table: torch.Tensor, *, max_q: int, max_k: int, is_causal: bool = False,
+             window_size: tuple[int, int] | None = None, scale: float | None = None) -> torch.Tensor:
+    """``varlen_attn`` over an 8-bit paged cache, plan and run in one call. ``window_size=(-1, 0)``
+    is the bottom-right causal mask, None every key."""
+    device = _require_gpu(query, *cache, cu_seq_q, seqused_k, block_table)
+    del device
+    _, _, page_size, n_kv, head_dim = _check_kv8(cache)
+    if query.ndim != 3:
+        raise ValueError("query must be [total_q, n_q_heads, head_dim].")
+    _, width, _ = _table_layout(block_table)
+    plan = Kv8AttnPlan(cu_seq_q, seqused_k, total_q=query.shape[0], max_q=max_q, max_k=max_k,
+                       n_q_heads=query.shape[1], n_kv_heads=n_kv, head_dim=head_dim, page_size=page_size,
+                       window=_window(window_size, is_causal), block_table_width=width)
+    return plan.run(query, cache, block_table, scale=scale)
+
+
 # --------------------------------------------------------------- rules on the logits
 class LogitRules(NamedTuple):
     """What the requests of a tick ask of their logit rows, all on the device, None: not asked.

@@ -50,7 +50,15 @@ extern "C" {
 /* ---- element types -------------------------------------------------------- */
 #define HX_DTYPE_BF16 0
 #define HX_DTYPE_FP16 1
-#define HX_DTYPE_FP32 2 /* hx_logit_rules only */
+#define HX_DTYPE_FP32 2 /* hx_logit_rules, hx_kv8_gather, hx_sample_tokens */
+
+/* ---- codes of the 8-bit cache --------------------------------------------- */
+#define HX_CODE_E4M3 0 /* 8-bit floats of 4 exponent and 3 mantissa bits, at most 448 */
+#define HX_CODE_INT8 1 /* whole numbers -127 .. 127 */
+
+/* ---- row kinds of hx_kv8_attn_run ------------------------------------------ */
+#define HX_KV8_FEW_ROWS 1   /* sequences of few new rows (a decode row, drafted ones) */
+#define HX_KV8_CHUNK_ROWS 2 /* the others */
 
 /* ---- bits of the workspace error word (hx_varlen_attn_error_word) --------- */
 #define HX_WERR_BAD_PAGE 1        /* a block-table entry outside [0, num_pages)     */
@@ -665,6 +673,83 @@ int hx_block_sparse_attn(const void* q, int64_t q_row_stride, int64_t q_head_str
                          int32_t n_kv_heads, int32_t head_dim, float scale, int32_t dtype,
                          void* out, int64_t out_row_stride, int64_t out_head_stride,
                          void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The 8-bit KV cache. Per layer: key and value codes, each [num_pages, page_size, n_kv_heads,
+ * head_dim] bytes, and their fp32 scales, each [num_pages, n_kv_heads, page_size]; an element
+ * stands for code * scale. head_dim is a multiple of 16 up to 256, codes are 16-byte aligned.
+ *
+ * hx_kv8_append stores token t's rows k_new[t][h] and v_new[t][h] (bf16 or fp16) at slot
+ * write_slots[t] = page * page_size + offset: with a = max |x|, and Q = 448 or 127,
+ *   scale = max(a * (1 / Q), 2^-100),  code = x / scale rounded to nearest even,
+ * in fp32, with 1 / Q rounded to it.
+ * A row with an infinite or NaN element gets a NaN scale and zero codes. Slots outside the pool
+ * are skipped; a slot listed twice holds codes and a scale of either row, perhaps not of the same.
+ */
+int hx_kv8_append(void* k_codes, void* v_codes, float* k_scales, float* v_scales, int32_t num_pages,
+                  int32_t page_size, int32_t n_kv_heads, int32_t head_dim, int32_t code,
+                  const void* k_new, int64_t k_row_stride, int64_t k_head_stride,
+                  const void* v_new, int64_t v_row_stride, int64_t v_head_stride,
+                  const int64_t* write_slots, int64_t n_tokens, int32_t dtype, void* stream);
+
+/*
+ * hx_qk_norm_rope_append into the 8-bit cache: RMSNorm of every query and key head, the position
+ * rotation (tables of rope_rows rows of head_dim; positions are clamped to them), queries to
+ * q_out, keys and values quantised as hx_kv8_append does. In fp32, rounded once. Norm weights and
+ * tables are 16-byte aligned.
+ */
+int hx_kv8_norm_rope_append(const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                            const void* k, int64_t k_row_stride, int64_t k_head_stride,
+                            const void* v, int64_t v_row_stride, int64_t v_head_stride,
+                            const float* q_norm_weight, const float* k_norm_weight,
+                            const float* cos, const float* sin, int64_t rope_rows,
+                            const int64_t* positions, int64_t n_rows, int32_t n_q_heads,
+                            int32_t n_kv_heads, int32_t head_dim, float eps, int32_t dtype,
+                            void* q_out, int64_t q_out_row_stride, int64_t q_out_head_stride,
+                            void* k_codes, void* v_codes, float* k_scales, float* v_scales,
+                            int32_t num_pages, int32_t page_size, int32_t code,
+                            const int64_t* write_slots, void* stream);
+
+/*
+ * Pages of codes read back: out[h][t][d] = code * scale of token t < length of the listed pages,
+ * rounded to dtype (bf16, fp16 or fp32); zeros where a page id is outside the pool. out is 16-byte
+ * aligned.
+ */
+int hx_kv8_gather(const void* codes, const float* scales, int32_t num_pages, int32_t page_size,
+                  int32_t n_kv_heads, int32_t head_dim, int32_t code, const int32_t* pages,
+                  int32_t n_pages, int64_t length, int32_t dtype, void* out, void* stream);
+
+/*
+ * Varlen GQA attention over the 8-bit cache, as hx_varlen_attn_plan / _run over the 16-bit one:
+ * rows cu_seq_q[b] .. cu_seq_q[b + 1] - 1 of q attend to the seqused_k[b] keys of sequence b, whose
+ * pages are block_table[b], row i of n being at position seqused_k[b] - n + i; window_left / right
+ * (-1: all) limit the keys around it. out = softmax(scale q k) v, rounded once; a row without a key
+ * gets zeros. One plan serves any number of runs with its shape; runs that share a workspace must
+ * be ordered. page_size is a multiple of 64, at most 128 query heads share a KV head; scales and q
+ * are 16-byte aligned, with strides of q that are multiples of 8, out 4-byte aligned with even
+ * strides. kinds (HX_KV8_*): which kinds of rows the tick has; rows of another kind stay unwritten.
+ * Pages outside the pool count as no keys and, like lengths past max_q, max_k or the table, set a
+ * bit of the error word at hx_kv8_attn_error_word_offset() of the workspace. The workspace is
+ * hx_kv8_attn_workspace_bytes() bytes (0: unsupported), 256-byte aligned.
+ */
+size_t hx_kv8_attn_workspace_bytes(int32_t batch, int32_t total_q, int32_t max_q, int32_t max_k,
+                                   int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                   int32_t page_size);
+size_t hx_kv8_attn_error_word_offset(void);
+int hx_kv8_attn_plan(const int32_t* cu_seq_q, const int32_t* seqused_k, int32_t batch,
+                     int32_t total_q, int32_t max_q, int32_t max_k, int32_t n_q_heads,
+                     int32_t n_kv_heads, int32_t head_dim, int32_t page_size,
+                     int32_t block_table_width, int32_t window_left, int32_t window_right,
+                     void* workspace, size_t workspace_bytes, void* stream);
+int hx_kv8_attn_run(const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                    const void* k_codes, const void* v_codes, const float* k_scales,
+                    const float* v_scales, int32_t num_pages, int32_t page_size, int32_t code,
+                    const int32_t* block_table, int64_t block_table_stride,
+                    int32_t block_table_width, int32_t batch, int32_t total_q, int32_t max_q,
+                    int32_t max_k, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                    float scale, int32_t window_left, int32_t window_right, int32_t dtype,
+                    void* out, int64_t out_row_stride, int64_t out_head_stride, int32_t kinds,
+                    void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Penalties, biases and allowed-token masks on logits [rows, vocab], and the greedy ids.
