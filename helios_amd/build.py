@@ -20,7 +20,7 @@ INCLUDE = PACKAGE_DIR.parent / "include"
 LIBRARY = PACKAGE_DIR / "libhelios_paged.so"
 SOURCES = ("kv_ops.hip", "paged_attn.hip", "tick_meta.hip", "qk_rope.hip", "block_ops.hip", "skinny_gemm.hip",
            "logits.hip", "int4_gemm.hip", "logit_rules.hip", "block_sparse.hip",
-           "kv8_ops.hip", "kv8_attn.hip")
+           "kv8_ops.hip", "kv8_attn.hip", "sample.hip")
 ARCH = "gfx950"
 
 

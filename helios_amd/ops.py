@@ -1167,6 +1167,62 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, *, out: torch.Ten
     return RuledLogits(out, token_ids)
 
 
+# ------------------------------------------------------------------- drawing tokens
+SAMPLE_MAX_VOCAB = 1 << 18  # tokens that sample_tokens can draw from
+
+
+class SampledTokens(NamedTuple):
+    """Result of ``sample_tokens``: ``token_ids`` int64 ``[rows]`` and ``logprobs`` float32
+    ``[rows]``, the logarithm of the token's share of the weights that were kept."""
+
+    token_ids: torch.Tensor
+    logprobs: torch.Tensor
+
+
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: torch.Tensor | None = None,
+                  top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
+                  min_p: torch.Tensor | None = None) -> SampledTokens:
+    """A token drawn from each row of ``logits`` ``[rows, vocab]`` (bfloat16, float16 or float32,
+    contiguous rows) by the numbers ``uniforms`` (float32 ``[rows]``, in [0, 1)).
+
+    With t = ``temperature[r]`` a token's weight is ``exp((logit - largest) / t)``. In order of
+    falling logit (equal ones: the lower id first) the first n tokens are kept: at most
+    ``top_k[r]`` (int32; 0 or less: all), no more than it takes to reach ``top_p[r]`` of the
+    weight of the first ``top_k``, those with a weight of at least ``min_p[r]``, and at least
+    one. The token drawn is the first in that order whose cumulative weight passes ``uniforms[r]``
+    of theirs. A temperature of 0 or less takes the first token (as ``torch.argmax``, logprob 0), as
+    does a row whose largest logit is +inf or NaN; a row of -inf alone gives -1 and -inf. Limits are
+    float32 (``top_k`` int32) ``[rows]``, None: none; a ``temperature`` of None is 1. Weights are exact to 2^-45 of the largest and
+    sums of them have no order: equal inputs give equal tokens."""
+    device = _require_gpu(logits, uniforms)
+    dtype = _capi.HX_DTYPE_FP32 if logits.dtype == torch.float32 else _SUPPORTED.get(logits.dtype)
+    if dtype is None or logits.ndim != 2 or logits.shape[1] < 1:
+        raise ValueError("logits must be bfloat16, float16 or float32 [rows, vocab].")
+    rows, vocab = logits.shape
+    if vocab > SAMPLE_MAX_VOCAB:
+        raise ValueError(f"sample_tokens draws from at most {SAMPLE_MAX_VOCAB} tokens.")
+    if (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
+        raise ValueError("logits need contiguous rows that do not overlap.")
+    for name, t, kind in (("uniforms", uniforms, torch.float32), ("temperature", temperature, torch.float32),
+                          ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                          ("min_p", min_p, torch.float32)):
+        if t is not None and (t.dtype != kind or t.shape != (rows,) or not t.is_contiguous() or t.device != device):
+            raise ValueError(f"{name} must be contiguous {kind} [{rows}] on the logits' device.")
+    token_ids = logits.new_empty(rows, dtype=torch.int64)
+    logprobs = logits.new_empty(rows, dtype=torch.float32)
+    if rows == 0:
+        return SampledTokens(token_ids, logprobs)
+    lib = _capi.lib()
+    ws_bytes = lib.hx_sample_workspace_bytes(rows, vocab)
+    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    code = _launch(
+        device, lib.hx_sample_tokens, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, dtype,
+        uniforms.data_ptr(), *(None if t is None else t.data_ptr() for t in (temperature, top_k, top_p, min_p)),
+        token_ids.data_ptr(), logprobs.data_ptr(), workspace.data_ptr(), ws_bytes)
+    _capi.check(code, "hx_sample_tokens")
+    return SampledTokens(token_ids, logprobs)
+
+
 # --------------------------------------------------------------- logits and argmax
 class GreedyHeads(NamedTuple):
     """Result of ``final_norm_logits_argmax``: ``token_ids`` int64 ``[n]`` (-1 for an index

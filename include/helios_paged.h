@@ -780,6 +780,25 @@ int hx_logit_rules(const void* logits, int64_t logits_row_stride, int64_t rows,
                    int64_t out_row_stride, int64_t* token_ids, void* workspace,
                    size_t workspace_bytes, void* stream);
 
+/*
+ * A token drawn from each row of logits [rows, vocab] (bf16, fp16 or fp32; contiguous rows). With
+ * t = temperature[r], e_v = exp((l_v - max l) / t), tokens in order of falling logit (equal ones by
+ * index): the first n tokens are kept, the least of top_k[r] (<= 0: all), of the least number whose
+ * weights reach top_p[r] of the first top_k tokens', and of those with e_v >= min_p[r], at least one;
+ * token_ids[r] is the first whose cumulative weight passes uniforms[r] (in [0, 1)) of theirs, and
+ * logprobs[r] the log of its share of them. t <= 0: the first token, 0. A row whose largest logit
+ * is +inf or NaN (which counts as larger): that token, 0. A row of -inf alone: -1, -inf. Weights
+ * below 2^-45 of the largest count as 0. temperature (1), top_k, top_p, min_p and logprobs may be
+ * NULL. At most 2^18 tokens and 2^20 rows. The workspace is hx_sample_workspace_bytes() bytes,
+ * 8-byte aligned; calls that share one must be ordered.
+ */
+size_t hx_sample_workspace_bytes(int64_t rows, int64_t vocab);
+int hx_sample_tokens(const void* logits, int64_t logits_row_stride, int64_t rows, int64_t vocab,
+                     int32_t dtype, const float* uniforms, const float* temperature,
+                     const int32_t* top_k, const float* top_p, const float* min_p,
+                     int64_t* token_ids, float* logprobs, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif
