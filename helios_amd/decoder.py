@@ -18,7 +18,9 @@ With ``weight_bits=4`` the four products' weights are ``ops.Int4Weight``s: ticks
 ``ops.INT4_MAX_ROWS`` rows run them through ``ops.int4_linear`` with the steps between them
 fused in, longer ones dequantise a weight, to its type, and take the library's product (slower
 there than 16-bit weights). ``rules`` puts the
-requests' penalties, biases and allowed tokens on the logits (``ops.apply_logit_rules``).
+requests' penalties, biases and allowed tokens on the logits (``ops.apply_logit_rules``), and
+``sampling`` draws their tokens (``ops.sample_tokens``). Caches of an 8-bit pool
+(``KVPagePool(kv_dtype=...)``) are written and attended to in 8 bits.
 """
 
 from __future__ import annotations
@@ -134,9 +136,11 @@ class PagedQwen3Decoder:
     @torch.inference_mode()
     def forward_packed(self, input_ids: torch.Tensor, cache: PackedBatchCache, *,
                        fused_rope: bool = True, attention_events: list | None = None,
-                       greedy: bool = False, rules: ops.LogitRules | None = None) -> torch.Tensor:
+                       greedy: bool = False, rules: ops.LogitRules | None = None,
+                       sampling: ops.Sampling | None = None) -> torch.Tensor | ops.SampledTokens:
         """Logits of the tick's logit rows (model.py:92-110), or with ``greedy`` their
-        argmax token ids (engine.py:470-473). ``attention_events`` collects (start, end)
+        argmax token ids (engine.py:470-473), or with ``sampling`` (a value per logit row) tokens
+        drawn from them. ``attention_events`` collects (start, end)
         CUDA events around each layer's attention step.
 
         With ``fused_rope`` (this build's sequence) the logits or greedy ids come from the
@@ -146,6 +150,8 @@ class PagedQwen3Decoder:
         ``rules`` (a row per logit row) are applied to the logits before they are returned or
         the ids taken; an id is then -1 where nothing is allowed."""
         config = self.config
+        if greedy and sampling is not None:
+            raise ValueError("a tick is greedy or draws its tokens, not both")
         if input_ids.shape != (1, sum(cache.counts)):
             raise ValueError(f"input_ids must be [1, {sum(cache.counts)}]: one token per packed row of the tick.")
         hq, hkv, d = config.n_heads * config.head_dim, config.n_kv_heads * config.head_dim, config.head_dim
@@ -206,12 +212,17 @@ class PagedQwen3Decoder:
         if fused_rope and self._fused_heads(cache.logit_indices, x.dtype):
             logits = ops.final_norm_logits_argmax(x, cache.logit_indices, self.final_norm, self.embedding, eps,
                                                   return_logits=True).logits
-            if rules is None:
+            if rules is None and sampling is None:
                 return logits
         else:
             x = x.index_select(1, cache.logit_indices)
             logits = (_rms_norm(x, self.final_norm, eps).to(config.dtype) @ self.embedding.t())[0]
         if rules is not None:
             ruled = ops.apply_logit_rules(logits, rules, out=logits)
-            return ruled.token_ids if greedy else ruled.logits
+            if sampling is None:
+                return ruled.token_ids if greedy else ruled.logits
+            logits = ruled.logits
+        if sampling is not None:
+            return ops.sample_tokens(logits, sampling.uniforms, temperature=sampling.temperature, top_k=sampling.top_k,
+                                     top_p=sampling.top_p, min_p=sampling.min_p)
         return logits.argmax(dim=-1) if greedy else logits

@@ -1179,6 +1179,17 @@ class SampledTokens(NamedTuple):
     logprobs: torch.Tensor
 
 
+class Sampling(NamedTuple):
+    """How the requests of a tick draw their tokens, a value per logit row: ``sample_tokens``'s
+    arguments, for callers that pass them on."""
+
+    uniforms: torch.Tensor
+    temperature: torch.Tensor | None = None
+    top_k: torch.Tensor | None = None
+    top_p: torch.Tensor | None = None
+    min_p: torch.Tensor | None = None
+
+
 def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: torch.Tensor | None = None,
                   top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
                   min_p: torch.Tensor | None = None) -> SampledTokens:
@@ -1192,8 +1203,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: 
     one. The token drawn is the first in that order whose cumulative weight passes ``uniforms[r]``
     of theirs. A temperature of 0 or less takes the first token (as ``torch.argmax``, logprob 0), as
     does a row whose largest logit is +inf or NaN; a row of -inf alone gives -1 and -inf. Limits are
-    float32 (``top_k`` int32) ``[rows]``, None: none; a ``temperature`` of None is 1. Weights are exact to 2^-45 of the largest and
-    sums of them have no order: equal inputs give equal tokens."""
+    float32 (``top_k`` int32) ``[rows]``, None: none; a ``temperature`` of None is 1. Weights are
+    exact to 2^-45 of the largest and sums of them have no order: equal inputs give equal tokens."""
     device = _require_gpu(logits, uniforms)
     dtype = _capi.HX_DTYPE_FP32 if logits.dtype == torch.float32 else _SUPPORTED.get(logits.dtype)
     if dtype is None or logits.ndim != 2 or logits.shape[1] < 1:

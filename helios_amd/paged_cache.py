@@ -21,8 +21,9 @@ this module unchanged. How they are computed is this module's own design:
   only the bookkeeping works.
 * Extensions, all off the reference's call path: ``restore_blocks(copy=...,
   private_tail=...)`` (copying restores on the page-copy kernel), ``attend_projected``
-  (q/k RMSNorm + RoPE fused with the append), the shared-prefix cascade, and attention
-  over selected blocks (``KVPagePool(block_size=...)``, ``BlockSparse``).
+  (q/k RMSNorm + RoPE fused with the append), the shared-prefix cascade, attention
+  over selected blocks (``KVPagePool(block_size=...)``, ``BlockSparse``), and a pool in 8 bits
+  (``KVPagePool(kv_dtype=...)``).
 """
 
 from __future__ import annotations
@@ -89,10 +90,16 @@ class KVPagePool:
     also keeps each block's key bounds, ``bounds[l]`` ``[num_pages, page_size //
     block_size, n_kv_heads, 2, head_dim]`` (2 / block_size of the keys' memory): every append
     of a batch brings them up to date, so that ``BlockSparse`` batches can select by them.
-    Keys written into the pool by other means need ``PagedKVCache.refresh_bounds``."""
+    Keys written into the pool by other means need ``PagedKVCache.refresh_bounds``.
+
+    With ``kv_dtype`` (float8_e4m3fn or int8) the pool holds 8-bit codes, and
+    ``key_scales[l]`` / ``value_scales[l]`` float32 ``[num_pages, n_kv_heads, page_size]`` what
+    they are scaled by (``ops.Kv8Cache``; ``kv8(l)`` is a layer's): 0.52 of the 16-bit memory at
+    heads of 128. Batches write and read it through the same calls; the shared-prefix cascade,
+    overlapped streams and selected blocks are for 16-bit pools."""
 
     def __init__(self, config: Qwen3Config, num_pages: int, *, device: torch.device,
-                 page_size: int = 256, block_size: int | None = None) -> None:
+                 page_size: int = 256, block_size: int | None = None, kv_dtype: torch.dtype | None = None) -> None:
         if num_pages < 1:
             raise ValueError(f"a KV page pool needs at least one page, not {num_pages}")
         if page_size < 1 or page_size % 256 != 0:
@@ -103,16 +110,32 @@ class KVPagePool:
                     f"block_size must be a power of two from 16 to 1024 that divides the page, not {block_size}")
             if config.dtype not in (torch.bfloat16, torch.float16) or config.head_dim % 8 or config.head_dim > 256:
                 raise ValueError("key bounds need bfloat16 or float16 heads of a multiple of 8 up to 256 elements")
+        if kv_dtype is not None:
+            if kv_dtype not in (torch.float8_e4m3fn, torch.int8):
+                raise ValueError(f"an 8-bit pool holds float8_e4m3fn or int8, not {kv_dtype}")
+            if block_size is not None:
+                raise ValueError("key bounds need a 16-bit pool")
+            if config.dtype not in (torch.bfloat16, torch.float16) or config.head_dim % 16 or config.head_dim > 256 \
+                    or config.group_size > 128:
+                raise ValueError("an 8-bit pool needs a bfloat16 or float16 model with heads of a multiple of 16 up to "
+                                 "256 elements, at most 128 to a KV head")
         self.config = config
         self.num_pages = int(num_pages)
         self.page_size = int(page_size)
         self.device = torch.device(device)
         self.storage = torch.empty(
             (2, config.n_layers, self.num_pages, self.page_size, config.n_kv_heads, config.head_dim),
-            dtype=config.dtype, device=self.device,
+            dtype=config.dtype if kv_dtype is None else kv_dtype, device=self.device,
         )
         self.keys = tuple(self.storage[0].unbind(0))
         self.values = tuple(self.storage[1].unbind(0))
+        self.kv_dtype = kv_dtype
+        self.key_scales: tuple[torch.Tensor, ...] | None = None
+        self.value_scales: tuple[torch.Tensor, ...] | None = None
+        if kv_dtype is not None:
+            scales = torch.empty((2, config.n_layers, self.num_pages, config.n_kv_heads, self.page_size),
+                                 dtype=torch.float32, device=self.device)
+            self.key_scales, self.value_scales = (tuple(t.unbind(0)) for t in scales)
         self.block_size = block_size
         self.bounds: tuple[torch.Tensor, ...] | None = None
         if block_size is not None:
@@ -130,9 +153,15 @@ class KVPagePool:
 
     @property
     def bytes_per_token(self) -> int:
-        """K and V bytes of one token over all layers."""
-        per_layer_row = self.config.n_kv_heads * self.config.head_dim * self.storage.element_size()
-        return 2 * self.config.n_layers * per_layer_row
+        """K and V bytes of one token over all layers, scales included."""
+        per_head = self.config.head_dim * self.storage.element_size() + (0 if self.kv_dtype is None else 4)
+        return 2 * self.config.n_layers * self.config.n_kv_heads * per_head
+
+    def kv8(self, layer: int) -> ops.Kv8Cache:
+        """A layer of an 8-bit pool."""
+        if self.key_scales is None:
+            raise RuntimeError("the pool holds 16-bit keys and values; create it with kv_dtype")
+        return ops.Kv8Cache(self.keys[layer], self.values[layer], self.key_scales[layer], self.value_scales[layer])
 
     @property
     def bytes_per_page(self) -> int:
@@ -174,9 +203,11 @@ class KVPagePool:
             n = len(released)
 
     def copy_pages(self, src_pages: Sequence[int], dst_pages: Sequence[int]) -> None:
-        """Bit-copy pages for every layer, keys, values and any key bounds, on the page-copy
-        kernel."""
+        """Bit-copy pages for every layer, keys, values and any scales or key bounds, on the
+        page-copy kernel."""
         ops.kv_copy_pages(self.keys, self.values, src_pages, dst_pages)
+        if self.key_scales is not None:
+            ops.kv_copy_pages(self.key_scales, self.value_scales, src_pages, dst_pages)
         if self.bounds is not None:
             ops.kv_copy_pages(self.bounds, None, src_pages, dst_pages)
 
@@ -778,7 +809,8 @@ class PagedBatchCache:
     decode workgroups, so the kernels interleave rather than overlap (the full Qwen3-4B
     tick measured 12.5 ms of attention with it, 12.0 ms without). ``sparse`` lets decode rows
     of long caches attend to selected blocks; a tick in which one does runs on one stream
-    and without the cascade."""
+    and without the cascade. On an 8-bit pool (``KVPagePool(kv_dtype=...)``) appends quantise and
+    attention reads codes (``ops.Kv8AttnPlan``); there is no cascade, overlap or selection."""
 
     def __init__(self, caches: Sequence[PagedKVCache], *, device_metadata: bool | None = None,
                  prefix_cascade: bool | None = None, overlap: bool = False,
@@ -798,6 +830,9 @@ class PagedBatchCache:
             raise ValueError("device metadata needs a pool on a ROCm device")
         if overlap and not on_gpu:
             raise ValueError("overlapped streams need a pool on a ROCm device")
+        kv8 = pool.kv_dtype is not None
+        if kv8 and (overlap or prefix_cascade):
+            raise ValueError("an 8-bit pool has no overlapped streams and no prefix cascade")
         if sparse is not None and pool.bounds is None:
             raise ValueError("block-sparse attention needs a pool with key bounds (block_size)")
         if sparse is not None and _page_count(pool.config.context_length, pool.page_size) \
@@ -812,10 +847,11 @@ class PagedBatchCache:
         self._staged: dict[str, tuple[torch.Tensor, np.ndarray]] = {}
         self._table_key: tuple | None = None
         self._device_meta = _DeviceTickMetadata(pool.device) if device_metadata else None
-        self._use_cascade = on_gpu if prefix_cascade is None else bool(prefix_cascade)
+        self._use_cascade = on_gpu and not kv8 if prefix_cascade is None else bool(prefix_cascade)
         self._overlap = bool(overlap)
         self._side_stream: torch.cuda.Stream | None = None
         self._plan: ops.VarlenAttnPlan | None = None
+        self._kv8_plan: ops.Kv8AttnPlan | None = None
         self._cascade: _PrefixCascade | None = None
         self._lens: tuple[list[int], list[int]] | None = None
         self._row_positions: torch.Tensor | None = None
@@ -919,7 +955,7 @@ class PagedBatchCache:
             ends = self._device_tick(lengths, counts, tails, tables, width)
         else:
             ends = self._host_tick(lengths, counts, tails, tables, width)
-        self._plan = None
+        self._plan = self._kv8_plan = None
         self._lens = (list(counts), ends)
         self._sparse_tick = self._cascade = None
         if self._sparse is not None and on_gpu and any(
@@ -991,6 +1027,17 @@ class PagedBatchCache:
             )
         return self._plan
 
+    def _attend_kv8(self, rows: torch.Tensor, layer: int) -> torch.Tensor:
+        """Attention of packed query rows whose new K/V is already in the 8-bit pool: one plan a
+        tick, as above."""
+        if self._kv8_plan is None:
+            config = self.pool.config
+            self._kv8_plan = ops.Kv8AttnPlan(
+                self.cu_seq_q, self.seqused_k, total_q=rows.shape[0], max_q=self.max_q, max_k=self.max_k,
+                n_q_heads=config.n_heads, n_kv_heads=config.n_kv_heads, head_dim=config.head_dim,
+                page_size=self.pool.page_size, window=(-1, 0), q_lens=self._lens[0])
+        return self._kv8_plan.run(rows, self.pool.kv8(layer), self.block_table)
+
     def _require_device(self) -> None:
         if self.pool.device.type != "cuda":
             raise RuntimeError(
@@ -1032,6 +1079,14 @@ class PagedBatchCache:
         if rows != self.write_slots.shape[0]:
             raise ValueError(f"{rows} projected rows do not match the {self.write_slots.shape[0]} prepared")
         self._require_device()
+        if self.pool.kv_dtype is not None:
+            q_rot = ops.kv8_norm_rope_append(
+                queries.reshape(rows, config.n_heads, config.head_dim),
+                keys.reshape(rows, config.n_kv_heads, config.head_dim),
+                values.reshape(rows, config.n_kv_heads, config.head_dim), q_norm_weight, k_norm_weight, cos, sin,
+                self._positions_for_rows(), self.pool.kv8(layer), self.write_slots, eps)
+            out = self._attend_kv8(q_rot, layer)
+            return out.view(queries.shape[0], queries.shape[1], config.n_heads, config.head_dim).transpose(1, 2)
         k_pool, v_pool = self.pool.keys[layer], self.pool.values[layer]
         q_rot = ops.qk_norm_rope_append_packed(
             queries, keys, values, config.n_heads, q_norm_weight, k_norm_weight, cos, sin, self._positions_for_rows(),
@@ -1079,12 +1134,18 @@ class PagedBatchCache:
         """KV append alone (paged_cache.py:335-345): ``[B, Hkv, T, d]`` rows to their
         write slots."""
         k_rows, v_rows = _as_rows(keys), _as_rows(values)
+        if self.pool.kv_dtype is not None:
+            ops.kv8_append(self.pool.kv8(layer), self.write_slots, k_rows, v_rows)
+            return
         ops.kv_append(self.pool.keys[layer], self.pool.values[layer], self.write_slots, k_rows, v_rows)
 
     def _append_and_attend(self, layer: int, rows: torch.Tensor, keys: torch.Tensor,
                            values: torch.Tensor) -> torch.Tensor:
         """``_write`` then paged attention: one fused call when the new rows allow 16-byte
         loads (always, for contiguous projections), else the append kernel first."""
+        if self.pool.kv_dtype is not None:
+            self._write(layer, keys, values)
+            return self._attend_kv8(rows, layer)
         k_rows, v_rows = _as_rows(keys), _as_rows(values)
         k_pool, v_pool = self.pool.keys[layer], self.pool.values[layer]
         fused = (self._cascade is None and self._sparse_tick is None and self._side() is None
@@ -1126,7 +1187,7 @@ class PackedBatchCache(PagedBatchCache):
                 f"packed attention takes [1, heads, {sum(self.counts)}, head_dim] queries, "
                 f"not {list(queries.shape)}")
         self._require_device()
-        if self._cascade is None and self._sparse_tick is None and not self._overlap:
+        if self._cascade is None and self._sparse_tick is None and not self._overlap and self.pool.kv_dtype is None:
             out = self._attention_plan(queries.shape[2]).append_attend(
                 queries, keys, values, self.pool.keys[layer], self.pool.values[layer], self.block_table,
                 self.write_slots)
