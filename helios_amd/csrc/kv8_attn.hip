@@ -27,8 +27,12 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kFewUnits = 16;     // (row, head) pairs of a few_kernel item
 constexpr int kFewThreads = 256;  // 4 waves, each on its own 32-key tiles
 constexpr int kFewTile = 32;
-constexpr int kFewWGs = 2048;     // workgroups that the split size aims at: 8 a CU
-constexpr int kFewLeast = 8;      // tiles of a split, at least (two a wave)
+// Work of few_kernel's rows is dealt in equal parts of the tick's tiles, whatever the sequences are:
+// a part ends in the middle of one and goes on in the next. A sequence counts kFewStart tiles more
+// than it has, for what its start costs (loads that wait for one another, the waves' merge).
+constexpr int kFewWGs = 768;      // workgroups, about: 3 a CU, all at once
+constexpr int kFewStart = 8;
+constexpr int kFewLeast = 24;     // of a part, at least: tiles and starts
 constexpr int kFewMost = 256;     // and at most
 constexpr int kChunkThreads = 512;
 constexpr int kChunkTile = 64;
@@ -37,7 +41,7 @@ constexpr int kChunkLeast = 4;    // tiles of a split, at least
 constexpr int kPlanThreads = 1024;
 
 // Plan header words.
-enum { H_FEW = 0, H_CHUNK = 1, H_JOIN = 2, H_ERR = 3, H_STAMP = 4, H_WORDS = 16 };
+enum { H_PARTS = 0, H_CHUNK = 1, H_JOIN = 2, H_ERR = 3, H_STAMP = 4, H_WORDS = 16 };
 
 __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -53,7 +57,7 @@ struct Sizes {
   int32_t group;
   int32_t few_heads, head_blocks;  // query heads of a few item, and items over a group's heads
   int32_t few_rows;                // rows of a sequence that few_kernel takes
-  int32_t few_cap;                 // most tiles of a few split
+  int32_t few_cap;                 // most tiles of a part
   int32_t chunk_rows;              // rows of a chunk block
 };
 
@@ -65,23 +69,24 @@ inline Sizes sizes_of(const Shape& s) {
   z.few_heads = z.group < kFewUnits ? z.group : kFewUnits;
   z.head_blocks = ceil_div(z.group, kFewUnits);
   z.few_rows = z.group <= kFewUnits ? kFewUnits / z.group : 1;
-  const int pages = 62 * (s.page / kFewTile);  // a wave holds a split's page ids, one a lane
-  z.few_cap = pages < kFewMost ? pages / 4 * 4 : kFewMost;
+  const int pages = 62 * (s.page / kFewTile);  // a wave holds a part's page ids of a sequence, one a lane
+  z.few_cap = pages < kFewMost ? pages : kFewMost;
   z.chunk_rows = chunk_units(s.head_dim) / z.group;
   return z;
 }
 
 struct Layout {
-  size_t seq, few, chunk, join, ml, o, total;
-  int64_t most_few, most_chunk, most_join, slots;
+  size_t seq, part, few, chunk, join, ml, o, total;
+  int64_t most_parts, most_few, most_chunk, most_join, slots;
 };
 
 inline Layout layout_of(const Shape& s) {
   const Sizes z = sizes_of(s);
   Layout l;
   const int64_t few_rows = s.max_q < z.few_rows ? s.max_q : z.few_rows;
-  l.most_few = ceil_div64(kFewWGs, (int64_t)s.hkv * z.head_blocks) +
-               (int64_t)s.batch * (2 + ceil_div64(s.max_k / kFewTile + 2, z.few_cap));
+  l.most_parts = ceil_div64(kFewWGs, (int64_t)s.hkv * z.head_blocks) +
+                 ceil_div64((int64_t)s.batch * (s.max_k / kFewTile + 2 + kFewStart), z.few_cap) + 1;
+  l.most_few = l.most_parts + s.batch;  // a part's end cuts one item in two
   l.slots = l.most_few * few_rows;
   l.most_join = (int64_t)s.batch * few_rows;
   l.most_chunk = 0;
@@ -97,6 +102,7 @@ inline Layout layout_of(const Shape& s) {
   }
   size_t off = align256(H_WORDS * sizeof(int32_t));
   l.seq = off;    off = align256(off + (size_t)s.batch * sizeof(int4));
+  l.part = off;   off = align256(off + (size_t)(l.most_parts + 1) * 3 * sizeof(int4));
   l.few = off;    off = align256(off + (size_t)l.most_few * 2 * sizeof(int4));
   l.chunk = off;  off = align256(off + (size_t)l.most_chunk * 2 * sizeof(int4));
   l.join = off;   off = align256(off + (size_t)l.most_join * sizeof(int4));
@@ -109,7 +115,9 @@ inline Layout layout_of(const Shape& s) {
 // -------------------------------------------------------------------------------- plan
 //
 // Work lists, two int4 an entry:
-//   few:   {sequence, first key, key end, slot or -1} {first query row, rows, keys, -}
+//   few:   {sequence, first key, key end, slot or -1} {first query row, rows, keys, -}, in the
+//          sequences' order
+//   part:  {its first entry of few} and that entry; it goes on to the next part's
 //   chunk: {sequence, first row, first tile, tile end} {first query row, rows, keys, slot or -1}
 //   join:  {output row, first slot, slots from one split to the next, splits}
 // A slot holds the partial result of one query row, all heads.
@@ -118,10 +126,11 @@ struct PlanArgs {
   const int32_t* used;
   int32_t* hdr;
   int4* seq;
+  int4* part;
   int4* few;
   int4* chunk;
   int4* join;
-  int64_t most_few, most_chunk, most_join, slots;
+  int64_t most_parts, most_few, most_chunk, most_join, slots;
   Shape s;
   Sizes z;
 };
@@ -184,9 +193,15 @@ __device__ __forceinline__ int block_tiles(const PlanArgs& a, int n, int L, int 
   return hi > lo ? ceil_div(hi, kChunkTile) - *first : 0;
 }
 
+// 32-key tiles of a sequence of few rows, and the first.
+__device__ __forceinline__ int few_tiles(const PlanArgs& a, int n, int L, int* lo, int* hi) {
+  keys_of(a.s, n, L, 0, n, lo, hi);
+  return *hi > *lo ? ceil_div(*hi, kFewTile) - *lo / kFewTile : 0;
+}
+
 __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanArgs a) {
   __shared__ int3 s_waves[kPlanThreads / 64];
-  __shared__ int s_items[kPlanThreads + 1], s_slots[kPlanThreads + 1], s_blocks[kPlanThreads + 1];
+  __shared__ int s_items[kPlanThreads], s_slots[kPlanThreads], s_blocks[kPlanThreads], s_cost[kPlanThreads];
   __shared__ unsigned long long s_few, s_tiles;
   __shared__ int s_err, s_nblocks;
   const int tid = hx::tid_x(), batch = a.s.batch;
@@ -222,8 +237,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanArgs a) {
       a.seq[b] = make_int4(q0, n, L, 0);
       if (n > 0 && n <= a.z.few_rows) {
         int lo, hi;
-        keys_of(a.s, n, L, 0, n, &lo, &hi);
-        if (hi > lo) atomicAdd(&s_few, (unsigned long long)(ceil_div(hi, kFewTile) - lo / kFewTile));
+        atomicAdd(&s_few, (unsigned long long)(few_tiles(a, n, L, &lo, &hi) + kFewStart));
       } else if (n > 0) {
         blocks = ceil_div(n, a.z.chunk_rows);
       }
@@ -244,41 +258,46 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanArgs a) {
     if (tiles) atomicAdd(&s_tiles, tiles);
     __syncthreads();
   }
-  // Split sizes: for few rows, so that about kFewWGs workgroups run; blocks of chunk rows only
-  // when they are fewer than kChunkWGs.
+  // Parts of the few rows' tiles; blocks of chunk rows are split only when they are fewer than
+  // kChunkWGs.
   const int64_t few_wgs = kFewWGs / (a.s.hkv * a.z.head_blocks) > 0 ? kFewWGs / (a.s.hkv * a.z.head_blocks) : 1;
-  int64_t fs = ((int64_t)s_few + few_wgs - 1) / few_wgs;
-  fs = (fs + 3) / 4 * 4;
-  const int few_split = (int)(fs < kFewLeast ? kFewLeast : fs > a.z.few_cap ? a.z.few_cap : fs);
+  const int64_t even = ((int64_t)s_few + few_wgs - 1) / few_wgs;
+  const int share = (int)(even > a.z.few_cap ? a.z.few_cap : even < kFewLeast ? kFewLeast : even);
+  const int parts = (int)(((int64_t)s_few + share - 1) / share);
   int chunk_split = 1 << 30;
   if ((int64_t)s_nblocks * a.s.hkv < kChunkWGs) {
     const int64_t t = ((int64_t)s_tiles * a.s.hkv + kChunkWGs - 1) / kChunkWGs;
     chunk_split = (int)(t < kChunkLeast ? kChunkLeast : t);
   }
-  int few_base = 0, chunk_base = 0, slot_base = 0, join_base = 0;
+  int few_base = 0, cost_base = 0, chunk_base = 0, slot_base = 0, join_base = 0;
   for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
     const int b = b0 + tid;
     int4 si = make_int4(0, 0, 0, 0);
-    int splits = 0, blocks = 0, rows = 0;
+    int cost = 0, tiles = 0, blocks = 0, rows = 0;
     if (b < batch) {
       si = a.seq[b];
       if (si.y > 0 && si.y <= a.z.few_rows) {
         int lo, hi;
-        keys_of(a.s, si.y, si.z, 0, si.y, &lo, &hi);
-        splits = hi > lo ? ceil_div(ceil_div(hi, kFewTile) - lo / kFewTile, few_split) : 1;
+        tiles = few_tiles(a, si.y, si.z, &lo, &hi);
+        cost = tiles + kFewStart;
         rows = si.y;
       } else if (si.y > 0) {
         blocks = ceil_div(si.y, a.z.chunk_rows);
       }
     }
+    int3 sum;
+    const int3 place = plan_scan(make_int3(cost, blocks, 0), &sum, s_waves);
+    // Tile x of the sequence lies at its place, and kFewStart, and x: its first and last part.
+    const int from = cost_base + place.x, first_part = (tiles ? from + kFewStart : from + cost - 1) / share;
+    const int splits = rows ? (from + cost - 1) / share - first_part + 1 : 0;
     const int joined = splits > 1 ? rows : 0;
-    int3 total, total2;
+    int3 total;
     const int3 at = plan_scan(make_int3(splits, joined * splits, joined), &total, s_waves);
-    const int3 at2 = plan_scan(make_int3(blocks, 0, 0), &total2, s_waves);
     __syncthreads();
     s_items[tid] = at.x;
     s_slots[tid] = at.y;
-    s_blocks[tid] = at2.x;
+    s_blocks[tid] = place.y;
+    s_cost[tid] = from;
     __syncthreads();
     for (int r = 0; r < joined; ++r) {
       const int64_t to = join_base + at.z + r;
@@ -288,19 +307,30 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanArgs a) {
       const int j = plan_find(s_items, kPlanThreads, i);
       const int4 of = a.seq[b0 + j];
       int lo, hi;
-      keys_of(a.s, of.y, of.z, 0, of.y, &lo, &hi);
-      const int t0 = lo / kFewTile, tiles = hi > lo ? ceil_div(hi, kFewTile) - t0 : 0;
-      const int n = tiles > 0 ? ceil_div(tiles, few_split) : 1, sp = i - s_items[j];
-      // Shares of whole rounds of the waves, as even as they come.
-      const int share = ceil_div(ceil_div(tiles, n), 4) * 4;
-      const int from = t0 + (sp * share < tiles ? sp * share : tiles), to = from + share < t0 + tiles ? from + share : t0 + tiles;
-      const int64_t entry = few_base + i;
+      const int n = few_tiles(a, of.y, of.z, &lo, &hi), sp = i - s_items[j], start = s_cost[j];
+      const int first = (n ? start + kFewStart : start + kFewStart - 1) / share, last = (start + kFewStart + n - 1) / share;
+      const int part = first + sp, t0 = lo / kFewTile, base = start + kFewStart;
+      int begin = part * share - base, end = begin + share;
+      begin = t0 + (begin > 0 ? begin : 0);
+      end = t0 + (end < n ? end : n);
+      const int64_t entry = (int64_t)few_base + i;
+      const int4 e0 = make_int4(b0 + j, begin * kFewTile > lo ? begin * kFewTile : lo, end * kFewTile < hi ? end * kFewTile : hi,
+                                last > first ? slot_base + s_slots[j] + sp * of.y : -1);
+      const int4 e1 = make_int4(of.x, of.y, of.z, 0);
       if (entry < a.most_few) {
-        a.few[2 * entry] = make_int4(b0 + j, from * kFewTile > lo ? from * kFewTile : lo, to * kFewTile < hi ? to * kFewTile : hi,
-                                     n > 1 ? slot_base + s_slots[j] + sp * of.y : -1);
-        a.few[2 * entry + 1] = make_int4(of.x, of.y, of.z, 0);
+        a.few[2 * entry] = e0;
+        a.few[2 * entry + 1] = e1;
       }
+      // The first entry of its part, and of parts that have none.
+      for (int q = sp ? part : start ? (start - 1) / share + 1 : 0; q <= part; ++q)
+        if (q < a.most_parts) {
+          a.part[3 * q] = make_int4((int)entry, 0, 0, 0);
+          a.part[3 * q + 1] = e0;
+          a.part[3 * q + 2] = e1;
+        }
     }
+    cost_base += sum.x;
+    const int3 total2 = make_int3(sum.y, 0, 0);
     few_base += total.x;
     slot_base += total.y;
     join_base += total.z;
@@ -343,8 +373,10 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanArgs a) {
   if (tid == 0) {
     int err = s_err;
     // By the bounds that the workspace was sized with none of these can happen.
-    if (few_base > a.most_few || chunk_base > a.most_chunk || join_base > a.most_join || slot_base > a.slots) err |= HX_WERR_GRID;
-    a.hdr[H_FEW] = few_base < a.most_few ? few_base : (int)a.most_few;
+    if (parts > a.most_parts || few_base > a.most_few || chunk_base > a.most_chunk || join_base > a.most_join || slot_base > a.slots) err |= HX_WERR_GRID;
+    const int most = (int)(parts < a.most_parts ? parts : a.most_parts);
+    a.hdr[H_PARTS] = most;
+    a.part[3 * most] = make_int4(few_base < a.most_few ? few_base : (int)a.most_few, 0, 0, 0);
     a.hdr[H_CHUNK] = chunk_base < a.most_chunk ? chunk_base : (int)a.most_chunk;
     a.hdr[H_JOIN] = join_base < a.most_join ? join_base : (int)a.most_join;
     a.hdr[H_ERR] = err;
@@ -368,6 +400,7 @@ struct RunArgs {
   uint16_t* out;
   int64_t out_row, out_head;
   int32_t* hdr;
+  const int4* part;
   const int4* few;
   const int4* chunk;
   const int4* join;
@@ -400,15 +433,22 @@ __device__ __forceinline__ int4 uniform4(const int4* p) {
 __device__ __forceinline__ float fit_up(uint32_t top) { return __uint_as_float((268u - max(top >> 23, 20u)) << 23); }
 __device__ __forceinline__ float fit_down(uint32_t top) { return __uint_as_float((max(top >> 23, 20u) - 14u) << 23); }
 
-// The largest finite magnitude's bits. (An infinite or NaN element passes through any power of two.)
-__device__ __forceinline__ uint32_t largest(const float (&x)[8], uint32_t top) {
+// The largest finite magnitude among packed elements, as their type's bits (a step further than
+// `top`), and those bits as fp32's. (An infinite or NaN element passes through any power of two.)
+template <typename T>
+__device__ __forceinline__ uint32_t largest(uint4 u, uint32_t top) {
+  constexpr uint32_t kInf = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t b = hx::raw_bits(x[e]) & 0x7fffffffu;
-    top = max(top, b < 0x7f800000u ? b : 0u);
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t lo = w[e] & 0x7fffu, hi = w[e] >> 16 & 0x7fffu;
+    top = max(top, lo < kInf ? lo : 0u);
+    top = max(top, hi < kInf ? hi : 0u);
   }
   return top;
 }
+template <typename T>
+__device__ __forceinline__ uint32_t magnitude(uint32_t top) { return __float_as_uint(hx::Elem<T>::lo(top)); }
 
 // Key positions `at + more`, which may lie far past the last key.
 __device__ __forceinline__ int beyond(int at, int more) {
@@ -443,245 +483,292 @@ __device__ __forceinline__ uint2 ld8_lds_tr8(const void* p) {
   return __builtin_bit_cast(uint2, r);
 }
 
-// LDS position of 16-byte piece p of value row r, of DP bytes: 16 rows' pieces of one dim block
-// then cover all banks once.
-template <int DP>
-__device__ __forceinline__ int v8_piece(int r, int p) {
-  return DP == 64 ? p ^ ((r >> 2) & 3) : DP == 128 ? p ^ ((r >> 1) & 7) : p ^ (r & 15);
-}
-
 constexpr float kFewShift = 14.f;  // weights are scaled by 2^14 into fp16, and their remainders stay normal
+constexpr float kFewLazy = 1.f;    // the reference maximum moves when exceeded by this, in log2
+
+template <int DP>
+struct FewLds {
+  union {
+    // The waves' codes. Rows of an odd number of 16-byte pieces: 16 rows' pieces of one dim block
+    // cover all banks once.
+    struct {
+      __attribute__((aligned(16))) uint8_t k[4][kFewTile * (DP + 16)];
+      __attribute__((aligned(16))) uint8_t v[4][kFewTile * (DP + 16)];
+    };
+    __attribute__((aligned(16))) float o[4][kFewUnits][DP];    // their results
+  };
+  __attribute__((aligned(16))) float scale[4][3][kFewTile];    // of a tile: keys' scales, log2 and inverse of values'
+  float m[4][kFewUnits], l[4][kFewUnits];
+};
+
+struct FewItem {
+  int seq, k0, k1, slot;  // keys [k0, k1)
+  int q0, n, L;
+  int h, head0, heads;    // KV head, first query head and how many
+};
 
 // One item and KV head (and block of 16 query heads) to a workgroup. The units, (row, head) pairs,
-// are the columns of S^T = K Q^T. A wave walks every fourth 32-key tile on its own, the next one's
-// codes in flight in registers: key codes are the MFMA's operand as they are loaded (lane r of a
-// 16-lane group takes key 8 (r / 4) + 4 u + r % 4 for block u, so that a lane's 8 scores belong to 8
-// consecutive keys), value codes pass through LDS to be read transposed. Up to 8 units have a
-// second set of columns, which carries the weights' remainders; more take a second MFMA: 22 bits.
-template <typename T, typename C, int DP>
-__global__ __launch_bounds__(kFewThreads) void kv8_few_kernel(RunArgs a, int n_wg) {
+// are the columns of S^T = K Q^T. A wave walks every fourth 32-key tile on its own through its part
+// of LDS, the next one's codes in flight in registers. Row r of the MFMA's operand for block u is key
+// 8 (r / 4) + 4 u + r % 4, so that a lane's 8 scores belong to 8 consecutive keys; value codes are
+// read transposed. TWICE: up to 8 units, whose
+// second set of columns carries the weights' remainders; more take a second MFMA: 22 bits.
+template <typename T, typename C, int DP, bool TWICE>
+__device__ __forceinline__ void few_item(const RunArgs& a, FewLds<DP>& lds, const FewItem& it) {
   typedef hx::f16x8_t v8;
   typedef hx::Elem<_Float16> E;
   constexpr int kLoads = DP / 64, kSteps = DP / 32, kDims = DP / 16, kPieces = DP / 16, kVLoads = DP / 32;
-  constexpr int kStage = kFewTile * DP;
-  constexpr int kLdsBytes = 4 * kStage > 4 * kFewUnits * DP * 4 ? 4 * kStage : 4 * kFewUnits * DP * 4;
-  __shared__ __attribute__((aligned(16))) uint8_t smem[kLdsBytes];
-  __shared__ float s_m[4][kFewUnits], s_l[4][kFewUnits];
   const int tid = hx::tid_x(), lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int4 counts;
-  if (!plan_ok(a, &counts)) return;
-  const int per_item = a.s.hkv * a.z.head_blocks, D = a.s.head_dim, page = a.s.page;
-  const int64_t work = (int64_t)counts.x * per_item;
+  const int D = a.s.head_dim, page = a.s.page, k0 = it.k0, k1 = it.k1, heads = it.heads, units = it.n * heads;
   const uint32_t row_bytes = (uint32_t)a.s.hkv * (uint32_t)D;
-  uint8_t* const vt = smem + w * kStage;
+  uint8_t *const kt = lds.k[w], *const vt = lds.v[w];
+  const int unit = TWICE ? lr & 7 : lr;
+  const bool live = unit < units;
+  const int urow = live ? unit / heads : 0, uhead = it.head0 + (live ? unit - urow * heads : 0);
 
-  for (int64_t i = hx::wg_x(); i < work; i += n_wg) {
-    const int item = (int)((uint32_t)i / (uint32_t)per_item), sub = (int)((uint32_t)i % (uint32_t)per_item);
-    const int hb = sub / a.s.hkv, h = sub - hb * a.s.hkv;
-    const int4 it = uniform4(a.few + 2 * (int64_t)item), si = uniform4(a.few + 2 * (int64_t)item + 1);
-    const int k0 = it.y, k1 = it.z, n = si.y, L = si.z;
-    const int heads = min(a.z.few_heads, a.z.group - hb * kFewUnits), units = n * heads;
-    const int head0 = h * a.z.group + hb * kFewUnits;
-    const bool twice = units <= 8;
-    const int unit = twice ? lr & 7 : lr;
-    const bool live = unit < units;
-    const int urow = live ? unit / heads : 0, uhead = head0 + (live ? unit - urow * heads : 0);
+  const int t0 = k0 / kFewTile, t1 = k1 > k0 ? (k1 + kFewTile - 1) / kFewTile : t0;
+  // Page ids of the item's keys: lane j holds that of page pg0 + j.
+  const int pg0 = t0 * kFewTile / page;
+  int ids = -1;
+  if (t1 > t0 && pg0 + lane <= (k1 - 1) / page) ids = a.table[(int64_t)it.seq * a.table_stride + pg0 + lane];
 
-    v8 qf[kSteps];
-    float qc;  // of this lane's unit: log2(e) scale, and what undoes q's power of two
-    {
-      float x[kSteps][8];
-      uint32_t top = 0;
-      const uint16_t* const qp = a.q + (int64_t)(si.x + urow) * a.q_row + (int64_t)uhead * a.q_head;
+  v8 qf[kSteps];
+  float qc;  // of this lane's unit: log2(e) scale, and what undoes q's power of two
+  {
+    uint4 raw[kSteps];
+    const uint16_t* const qp = a.q + (int64_t)(it.q0 + urow) * a.q_row + (int64_t)uhead * a.q_head;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int d = 64 * (s >> 1) + 16 * lg + 8 * (s & 1);
-        widen8<T>(live && d < D ? *reinterpret_cast<const uint4*>(qp + d) : hx::zero4(), x[s]);
-        top = largest(x[s], top);
-      }
-      top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-      top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-      const float up = fit_up(top);
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) qf[s] = hx::as_v8<_Float16>(pack8(x[s], up));
-      qc = a.scale_log2 * fit_down(top);
+    for (int s = 0; s < kSteps; ++s) {
+      const int d = 64 * (s >> 1) + 16 * lg + 8 * (s & 1);
+      raw[s] = live && d < D ? *reinterpret_cast<const uint4*>(qp + d) : hx::zero4();
     }
-    // Keys this lane's unit sees of the item's. (Columns without a unit have q = 0 and go nowhere.)
-    int klo = k0, khi = k1 - 1;
-    {
-      const int at = L - n + urow;
-      if (a.s.left >= 0) klo = max(klo, at > a.s.left ? at - a.s.left : 0);
-      if (a.s.right >= 0) khi = min(khi, beyond(at, a.s.right));
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) top = largest<T>(raw[s], top);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    top = magnitude<T>(top);
+    const float up = fit_up(top);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      float x[8];
+      widen8<T>(raw[s], x);
+      qf[s] = hx::as_v8<_Float16>(pack8(x, up));
     }
+    qc = a.scale_log2 * fit_down(top);
+  }
+  // Keys this lane's unit sees of the item's. (Columns without a unit have q = 0 and go nowhere.)
+  int klo = k0, khi = k1 - 1;
+  {
+    const int at = it.L - it.n + urow;
+    if (a.s.left >= 0) klo = max(klo, at > a.s.left ? at - a.s.left : 0);
+    if (a.s.right >= 0) khi = min(khi, beyond(at, a.s.right));
+  }
 
-    const int t0 = k0 / kFewTile, t1 = k1 > k0 ? (k1 + kFewTile - 1) / kFewTile : t0;
-    // Page ids of the item's keys: lane j holds that of page pg0 + j.
-    const int pg0 = t0 * kFewTile / page;
-    int ids = -1;
-    if (t1 > t0 && pg0 + lane <= (k1 - 1) / page) ids = a.table[(int64_t)it.x * a.table_stride + pg0 + lane];
+  // Lane l of a load takes piece l % kPieces of row l / kPieces: whole rows, side by side. Past
+  // head_dim its offset is one that no tile reaches.
+  constexpr int kRows = 64 / kPieces;  // rows of a load
+  const uint32_t off = 16 * (lane % kPieces) < D ? (uint32_t)(lane / kPieces) * row_bytes + 16u * (lane % kPieces) : 0x7ffffff0u;
+  const int to = lane / kPieces * (DP + 16) + 16 * (lane % kPieces);
+  uint4 kb[kVLoads], vb[kVLoads];
+  float sreg;  // lanes 0-31: the keys' scales, 32-63: the values'
+  int next_cnt = 0;
+  bool bad = false;
+  auto load = [&](int t) __attribute__((always_inline)) {
+    const int key0 = t * kFewTile, j = key0 / page;
+    int id = __builtin_amdgcn_readlane(ids, j - pg0);
+    const bool none = (unsigned)id >= (unsigned)a.num_pages;
+    bad |= none;
+    id = none ? 0 : id;
+    const int cnt = none ? 0 : min(kFewTile, k1 - key0);
+    next_cnt = cnt;
+    const int64_t in = key0 - j * page;
+    const int64_t base = (((int64_t)id * page + in) * a.s.hkv + it.h) * D;
+    const uint32_t bytes = cnt > 0 ? (uint32_t)(cnt - 1) * row_bytes + (uint32_t)D : 0u;
+    const __amdgpu_buffer_rsrc_t kr = hx::buffer_rsrc(a.k + base, bytes), vr = hx::buffer_rsrc(a.v + base, bytes);
+#pragma unroll
+    for (int q = 0; q < kVLoads; ++q) kb[q] = hx::ld16_stream(kr, off, q * kRows * row_bytes);
+    const float* const sp = lane < 32 ? a.k_scale : a.v_scale;
+    sreg = sp[((int64_t)id * a.s.hkv + it.h) * page + in + (lane & 31)];
+#pragma unroll
+    for (int q = 0; q < kVLoads; ++q) vb[q] = hx::ld16_stream(vr, off, q * kRows * row_bytes);
+  };
 
-    uint4 kb[2][kLoads], vb[kVLoads];
-    float4 ks[2], vs[2];
-    int next_cnt = 0;
-    bool bad = false;
-    auto load = [&](int t) __attribute__((always_inline)) {
-      const int key0 = t * kFewTile, j = key0 / page;
-      int id = __builtin_amdgcn_readlane(ids, j - pg0);
-      const bool off = (unsigned)id >= (unsigned)a.num_pages;
-      bad |= off;
-      id = off ? 0 : id;
-      const int cnt = off ? 0 : min(kFewTile, k1 - key0);
-      next_cnt = cnt;
-      const int64_t in = key0 - j * page;
-      const int64_t base = (((int64_t)id * page + in) * a.s.hkv + h) * D;
-      const uint32_t bytes = cnt > 0 ? (uint32_t)(cnt - 1) * row_bytes + (uint32_t)D : 0u;
-      const __amdgpu_buffer_rsrc_t kr = hx::buffer_rsrc(a.k + base, bytes), vr = hx::buffer_rsrc(a.v + base, bytes);
+  float m_run = -INFINITY, l_run = 0.f;
+  hx::f32x4_t o[kDims];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int q = 0; q < kLoads; ++q) {
-          const int d = 64 * q + 16 * lg;
-          const uint32_t at = (uint32_t)(8 * (lr >> 2) + 4 * u + (lr & 3)) * row_bytes + (uint32_t)d;
-          kb[u][q] = hx::ld16_stream(kr, d < D ? at : 0x7ffffff0u, 0);
-        }
-      const int piece = lane % kPieces, tok = lane / kPieces;
-#pragma unroll
-      for (int q = 0; q < kVLoads; ++q)
-        vb[q] = hx::ld16_stream(vr, 16 * piece < D ? (uint32_t)(tok + q * (64 / kPieces)) * row_bytes + 16u * piece : 0x7ffffff0u, 0);
-      const int64_t st = ((int64_t)id * a.s.hkv + h) * page + in + 8 * lg;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        ks[e] = *reinterpret_cast<const float4*>(a.k_scale + st + 4 * e);
-        vs[e] = *reinterpret_cast<const float4*>(a.v_scale + st + 4 * e);
-      }
-    };
+  for (int d = 0; d < kDims; ++d) o[d] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-    float m_run = -INFINITY, l_run = 0.f;
-    hx::f32x4_t o[kDims];
+  int t = t0 + w;
+  if (t < t1) load(t);
+  while (t < t1) {
+    const int key0 = t * kFewTile, cnt = next_cnt;
+    t += 4;
 #pragma unroll
-    for (int d = 0; d < kDims; ++d) o[d] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-    int t = t0 + w;
+    for (int q = 0; q < kVLoads; ++q) {
+      *reinterpret_cast<uint4*>(kt + to + q * kRows * (DP + 16)) = kb[q];
+      *reinterpret_cast<uint4*>(vt + to + q * kRows * (DP + 16)) = vb[q];
+    }
+    // A lane's key or value scale to where its 16 columns' lanes find 8 in a row.
+    {
+      const float lv = __builtin_amdgcn_logf(sreg), iv = __builtin_amdgcn_rcpf(sreg);
+      lds.scale[w][lane < 32 ? 0 : 1][lane & 31] = lane < 32 ? sreg : lv;
+      if (lane >= 32) lds.scale[w][2][lane & 31] = iv;
+    }
+    // Lanes read what others of the wave stored: a wave's LDS accesses complete in order, the
+    // fences hold the compiler to it.
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (t < t1) load(t);
-    while (t < t1) {
-      const int key0 = t * kFewTile, cnt = next_cnt;
+    hx::f32x4_t sc[2];
 #pragma unroll
-      for (int q = 0; q < kVLoads; ++q) {
-        const int r = lane / kPieces + q * (64 / kPieces);
-        *reinterpret_cast<uint4*>(vt + r * DP + 16 * v8_piece<DP>(r, lane % kPieces)) = vb[q];
+    for (int u = 0; u < 2; ++u) {
+      sc[u] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) {
+        const uint4 kw = *reinterpret_cast<const uint4*>(kt + (8 * (lr >> 2) + 4 * u + (lr & 3)) * (DP + 16) + 64 * q + 16 * lg);
+        sc[u] = E::mfma16x16x32(codes8<C>(make_uint2(kw.x, kw.y)), qf[2 * q], sc[u]);
+        sc[u] = E::mfma16x16x32(codes8<C>(make_uint2(kw.z, kw.w)), qf[2 * q + 1], sc[u]);
       }
-      // Lanes read what others of the wave stored: a wave's LDS accesses complete in order, the
-      // fences hold the compiler to it.
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      hx::f32x4_t sc[2];
+    }
+    float u[8], inv[8];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        sc[u] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int q = 0; q < kLoads; ++q) {
-          sc[u] = E::mfma16x16x32(codes8<C>(make_uint2(kb[u][q].x, kb[u][q].y)), qf[2 * q], sc[u]);
-          sc[u] = E::mfma16x16x32(codes8<C>(make_uint2(kb[u][q].z, kb[u][q].w)), qf[2 * q + 1], sc[u]);
-        }
-      }
-      const float kf[8] = {ks[0].x, ks[0].y, ks[0].z, ks[0].w, ks[1].x, ks[1].y, ks[1].z, ks[1].w};
-      const float vf[8] = {vs[0].x, vs[0].y, vs[0].z, vs[0].w, vs[1].x, vs[1].y, vs[1].z, vs[1].w};
-      float u[8], inv[8];
-      t += 4;
-      const int next = t;
+    for (int e = 0; e < 8; e += 4) {
+      const float4 ks = *reinterpret_cast<const float4*>(&lds.scale[w][0][8 * lg + e]);
+      const float4 lv = *reinterpret_cast<const float4*>(&lds.scale[w][1][8 * lg + e]);
+      const float4 iv = *reinterpret_cast<const float4*>(&lds.scale[w][2][8 * lg + e]);
+      u[e] = fmaf(sc[e / 4][0], ks.x * qc, lv.x);
+      u[e + 1] = fmaf(sc[e / 4][1], ks.y * qc, lv.y);
+      u[e + 2] = fmaf(sc[e / 4][2], ks.z * qc, lv.z);
+      u[e + 3] = fmaf(sc[e / 4][3], ks.w * qc, lv.w);
+      inv[e] = iv.x;
+      inv[e + 1] = iv.y;
+      inv[e + 2] = iv.z;
+      inv[e + 3] = iv.w;
+    }
+    const int from = key0 + 8 * lg, last = min(khi, key0 + cnt - 1);
+    if (__any(from < klo || from + 7 > last)) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        u[e] = fmaf(sc[e >> 2][e & 3], kf[e] * qc, __builtin_amdgcn_logf(vf[e]));
-        inv[e] = __builtin_amdgcn_rcpf(vf[e]);
+        const bool seen = from + e >= klo && from + e <= last;
+        u[e] = seen ? u[e] : -INFINITY;
+        inv[e] = seen ? inv[e] : 0.f;
       }
-      if (next < t1) load(next);
-      const int from = key0 + 8 * lg, last = min(khi, key0 + cnt - 1);
-      if (__any(from < klo || from + 7 > last)) {
+    }
+    float mx = fmaxf(u[0], u[1]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const bool seen = from + e >= klo && from + e <= last;
-          u[e] = seen ? u[e] : -INFINITY;
-          inv[e] = seen ? inv[e] : 0.f;
-        }
-      }
-      float mx = m_run;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, u[e]);
-      mx = hx::max_xor32(hx::max_xor16(mx));
-      const float alpha = mx == -INFINITY ? 1.f : hx::fast_exp2(m_run - mx);
-      const float neg = mx == -INFINITY ? 0.f : kFewShift - mx;
-      m_run = mx;
+    for (int e = 2; e < 8; ++e) mx = fmaxf(mx, u[e]);
+    mx = hx::max_xor32(hx::max_xor16(mx));
+    const bool move = mx > m_run + kFewLazy;
+    if (__any(move)) {
+      const float alpha = move ? hx::fast_exp2(m_run - mx) : 1.f;
+      m_run = move ? mx : m_run;
       l_run *= alpha;
 #pragma unroll
       for (int d = 0; d < kDims; ++d) o[d] *= alpha;
-      uint32_t pw[4], pr[4];
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const float p0 = hx::fast_exp2(u[e] + neg), p1 = hx::fast_exp2(u[e + 1] + neg);
-        l_run = fmaf(p0, inv[e], l_run);
-        l_run = fmaf(p1, inv[e + 1], l_run);
-        const uint32_t top = hx::pack2_round<_Float16>(p0, p1);
-        pr[e / 2] = hx::pack2_round<_Float16>(p0 - E::lo(top), p1 - E::hi(top));
-        pw[e / 2] = twice && lr >= 8 ? pr[e / 2] : top;
-      }
-      const v8 pf = hx::as_v8<_Float16>(make_uint4(pw[0], pw[1], pw[2], pw[3]));
-      const v8 pf2 = hx::as_v8<_Float16>(make_uint4(pr[0], pr[1], pr[2], pr[3]));
-#pragma unroll
-      for (int d = 0; d < kDims; ++d) {
-        const int r = 8 * lg + (lr >> 1);
-        const v8 vv = codes8<C>(ld8_lds_tr8(vt + r * DP + 16 * v8_piece<DP>(r, d) + 8 * (lr & 1)));
-        o[d] = E::mfma16x16x32(vv, pf, o[d]);
-        if (!twice) o[d] = E::mfma16x16x32(vv, pf2, o[d]);
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    if (bad && lane == 0) atomicOr(&a.hdr[H_ERR], HX_WERR_BAD_PAGE);
+    const float neg = m_run == -INFINITY ? 0.f : kFewShift - m_run;
+    uint32_t pw[4], pr[4];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float p0 = hx::fast_exp2(u[e] + neg), p1 = hx::fast_exp2(u[e + 1] + neg);
+      l_run = fmaf(p0, inv[e], l_run);
+      l_run = fmaf(p1, inv[e + 1], l_run);
+      pw[e / 2] = hx::pack2_round<_Float16>(p0, p1);
+      pr[e / 2] = hx::pack2_round<_Float16>(p0 - E::lo(pw[e / 2]), p1 - E::hi(pw[e / 2]));
+      if (TWICE) pw[e / 2] = lr >= 8 ? pr[e / 2] : pw[e / 2];
+    }
+    const v8 pf = hx::as_v8<_Float16>(make_uint4(pw[0], pw[1], pw[2], pw[3]));
+    const v8 pf2 = hx::as_v8<_Float16>(make_uint4(pr[0], pr[1], pr[2], pr[3]));
+    const uint8_t* const vp = vt + (8 * lg + (lr >> 1)) * (DP + 16) + 8 * (lr & 1);
+#pragma unroll
+    for (int d0 = 0; d0 < kDims; d0 += 4) {
+      uint2 vw[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) vw[e] = ld8_lds_tr8(vp + 16 * (d0 + e));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const v8 vv = codes8<C>(vw[e]);
+        o[d0 + e] = E::mfma16x16x32(vv, pf, o[d0 + e]);
+        if (!TWICE) o[d0 + e] = E::mfma16x16x32(vv, pf2, o[d0 + e]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  if (bad && lane == 0) atomicOr(&a.hdr[H_ERR], HX_WERR_BAD_PAGE);
 
-    // Lane: dims 16 d + 4 lg .. + 3 of its unit; remainders' columns added.
-    l_run = hx::add_xor32(hx::add_xor16(l_run));
-    if (twice) {
-#pragma unroll
-      for (int d = 0; d < kDims; ++d)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[d][e] += hx::dpp<0x128>(o[d][e]);  // the lane 8 apart in its row of 16
-    }
-    __syncthreads();  // every wave is done with its stage
-    float (*const s_o)[kFewUnits][DP] = reinterpret_cast<float (*)[kFewUnits][DP]>(smem);
+  // Lane: dims 16 d + 4 lg .. + 3 of its unit; remainders' columns added.
+  l_run = hx::add_xor32(hx::add_xor16(l_run));
+  if (TWICE) {
 #pragma unroll
     for (int d = 0; d < kDims; ++d)
-      *reinterpret_cast<float4*>(&s_o[w][lr][16 * d + 4 * lg]) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[d][e] += hx::dpp<0x128>(o[d][e]);  // the lane 8 apart in its row of 16
+  }
+  __syncthreads();  // every wave is done with its stage
+  if (lr < units) {
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+      *reinterpret_cast<float4*>(&lds.o[w][lr][16 * d + 4 * lg]) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
     if (lg == 0) {
-      s_m[w][lr] = m_run;
-      s_l[w][lr] = l_run;
+      lds.m[w][lr] = m_run;
+      lds.l[w][lr] = l_run;
     }
-    __syncthreads();
-    const int half = D / 2;
-    for (int e = tid; e < units * half; e += kFewThreads) {
-      const int un = e / half, d = 2 * (e % half);
-      float m = s_m[0][un];
+  }
+  __syncthreads();
+  const int half = D / 2;
+  for (int e = tid; e < units * half; e += kFewThreads) {
+    const int un = e / half, d = 2 * (e % half);
+    float m = lds.m[0][un];
 #pragma unroll
-      for (int ww = 1; ww < 4; ++ww) m = fmaxf(m, s_m[ww][un]);
-      const float ref = m == -INFINITY ? 0.f : m;
-      float l = 0.f, x = 0.f, y = 0.f;
+    for (int ww = 1; ww < 4; ++ww) m = fmaxf(m, lds.m[ww][un]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-      for (int ww = 0; ww < 4; ++ww) {
-        const float f = hx::fast_exp2(s_m[ww][un] - ref);
-        l = fmaf(f, s_l[ww][un], l);
-        x = fmaf(f, s_o[ww][un][d], x);
-        y = fmaf(f, s_o[ww][un][d + 1], y);
-      }
-      const int row = un / heads, head = head0 + un - row * heads;
-      if (it.w < 0) {
-        const float r = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-        *reinterpret_cast<uint32_t*>(a.out + (int64_t)(si.x + row) * a.out_row + (int64_t)head * a.out_head + d) =
-            hx::pack2_round<T>(x * r, y * r);
-      } else if ((int64_t)it.w + row < a.slots) {
-        const int64_t p = ((int64_t)it.w + row) * a.s.hq + head;
-        *reinterpret_cast<float2*>(a.part_o + p * D + d) = make_float2(x, y);
-        if (d == 0) a.part_ml[p] = make_float2(m, l);
-      }
+    for (int ww = 0; ww < 4; ++ww) {
+      const float f = hx::fast_exp2(lds.m[ww][un] - ref);
+      l = fmaf(f, lds.l[ww][un], l);
+      x = fmaf(f, lds.o[ww][un][d], x);
+      y = fmaf(f, lds.o[ww][un][d + 1], y);
     }
-    __syncthreads();  // the next item's stages take the place of s_o
+    const int row = un / heads, head = it.head0 + un - row * heads;
+    if (it.slot < 0) {
+      const float r = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+      *reinterpret_cast<uint32_t*>(a.out + (int64_t)(it.q0 + row) * a.out_row + (int64_t)head * a.out_head + d) =
+          hx::pack2_round<T>(x * r, y * r);
+    } else if ((int64_t)it.slot + row < a.slots) {
+      const int64_t p = ((int64_t)it.slot + row) * a.s.hq + head;
+      *reinterpret_cast<float2*>(a.part_o + p * D + d) = make_float2(x, y);
+      if (d == 0) a.part_ml[p] = make_float2(m, l);
+    }
+  }
+  __syncthreads();  // the next item's stages take the place of the results
+}
+
+template <typename T, typename C, int DP>
+__global__ __launch_bounds__(kFewThreads, DP == 256 ? 2 : DP == 128 ? 3 : 4) void kv8_few_kernel(RunArgs a, int n_wg) {
+  __shared__ FewLds<DP> lds;
+  // All parts of one head, then of the next: a head's rows are every eighth 128 bytes of memory, say,
+  // and what one head's reads bring along of its neighbours' is there when theirs come. (Heads side
+  // by side: 3.9 to 5.4 TB/s of loads alone; this way 5.8 to 6.4.)
+  int4 counts;
+  if (!plan_ok(a, &counts)) return;
+  const int64_t work = (int64_t)counts.x * a.s.hkv * a.z.head_blocks;
+  for (int64_t i = hx::wg_x(); i < work; i += n_wg) {
+    const int sub = (int)((uint32_t)i / (uint32_t)counts.x), part = (int)((uint32_t)i - (uint32_t)sub * (uint32_t)counts.x);
+    const int hb = sub / a.s.hkv, h = sub - hb * a.s.hkv;
+    int4 e0 = uniform4(a.part + 3 * part + 1), e1 = uniform4(a.part + 3 * part + 2);
+    const int first = __builtin_amdgcn_readfirstlane(a.part[3 * part].x), end = __builtin_amdgcn_readfirstlane(a.part[3 * part + 3].x);
+    for (int item = first; item < end; ++item) {
+      if (item > first) {
+        e0 = uniform4(a.few + 2 * (int64_t)item);
+        e1 = uniform4(a.few + 2 * (int64_t)item + 1);
+      }
+      const FewItem it{e0.x, e0.y, e0.z, e0.w, e1.x, e1.y, e1.z, h, h * a.z.group + hb * kFewUnits,
+                       min(a.z.few_heads, a.z.group - hb * kFewUnits)};
+      if (it.n * it.heads <= 8) few_item<T, C, DP, true>(a, lds, it);
+      else few_item<T, C, DP, false>(a, lds, it);
+    }
   }
 }
 
@@ -749,14 +836,12 @@ __global__ __launch_bounds__(kChunkThreads, 2) void kv8_chunk_kernel(RunArgs a, 
         for (int s = 0; s < kSteps; ++s) {
           const int d = 32 * s + 8 * lg;
           raw[rb][s] = live[rb] && d < D ? *reinterpret_cast<const uint4*>(qp + d) : hx::zero4();
-          float x[8];
-          widen8<T>(raw[rb][s], x);
-          top = largest(x, top);
+          top = largest<T>(raw[rb][s], top);
         }
       }
       // One power of two for the wave's units.
       for (int m = 1; m < 64; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m));
-      top = __builtin_amdgcn_readfirstlane((int)top);
+      top = magnitude<T>((uint32_t)__builtin_amdgcn_readfirstlane((int)top));
       const float up = fit_up(top);
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
@@ -1101,8 +1186,8 @@ template <typename T, typename C, int DP>
 void launch_run(const Run& r, bool few, bool chunk) {
   const RunArgs& a = r.a;
   if (few) {
-    const int64_t most = r.l.most_few * a.s.hkv * a.z.head_blocks;
-    const int n = (int)(most < 8192 ? most : 8192);
+    const int64_t most = r.l.most_parts * a.s.hkv * a.z.head_blocks;
+    const int n = (int)(most < 65536 ? most : 65536);
     hipLaunchKernelGGL((kv8_few_kernel<T, C, DP>), dim3(n), dim3(kFewThreads), 0, r.s, a, n);
   }
   if (chunk) {
@@ -1123,8 +1208,8 @@ template <typename T>
 int launch_run(const Run& r, int32_t code, bool few, bool chunk) {
   if (code == HX_CODE_E4M3) launch_run<T, hx8::E4m3>(r, few, chunk);
   else launch_run<T, hx8::Int8>(r, few, chunk);
-  // Splits exist past the least split of a few item, and among few chunk blocks.
-  if ((few && r.a.s.max_k > kFewLeast * kFewTile - kFewTile) || (chunk && r.a.s.max_k > kChunkLeast * kChunkTile - kChunkTile)) {
+  // Sequences may be cut wherever a part ends; blocks of chunk rows past the least of a split.
+  if (few || (chunk && r.a.s.max_k > kChunkLeast * kChunkTile - kChunkTile)) {
     const int64_t most = r.l.most_join * r.a.s.hq;
     const int n = (int)(most < 4096 ? most : 4096);
     hipLaunchKernelGGL(kv8_join_kernel<T>, dim3(n), dim3(kJoinThreads), 0, r.s, r.a, n);
@@ -1156,16 +1241,18 @@ extern "C" int hx_kv8_attn_plan(const int32_t* cu_seq_q, const int32_t* seqused_
   if (!cu_seq_q || !seqused_k) return HX_E_INVALID_ARG;
   const Layout l = layout_of(s);
   if (!workspace || misaligned(workspace, 256) || workspace_bytes < l.total) return HX_E_WORKSPACE;
-  if (l.slots > 0x7fffffff || l.most_chunk > 0x7fffffff / n_kv_heads || l.most_few > 0x7fffffff / n_q_heads) return HX_E_UNSUPPORTED;
+  if (l.slots > 0x7fffffff || l.most_chunk > 0x7fffffff / n_kv_heads || l.most_parts > 0x7ffffff / n_q_heads) return HX_E_UNSUPPORTED;
   uint8_t* const base = static_cast<uint8_t*>(workspace);
   PlanArgs a;
   a.cu_q = cu_seq_q;
   a.used = seqused_k;
   a.hdr = reinterpret_cast<int32_t*>(base);
   a.seq = reinterpret_cast<int4*>(base + l.seq);
+  a.part = reinterpret_cast<int4*>(base + l.part);
   a.few = reinterpret_cast<int4*>(base + l.few);
   a.chunk = reinterpret_cast<int4*>(base + l.chunk);
   a.join = reinterpret_cast<int4*>(base + l.join);
+  a.most_parts = l.most_parts;
   a.most_few = l.most_few;
   a.most_chunk = l.most_chunk;
   a.most_join = l.most_join;
@@ -1215,6 +1302,7 @@ extern "C" int hx_kv8_attn_run(const void* q, int64_t q_row_stride, int64_t q_he
   a.out_row = out_row_stride;
   a.out_head = out_head_stride;
   a.hdr = reinterpret_cast<int32_t*>(base);
+  a.part = reinterpret_cast<const int4*>(base + r.l.part);
   a.few = reinterpret_cast<const int4*>(base + r.l.few);
   a.chunk = reinterpret_cast<const int4*>(base + r.l.chunk);
   a.join = reinterpret_cast<const int4*>(base + r.l.join);
