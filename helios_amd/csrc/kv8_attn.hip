@@ -34,7 +34,7 @@ constexpr int kFewWGs = 768;      // workgroups, about: 3 a CU, all at once
 constexpr int kFewStart = 8;
 constexpr int kFewLeast = 24;     // of a part, at least: tiles and starts
 constexpr int kFewMost = 256;     // and at most
-constexpr int kChunkThreads = 512;
+constexpr int kChunkUnits = 128;  // (row, head) pairs of a chunk block
 constexpr int kChunkTile = 64;
 constexpr int kChunkWGs = 512;    // workgroups below which row blocks are split
 constexpr int kChunkLeast = 4;    // tiles of a split, at least
@@ -61,7 +61,6 @@ struct Sizes {
   int32_t chunk_rows;              // rows of a chunk block
 };
 
-__host__ __device__ inline int chunk_units(int head_dim) { return head_dim > 128 ? 128 : 256; }
 
 inline Sizes sizes_of(const Shape& s) {
   Sizes z;
@@ -71,7 +70,7 @@ inline Sizes sizes_of(const Shape& s) {
   z.few_rows = z.group <= kFewUnits ? kFewUnits / z.group : 1;
   const int pages = 62 * (s.page / kFewTile);  // a wave holds a part's page ids of a sequence, one a lane
   z.few_cap = pages < kFewMost ? pages : kFewMost;
-  z.chunk_rows = chunk_units(s.head_dim) / z.group;
+  z.chunk_rows = kChunkUnits / z.group;
   return z;
 }
 
@@ -450,6 +449,17 @@ __device__ __forceinline__ uint32_t largest(uint4 u, uint32_t top) {
 template <typename T>
 __device__ __forceinline__ uint32_t magnitude(uint32_t top) { return __float_as_uint(hx::Elem<T>::lo(top)); }
 
+// A value's scale as the softmax takes it. A NaN makes the weight NaN through its logarithm, and has
+// an inverse that leaves the weight 0 of a row that does not see the key alone.
+struct ValueScale {
+  float log, inverse;
+};
+__device__ __forceinline__ ValueScale value_scale(float s) {
+  const bool nan = (hx::raw_bits(s) & 0x7fffffffu) > 0x7f800000u;
+  const float at_least = nan ? 1.f : fmaxf(s, hx8::kLeastScale);
+  return {nan ? __uint_as_float(0x7fc00000u) : __builtin_amdgcn_logf(at_least), __builtin_amdgcn_rcpf(at_least)};
+}
+
 // Key positions `at + more`, which may lie far past the last key.
 __device__ __forceinline__ int beyond(int at, int more) {
   const int64_t x = (int64_t)at + more;
@@ -612,9 +622,9 @@ __device__ __forceinline__ void few_item(const RunArgs& a, FewLds<DP>& lds, cons
     }
     // A lane's key or value scale to where its 16 columns' lanes find 8 in a row.
     {
-      const float lv = __builtin_amdgcn_logf(sreg), iv = __builtin_amdgcn_rcpf(sreg);
-      lds.scale[w][lane < 32 ? 0 : 1][lane & 31] = lane < 32 ? sreg : lv;
-      if (lane >= 32) lds.scale[w][2][lane & 31] = iv;
+      const ValueScale v = value_scale(sreg);
+      lds.scale[w][lane < 32 ? 0 : 1][lane & 31] = lane < 32 ? sreg : v.log;
+      if (lane >= 32) lds.scale[w][2][lane & 31] = v.inverse;
     }
     // Lanes read what others of the wave stored: a wave's LDS accesses complete in order, the
     // fences hold the compiler to it.
@@ -652,7 +662,6 @@ __device__ __forceinline__ void few_item(const RunArgs& a, FewLds<DP>& lds, cons
       for (int e = 0; e < 8; ++e) {
         const bool seen = from + e >= klo && from + e <= last;
         u[e] = seen ? u[e] : -INFINITY;
-        inv[e] = seen ? inv[e] : 0.f;
       }
     }
     float mx = fmaxf(u[0], u[1]);
@@ -773,30 +782,35 @@ __global__ __launch_bounds__(kFewThreads, DP == 256 ? 2 : DP == 128 ? 3 : 4) voi
 }
 
 // ------------------------------------------------------------------------------- chunks
+constexpr int chunk_threads(int dp) { return dp == 256 ? 512 : 256; }
 constexpr float kChunkShift = 7.f;  // 2^7 times weights of up to 2^8 fits fp16
 constexpr float kLazy = 8.f;        // the reference maximum moves when exceeded by this, in log2
 
-template <int DP>
-__device__ __forceinline__ int k16_piece(int r, int c) { return DP == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15); }
-template <int DP>
-__device__ __forceinline__ int v16_piece(int r, int c) { return DP == 64 ? c ^ (2 * ((r >> 1) & 3)) : c ^ (2 * (r & 7)); }
-
-// One item and KV head to a workgroup of 8 waves: wave w owns units 16 RB w .. + 16 RB - 1, (row,
-// head) pairs with the group's heads fastest. 64-key tiles of K and V go from HBM through registers,
-// where the workgroup widens their codes to fp16 once for all waves, into two LDS buffers in turn:
-// a tile's loads are in flight for a whole tile, and one barrier a tile suffices.
+// One item and KV head to a workgroup: wave w owns units 16 RB w .. + 16 RB - 1, (row, head) pairs
+// with the group's heads fastest. 64-key tiles of K and V go from HBM through registers, where the
+// workgroup widens their codes to fp16 once for all waves, into two LDS buffers in turn: a tile's
+// loads are in flight for a whole tile, and one barrier a tile suffices.
+// Up to 128 dims a workgroup is 4 waves, and the two on a CU are out of step: one's products run
+// under the other's softmax. 8 waves with 256 units halve the staging but wait in step: 1 % faster
+// on a long prompt, 14 % slower on a tick of chunks, whose blocks and splits are then twice as large.
 // The weights go into P V as one fp16 (11 bits, an eighth of a bf16 output's rounding), or with
 // fp16 outputs as two.
 template <typename T, typename C, int DP>
-__global__ __launch_bounds__(kChunkThreads, 2) void kv8_chunk_kernel(RunArgs a, int n_wg) {
+__global__ __launch_bounds__(chunk_threads(DP), 2) void kv8_chunk_kernel(RunArgs a, int n_wg) {
   typedef hx::f16x8_t v8;
   typedef hx::Elem<_Float16> E;
   constexpr bool kTwo = __is_same(T, _Float16);
   constexpr int RB = DP == 256 ? 1 : 2, kSteps = DP / 32, kDims = DP / 16, kPieces = DP / 16;
-  constexpr int kRow = 2 * DP, kTileBytes = kChunkTile * kRow, kMine = DP / 64;  // pieces a thread moves
-  __shared__ __attribute__((aligned(16))) uint8_t s_k[2][kTileBytes];
-  __shared__ __attribute__((aligned(16))) uint8_t s_v[2][kTileBytes];
+  constexpr int kThreads = chunk_threads(DP), kWaves = kThreads / 64;
+  constexpr int kAhead = 2;  // operands of V read before the softmax, and ahead of their products
+  constexpr int kMine = 8 * DP / kThreads;  // 16-byte pieces of codes that a thread moves
+  // Rows of fp16 with 16 and 32 bytes more: 16 keys' fragments, and the 8 rows of 32 bytes that half a
+  // wave reads transposed, then cover all banks once.
+  constexpr int kKRow = 2 * DP + 16, kVRow = 2 * DP + 32;
+  __shared__ __attribute__((aligned(16))) uint8_t s_k[2][kChunkTile * kKRow];
+  __shared__ __attribute__((aligned(16))) uint8_t s_v[2][kChunkTile * kVRow];
   __shared__ __attribute__((aligned(16))) float s_ks[2][kChunkTile], s_lv[2][kChunkTile], s_iv[2][kChunkTile];
+  __shared__ uint32_t s_top[kWaves];
   const int tid = hx::tid_x(), lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   int4 counts;
@@ -839,8 +853,12 @@ __global__ __launch_bounds__(kChunkThreads, 2) void kv8_chunk_kernel(RunArgs a, 
           top = largest<T>(raw[rb][s], top);
         }
       }
-      // One power of two for the wave's units.
+      // One power of two for all units.
       for (int m = 1; m < 64; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m));
+      if (lane == 0) s_top[w] = top;
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < kWaves; ++e) top = max(top, s_top[e]);
       top = magnitude<T>((uint32_t)__builtin_amdgcn_readfirstlane((int)top));
       const float up = fit_up(top);
 #pragma unroll
@@ -901,9 +919,9 @@ __global__ __launch_bounds__(kChunkThreads, 2) void kv8_chunk_kernel(RunArgs a, 
       const __amdgpu_buffer_rsrc_t kr = hx::buffer_rsrc(a.k + base, bytes), vr = hx::buffer_rsrc(a.v + base, bytes);
 #pragma unroll
       for (int e = 0; e < kMine; ++e) {
-        // The first half of the pieces are K's (DP = 64: of the threads).
-        const bool of_v = DP == 64 ? w >= 4 : 2 * e >= kMine;
-        const int p = DP == 64 ? tid & 255 : tid + (2 * e >= kMine ? e - kMine / 2 : e) * kChunkThreads;
+        // The first half of the pieces are K's.
+        const bool of_v = 2 * e >= kMine;
+        const int p = tid + (of_v ? e - kMine / 2 : e) * kThreads;
         const int r = p / kPieces, c = p % kPieces;
         reg[e] = hx::ld16_buf(of_v ? vr : kr, 16 * c < D ? (uint32_t)r * row_bytes + 16u * c : 0x7ffffff0u);
       }
@@ -913,22 +931,21 @@ __global__ __launch_bounds__(kChunkThreads, 2) void kv8_chunk_kernel(RunArgs a, 
     auto store = [&](int b, int cnt) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < kMine; ++e) {
-        const bool of_v = DP == 64 ? w >= 4 : 2 * e >= kMine;
-        const int p = DP == 64 ? tid & 255 : tid + (2 * e >= kMine ? e - kMine / 2 : e) * kChunkThreads;
+        const bool of_v = 2 * e >= kMine;
+        const int p = tid + (of_v ? e - kMine / 2 : e) * kThreads;
         const int r = p / kPieces, c = p % kPieces;
         const uint2 x0 = hx8::to_f16<C>(reg[e].x), x1 = hx8::to_f16<C>(reg[e].y), x2 = hx8::to_f16<C>(reg[e].z),
                     x3 = hx8::to_f16<C>(reg[e].w);
-        uint8_t* const to = (of_v ? s_v[b] : s_k[b]) + r * kRow;
-        const int c0 = of_v ? v16_piece<DP>(r, 2 * c) : k16_piece<DP>(r, 2 * c);
-        const int c1 = of_v ? v16_piece<DP>(r, 2 * c + 1) : k16_piece<DP>(r, 2 * c + 1);
-        *reinterpret_cast<uint4*>(to + 16 * c0) = make_uint4(x0.x, x0.y, x1.x, x1.y);
-        *reinterpret_cast<uint4*>(to + 16 * c1) = make_uint4(x2.x, x2.y, x3.x, x3.y);
+        uint8_t* const to = (of_v ? s_v[b] + r * kVRow : s_k[b] + r * kKRow) + 32 * c;
+        *reinterpret_cast<uint4*>(to) = make_uint4(x0.x, x0.y, x1.x, x1.y);
+        *reinterpret_cast<uint4*>(to + 16) = make_uint4(x2.x, x2.y, x3.x, x3.y);
       }
       if (w == 0) {
-        s_ks[b][lane] = lane < cnt ? sreg : 0.f;
+        s_ks[b][lane] = lane < cnt ? sreg * qc : 0.f;
       } else if (w == 1) {
-        s_lv[b][lane] = lane < cnt ? __builtin_amdgcn_logf(sreg) : 0.f;
-        s_iv[b][lane] = lane < cnt ? __builtin_amdgcn_rcpf(sreg) : 0.f;
+        const ValueScale v = value_scale(lane < cnt ? sreg : 1.f);
+        s_lv[b][lane] = v.log;
+        s_iv[b][lane] = v.inverse;
       }
     };
 
@@ -961,6 +978,8 @@ __global__ __launch_bounds__(kChunkThreads, 2) void kv8_chunk_kernel(RunArgs a, 
       }
       if (key0 > any_hi || key0 + kChunkTile - 1 < any_lo) continue;
 
+      const uint8_t* const kp = s_k[b] + lr * kKRow + 16 * lg;
+      const uint8_t* const vp = s_v[b] + (4 * lg + (lr >> 2)) * kVRow + 16 * ((lr >> 1) & 1) + 8 * (lr & 1);
       hx::f32x4_t sc[4][RB];
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
@@ -970,19 +989,25 @@ __global__ __launch_bounds__(kChunkThreads, 2) void kv8_chunk_kernel(RunArgs a, 
       for (int s = 0; s < kSteps; ++s)
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
-          const int r = 16 * kb + lr;
-          const v8 kf = hx::as_v8<_Float16>(*reinterpret_cast<const uint4*>(s_k[b] + r * kRow + 16 * k16_piece<DP>(r, 4 * s + lg)));
+          const v8 kf = hx::as_v8<_Float16>(*reinterpret_cast<const uint4*>(kp + 16 * kb * kKRow + 64 * s));
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) sc[kb][rb] = E::mfma16x16x32(kf, qf[rb][s], sc[kb][rb]);
         }
+      // V^T operands, read transposed: keys 32 ks + 4 lg + 0..3 and 16 further of dim 16 d + lr.
+      auto read_v = [&](int ks, int d) __attribute__((always_inline)) {
+        const uint2 lo = hx::ld8_lds_tr16(vp + 32 * ks * kVRow + 32 * d);
+        const uint2 hi = hx::ld8_lds_tr16(vp + (32 * ks + 16) * kVRow + 32 * d);
+        return hx::as_v8<_Float16>(make_uint4(lo.x, lo.y, hi.x, hi.y));
+      };
+      v8 vf[kAhead];
+#pragma unroll
+      for (int d = 0; d < kAhead; ++d) vf[d] = read_v(0, d);
       // Lane: keys 16 kb + 4 lg + e of its units.
-      float4 iv[4];
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) {
         const float4 ks = *reinterpret_cast<const float4*>(&s_ks[b][16 * kb + 4 * lg]);
         const float4 lv = *reinterpret_cast<const float4*>(&s_lv[b][16 * kb + 4 * lg]);
-        iv[kb] = *reinterpret_cast<const float4*>(&s_iv[b][16 * kb + 4 * lg]);
-        const float k4[4] = {ks.x * qc, ks.y * qc, ks.z * qc, ks.w * qc}, l4[4] = {lv.x, lv.y, lv.z, lv.w};
+        const float k4[4] = {ks.x, ks.y, ks.z, ks.w}, l4[4] = {lv.x, lv.y, lv.z, lv.w};
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
@@ -1031,13 +1056,13 @@ __global__ __launch_bounds__(kChunkThreads, 2) void kv8_chunk_kernel(RunArgs a, 
         float sum = 0.f;
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
-          const float i4[4] = {iv[kb].x, iv[kb].y, iv[kb].z, iv[kb].w};
+          const float4 iv = *reinterpret_cast<const float4*>(&s_iv[b][16 * kb + 4 * lg]);
+          const float i4[4] = {iv.x, iv.y, iv.z, iv.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             sc[kb][rb][e] = hx::fast_exp2(sc[kb][rb][e] + neg);
             // A key that is hidden has the weight 0 under any scale, a NaN too.
-            if (whole) sum = fmaf(sc[kb][rb][e], i4[e], sum);
-            else sum += sc[kb][rb][e] == 0.f ? 0.f : sc[kb][rb][e] * i4[e];
+            sum = fmaf(sc[kb][rb][e], i4[e], sum);
           }
         }
         l_run[rb] += sum;
@@ -1055,23 +1080,20 @@ __global__ __launch_bounds__(kChunkThreads, 2) void kv8_chunk_kernel(RunArgs a, 
                            hx::pack2_round<_Float16>(y[2] - E::lo(p[3]), y[3] - E::hi(p[3]))));
         }
       }
-      // O^T += V^T P^T, V^T read transposed: keys 32 ks + 4 lg + 0..3 and 16 further of dim 16 d + lr.
+      // O^T += V^T P^T
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const int r0 = 32 * ks + 4 * lg + (lr >> 2), r1 = r0 + 16;
+      for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
         for (int d = 0; d < kDims; ++d) {
-          const int c = 2 * d + ((lr >> 1) & 1);
-          const uint2 lo = hx::ld8_lds_tr16(s_v[b] + r0 * kRow + 16 * v16_piece<DP>(r0, c) + 8 * (lr & 1));
-          const uint2 hi = hx::ld8_lds_tr16(s_v[b] + r1 * kRow + 16 * v16_piece<DP>(r1, c) + 8 * (lr & 1));
-          const v8 vv = hx::as_v8<_Float16>(make_uint4(lo.x, lo.y, hi.x, hi.y));
+          const int i = ks * kDims + d, next = i + kAhead;
+          const v8 vv = vf[i % kAhead];
+          if (next < 2 * kDims) vf[i % kAhead] = read_v(next / kDims, next % kDims);
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) {
             o[d][rb] = E::mfma16x16x32(vv, pf[ks][rb], o[d][rb]);
             if constexpr (kTwo) o[d][rb] = E::mfma16x16x32(vv, pf2[ks][rb], o[d][rb]);
           }
         }
-      }
     }
     if (bad && tid == 0) atomicOr(&a.hdr[H_ERR], HX_WERR_BAD_PAGE);
 
@@ -1193,7 +1215,7 @@ void launch_run(const Run& r, bool few, bool chunk) {
   if (chunk) {
     const int64_t most = r.l.most_chunk * a.s.hkv;
     const int n = (int)(most < 8192 ? most : 8192);
-    hipLaunchKernelGGL((kv8_chunk_kernel<T, C, DP>), dim3(n), dim3(kChunkThreads), 0, r.s, a, n);
+    hipLaunchKernelGGL((kv8_chunk_kernel<T, C, DP>), dim3(n), dim3(chunk_threads(DP)), 0, r.s, a, n);
   }
 }
 
