@@ -15,10 +15,19 @@
 // from fp64 (the argument of exp loses 2^-24 of itself in fp32, more than a token's share of a flat
 // row over 10^5 tokens).
 //
-// Three launches: the rows' largest and smallest logits (many workgroups a row), the histogram of
-// counts and weights over 2048 bins of equal width between them (many workgroups a row), and a
-// workgroup a row that finds the bins where the limits and the drawn position fall, gathers their
-// tokens and orders those. Bound by reading the logits three times, of which HBM sees the first.
+// Three launches:
+//   range  (many workgroups a row) the row's largest and smallest logit, and the largest of each
+//          group of 32 tokens
+//   limits (many workgroups a row) rows of a small top_k: the k-th largest of the groups' maxima is a
+//          bound that the k first tokens reach and few others do; the groups that reach it are read
+//          again and their tokens listed, and the row's last workgroup orders them and draws. Other
+//          rows: counts and weights over 2048 bins of equal width between the extremes.
+//   row    (a workgroup a row) of those finds the bins where the limits and the drawn position fall,
+//          gathers their tokens and orders those.
+// Bound by reading the logits from HBM, once; what is read again is in the last-level cache.
+// 96 rows of 151936 fp32 logits, top_k about 1000: 54 us (range 12, limits 34, row 4; the bins alone
+// 115), one bf16 row of them, top_k about 50: 19.5 us (31). Rows without a top_k: 75 to 110 us, of
+// which the fp64 weights of all tokens are 34 and a workgroup a row's pass over its logits 15 to 40.
 
 #include "hx_common.h"
 
@@ -26,8 +35,13 @@ namespace {
 
 constexpr int kBins = 2048;
 constexpr int kList = 2048;      // tokens that the last launch orders at once
-constexpr int kThreads = 256;    // of the first two launches
+constexpr int kThreads = 256;    // of the three launches
+constexpr int kLimitThreads = 512;
 constexpr int kRowThreads = 1024;
+constexpr int kGroup = 32;       // tokens of a group
+// A small top_k: of k tokens drawn at random over g groups the bound lets through about
+// -g ln(1 - k / g) tokens, 1.22 k at k = g / 3; kList must hold them.
+constexpr int kMostPicked = 1536;
 constexpr int kFixed = 44;       // fraction bits of a weight
 constexpr int kMostVocab = 1 << 18;
 constexpr int kMostChunks = 64;
@@ -46,7 +60,10 @@ struct SampleArgs {
   uint64_t* best;   // [rows][chunks]: the first token in order
   uint32_t* least;  // [rows][chunks]: the smallest finite logit's order
   uint32_t* count;  // [rows][kBins]
-  uint64_t* mass;   // [rows][kBins]
+  uint64_t* mass;   // [rows][kBins]; or [rows][kList], the listed tokens of a row of a small top_k
+  uint32_t* most;   // [rows][groups]: the order of a group's largest logit
+  uint32_t* listed; // [rows][2]: tokens that a row of a small top_k lists, and workgroups that have
+  int32_t groups;
   int32_t chunks, chunk;    // of the first launch, and their tokens
   int32_t chunks2, chunk2;  // of the second
 };
@@ -63,22 +80,33 @@ struct Logit<float> {
   static constexpr int kVec = 4;
 };
 
-// Calls f(logit, index) for tokens [begin, end) of a row, spread over a workgroup's threads, 16
-// bytes at a time (at any alignment: the hardware's loads take it).
+// 16 bytes of logits, at any alignment: the hardware's loads take it.
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Piece {
+  uint32_t w[4];
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+    else return Logit<T>::get(w[e / 2], e & 1);
+  }
+};
+
+// Calls f(logit, index) for tokens [begin, end) of a row, spread over a workgroup's threads.
 template <typename T, int THREADS, typename F>
 __device__ __forceinline__ void each_logit(const void* row, int begin, int end, F f) {
-  struct __attribute__((packed, aligned(sizeof(T)))) Piece {
-    uint32_t w[4];
-  };
-  constexpr int kVec = Logit<T>::kVec;
+  constexpr int kVec = Logit<T>::kVec, kAhead = 4;
   const T* const p = static_cast<const T*>(row);
   const int whole = (end - begin) / kVec;
-  for (int j = hx::tid_x(); j < whole; j += THREADS) {
-    const Piece u = *reinterpret_cast<const Piece*>(p + begin + j * kVec);
+  for (int j0 = hx::tid_x(); j0 < whole; j0 += kAhead * THREADS) {
+    Piece<T> u[kAhead];  // in flight together
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      if constexpr (sizeof(T) == 4) f(__uint_as_float(u.w[e]), begin + j * kVec + e);
-      else f(Logit<T>::get(u.w[e / 2], e & 1), begin + j * kVec + e);
+    for (int i = 0; i < kAhead; ++i)
+      u[i] = *reinterpret_cast<const Piece<T>*>(p + begin + min(j0 + i * THREADS, whole - 1) * kVec);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int j = j0 + i * THREADS;
+      if (j >= whole) break;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) f(u[i].get(e), begin + j * kVec + e);
     }
   }
   const int v = begin + whole * kVec + hx::tid_x();
@@ -103,6 +131,22 @@ __device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t x, int m) {
   return (uint64_t)(uint32_t)__shfl_xor((int)(uint32_t)x, m) | (uint64_t)(uint32_t)__shfl_xor((int)(x >> 32), m) << 32;
 }
 
+// Whether a row goes by its groups' maxima.
+__device__ __forceinline__ bool small_top_k(const SampleArgs& a, int64_t row) {
+  const int k = a.top_k != nullptr ? a.top_k[row] : 0;
+  return k > 0 && k <= kMostPicked && 3 * k <= a.groups;
+}
+
+// Largest of 2^n neighbouring lanes.
+template <int LANES>
+__device__ __forceinline__ uint32_t max_of_lanes(uint32_t x) {
+  static_assert(LANES == 4 || LANES == 8);
+  x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true));  // lane ^ 1
+  x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true));  // lane ^ 2
+  if constexpr (LANES == 8) x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xf, 0xf, true));  // 7 - lane
+  return x;
+}
+
 // ---------------------------------------------------------------------------- extremes
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_range_kernel(SampleArgs a) {
@@ -110,19 +154,48 @@ __global__ __launch_bounds__(kThreads) void sample_range_kernel(SampleArgs a) {
   __shared__ uint32_t s_least[kThreads / 64];
   const int64_t row = hx::wg_x() / a.chunks;
   const int c = hx::wg_x() % a.chunks, tid = hx::tid_x();
-  for (int b = c * kThreads + tid; b < kBins; b += a.chunks * kThreads) {
-    a.count[row * kBins + b] = 0;
-    a.mass[row * kBins + b] = 0;
+  if (!small_top_k(a, row)) {
+    for (int b = c * kThreads + tid; b < kBins; b += a.chunks * kThreads) {
+      a.count[row * kBins + b] = 0;
+      a.mass[row * kBins + b] = 0;
+    }
+  } else if (c == 0 && tid < 2) {
+    a.listed[2 * row + tid] = 0;
   }
+  constexpr int kVec = Logit<T>::kVec, kLanes = kGroup / kVec, kAhead = 4;
   uint32_t top = 0, at = 0xffffffffu, low = 0xffffffffu;
   const int begin = min(a.vocab, c * a.chunk), end = min(a.vocab, begin + a.chunk);
-  each_logit<T, kThreads>(static_cast<const T*>(a.logits) + row * a.row_stride, begin, end, [&](float l, int v) {
-    const uint32_t o = order_of(l);
-    // Tokens come in rising order to a thread: the first of equal ones stays.
-    at = o > top ? (uint32_t)v : at;
-    top = o > top ? o : top;
-    low = o > kOrderNegInf && o < low ? o : low;
-  });
+  const T* const p = static_cast<const T*>(a.logits) + row * a.row_stride;
+  // Chunks begin with a group, and every thread of a group takes each turn.
+  for (int v0 = begin; v0 < end; v0 += kAhead * kThreads * kVec) {
+    Piece<T> u[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int v = v0 + (i * kThreads + tid) * kVec;
+      if (v + kVec <= end) u[i] = *reinterpret_cast<const Piece<T>*>(p + v);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int v = v0 + (i * kThreads + tid) * kVec;
+      uint32_t here = 0;
+      auto take = [&](float l, int v) __attribute__((always_inline)) {
+        const uint32_t o = order_of(l);
+        // Tokens come in rising order to a thread: the first of equal ones stays.
+        at = o > top ? (uint32_t)v : at;
+        top = o > top ? o : top;
+        low = o > kOrderNegInf && o < low ? o : low;
+        here = max(here, o);
+      };
+      if (v + kVec <= end) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) take(u[i].get(e), v + e);
+      } else {
+        for (int e = v; e < end; ++e) take((float)p[e], e);
+      }
+      here = max_of_lanes<kLanes>(here);
+      if (tid % kLanes == 0 && v < end) a.most[row * a.groups + v / kGroup] = here;
+    }
+  }
   uint64_t best = (uint64_t)top << 32 | (uint32_t)~at;
   for (int m = 1; m < 64; m <<= 1) {
     best = max_u64(best, shfl_xor_u64(best, m));
@@ -148,6 +221,7 @@ struct Row {
   uint64_t best;    // the first token in order
   float top;        // its logit
   bool drawn;       // a temperature, and a finite largest logit
+  bool cut;         // the last bin's weights are all 0
   float per_bin;    // bins per unit of logit
   double scale;     // log2(e) / t
 };
@@ -167,23 +241,26 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t row) {
   r.best = best;
   r.top = logit_of(order);
   r.drawn = order > kOrderNegInf && order < kOrderInf && t > 0.f;
+  r.cut = false;
   r.per_bin = 0.f;
   r.scale = 0.;
   if (r.drawn) {
     t = fminf(fmaxf(t, 1e-30f), 1e30f);  // past these every weight is 0 or 1 already
     // Weights below 2^-46 are 0: what lies lower is one bin.
-    const float range = fminf(r.top - logit_of(low), 32.f * t);
+    const float all = r.top - logit_of(low), range = fminf(all, 32.f * t);
+    r.cut = all > range;
     r.per_bin = range > 0.f ? fminf((float)(kBins - 1) / range, 3e38f) : 0.f;
     r.scale = 1.4426950408889634074 / (double)t;
   }
   return r;
 }
 
-// Rises as the logit falls.
+// Rises as the logit falls; kBins for -inf and where all weights are 0, whose tokens no limit and no
+// drawn position needs.
 __device__ __forceinline__ int bin_of(const Row& r, float l) {
-  const float d = r.top - l;
-  const float x = d > 3e38f ? (float)kBins : d * r.per_bin;  // (-inf where all finite logits are equal: not inf * 0)
-  return x < (float)(kBins - 1) ? (int)x : kBins - 1;
+  if (hx::raw_bits(l) == 0xff800000u) return kBins;
+  const float x = (r.top - l) * r.per_bin;
+  return x < (float)(kBins - 1) ? (int)x : r.cut ? kBins : kBins - 1;
 }
 
 // log2 of a weight, and the weight 2^y, y <= 0, to about 1e-13 of itself.
@@ -213,60 +290,33 @@ __device__ __forceinline__ uint64_t fixed_of(double e) {
   return __builtin_bit_cast(uint64_t, x) & 0xfffffffffffffull;
 }
 
-// --------------------------------------------------------------------------- histogram
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a) {
-  __shared__ uint32_t s_count[kBins];
-  __shared__ unsigned long long s_mass[kBins];
-  const int64_t row = hx::wg_x() / a.chunks2;
-  const int c = hx::wg_x() % a.chunks2, tid = hx::tid_x();
-  const Row r = row_of(a, row);
-  if (!r.drawn) return;
-  for (int b = tid; b < kBins; b += kThreads) {
-    s_count[b] = 0;
-    s_mass[b] = 0;
-  }
-  __syncthreads();
-  const int begin = min(a.vocab, c * a.chunk2), end = min(a.vocab, begin + a.chunk2);
-  each_logit<T, kThreads>(static_cast<const T*>(a.logits) + row * a.row_stride, begin, end, [&](float l, int) {
-    const int b = bin_of(r, l);
-    atomicAdd(&s_count[b], 1u);
-    atomicAdd(&s_mass[b], (unsigned long long)fixed_of(weight_of(log_weight(r, l))));
-  });
-  __syncthreads();
-  for (int b = tid; b < kBins; b += kThreads) {
-    if (!s_count[b]) continue;
-    atomicAdd(&a.count[row * kBins + b], s_count[b]);
-    if (s_mass[b]) atomicAdd(reinterpret_cast<unsigned long long*>(&a.mass[row * kBins + b]), s_mass[b]);
-  }
-}
-
-// ---------------------------------------------------------------------------- the row
-struct RowLds {
-  uint32_t count[kBins];  // tokens up to and with a bin
-  uint64_t mass[kBins];   // their weight
-  uint64_t list[kList];   // gathered tokens: order falling in the high half, index in the low
+// ------------------------------------------------------------------------ listed tokens
+template <int THREADS>
+struct List {
+  uint32_t bins[kBins];
+  uint64_t list[kList];    // gathered tokens: order falling in the high half, index in the low
   uint64_t sorted[kList];
-  uint64_t cum[kList];    // weight up to and with a token of the sorted list
-  uint32_t digit_count[256];
-  unsigned long long digit_mass[256];
-  uint64_t waves[kRowThreads / 64];
-  uint32_t listed;
+  uint64_t waves[THREADS / 64];
+  uint32_t listed, crowd;
+  // Weight up to and with a token of the sorted list: in the list's place once that is sorted.
+  __device__ __forceinline__ uint64_t* cum() { return list; }
 };
 
-__device__ uint64_t block_sum(RowLds& s, uint64_t x) {
+template <int THREADS>
+__device__ uint64_t block_sum(List<THREADS>& s, uint64_t x) {
   for (int m = 1; m < 64; m <<= 1) x += shfl_xor_u64(x, m);
   __syncthreads();
   if ((hx::tid_x() & 63) == 0) s.waves[hx::tid_x() >> 6] = x;
   __syncthreads();
   uint64_t all = 0;
 #pragma unroll
-  for (int w = 0; w < kRowThreads / 64; ++w) all += s.waves[w];
+  for (int w = 0; w < THREADS / 64; ++w) all += s.waves[w];
   return all;
 }
 
 // Sum over the threads before this one.
-__device__ uint64_t block_before(RowLds& s, uint64_t x) {
+template <int THREADS>
+__device__ uint64_t block_before(List<THREADS>& s, uint64_t x) {
   const int lane = hx::tid_x() & 63;
   uint64_t sum = x;
   for (int m = 1; m < 64; m <<= 1) {
@@ -277,7 +327,8 @@ __device__ uint64_t block_before(RowLds& s, uint64_t x) {
   if (lane == 63) s.waves[hx::tid_x() >> 6] = sum;
   __syncthreads();
   uint64_t before = sum - x;
-  for (int w = 0; w < hx::tid_x() >> 6; ++w) before += s.waves[w];
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) before += w < hx::tid_x() >> 6 ? s.waves[w] : 0;
   return before;
 }
 
@@ -296,58 +347,346 @@ __device__ __forceinline__ int first_from(const P* p, int n, X x) {
 __device__ __forceinline__ uint64_t place_of(float l, int v) { return (uint64_t)(uint32_t)~order_of(l) << 32 | (uint32_t)v; }
 __device__ __forceinline__ float place_logit(uint64_t place) { return logit_of(~(uint32_t)(place >> 32)); }
 
-// Orders the n listed tokens and sums their weights onto `base`. By all threads.
-__device__ void order_list(RowLds& s, const Row& r, int n, uint64_t base) {
+// Orders the n listed tokens and sums their weights onto `base`. By all threads. The tokens are of
+// all bins, or of one bin alone.
+template <int THREADS>
+__device__ void order_list(List<THREADS>& s, const Row& r, int n, uint64_t base, int one = -1) {
+  constexpr int kEach = kList / THREADS, kBinsEach = kBins / THREADS;
   const int tid = hx::tid_x();
   __syncthreads();
-  if (n <= kRowThreads) {
-    // A token's place is the number of those before it.
-    if (tid < n) {
-      const uint64_t mine = s.list[tid];
-      int before = 0;
-      for (int i = 0; i < n; ++i) before += s.list[i] < mine ? 1 : 0;
-      s.sorted[before] = mine;
+  // Tokens to their bins' places (one bin's: parts of it), in any order; then a token's place is the
+  // number of its bin's tokens before it. Lists with a crowded bin are sorted instead.
+  for (int b = tid; b < kBins; b += THREADS) s.bins[b] = 0;
+  if (tid == 0) s.crowd = 0;
+  __syncthreads();
+  uint64_t mine[kEach];
+  int bin[kEach];
+  uint32_t turn[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = tid + e * THREADS;
+    if (i >= n) break;
+    mine[e] = s.list[i];
+    const float x = (r.top - place_logit(mine[e])) * r.per_bin;
+    bin[e] = (int)fminf(one < 0 ? x : (x - (float)one) * (float)kBins, (float)(kBins - 1));
+    turn[e] = atomicAdd(&s.bins[bin[e]], 1u);
+  }
+  __syncthreads();
+  uint32_t here[kBinsEach], sum = 0, most = 0;
+#pragma unroll
+  for (int e = 0; e < kBinsEach; ++e) {
+    here[e] = s.bins[kBinsEach * tid + e];
+    most = max(most, here[e]);
+    sum += here[e];
+  }
+  if (most > 256) s.crowd = 1;
+  uint32_t before = (uint32_t)block_before(s, (uint64_t)sum);
+#pragma unroll
+  for (int e = 0; e < kBinsEach; ++e) {
+    s.bins[kBinsEach * tid + e] = before;
+    before += here[e];
+  }
+  __syncthreads();
+  if (!s.crowd) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      if (tid + e * THREADS < n) s.list[s.bins[bin[e]] + turn[e]] = mine[e];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      if (tid + e * THREADS >= n) break;
+      const int from = (int)s.bins[bin[e]], to = bin[e] + 1 < kBins ? (int)s.bins[bin[e] + 1] : n;
+      int at = from;
+      for (int i = from; i < to; ++i) at += s.list[i] < mine[e] ? 1 : 0;
+      s.sorted[at] = mine[e];
     }
   } else {
-    int size = 2 * kRowThreads;
-    static_assert(kList == 2 * kRowThreads, "two of a list to a thread");
-    for (int i = tid; i < size; i += kRowThreads) s.sorted[i] = i < n ? s.list[i] : ~0ull;
+    int size = 2;
+    while (size < n) size <<= 1;
+    for (int i = tid; i < size; i += THREADS) s.sorted[i] = i < n ? s.list[i] : ~0ull;
     for (int k = 2; k <= size; k <<= 1)
       for (int j = k >> 1; j > 0; j >>= 1) {
         __syncthreads();
-        const int i = (tid / j) * 2 * j + tid % j;
-        const uint64_t x = s.sorted[i], y = s.sorted[i + j];
-        if ((x > y) == ((i & k) == 0)) {
-          s.sorted[i] = y;
-          s.sorted[i + j] = x;
+        for (int pair = tid; pair < size / 2; pair += THREADS) {
+          const int i = 2 * pair - (pair & (j - 1));
+          const uint64_t x = s.sorted[i], y = s.sorted[i + j];
+          if ((x > y) == ((i & k) == 0)) {
+            s.sorted[i] = y;
+            s.sorted[i + j] = x;
+          }
         }
       }
   }
   __syncthreads();
-  uint64_t w[2];
+  uint64_t w[kEach], all = 0;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int i = 2 * tid + e;
+  for (int e = 0; e < kEach; ++e) {
+    const int i = kEach * tid + e;
     w[e] = i < n ? fixed_of(weight_of(log_weight(r, place_logit(s.sorted[i])))) : 0;
+    all += w[e];
   }
-  const uint64_t before = base + block_before(s, w[0] + w[1]);
-  s.cum[2 * tid] = before + w[0];
-  s.cum[2 * tid + 1] = before + w[0] + w[1];
+  uint64_t up_to = base + block_before(s, all);
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    up_to += w[e];
+    s.cum()[kEach * tid + e] = up_to;
+  }
   __syncthreads();
 }
 
-// Lists the row's tokens that `take` says, at most kList. By all threads; their number.
+// ------------------------------------------------------------------------ a row's limits
+struct Limits {
+  bool limited, by_p, by_min;
+  uint32_t k;
+  double p, min_p, u;
+
+  // Weights are whole: the first cumulative one above u W is the first above its whole part, which
+  // rounding must not take to W. The weight to reach:
+  __device__ __forceinline__ uint64_t target(uint64_t w) const {
+    const uint64_t t = (uint64_t)(u * (double)w);
+    return (t < w ? t : w - 1) + 1;
+  }
+};
+
+__device__ __forceinline__ Limits limits_of(const SampleArgs& a, int64_t row) {
+  Limits m;
+  const int asked = a.top_k != nullptr ? a.top_k[row] : 0;
+  m.limited = asked > 0 && asked < a.vocab;
+  m.k = m.limited ? (uint32_t)asked : (uint32_t)a.vocab;
+  const float top_p = a.top_p != nullptr ? a.top_p[row] : 1.f;
+  m.by_p = top_p < 1.f;
+  m.p = top_p > 0.f ? (double)top_p : 0.;
+  m.min_p = a.min_p != nullptr ? (double)a.min_p[row] : 0.;
+  m.by_min = m.min_p > 0.;
+  const float given = a.uniforms[row];
+  m.u = given > 0.f ? fmin((double)given, 1.) : 0.;
+  return m;
+}
+
+// By one thread: the token, and its share of the kept weight.
+__device__ __forceinline__ void answer(const SampleArgs& a, const Row& r, int64_t row, uint64_t place, uint64_t kept) {
+  a.token_ids[row] = (int64_t)(uint32_t)place;
+  if (a.logprobs != nullptr)
+    a.logprobs[row] = (float)(log_weight(r, place_logit(place)) * 0.69314718055994530942 -
+                              log((double)kept * (1. / (double)(1ull << kFixed))));
+}
+
+// Draws from a list that holds the row's first tokens, all that the limits can keep. `total` is the
+// weight of the row where the limits need it (no top_k).
+template <int THREADS>
+__device__ void draw_from(const SampleArgs& a, List<THREADS>& s, const Row& r, int64_t row, const Limits& m, int listed,
+                          uint64_t total) {
+  order_list(s, r, listed, 0);
+  const uint64_t* const cum = s.cum();
+  uint32_t n = min(m.k, (uint32_t)listed);
+  if (m.by_p) {
+    const uint64_t of = m.limited ? cum[n - 1] : total;
+    n = min(n, (uint32_t)first_from(cum, listed, m.p * (double)of) + 1);
+  }
+  if (m.by_min) {
+    uint64_t mine = 0;
+    for (int i = hx::tid_x(); i < listed; i += THREADS) mine += weight_of(log_weight(r, place_logit(s.sorted[i]))) >= m.min_p ? 1 : 0;
+    n = min(n, (uint32_t)block_sum(s, mine));
+  }
+  n = max(n, 1u);
+  const uint64_t kept = !m.limited && !m.by_p && !m.by_min ? total : cum[n - 1];
+  const int at = first_from(cum, listed, m.target(kept));
+  if (hx::tid_x() == 0) answer(a, r, row, s.sorted[at], kept);
+}
+
+// ----------------------------------------------------------------- bounds and histograms
+struct Bins {
+  uint32_t count[kBins];
+  unsigned long long mass[kBins];
+};
+
+// Counts and weights of a workgroup's tokens over the row's bins.
+template <typename T, int THREADS>
+__device__ void fill_bins(Bins& s, const Row& r, const void* row, int begin, int end) {
+  for (int b = hx::tid_x(); b < kBins; b += THREADS) {
+    s.count[b] = 0;
+    s.mass[b] = 0;
+  }
+  __syncthreads();
+  each_logit<T, THREADS>(row, begin, end, [&](float l, int) {
+    const int b = bin_of(r, l);
+    if (b == kBins) return;
+    atomicAdd(&s.count[b], 1u);
+    const uint64_t w = fixed_of(weight_of(log_weight(r, l)));
+    if (w) atomicAdd(&s.mass[b], (unsigned long long)w);
+  });
+  __syncthreads();
+}
+
+// The last bin of the bound: k groups have their largest logit in it or before it.
+template <int THREADS>
+__device__ int bound_of(const SampleArgs& a, List<THREADS>& s, const Row& r, int64_t row, uint32_t k) {
+  constexpr int kEach = kBins / THREADS, kAhead = 8;
+  const int tid = hx::tid_x();
+  for (int b = tid; b < kBins; b += THREADS) s.bins[b] = 0;
+  if (tid == 0) s.crowd = kBins - 1;
+  __syncthreads();
+  for (int g0 = tid; g0 < a.groups; g0 += kAhead * THREADS) {
+    uint32_t most[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) most[i] = g0 + i * THREADS < a.groups ? a.most[row * a.groups + g0 + i * THREADS] : kOrderNegInf;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int b = bin_of(r, logit_of(most[i]));
+      if (b < kBins) atomicAdd(&s.bins[b], 1u);
+    }
+  }
+  __syncthreads();
+  uint32_t here[kEach], sum = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    here[e] = s.bins[kEach * tid + e];
+    sum += here[e];
+  }
+  uint32_t up_to = (uint32_t)block_before(s, (uint64_t)sum);
+  if (up_to < k && up_to + sum >= k) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const bool here_it = up_to < k && up_to + here[e] >= k;
+      up_to += here[e];
+      if (here_it) s.crowd = kEach * tid + e;
+    }
+  }
+  __syncthreads();
+  return (int)s.crowd;
+}
+
+// Lists a workgroup's tokens within the row's bound; the row's last workgroup draws.
+template <typename T, int THREADS>
+__device__ void pick(const SampleArgs& a, List<THREADS>& s, const Row& r, int64_t row, int begin, int end) {
+  constexpr int kVec = Logit<T>::kVec, kLanes = kGroup / kVec;
+  const int tid = hx::tid_x();
+  const Limits m = limits_of(a, row);
+  const int bound = bound_of(a, s, r, row, m.k);
+  static_assert(kMostVocab / kGroup * sizeof(uint16_t) <= sizeof(s.sorted));
+  uint16_t* const reach = reinterpret_cast<uint16_t*>(s.sorted);  // the workgroup's groups that reach the bound
+  __syncthreads();
+  if (tid == 0) s.listed = s.crowd = 0;
+  __syncthreads();
+  const int g_end = (end + kGroup - 1) / kGroup;
+  for (int g = begin / kGroup + tid; g < g_end; g += THREADS)
+    if (bin_of(r, logit_of(a.most[row * a.groups + g])) <= bound) reach[atomicAdd(&s.crowd, 1u)] = (uint16_t)g;
+  __syncthreads();
+  const int groups = (int)s.crowd;
+  const T* const p = static_cast<const T*>(a.logits) + row * a.row_stride;
+  constexpr int kAhead = 4;
+  for (int i0 = tid; i0 < groups * kLanes; i0 += kAhead * THREADS) {
+    Piece<T> u[kAhead];  // in flight together
+    int at[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int j = i0 + i * THREADS;
+      at[i] = j < groups * kLanes ? reach[j / kLanes] * kGroup + j % kLanes * kVec : end;
+      if (at[i] + kVec <= end) u[i] = *reinterpret_cast<const Piece<T>*>(p + at[i]);
+    }
+    auto take = [&](float l, int v) __attribute__((always_inline)) {
+      if (bin_of(r, l) > bound) return;
+      const uint32_t to = atomicAdd(&s.listed, 1u);
+      if (to < (uint32_t)kList) s.list[to] = place_of(l, v);
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (at[i] + kVec <= end) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) take(u[i].get(e), at[i] + e);
+      } else {
+        for (int e = at[i]; e < end; ++e) take((float)p[e], e);
+      }
+    }
+  }
+  __syncthreads();
+  const uint32_t mine = s.listed;
+  __syncthreads();
+  if (tid == 0) s.crowd = mine ? atomicAdd(&a.listed[2 * row], mine) : 0;
+  __syncthreads();
+  const uint32_t base = s.crowd;
+  static_assert(kList <= kBins);
+  uint64_t* const list = a.mass + row * kBins;
+  for (uint32_t i = tid; i < mine && base + i < (uint32_t)kList && i < (uint32_t)kList; i += THREADS) list[base + i] = s.list[i];
+  __syncthreads();
+  // What the workgroups wrote is seen by the one that counts itself last.
+  if (tid == 0) s.crowd = __hip_atomic_fetch_add(&a.listed[2 * row + 1], 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (s.crowd != (uint32_t)a.chunks2 - 1) return;
+  const uint32_t all = __hip_atomic_load(&a.listed[2 * row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (all > (uint32_t)kList) return;  // the next launch's
+  for (uint32_t i = tid; i < all; i += THREADS) s.list[i] = list[i];
+  draw_from(a, s, r, row, m, (int)all, 0);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kLimitThreads) void sample_limits_kernel(SampleArgs a) {
+  __shared__ union Lds {
+    Bins bins;
+    List<kLimitThreads> list;
+  } s;
+  const int64_t row = hx::wg_x() / a.chunks2;
+  const int c = hx::wg_x() % a.chunks2;
+  const Row r = row_of(a, row);
+  if (!r.drawn) return;
+  const int begin = min(a.vocab, c * a.chunk2), end = min(a.vocab, begin + a.chunk2);
+  if (small_top_k(a, row)) {
+    pick<T>(a, s.list, r, row, begin, end);
+    return;
+  }
+  fill_bins<T, kLimitThreads>(s.bins, r, static_cast<const T*>(a.logits) + row * a.row_stride, begin, end);
+  for (int b = hx::tid_x(); b < kBins; b += kLimitThreads) {
+    if (!s.bins.count[b]) continue;
+    atomicAdd(&a.count[row * kBins + b], s.bins.count[b]);
+    if (s.bins.mass[b]) atomicAdd(reinterpret_cast<unsigned long long*>(&a.mass[row * kBins + b]), s.bins.mass[b]);
+  }
+}
+
+// ---------------------------------------------------------------------------- the row
+struct RowLds : List<kRowThreads> {
+  Bins to;  // tokens up to and with a bin, and their weight
+  uint32_t digit_count[256];
+  unsigned long long digit_mass[256];
+};
+
+// Lists the row's tokens of the bins [first, last] that `take` says, at most kList. By all threads;
+// their number. One test of 16 bytes' tokens comes before the tokens' own: few are of the bins.
 template <typename T, typename F>
-__device__ int gather(const SampleArgs& a, RowLds& s, const void* row, F take) {
+__device__ int gather(const SampleArgs& a, RowLds& s, const Row& r, const void* row, int first, int last, F take) {
+  constexpr int kVec = Logit<T>::kVec, kAhead = 4;
   __syncthreads();
   if (hx::tid_x() == 0) s.listed = 0;
   __syncthreads();
-  each_logit<T, kRowThreads>(row, 0, a.vocab, [&](float l, int v) {
-    if (take(l, v)) {
-      const uint32_t at = atomicAdd(&s.listed, 1u);
-      if (at < (uint32_t)kList) s.list[at] = place_of(l, v);
+  // (An x that is infinite, or NaN from an infinite distance and bins of no width, is in no bin.)
+  const float from = (float)first, to = last < kBins - 1 ? (float)(last + 1) : r.cut ? (float)(kBins - 1) : 3.4e38f;
+  auto within = [&](float l) __attribute__((always_inline)) {
+    const float x = (r.top - l) * r.per_bin;
+    return x >= from && x < to;
+  };
+  auto list = [&](float l, int v) __attribute__((always_inline)) {
+    if (!within(l) || !take(place_of(l, v))) return;
+    const uint32_t at = atomicAdd(&s.listed, 1u);
+    if (at < (uint32_t)kList) s.list[at] = place_of(l, v);
+  };
+  const T* const p = static_cast<const T*>(row);
+  const int whole = a.vocab / kVec;
+  for (int j0 = hx::tid_x(); j0 < whole; j0 += kAhead * kRowThreads) {
+    Piece<T> u[kAhead];  // in flight together
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) u[i] = *reinterpret_cast<const Piece<T>*>(p + min(j0 + i * kRowThreads, whole - 1) * kVec);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int j = j0 + i * kRowThreads;
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) any |= within(u[i].get(e));
+      if (!any || j >= whole) continue;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) list(u[i].get(e), j * kVec + e);
     }
-  });
+  }
+  const int v = whole * kVec + hx::tid_x();
+  if (v < a.vocab) list((float)p[v], v);
   __syncthreads();
   return min((int)s.listed, kList);
 }
@@ -363,9 +702,9 @@ struct Found {
 template <typename T>
 __device__ Found resolve(const SampleArgs& a, RowLds& s, const Row& r, const void* row, int bin, bool by_count, uint64_t target) {
   const int tid = hx::tid_x();
-  uint32_t before = bin ? s.count[bin - 1] : 0;
-  uint64_t mass = bin ? s.mass[bin - 1] : 0;
-  uint32_t size = s.count[bin] - before;
+  uint32_t before = bin ? s.to.count[bin - 1] : 0;
+  uint64_t mass = bin ? s.to.mass[bin - 1] : 0;
+  uint32_t size = s.to.count[bin] - before;
   int shift = 64;
   uint64_t prefix = 0;
   while (size > (uint32_t)kList && shift > 0) {
@@ -409,10 +748,8 @@ __device__ Found resolve(const SampleArgs& a, RowLds& s, const Row& r, const voi
     size = count_here;
     prefix = from < 64 ? prefix << 8 | (uint64_t)at : (uint64_t)at;
   }
-  const int n = gather<T>(a, s, row, [&](float l, int v) {
-    return bin_of(r, l) == bin && (shift == 64 || (place_of(l, v) >> shift) == prefix);
-  });
-  order_list(s, r, n, mass);
+  const int n = gather<T>(a, s, r, row, bin, bin, [&](uint64_t place) { return shift == 64 || place >> shift == prefix; });
+  order_list(s, r, n, mass, bin);
   return {n, before};
 }
 
@@ -431,114 +768,87 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
     }
     return;
   }
+  const bool picked = small_top_k(a, row);
+  if (picked && a.listed[2 * row] <= (uint32_t)kList) return;  // drawn already
   const void* const logits = static_cast<const T*>(a.logits) + row * a.row_stride;
+  if (picked) {
+    fill_bins<T, kRowThreads>(s.to, r, logits, 0, a.vocab);
+  } else {
+    for (int b = tid; b < kBins; b += kRowThreads) {
+      s.to.count[b] = a.count[row * kBins + b];
+      s.to.mass[b] = a.mass[row * kBins + b];
+    }
+    __syncthreads();
+  }
   {
     // Prefix sums over the bins, two a thread.
-    const uint32_t c0 = a.count[row * kBins + 2 * tid], c1 = a.count[row * kBins + 2 * tid + 1];
-    const uint64_t m0 = a.mass[row * kBins + 2 * tid], m1 = a.mass[row * kBins + 2 * tid + 1];
+    static_assert(kBins == 2 * kRowThreads);
+    const uint32_t c0 = s.to.count[2 * tid], c1 = s.to.count[2 * tid + 1];
+    const uint64_t m0 = s.to.mass[2 * tid], m1 = s.to.mass[2 * tid + 1];
     const uint32_t c = (uint32_t)block_before(s, (uint64_t)c0 + c1);
     const uint64_t m = block_before(s, m0 + m1);
-    s.count[2 * tid] = c + c0;
-    s.count[2 * tid + 1] = c + c0 + c1;
-    s.mass[2 * tid] = m + m0;
-    s.mass[2 * tid + 1] = m + m0 + m1;
+    s.to.count[2 * tid] = c + c0;
+    s.to.count[2 * tid + 1] = c + c0 + c1;
+    s.to.mass[2 * tid] = m + m0;
+    s.to.mass[2 * tid + 1] = m + m0 + m1;
   }
   __syncthreads();
-  const int asked = a.top_k != nullptr ? a.top_k[row] : 0;
-  const bool limited = asked > 0 && asked < a.vocab;
-  const uint32_t nk = limited ? (uint32_t)asked : (uint32_t)a.vocab;
-  const float top_p = a.top_p != nullptr ? a.top_p[row] : 1.f;
-  const bool by_p = top_p < 1.f;
-  const double p = top_p > 0.f ? (double)top_p : 0.;
-  const double min_p = a.min_p != nullptr ? (double)a.min_p[row] : 0.;
-  const bool by_min = min_p > 0.;
-  const float given = a.uniforms[row];
-  const double u = given > 0.f ? fmin((double)given, 1.) : 0.;
-
-  const int bin_k = first_from(s.count, kBins, nk);
+  const Limits m = limits_of(a, row);
+  const uint32_t nk = min(m.k, s.to.count[kBins - 1]);
+  const int bin_k = first_from(s.to.count, kBins, nk);
   // No kept token lies in a bin past `last`.
   int last = bin_k;
-  if (by_p) last = min(last, first_from(s.mass, kBins, p * (double)s.mass[bin_k]));
-  if (by_min) {
+  if (m.by_p) last = min(last, first_from(s.to.mass, kBins, m.p * (double)s.to.mass[bin_k]));
+  if (m.by_min) {
     // How far below the largest logit the border lies, and two bins more for what is rounded.
-    const float x = -logf((float)min_p) * (float)(1.4426950408889634074 / r.scale) * r.per_bin * 1.00001f;
+    const float x = -logf((float)m.min_p) * (float)(1.4426950408889634074 / r.scale) * r.per_bin * 1.00001f;
     last = min(last, x < (float)(kBins - 3) ? max((int)x, 0) + 2 : kBins - 1);
   }
-  const int until = limited && by_p ? bin_k : last;  // the top_k tokens' weight needs all of them
-  uint32_t n;
-  uint64_t kept;
-  int at;
-  auto fewest = [&](uint32_t m, uint64_t w) __attribute__((always_inline)) {
-    if (m < n) {
-      n = m;
+  const int until = m.limited && m.by_p ? bin_k : last;  // the top_k tokens' weight needs all of them
+  if (s.to.count[until] <= (uint32_t)kList) {
+    const int listed = gather<T>(a, s, r, logits, 0, until, [](uint64_t) { return true; });
+    draw_from(a, s, r, row, m, listed, s.to.mass[kBins - 1]);
+    return;
+  }
+  uint32_t n = nk;
+  uint64_t kept = s.to.mass[kBins - 1], of = kept;
+  const uint64_t* const cum = s.cum();
+  auto fewest = [&](uint32_t fewer, uint64_t w) __attribute__((always_inline)) {
+    if (fewer < n) {
+      n = fewer;
       kept = w;
     }
   };
-  auto target_of = [&](uint64_t w) __attribute__((always_inline)) {
-    // Weights are whole: the first cumulative one above u W is the first above its whole part,
-    // which rounding must not take to W.
-    const uint64_t t = (uint64_t)(u * (double)w);
-    return t < w ? t : w - 1;
-  };
-  if (s.count[until] <= (uint32_t)kList) {
-    const int listed = gather<T>(a, s, logits, [&](float l, int) { return bin_of(r, l) <= until; });
-    order_list(s, r, listed, 0);
-    n = min(nk, (uint32_t)listed);
-    if (by_p) {
-      const uint64_t of = limited ? s.cum[n - 1] : s.mass[kBins - 1];
-      n = min(n, (uint32_t)first_from(s.cum, listed, p * (double)of) + 1);
-    }
-    if (by_min) {
-      uint64_t mine = 0;
-      for (int i = tid; i < listed; i += kRowThreads) mine += weight_of(log_weight(r, place_logit(s.sorted[i]))) >= min_p ? 1 : 0;
-      n = min(n, (uint32_t)block_sum(s, mine));
-    }
-    n = max(n, 1u);
-    kept = !limited && !by_p && !by_min ? s.mass[kBins - 1] : s.cum[n - 1];
-    at = first_from(s.cum, listed, target_of(kept) + 1);
-  } else {
-    n = (uint32_t)a.vocab;
-    kept = s.mass[kBins - 1];
-    uint64_t of = kept;
-    if (limited) {
-      const Found f = resolve<T>(a, s, r, logits, bin_k, true, nk);
-      of = s.cum[nk - f.before - 1];
-      fewest(nk, of);
-      __syncthreads();
-    }
-    if (by_p) {
-      const double border = p * (double)of;
-      const int bin = min(first_from(s.mass, kBins, border), kBins - 1);
-      const uint64_t whole = (uint64_t)border + ((double)(uint64_t)border < border ? 1 : 0);
-      const Found f = resolve<T>(a, s, r, logits, bin, false, whole);
-      const int i = min(first_from(s.cum, f.n, border), f.n - 1);
-      fewest(f.before + (uint32_t)i + 1, s.cum[i]);
-      __syncthreads();
-    }
-    if (by_min) {
-      uint64_t count = 0, mass = 0;
-      each_logit<T, kRowThreads>(logits, 0, a.vocab, [&](float l, int) {
-        const double e = weight_of(log_weight(r, l));
-        if (e >= min_p) {
-          ++count;
-          mass += fixed_of(e);
-        }
-      });
-      count = block_sum(s, count);
-      mass = block_sum(s, mass);
-      fewest(max((uint32_t)count, 1u), mass);
-    }
-    const uint64_t target = target_of(kept) + 1;
-    const Found f = resolve<T>(a, s, r, logits, first_from(s.mass, kBins, target), false, target);
-    at = first_from(s.cum, f.n, target);
+  if (m.limited) {
+    const Found f = resolve<T>(a, s, r, logits, bin_k, true, nk);
+    kept = of = cum[nk - f.before - 1];
+    __syncthreads();
   }
-  if (tid == 0) {
-    const uint64_t place = s.sorted[at];
-    a.token_ids[row] = (int64_t)(uint32_t)place;
-    if (a.logprobs != nullptr)
-      a.logprobs[row] = (float)(log_weight(r, place_logit(place)) * 0.69314718055994530942 -
-                                log((double)kept * (1. / (double)(1ull << kFixed))));
+  if (m.by_p) {
+    const double border = m.p * (double)of;
+    const int bin = min(first_from(s.to.mass, kBins, border), kBins - 1);
+    const uint64_t whole = (uint64_t)border + ((double)(uint64_t)border < border ? 1 : 0);
+    const Found f = resolve<T>(a, s, r, logits, bin, false, whole);
+    const int i = min(first_from(cum, f.n, border), f.n - 1);
+    fewest(f.before + (uint32_t)i + 1, cum[i]);
+    __syncthreads();
   }
+  if (m.by_min) {
+    uint64_t count = 0, mass = 0;
+    each_logit<T, kRowThreads>(logits, 0, a.vocab, [&](float l, int) {
+      const double e = weight_of(log_weight(r, l));
+      if (e >= m.min_p) {
+        ++count;
+        mass += fixed_of(e);
+      }
+    });
+    count = block_sum(s, count);
+    mass = block_sum(s, mass);
+    fewest(max((uint32_t)count, 1u), mass);
+  }
+  const uint64_t target = m.target(kept);
+  const Found f = resolve<T>(a, s, r, logits, first_from(s.to.mass, kBins, target), false, target);
+  if (tid == 0) answer(a, r, row, s.sorted[first_from(cum, f.n, target)], kept);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -555,7 +865,7 @@ void cut(int64_t rows, int32_t vocab, int64_t wgs, int32_t* chunks, int32_t* chu
 template <typename T>
 void launch(const SampleArgs& a, int64_t rows, hipStream_t s) {
   hipLaunchKernelGGL(sample_range_kernel<T>, dim3((unsigned)(rows * a.chunks)), dim3(kThreads), 0, s, a);
-  hipLaunchKernelGGL(sample_bins_kernel<T>, dim3((unsigned)(rows * a.chunks2)), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(sample_limits_kernel<T>, dim3((unsigned)(rows * a.chunks2)), dim3(kLimitThreads), 0, s, a);
   hipLaunchKernelGGL(sample_row_kernel<T>, dim3((unsigned)rows), dim3(kRowThreads), 0, s, a);
 }
 
@@ -563,7 +873,8 @@ void launch(const SampleArgs& a, int64_t rows, hipStream_t s) {
 
 extern "C" size_t hx_sample_workspace_bytes(int64_t rows, int64_t vocab) {
   if (rows < 1 || vocab < 1 || vocab > kMostVocab || rows > (1 << 20)) return 0;
-  return (size_t)rows * (kMostChunks * (sizeof(uint64_t) + sizeof(uint32_t)) + kBins * (sizeof(uint64_t) + sizeof(uint32_t)));
+  return (size_t)rows * ((kMostChunks + kBins) * (sizeof(uint64_t) + sizeof(uint32_t)) +
+                         (size_t)(ceil_div(vocab, kGroup) + 2) * sizeof(uint32_t));
 }
 
 extern "C" int hx_sample_tokens(const void* logits, int64_t logits_row_stride, int64_t rows, int64_t vocab, int32_t dtype,
@@ -593,8 +904,11 @@ extern "C" int hx_sample_tokens(const void* logits, int64_t logits_row_stride, i
   a.mass = a.best + rows * kMostChunks;
   a.least = reinterpret_cast<uint32_t*>(a.mass + rows * kBins);
   a.count = a.least + rows * kMostChunks;
+  a.listed = a.count + rows * kBins;
+  a.most = a.listed + rows * 2;
+  a.groups = (int32_t)ceil_div(vocab, kGroup);
   cut(rows, a.vocab, 2048, &a.chunks, &a.chunk);
-  cut(rows, a.vocab, 1024, &a.chunks2, &a.chunk2);
+  cut(rows, a.vocab, 384, &a.chunks2, &a.chunk2);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == HX_DTYPE_BF16) launch<__bf16>(a, rows, s);
   else if (dtype == HX_DTYPE_FP16) launch<_Float16>(a, rows, s);

@@ -98,6 +98,54 @@ def test_ties(device, dtype):
         _check(device, logits, u, **limits)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [20011, 151936])
+def test_small_top_k(device, vocab, dtype):
+    """A small top_k where its first tokens lie together, are tied, or few are allowed at all: more
+    tokens at its bound than one list holds, and fewer than top_k."""
+    say("sample small top_k", vocab, dtype)
+    g = torch.Generator().manual_seed(vocab % 97)
+    rising = torch.arange(vocab) * (8.0 / vocab)
+    logits = torch.zeros(11, vocab)
+    logits[0] = torch.randn(vocab, generator=g) * 3
+    logits[1] = rising.flip(0)
+    logits[2] = rising
+    logits[3, 77::7] = 2.0                # a seventh of the largest
+    logits[4] = -INF
+    logits[4, 5000:8000] = torch.randn(3000, generator=g)
+    logits[5] = torch.finfo(dtype).min
+    logits[5, 9::400] = torch.randn(logits[5, 9::400].shape, generator=g)
+    logits[6] = -INF
+    logits[6, vocab - 1] = -2.0
+    logits[7, :100] = 1.0
+    logits[8] = torch.randn(vocab, generator=g)
+    logits[8, 40:72] += 20.0              # a group's 32 tokens far above the others
+    logits[9] = torch.randn(vocab, generator=g) * 1e-3
+    logits[10] = -INF
+    logits[10, ::97] = 1.5
+    logits = logits.to(dtype)
+    u = torch.rand(11, generator=g)
+    k = torch.tensor([1, 33, 200, 64, 150, 100, 5, 120, 207, 208, 90], dtype=torch.int32)
+    _check(device, logits, u, top_k=k)
+    _check(device, logits, u, top_k=k, top_p=torch.rand(11, generator=g), temperature=0.1 + 2 * torch.rand(11, generator=g))
+    _check(device, logits, u, top_k=k.flip(0), min_p=torch.rand(11, generator=g))
+    _check(device, logits, u, top_k=7 * k, top_p=torch.full((11,), 0.99), min_p=torch.full((11,), 1e-4))
+    store = torch.zeros(11, vocab + 3, dtype=dtype)
+    store[:, 1:vocab + 1] = logits       # rows that begin anywhere
+    got = ops.sample_tokens(store.to(device)[:, 1:vocab + 1], u.to(device), top_k=k.to(device))
+    _check(device, logits, u, got, top_k=k)
+
+
+def test_small_top_k_of_many_rows(device):
+    """One workgroup a row, and rows of every kind side by side."""
+    say("sample small top_k, many rows")
+    g = torch.Generator().manual_seed(3)
+    rows = 900
+    logits = torch.randn(rows, 4099, generator=g) * 2
+    _check(device, logits, torch.rand(rows, generator=g), top_k=torch.randint(-1, 90, (rows,), generator=g).to(torch.int32),
+           top_p=0.5 + torch.rand(rows, generator=g), temperature=torch.rand(rows, generator=g))
+
+
 def test_special_logits(device):
     """Infinities and NaN; rows that nothing is allowed in."""
     say("sample special")
