@@ -36,12 +36,16 @@ constexpr int kFewLeast = 24;     // of a part, at least: tiles and starts
 constexpr int kFewMost = 256;     // and at most
 constexpr int kChunkUnits = 128;  // (row, head) pairs of a chunk block
 constexpr int kChunkTile = 64;
-constexpr int kChunkWGs = 512;    // workgroups below which row blocks are split
+// Workgroups below which row blocks are split, and into about as many. (512 would be on the CUs at
+// once, but partial results cost too: a tick whose blocks are 344 workgroups takes 106 us split for
+// 384, 114 for 512, 127 as it is.)
+constexpr int kChunkWGs = 384;
 constexpr int kChunkLeast = 4;    // tiles of a split, at least
+constexpr int kShortJoin = 4;     // splits that a part of a wave joins; a workgroup does more
 constexpr int kPlanThreads = 1024;
 
 // Plan header words.
-enum { H_PARTS = 0, H_CHUNK = 1, H_JOIN = 2, H_ERR = 3, H_STAMP = 4, H_WORDS = 16 };
+enum { H_PARTS = 0, H_CHUNK = 1, H_JOIN = 2, H_ERR = 3, H_STAMP = 4, H_SHORT = 12, H_WORDS = 16 };
 
 __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -118,7 +122,8 @@ inline Layout layout_of(const Shape& s) {
 //          sequences' order
 //   part:  {its first entry of few} and that entry; it goes on to the next part's
 //   chunk: {sequence, first row, first tile, tile end} {first query row, rows, keys, slot or -1}
-//   join:  {output row, first slot, slots from one split to the next, splits}
+//   join:  {output row, first slot, slots from one split to the next, splits}; those of up to
+//          kShortJoin splits from the list's end backwards
 // A slot holds the partial result of one query row, all heads.
 struct PlanArgs {
   const int32_t* cu_q;
@@ -202,11 +207,11 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanArgs a) {
   __shared__ int3 s_waves[kPlanThreads / 64];
   __shared__ int s_items[kPlanThreads], s_slots[kPlanThreads], s_blocks[kPlanThreads], s_cost[kPlanThreads];
   __shared__ unsigned long long s_few, s_tiles;
-  __shared__ int s_err, s_nblocks;
+  __shared__ int s_err, s_nblocks, s_join, s_short;
   const int tid = hx::tid_x(), batch = a.s.batch;
   if (tid == 0) {
     s_few = s_tiles = 0;
-    s_err = s_nblocks = 0;
+    s_err = s_nblocks = s_join = s_short = 0;
   }
   __syncthreads();
   const int64_t room = (int64_t)a.s.width * a.s.page;
@@ -268,7 +273,16 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanArgs a) {
     const int64_t t = ((int64_t)s_tiles * a.s.hkv + kChunkWGs - 1) / kChunkWGs;
     chunk_split = (int)(t < kChunkLeast ? kChunkLeast : t);
   }
-  int few_base = 0, cost_base = 0, chunk_base = 0, slot_base = 0, join_base = 0;
+  int few_base = 0, cost_base = 0, chunk_base = 0, slot_base = 0;
+  // Rows to join, from `of` on; their order in the list is of no account.
+  auto add_joins = [&](int4 of, int rows) {
+    const bool is_short = of.w <= kShortJoin;
+    const int at = atomicAdd(is_short ? &s_short : &s_join, rows);
+    for (int r = 0; r < rows; ++r) {
+      const int64_t to = is_short ? a.most_join - 1 - (at + r) : at + r;
+      if (to >= 0 && to < a.most_join) a.join[to] = make_int4(of.x + r, of.y + r, of.z, of.w);
+    }
+  };
   for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
     const int b = b0 + tid;
     int4 si = make_int4(0, 0, 0, 0);
@@ -291,17 +305,14 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanArgs a) {
     const int splits = rows ? (from + cost - 1) / share - first_part + 1 : 0;
     const int joined = splits > 1 ? rows : 0;
     int3 total;
-    const int3 at = plan_scan(make_int3(splits, joined * splits, joined), &total, s_waves);
+    const int3 at = plan_scan(make_int3(splits, joined * splits, 0), &total, s_waves);
     __syncthreads();
     s_items[tid] = at.x;
     s_slots[tid] = at.y;
     s_blocks[tid] = place.y;
     s_cost[tid] = from;
     __syncthreads();
-    for (int r = 0; r < joined; ++r) {
-      const int64_t to = join_base + at.z + r;
-      if (to < a.most_join) a.join[to] = make_int4(si.x + r, slot_base + at.y + r, rows, splits);
-    }
+    if (joined) add_joins(make_int4(si.x, slot_base + at.y, rows, splits), joined);
     for (int i = tid; i < total.x; i += kPlanThreads) {
       const int j = plan_find(s_items, kPlanThreads, i);
       const int4 of = a.seq[b0 + j];
@@ -332,7 +343,6 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanArgs a) {
     const int3 total2 = make_int3(sum.y, 0, 0);
     few_base += total.x;
     slot_base += total.y;
-    join_base += total.z;
     // Chunk blocks, a round of the threads at a time: their items, slots and joined rows follow
     // those of the blocks before them. Later blocks of a sequence first: they see more keys.
     for (int i0 = 0; i0 < total2.x; i0 += kPlanThreads) {
@@ -349,7 +359,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanArgs a) {
       }
       const int joins = n > 1 ? rows_here : 0;
       int3 all;
-      const int3 to = plan_scan(make_int3(n, joins * n, joins), &all, s_waves);
+      const int3 to = plan_scan(make_int3(n, joins * n, 0), &all, s_waves);
       const int share = n > 0 ? ceil_div(tiles, n) : 0;
       for (int sp = 0; sp < n; ++sp) {
         const int64_t entry = (int64_t)chunk_base + to.x + sp;
@@ -359,25 +369,23 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanArgs a) {
         a.chunk[2 * entry] = make_int4(b0 + j, row0, from, end);
         a.chunk[2 * entry + 1] = make_int4(of.x, of.y, of.z, n > 1 ? slot_base + to.y + sp * rows_here : -1);
       }
-      for (int r = 0; r < joins; ++r) {
-        const int64_t entry = (int64_t)join_base + to.z + r;
-        if (entry < a.most_join) a.join[entry] = make_int4(of.x + row0 + r, slot_base + to.y + r, rows_here, n);
-      }
+      if (joins) add_joins(make_int4(of.x + row0, slot_base + to.y, rows_here, n), joins);
       chunk_base += all.x;
       slot_base += all.y;
-      join_base += all.z;
     }
     __syncthreads();
   }
   if (tid == 0) {
     int err = s_err;
     // By the bounds that the workspace was sized with none of these can happen.
-    if (parts > a.most_parts || few_base > a.most_few || chunk_base > a.most_chunk || join_base > a.most_join || slot_base > a.slots) err |= HX_WERR_GRID;
+    if (parts > a.most_parts || few_base > a.most_few || chunk_base > a.most_chunk ||
+        (int64_t)s_join + s_short > a.most_join || slot_base > a.slots) err |= HX_WERR_GRID;
     const int most = (int)(parts < a.most_parts ? parts : a.most_parts);
     a.hdr[H_PARTS] = most;
     a.part[3 * most] = make_int4(few_base < a.most_few ? few_base : (int)a.most_few, 0, 0, 0);
     a.hdr[H_CHUNK] = chunk_base < a.most_chunk ? chunk_base : (int)a.most_chunk;
-    a.hdr[H_JOIN] = join_base < a.most_join ? join_base : (int)a.most_join;
+    a.hdr[H_JOIN] = s_join < a.most_join ? s_join : (int)a.most_join;
+    a.hdr[H_SHORT] = s_short < a.most_join ? s_short : (int)a.most_join;
     a.hdr[H_ERR] = err;
     const int32_t stamp[8] = {a.s.batch, a.s.total_q, a.s.max_q, a.s.max_k, a.s.hq, a.s.hkv, a.s.head_dim, a.s.page};
     for (int i = 0; i < 8; ++i) a.hdr[H_STAMP + i] = stamp[i];
@@ -405,7 +413,7 @@ struct RunArgs {
   const int4* join;
   float2* part_ml;
   float* part_o;
-  int64_t slots;
+  int64_t slots, most_join;
   Shape s;
   Sizes z;
 };
@@ -1125,8 +1133,9 @@ __global__ __launch_bounds__(chunk_threads(DP), 2) void kv8_chunk_kernel(RunArgs
 }
 
 // -------------------------------------------------------------------------------- join
-// The splits of an output row and query head: a thread takes four dims of every n-th split, in
-// order, then the groups of threads are summed in order.
+// The splits of an output row and query head. Many: a workgroup's thread takes four dims of every
+// n-th split, in order, then the groups of threads are summed in order. Few: a part of a wave with
+// four dims a lane takes them in order, four loads at once.
 constexpr int kJoinThreads = 256;
 
 template <typename T>
@@ -1184,6 +1193,51 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(RunArgs a, int n
       to[1] = hx::pack2_round<T>(x.z * inv, x.w * inv);
     }
     __syncthreads();
+  }
+  const int lane = tid & 63, each = 64 / quads, mine = lane / quads, d4 = 4 * (lane % quads);
+  if (mine >= each) return;
+  const int64_t short_work = (int64_t)a.hdr[H_SHORT] * a.s.hq, step = (int64_t)n_wg * (kJoinThreads / 64) * each;
+  for (int64_t i = ((int64_t)hx::wg_x() * (kJoinThreads / 64) + (tid >> 6)) * each + mine; i < short_work; i += step) {
+    const int rec = (int)((uint32_t)i / (uint32_t)a.s.hq), head = (int)((uint32_t)i % (uint32_t)a.s.hq);
+    const int4 r = a.join[a.most_join - 1 - rec];
+    const int splits = r.w;
+    if (r.x < 0 || r.x >= a.s.total_q || r.y < 0 || splits < 1 || (int64_t)r.y + (int64_t)(splits - 1) * r.z >= a.slots) continue;
+    float m = -INFINITY, l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < splits; s0 += 4) {
+      float2 ml[4];
+      float4 o[4];
+      float top = m;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t p = ((int64_t)r.y + (int64_t)min(s0 + e, splits - 1) * r.z) * a.s.hq + head;
+        ml[e] = a.part_ml[p];
+        o[e] = *reinterpret_cast<const float4*>(a.part_o + p * D + d4);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, ml[e].x);
+      const float ref = top == -INFINITY ? 0.f : top, before = hx::fast_exp2(m - ref);
+      l *= before;
+      x.x *= before;
+      x.y *= before;
+      x.z *= before;
+      x.w *= before;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (s0 + e >= splits) break;
+        const float f = hx::fast_exp2(ml[e].x - ref);
+        l = fmaf(f, ml[e].y, l);
+        x.x = fmaf(f, o[e].x, x.x);
+        x.y = fmaf(f, o[e].y, x.y);
+        x.z = fmaf(f, o[e].z, x.z);
+        x.w = fmaf(f, o[e].w, x.w);
+      }
+      m = top;
+    }
+    const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+    uint32_t* const to = reinterpret_cast<uint32_t*>(a.out + (int64_t)r.x * a.out_row + (int64_t)head * a.out_head + d4);
+    to[0] = hx::pack2_round<T>(x.x * inv, x.y * inv);
+    to[1] = hx::pack2_round<T>(x.z * inv, x.w * inv);
   }
 }
 
@@ -1331,6 +1385,7 @@ extern "C" int hx_kv8_attn_run(const void* q, int64_t q_row_stride, int64_t q_he
   a.part_ml = reinterpret_cast<float2*>(base + r.l.ml);
   a.part_o = reinterpret_cast<float*>(base + r.l.o);
   a.slots = r.l.slots;
+  a.most_join = r.l.most_join;
   a.s = s;
   a.z = sizes_of(s);
   const bool chunk = max_q > a.z.few_rows && (kinds & HX_KV8_CHUNK_ROWS), few = (kinds & HX_KV8_FEW_ROWS) != 0;
