@@ -824,6 +824,15 @@ def _check_kv8(cache: Kv8Cache) -> tuple[int, int, int, int, int]:
     return layout
 
 
+def _gpu_of(tensors: Sequence[torch.Tensor]) -> torch.device:
+    """``_require_gpu`` by the devices' indexes alone: a third of its time for a dozen tensors."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index:
+            return _require_gpu(*tensors)
+    return tensors[0].device if index >= 0 else _require_gpu(*tensors)
+
+
 def _check_kv8_rows(keys: torch.Tensor, values: torch.Tensor, write_slots: torch.Tensor, n_kv: int,
                     head_dim: int) -> int:
     """Checks of new keys and values for an 8-bit cache; their dtype code."""
@@ -848,7 +857,7 @@ def kv8_append(cache: Kv8Cache, write_slots: torch.Tensor, keys: torch.Tensor, v
     skipped; listed twice: one of its tokens, or parts of several). ``keys`` / ``values``
     ``[T, kv_heads, head_dim]`` bfloat16 or float16, any row and head strides. A row with an
     infinite or NaN element is stored as NaN: under a NaN scale."""
-    device = _require_gpu(*cache, write_slots, keys, values)
+    device = _gpu_of((*cache, write_slots, keys, values))
     code, pages, page_size, n_kv, head_dim = _check_kv8(cache)
     dtype = _check_kv8_rows(keys, values, write_slots, n_kv, head_dim)
     write_slots = write_slots.contiguous()
@@ -870,8 +879,7 @@ def kv8_norm_rope_append(
     normalised, rotated queries (``out`` if given). In fp32 and rounded once, to the queries'
     dtype or to the codes (``qk_norm_rope_append`` rounds between the norm and the rotation, as
     its reference does). Arguments as there, ``write_slots`` as for ``kv8_append``."""
-    device = _require_gpu(queries, keys, values, q_norm_weight, k_norm_weight, cos, sin, positions, *cache,
-                          write_slots)
+    device = _gpu_of((queries, keys, values, q_norm_weight, k_norm_weight, cos, sin, positions, *cache, write_slots))
     code, pages, page_size, n_kv, head_dim = _check_kv8(cache)
     dtype = _check_kv8_rows(keys, values, write_slots, n_kv, head_dim)
     if queries.ndim != 3 or queries.shape[0] != keys.shape[0] or queries.shape[2] != head_dim or queries.shape[1] < 1:
@@ -881,22 +889,30 @@ def kv8_norm_rope_append(
     _check_rope(q_norm_weight, k_norm_weight, cos, sin, head_dim)
     if cos.shape[0] < 1:
         raise ValueError("cos/sin need at least one row.")
-    positions = positions.reshape(-1)
-    if positions.dtype != torch.int64 or positions.numel() != queries.shape[0]:
+    tokens, n_q, _ = queries.shape
+    if positions.dtype != torch.int64 or positions.numel() != tokens:
         raise ValueError("positions must be int64 with one entry per row.")
+    if positions.ndim != 1:
+        positions = positions.reshape(-1)
     positions, write_slots = positions.contiguous(), write_slots.contiguous()
     if out is None:
-        out = torch.empty(queries.shape, dtype=queries.dtype, device=device)
+        out = torch.empty((tokens, n_q, head_dim), dtype=queries.dtype, device=device)
     elif out.shape != queries.shape or out.dtype != queries.dtype or out.device != device or out.stride(2) != 1:
         raise ValueError("out must match the queries' shape, dtype and device.")
-    q_norm_weight, k_norm_weight, cos, sin = (
-        t if t.data_ptr() % 16 == 0 else t.clone() for t in (q_norm_weight, k_norm_weight, cos, sin))
+    tables = [q_norm_weight, k_norm_weight, cos, sin]
+    at = [t.data_ptr() for t in tables]
+    for i in range(4):
+        if at[i] % 16:
+            tables[i] = tables[i].clone()
+            at[i] = tables[i].data_ptr()
+    q_row, q_head, _ = queries.stride()
+    k_row, k_head, _ = keys.stride()
+    v_row, v_head, _ = values.stride()
+    out_row, out_head, _ = out.stride()
     status = _launch(
-        device, _capi.lib().hx_kv8_norm_rope_append, queries.data_ptr(), queries.stride(0), queries.stride(1),
-        keys.data_ptr(), keys.stride(0), keys.stride(1), values.data_ptr(), values.stride(0), values.stride(1),
-        q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-        positions.data_ptr(), queries.shape[0], queries.shape[1], n_kv, head_dim, eps, dtype,
-        out.data_ptr(), out.stride(0), out.stride(1), cache.keys.data_ptr(), cache.values.data_ptr(),
+        device, _capi.lib().hx_kv8_norm_rope_append, queries.data_ptr(), q_row, q_head, keys.data_ptr(), k_row, k_head,
+        values.data_ptr(), v_row, v_head, *at, cos.shape[0], positions.data_ptr(), tokens, n_q, n_kv, head_dim, eps, dtype,
+        out.data_ptr(), out_row, out_head, cache.keys.data_ptr(), cache.values.data_ptr(),
         cache.key_scales.data_ptr(), cache.value_scales.data_ptr(), pages, page_size, code, write_slots.data_ptr())
     _capi.check(status, "hx_kv8_norm_rope_append")
     return out
@@ -1214,10 +1230,11 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: 
         raise ValueError(f"sample_tokens draws from at most {SAMPLE_MAX_VOCAB} tokens.")
     if (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
         raise ValueError("logits need contiguous rows that do not overlap.")
+    index = device.index
     for name, t, kind in (("uniforms", uniforms, torch.float32), ("temperature", temperature, torch.float32),
                           ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
                           ("min_p", min_p, torch.float32)):
-        if t is not None and (t.dtype != kind or t.shape != (rows,) or not t.is_contiguous() or t.device != device):
+        if t is not None and (t.dtype != kind or t.shape != (rows,) or not t.is_contiguous() or t.get_device() != index):
             raise ValueError(f"{name} must be contiguous {kind} [{rows}] on the logits' device.")
     token_ids = logits.new_empty(rows, dtype=torch.int64)
     logprobs = logits.new_empty(rows, dtype=torch.float32)
