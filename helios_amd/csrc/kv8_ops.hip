@@ -65,8 +65,28 @@ __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
   x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
 }
 
+// Over LANES neighbouring lanes, each of which gets the result: two lanes of a quad, two quads, two
+// halves of 16, and further ones through the shuffle.
+template <int CTRL, typename X>
+__device__ __forceinline__ X other_lane(X x) {
+  return __builtin_bit_cast(X, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+template <int LANES, typename X, typename F>
+__device__ __forceinline__ X over_lanes(X x, F f) {
+  x = f(x, other_lane<0xb1>(x));   // lane ^ 1
+  x = f(x, other_lane<0x4e>(x));   // lane ^ 2
+  x = f(x, other_lane<0x141>(x));  // 7 - lane
+  if constexpr (LANES >= 16) x = f(x, other_lane<0x140>(x));  // 15 - lane
+  if constexpr (LANES >= 32) x = f(x, __builtin_bit_cast(X, __shfl_xor(__builtin_bit_cast(int, x), 16)));
+  return x;
+}
+
 // A head row to LANES lanes, 8 elements each (lanes past head_dim idle along); a workgroup takes
-// kThreads / LANES of them, a token's query, key and value heads in turn.
+// kThreads / LANES of them, a token's query, key and value heads in turn. 2381 tokens of 32 + 8 + 8
+// heads of 128, with norms and rotation: 17.3 us, 3.3 TB/s, 11.7 without the rotation, whose weights,
+// cosines and sines are 6 times a row's own bytes, from L2, and whose sum and turn are chains across
+// lanes. (Two heads to a lane, which then share the cosines: 16.3, but 64 tokens 4.7 instead of 3.6.)
+// Few tokens are a launch's latency.
 template <typename T, typename C, int LANES, bool ROPE, bool VEC>
 __global__ __launch_bounds__(kThreads) void kv8_write_kernel(WriteArgs a) {
   const int lane = hx::tid_x() & (LANES - 1);
@@ -104,8 +124,7 @@ __global__ __launch_bounds__(kThreads) void kv8_write_kernel(WriteArgs a) {
     float ss = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-    for (int m = 1; m < LANES; m <<= 1) ss += __shfl_xor(ss, m);
+    ss = over_lanes<LANES>(ss, [](float p, float q) { return p + q; });
     const float r = rsqrtf(ss / (float)a.head_dim + a.eps);
     const int half = a.head_dim / 16;  // lanes of half a head row
     const bool low = lane < half;
@@ -138,15 +157,21 @@ __global__ __launch_bounds__(kThreads) void kv8_write_kernel(WriteArgs a) {
   uint32_t top = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) top = max(top, hx::raw_bits(x[e]) & 0x7fffffffu);
-#pragma unroll
-  for (int m = 1; m < LANES; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m));
+  top = over_lanes<LANES>(top, [](uint32_t p, uint32_t q) { return max(p, q); });
   const bool finite = top < 0x7f800000u;
   const float scale = fmaxf(__fmul_rn(__uint_as_float(finite ? top : 0u), 1.f / C::kMost), hx8::kLeastScale);
+  // x / scale, rounded once, from the rounded reciprocal, of which a row needs one (Markstein 1990):
+  // with r = 1 / s rounded to nearest and y = x r, the remainder x - y s is exact and y + (x - y s) r
+  // rounds to the quotient. A small scale goes up by 2^64 first, and x with it: remainders stay normal.
+  const float up = scale < 0x1p-64f ? 0x1p64f : 1.f, s = scale * up, r = __fdiv_rn(1.f, s);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float n = x[e] * up, y = n * r;
+    x[e] = copysignf(fmaf(fmaf(-y, s, n), r, y), n);  // (-0 stays)
+  }
   uint32_t code[2];
 #pragma unroll
-  for (int e = 0; e < 8; e += 4)
-    code[e / 4] = hx8::encode4<C>(__fdiv_rn(x[e], scale), __fdiv_rn(x[e + 1], scale), __fdiv_rn(x[e + 2], scale),
-                                  __fdiv_rn(x[e + 3], scale));
+  for (int e = 0; e < 8; e += 4) code[e / 4] = hx8::encode4<C>(x[e], x[e + 1], x[e + 2], x[e + 3]);
   if (mine)
     hx::st8_nt(a.codes[which] + (slot * a.hkv + hh) * a.head_dim + d, finite ? code[0] : 0u, finite ? code[1] : 0u);
   if (lane == 0) {
@@ -166,47 +191,66 @@ struct ReadArgs {
   void* out;
 };
 
-// 16 codes to a lane; consecutive lanes walk a head's rows, whose codes are whole 16-byte pieces
-// and whose results are consecutive in memory.
+// 16 bytes of results to a lane, from 8 codes (4 for fp32); consecutive lanes walk a head's rows, whose
+// results are consecutive in memory. A thread's loads for four such pieces are in flight together, and
+// one head's workgroups follow another's. 40001 tokens of 8 heads of 128 to fp16: 22 us, 5.5 TB/s (24
+// with two pieces, 24 with the heads side by side, 33 with 16 codes to a lane, whose stores leave gaps).
 template <typename T, typename C>
 __global__ __launch_bounds__(kThreads) void kv8_read_kernel(ReadArgs a, int pieces, uint32_t wgs) {
-  const int h = (int)((uint32_t)hx::wg_x() % (uint32_t)a.hkv);
-  const uint32_t at = (uint32_t)hx::wg_x() / (uint32_t)a.hkv;
-  for (int64_t i = (int64_t)at * kThreads + hx::tid_x(); i < a.length * pieces; i += (int64_t)wgs * kThreads) {
-    const int64_t t = (i >> 32) == 0 ? (int64_t)((uint32_t)i / (uint32_t)pieces) : i / pieces;
-    const int d = 16 * (int)(i - t * pieces);
-    const int64_t j = (t >> 32) == 0 ? (int64_t)((uint32_t)t / (uint32_t)a.page) : t / a.page;
-    const int off = (int)(t - j * a.page);
-    const int64_t page = a.pages[j];
-    float x[16];
+  constexpr int kCodes = 16 / sizeof(T), kAhead = 4;
+  const int h = (int)((uint32_t)hx::wg_x() / wgs);
+  const uint32_t at = (uint32_t)hx::wg_x() - (uint32_t)h * wgs;
+  const int64_t all = a.length * pieces;
+  for (int64_t i0 = (int64_t)at * (kAhead * kThreads) + hx::tid_x(); i0 < all; i0 += (int64_t)wgs * (kAhead * kThreads)) {
+    uint32_t w[kAhead][kCodes / 4];
+    float s[kAhead];
+    int64_t page[kAhead], in[kAhead];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = 0.f;
-    if (page >= 0 && page < a.num_pages) {
-      const uint4 u = hx::ld16_stream(a.codes + ((page * a.page + off) * a.hkv + h) * a.head_dim + d);
-      const float s = a.scales[(page * a.hkv + h) * a.page + off];
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t i = i0 + u * kThreads < all ? i0 + u * kThreads : all - 1;
+      const int64_t t = (i >> 32) == 0 ? (int64_t)((uint32_t)i / (uint32_t)pieces) : i / pieces;
+      const int64_t j = (t >> 32) == 0 ? (int64_t)((uint32_t)t / (uint32_t)a.page) : t / a.page;
+      page[u] = a.pages[j];
+      const bool off = page[u] < 0 || page[u] >= a.num_pages;
+      page[u] = off ? 0 : page[u];
+      const int64_t row = t - j * a.page;
+      in[u] = (row * a.hkv + h) * a.head_dim + kCodes * (i - t * pieces);
+      s[u] = off ? 0.f : a.scales[(page[u] * a.hkv + h) * a.page + row];
+      page[u] = off ? -1 : page[u];
+    }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float f[4];
-        hx8::decode4<C>(w[e], f);
+    for (int u = 0; u < kAhead; ++u) {
+      const uint8_t* const from = a.codes + (page[u] < 0 ? 0 : page[u]) * a.page * a.hkv * a.head_dim + in[u];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[4 * e + k] = f[k] * s;
+      for (int e = 0; e < kCodes / 4; ++e) w[u][e] = 0;
+      if (page[u] < 0) continue;
+      if constexpr (kCodes == 8) {
+        const uint2 x = *reinterpret_cast<const uint2*>(from);
+        w[u][0] = x.x;
+        w[u][1] = x.y;
+      } else {
+        w[u][0] = *reinterpret_cast<const uint32_t*>(from);
       }
     }
-    const int64_t to = ((int64_t)h * a.length + t) * a.head_dim + d;
-    if constexpr (sizeof(T) == 4) {
-      uint4* const o = reinterpret_cast<uint4*>(static_cast<float*>(a.out) + to);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        hx::st16_nt(o + e, make_uint4(__float_as_uint(x[4 * e]), __float_as_uint(x[4 * e + 1]),
-                                      __float_as_uint(x[4 * e + 2]), __float_as_uint(x[4 * e + 3])));
-    } else {
-      uint4* const o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + to);
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t i = i0 + u * kThreads;
+      if (i >= all) break;
+      float x[kCodes];
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        hx::st16_nt(o + e, make_uint4(hx::pack2_round<T>(x[8 * e], x[8 * e + 1]), hx::pack2_round<T>(x[8 * e + 2], x[8 * e + 3]),
-                                      hx::pack2_round<T>(x[8 * e + 4], x[8 * e + 5]),
-                                      hx::pack2_round<T>(x[8 * e + 6], x[8 * e + 7])));
+      for (int e = 0; e < kCodes / 4; ++e) {
+        float f[4];
+        hx8::decode4<C>(w[u][e], f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[4 * e + k] = f[k] * s[u];
+      }
+      uint4 o;
+      if constexpr (sizeof(T) == 4)
+        o = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+      else
+        o = make_uint4(hx::pack2_round<T>(x[0], x[1]), hx::pack2_round<T>(x[2], x[3]),
+                       hx::pack2_round<T>(x[4], x[5]), hx::pack2_round<T>(x[6], x[7]));
+      hx::st16_nt(static_cast<uint8_t*>(a.out) + ((int64_t)h * all + i) * 16, o);
     }
   }
 }
@@ -346,8 +390,8 @@ extern "C" int hx_kv8_gather(const void* codes, const float* scales, int32_t num
   if (length == 0) return HX_OK;
   if (!codes || !scales || !pages || !out || misaligned(codes, 16) || misaligned(out, 16)) return HX_E_INVALID_ARG;
   ReadArgs a{static_cast<const uint8_t*>(codes), scales, num_pages, page_size, n_kv_heads, head_dim, pages, length, out};
-  const int pieces = head_dim / 16;
-  int64_t wgs = (length * pieces + kThreads - 1) / kThreads;
+  const int pieces = head_dim / (dtype == HX_DTYPE_FP32 ? 4 : 8);
+  int64_t wgs = (length * pieces + 4 * kThreads - 1) / (4 * kThreads);
   const int64_t most = 65536 / n_kv_heads + 1;
   wgs = wgs < most ? wgs : most;
   if (wgs * n_kv_heads > kMostItems / kThreads) return HX_E_UNSUPPORTED;

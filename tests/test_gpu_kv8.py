@@ -84,6 +84,21 @@ def test_append(device, heads, d, page, tokens, code, dtype):
         _same_cache(cache, want)
 
 
+@pytest.mark.parametrize("code", CODES)
+def test_append_of_any_magnitude(device, code):
+    """Rows at every power of two that bfloat16 has, subnormal ones among them, with 0 and -0."""
+    say("kv8 append magnitudes", code)
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(320, 2, 64, generator=g).double() * 2.0 ** torch.randint(-9, 1, (320, 2, 64), generator=g)
+    x = (x * 2.0 ** (torch.arange(320) * 0.8 - 133)[:, None, None]).float().clamp(-3e38, 3e38).to(torch.bfloat16)
+    x[:, :, 5], x[:, :, 6] = 0.0, -0.0
+    cache = _cache(3, 128, 2, 64, code, device)
+    slots = torch.randperm(384, generator=g)[:320]
+    want = _expected_append(cache, slots, x, -x)
+    ops.kv8_append(cache, slots.to(device), x.to(device), (-x).to(device))
+    _same_cache(cache, want)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("code", CODES)
 def test_append_special_rows(device, code, dtype):
