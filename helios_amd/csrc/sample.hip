@@ -15,19 +15,18 @@
 // from fp64 (the argument of exp loses 2^-24 of itself in fp32, more than a token's share of a flat
 // row over 10^5 tokens).
 //
-// Three launches:
-//   range  (many workgroups a row) the row's largest and smallest logit, and the largest of each
-//          group of 32 tokens
-//   limits (many workgroups a row) rows of a small top_k: the k-th largest of the groups' maxima is a
-//          bound that the k first tokens reach and few others do; the groups that reach it are read
-//          again and their tokens listed, and the row's last workgroup orders them and draws. Other
-//          rows: counts and weights over 2048 bins of equal width between the extremes.
-//   row    (a workgroup a row) of those finds the bins where the limits and the drawn position fall,
-//          gathers their tokens and orders those.
-// Bound by reading the logits from HBM, once; what is read again is in the last-level cache.
-// 96 rows of 151936 fp32 logits, top_k about 1000: 54 us (range 12, limits 34, row 4; the bins alone
-// 115), one bf16 row of them, top_k about 50: 19.5 us (31). Rows without a top_k: 75 to 110 us, of
-// which the fp64 weights of all tokens are 34 and a workgroup a row's pass over its logits 15 to 40.
+// Two launches of many workgroups a row:
+//   range  the row's largest and smallest logit, and the largest of each group of 32 tokens
+//   row    rows of a small top_k: the k-th largest of the groups' maxima is a bound that the k first
+//          tokens reach and few others do; the groups that reach it are read again and their tokens
+//          listed. Other rows: counts and weights over 2048 bins of equal width between the extremes.
+//          A row's last workgroup orders the list and draws, or finds the bins where the limits and
+//          the drawn position fall, gathers their tokens and orders those.
+// Bound by reading the logits from HBM, once (what is read again is in the last-level cache), and by
+// the last workgroups' chain of steps. 96 rows of 151936 fp32 logits, top_k about 1000: 43 us, of
+// which the first launch is 12; one bf16 row of them, top_k about 50: 19. (By the bins, in three
+// launches: 115 and 31.) 96 rows without a top_k: 75 to 130 us, of which the fp64 weights of all
+// tokens are 34 and each of the last workgroups' passes over its row 15.
 
 #include "hx_common.h"
 
@@ -35,9 +34,8 @@ namespace {
 
 constexpr int kBins = 2048;
 constexpr int kList = 2048;      // tokens that the last launch orders at once
-constexpr int kThreads = 256;    // of the three launches
-constexpr int kLimitThreads = 512;
-constexpr int kRowThreads = 1024;
+constexpr int kThreads = 256;    // of the first launch
+constexpr int kRowThreads = 1024;  // and of the second
 constexpr int kGroup = 32;       // tokens of a group
 // A small top_k: of k tokens drawn at random over g groups the bound lets through about
 // -g ln(1 - k / g) tokens, 1.22 k at k = g / 3; kList must hold them.
@@ -62,7 +60,7 @@ struct SampleArgs {
   uint32_t* count;  // [rows][kBins]
   uint64_t* mass;   // [rows][kBins]; or [rows][kList], the listed tokens of a row of a small top_k
   uint32_t* most;   // [rows][groups]: the order of a group's largest logit
-  uint32_t* listed; // [rows][2]: tokens that a row of a small top_k lists, and workgroups that have
+  uint32_t* listed; // [rows][2]: tokens that a row of a small top_k lists, and its workgroups that are done
   int32_t groups;
   int32_t chunks, chunk;    // of the first launch, and their tokens
   int32_t chunks2, chunk2;  // of the second
@@ -88,25 +86,31 @@ struct __attribute__((packed, aligned(sizeof(T)))) Piece {
     if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
     else return Logit<T>::get(w[e / 2], e & 1);
   }
+  // f(logit, index from `at`) for each.
+  template <typename F>
+  __device__ __forceinline__ void each(int at, F f) const {
+#pragma unroll
+    for (int e = 0; e < Logit<T>::kVec; ++e) f(get(e), at + e);
+  }
 };
 
 // Calls f(logit, index) for tokens [begin, end) of a row, spread over a workgroup's threads.
-template <typename T, int THREADS, typename F>
+template <typename T, typename F>
 __device__ __forceinline__ void each_logit(const void* row, int begin, int end, F f) {
   constexpr int kVec = Logit<T>::kVec, kAhead = 4;
   const T* const p = static_cast<const T*>(row);
   const int whole = (end - begin) / kVec;
-  for (int j0 = hx::tid_x(); j0 < whole; j0 += kAhead * THREADS) {
+  for (int j0 = hx::tid_x(); j0 < whole; j0 += kAhead * kRowThreads) {
     Piece<T> u[kAhead];  // in flight together
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
-      u[i] = *reinterpret_cast<const Piece<T>*>(p + begin + min(j0 + i * THREADS, whole - 1) * kVec);
+      u[i] = *reinterpret_cast<const Piece<T>*>(p + begin + min(j0 + i * kRowThreads, whole - 1) * kVec);
+    // (One copy of f's code, which is large: a workgroup's few turns cost less than fetching more.)
+#pragma nounroll
+    for (int j = j0; j < min(whole, j0 + kAhead * kRowThreads); j += kRowThreads) {
+      u[0].each(begin + j * kVec, f);
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int j = j0 + i * THREADS;
-      if (j >= whole) break;
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) f(u[i].get(e), begin + j * kVec + e);
+      for (int i = 0; i + 1 < kAhead; ++i) u[i] = u[i + 1];
     }
   }
   const int v = begin + whole * kVec + hx::tid_x();
@@ -159,9 +163,8 @@ __global__ __launch_bounds__(kThreads) void sample_range_kernel(SampleArgs a) {
       a.count[row * kBins + b] = 0;
       a.mass[row * kBins + b] = 0;
     }
-  } else if (c == 0 && tid < 2) {
-    a.listed[2 * row + tid] = 0;
   }
+  if (c == 0 && tid < 2) a.listed[2 * row + tid] = 0;
   constexpr int kVec = Logit<T>::kVec, kLanes = kGroup / kVec, kAhead = 4;
   uint32_t top = 0, at = 0xffffffffu, low = 0xffffffffu;
   const int begin = min(a.vocab, c * a.chunk), end = min(a.vocab, begin + a.chunk);
@@ -291,32 +294,29 @@ __device__ __forceinline__ uint64_t fixed_of(double e) {
 }
 
 // ------------------------------------------------------------------------ listed tokens
-template <int THREADS>
 struct List {
   uint32_t bins[kBins];
   uint64_t list[kList];    // gathered tokens: order falling in the high half, index in the low
   uint64_t sorted[kList];
-  uint64_t waves[THREADS / 64];
+  uint64_t waves[kRowThreads / 64];
   uint32_t listed, crowd;
   // Weight up to and with a token of the sorted list: in the list's place once that is sorted.
   __device__ __forceinline__ uint64_t* cum() { return list; }
 };
 
-template <int THREADS>
-__device__ uint64_t block_sum(List<THREADS>& s, uint64_t x) {
+__device__ uint64_t block_sum(List& s, uint64_t x) {
   for (int m = 1; m < 64; m <<= 1) x += shfl_xor_u64(x, m);
   __syncthreads();
   if ((hx::tid_x() & 63) == 0) s.waves[hx::tid_x() >> 6] = x;
   __syncthreads();
   uint64_t all = 0;
 #pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) all += s.waves[w];
+  for (int w = 0; w < kRowThreads / 64; ++w) all += s.waves[w];
   return all;
 }
 
 // Sum over the threads before this one.
-template <int THREADS>
-__device__ uint64_t block_before(List<THREADS>& s, uint64_t x) {
+__device__ uint64_t block_before(List& s, uint64_t x) {
   const int lane = hx::tid_x() & 63;
   uint64_t sum = x;
   for (int m = 1; m < 64; m <<= 1) {
@@ -328,7 +328,7 @@ __device__ uint64_t block_before(List<THREADS>& s, uint64_t x) {
   __syncthreads();
   uint64_t before = sum - x;
 #pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) before += w < hx::tid_x() >> 6 ? s.waves[w] : 0;
+  for (int w = 0; w < kRowThreads / 64; ++w) before += w < hx::tid_x() >> 6 ? s.waves[w] : 0;
   return before;
 }
 
@@ -349,14 +349,13 @@ __device__ __forceinline__ float place_logit(uint64_t place) { return logit_of(~
 
 // Orders the n listed tokens and sums their weights onto `base`. By all threads. The tokens are of
 // all bins, or of one bin alone.
-template <int THREADS>
-__device__ void order_list(List<THREADS>& s, const Row& r, int n, uint64_t base, int one = -1) {
-  constexpr int kEach = kList / THREADS, kBinsEach = kBins / THREADS;
+__device__ void order_list(List& s, const Row& r, int n, uint64_t base, int one = -1) {
+  constexpr int kEach = kList / kRowThreads, kBinsEach = kBins / kRowThreads;
   const int tid = hx::tid_x();
   __syncthreads();
   // Tokens to their bins' places (one bin's: parts of it), in any order; then a token's place is the
   // number of its bin's tokens before it. Lists with a crowded bin are sorted instead.
-  for (int b = tid; b < kBins; b += THREADS) s.bins[b] = 0;
+  for (int b = tid; b < kBins; b += kRowThreads) s.bins[b] = 0;
   if (tid == 0) s.crowd = 0;
   __syncthreads();
   uint64_t mine[kEach];
@@ -364,7 +363,7 @@ __device__ void order_list(List<THREADS>& s, const Row& r, int n, uint64_t base,
   uint32_t turn[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    const int i = tid + e * THREADS;
+    const int i = tid + e * kRowThreads;
     if (i >= n) break;
     mine[e] = s.list[i];
     const float x = (r.top - place_logit(mine[e])) * r.per_bin;
@@ -390,11 +389,11 @@ __device__ void order_list(List<THREADS>& s, const Row& r, int n, uint64_t base,
   if (!s.crowd) {
 #pragma unroll
     for (int e = 0; e < kEach; ++e)
-      if (tid + e * THREADS < n) s.list[s.bins[bin[e]] + turn[e]] = mine[e];
+      if (tid + e * kRowThreads < n) s.list[s.bins[bin[e]] + turn[e]] = mine[e];
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      if (tid + e * THREADS >= n) break;
+      if (tid + e * kRowThreads >= n) break;
       const int from = (int)s.bins[bin[e]], to = bin[e] + 1 < kBins ? (int)s.bins[bin[e] + 1] : n;
       int at = from;
       for (int i = from; i < to; ++i) at += s.list[i] < mine[e] ? 1 : 0;
@@ -403,11 +402,11 @@ __device__ void order_list(List<THREADS>& s, const Row& r, int n, uint64_t base,
   } else {
     int size = 2;
     while (size < n) size <<= 1;
-    for (int i = tid; i < size; i += THREADS) s.sorted[i] = i < n ? s.list[i] : ~0ull;
+    for (int i = tid; i < size; i += kRowThreads) s.sorted[i] = i < n ? s.list[i] : ~0ull;
     for (int k = 2; k <= size; k <<= 1)
       for (int j = k >> 1; j > 0; j >>= 1) {
         __syncthreads();
-        for (int pair = tid; pair < size / 2; pair += THREADS) {
+        for (int pair = tid; pair < size / 2; pair += kRowThreads) {
           const int i = 2 * pair - (pair & (j - 1));
           const uint64_t x = s.sorted[i], y = s.sorted[i + j];
           if ((x > y) == ((i & k) == 0)) {
@@ -473,8 +472,7 @@ __device__ __forceinline__ void answer(const SampleArgs& a, const Row& r, int64_
 
 // Draws from a list that holds the row's first tokens, all that the limits can keep. `total` is the
 // weight of the row where the limits need it (no top_k).
-template <int THREADS>
-__device__ void draw_from(const SampleArgs& a, List<THREADS>& s, const Row& r, int64_t row, const Limits& m, int listed,
+__device__ void draw_from(const SampleArgs& a, List& s, const Row& r, int64_t row, const Limits& m, int listed,
                           uint64_t total) {
   order_list(s, r, listed, 0);
   const uint64_t* const cum = s.cum();
@@ -485,7 +483,7 @@ __device__ void draw_from(const SampleArgs& a, List<THREADS>& s, const Row& r, i
   }
   if (m.by_min) {
     uint64_t mine = 0;
-    for (int i = hx::tid_x(); i < listed; i += THREADS) mine += weight_of(log_weight(r, place_logit(s.sorted[i]))) >= m.min_p ? 1 : 0;
+    for (int i = hx::tid_x(); i < listed; i += kRowThreads) mine += weight_of(log_weight(r, place_logit(s.sorted[i]))) >= m.min_p ? 1 : 0;
     n = min(n, (uint32_t)block_sum(s, mine));
   }
   n = max(n, 1u);
@@ -501,14 +499,14 @@ struct Bins {
 };
 
 // Counts and weights of a workgroup's tokens over the row's bins.
-template <typename T, int THREADS>
+template <typename T>
 __device__ void fill_bins(Bins& s, const Row& r, const void* row, int begin, int end) {
-  for (int b = hx::tid_x(); b < kBins; b += THREADS) {
+  for (int b = hx::tid_x(); b < kBins; b += kRowThreads) {
     s.count[b] = 0;
     s.mass[b] = 0;
   }
   __syncthreads();
-  each_logit<T, THREADS>(row, begin, end, [&](float l, int) {
+  each_logit<T>(row, begin, end, [&](float l, int) {
     const int b = bin_of(r, l);
     if (b == kBins) return;
     atomicAdd(&s.count[b], 1u);
@@ -519,17 +517,16 @@ __device__ void fill_bins(Bins& s, const Row& r, const void* row, int begin, int
 }
 
 // The last bin of the bound: k groups have their largest logit in it or before it.
-template <int THREADS>
-__device__ int bound_of(const SampleArgs& a, List<THREADS>& s, const Row& r, int64_t row, uint32_t k) {
-  constexpr int kEach = kBins / THREADS, kAhead = 8;
+__device__ int bound_of(const SampleArgs& a, List& s, const Row& r, int64_t row, uint32_t k) {
+  constexpr int kEach = kBins / kRowThreads, kAhead = 8;
   const int tid = hx::tid_x();
-  for (int b = tid; b < kBins; b += THREADS) s.bins[b] = 0;
+  for (int b = tid; b < kBins; b += kRowThreads) s.bins[b] = 0;
   if (tid == 0) s.crowd = kBins - 1;
   __syncthreads();
-  for (int g0 = tid; g0 < a.groups; g0 += kAhead * THREADS) {
+  for (int g0 = tid; g0 < a.groups; g0 += kAhead * kRowThreads) {
     uint32_t most[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) most[i] = g0 + i * THREADS < a.groups ? a.most[row * a.groups + g0 + i * THREADS] : kOrderNegInf;
+    for (int i = 0; i < kAhead; ++i) most[i] = g0 + i * kRowThreads < a.groups ? a.most[row * a.groups + g0 + i * kRowThreads] : kOrderNegInf;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int b = bin_of(r, logit_of(most[i]));
@@ -556,31 +553,30 @@ __device__ int bound_of(const SampleArgs& a, List<THREADS>& s, const Row& r, int
   return (int)s.crowd;
 }
 
-// Lists a workgroup's tokens within the row's bound; the row's last workgroup draws.
-template <typename T, int THREADS>
-__device__ void pick(const SampleArgs& a, List<THREADS>& s, const Row& r, int64_t row, int begin, int end) {
+// Lists a workgroup's tokens within the row's bound.
+template <typename T>
+__device__ void pick(const SampleArgs& a, List& s, const Row& r, int64_t row, int begin, int end) {
   constexpr int kVec = Logit<T>::kVec, kLanes = kGroup / kVec;
   const int tid = hx::tid_x();
-  const Limits m = limits_of(a, row);
-  const int bound = bound_of(a, s, r, row, m.k);
+  const int bound = bound_of(a, s, r, row, (uint32_t)a.top_k[row]);
   static_assert(kMostVocab / kGroup * sizeof(uint16_t) <= sizeof(s.sorted));
   uint16_t* const reach = reinterpret_cast<uint16_t*>(s.sorted);  // the workgroup's groups that reach the bound
   __syncthreads();
   if (tid == 0) s.listed = s.crowd = 0;
   __syncthreads();
   const int g_end = (end + kGroup - 1) / kGroup;
-  for (int g = begin / kGroup + tid; g < g_end; g += THREADS)
+  for (int g = begin / kGroup + tid; g < g_end; g += kRowThreads)
     if (bin_of(r, logit_of(a.most[row * a.groups + g])) <= bound) reach[atomicAdd(&s.crowd, 1u)] = (uint16_t)g;
   __syncthreads();
   const int groups = (int)s.crowd;
   const T* const p = static_cast<const T*>(a.logits) + row * a.row_stride;
   constexpr int kAhead = 4;
-  for (int i0 = tid; i0 < groups * kLanes; i0 += kAhead * THREADS) {
+  for (int i0 = tid; i0 < groups * kLanes; i0 += kAhead * kRowThreads) {
     Piece<T> u[kAhead];  // in flight together
     int at[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int j = i0 + i * THREADS;
+      const int j = i0 + i * kRowThreads;
       at[i] = j < groups * kLanes ? reach[j / kLanes] * kGroup + j % kLanes * kVec : end;
       if (at[i] + kVec <= end) u[i] = *reinterpret_cast<const Piece<T>*>(p + at[i]);
     }
@@ -589,13 +585,18 @@ __device__ void pick(const SampleArgs& a, List<THREADS>& s, const Row& r, int64_
       const uint32_t to = atomicAdd(&s.listed, 1u);
       if (to < (uint32_t)kList) s.list[to] = place_of(l, v);
     };
-#pragma unroll
+#pragma nounroll
     for (int i = 0; i < kAhead; ++i) {
-      if (at[i] + kVec <= end) {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) take(u[i].get(e), at[i] + e);
+      if (at[0] + kVec <= end) {
+        u[0].each(at[0], take);
       } else {
-        for (int e = at[i]; e < end; ++e) take((float)p[e], e);
+#pragma nounroll
+        for (int e = at[0]; e < end; ++e) take((float)p[e], e);
+      }
+#pragma unroll
+      for (int k = 0; k + 1 < kAhead; ++k) {
+        u[k] = u[k + 1];
+        at[k] = at[k + 1];
       }
     }
   }
@@ -607,43 +608,12 @@ __device__ void pick(const SampleArgs& a, List<THREADS>& s, const Row& r, int64_
   const uint32_t base = s.crowd;
   static_assert(kList <= kBins);
   uint64_t* const list = a.mass + row * kBins;
-  for (uint32_t i = tid; i < mine && base + i < (uint32_t)kList && i < (uint32_t)kList; i += THREADS) list[base + i] = s.list[i];
-  __syncthreads();
-  // What the workgroups wrote is seen by the one that counts itself last.
-  if (tid == 0) s.crowd = __hip_atomic_fetch_add(&a.listed[2 * row + 1], 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  if (s.crowd != (uint32_t)a.chunks2 - 1) return;
-  const uint32_t all = __hip_atomic_load(&a.listed[2 * row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  if (all > (uint32_t)kList) return;  // the next launch's
-  for (uint32_t i = tid; i < all; i += THREADS) s.list[i] = list[i];
-  draw_from(a, s, r, row, m, (int)all, 0);
-}
-
-template <typename T>
-__global__ __launch_bounds__(kLimitThreads) void sample_limits_kernel(SampleArgs a) {
-  __shared__ union Lds {
-    Bins bins;
-    List<kLimitThreads> list;
-  } s;
-  const int64_t row = hx::wg_x() / a.chunks2;
-  const int c = hx::wg_x() % a.chunks2;
-  const Row r = row_of(a, row);
-  if (!r.drawn) return;
-  const int begin = min(a.vocab, c * a.chunk2), end = min(a.vocab, begin + a.chunk2);
-  if (small_top_k(a, row)) {
-    pick<T>(a, s.list, r, row, begin, end);
-    return;
-  }
-  fill_bins<T, kLimitThreads>(s.bins, r, static_cast<const T*>(a.logits) + row * a.row_stride, begin, end);
-  for (int b = hx::tid_x(); b < kBins; b += kLimitThreads) {
-    if (!s.bins.count[b]) continue;
-    atomicAdd(&a.count[row * kBins + b], s.bins.count[b]);
-    if (s.bins.mass[b]) atomicAdd(reinterpret_cast<unsigned long long*>(&a.mass[row * kBins + b]), s.bins.mass[b]);
-  }
+  for (uint32_t i = tid; i < min(mine, (uint32_t)kList) && base + i < (uint32_t)kList; i += kRowThreads)
+    __hip_atomic_store(&list[base + i], s.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // ---------------------------------------------------------------------------- the row
-struct RowLds : List<kRowThreads> {
+struct RowLds : List {
   Bins to;  // tokens up to and with a bin, and their weight
   uint32_t digit_count[256];
   unsigned long long digit_mass[256];
@@ -674,15 +644,14 @@ __device__ int gather(const SampleArgs& a, RowLds& s, const Row& r, const void* 
     Piece<T> u[kAhead];  // in flight together
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) u[i] = *reinterpret_cast<const Piece<T>*>(p + min(j0 + i * kRowThreads, whole - 1) * kVec);
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int j = j0 + i * kRowThreads;
+#pragma nounroll
+    for (int j = j0; j < min(whole, j0 + kAhead * kRowThreads); j += kRowThreads) {
       bool any = false;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) any |= within(u[i].get(e));
-      if (!any || j >= whole) continue;
+      for (int e = 0; e < kVec; ++e) any |= within(u[0].get(e));
+      if (any) u[0].each(j * kVec, list);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) list(u[i].get(e), j * kVec + e);
+      for (int i = 0; i + 1 < kAhead; ++i) u[i] = u[i + 1];
     }
   }
   const int v = whole * kVec + hx::tid_x();
@@ -716,7 +685,7 @@ __device__ Found resolve(const SampleArgs& a, RowLds& s, const Row& r, const voi
       s.digit_mass[tid] = 0;
     }
     __syncthreads();
-    each_logit<T, kRowThreads>(row, 0, a.vocab, [&](float l, int v) {
+    each_logit<T>(row, 0, a.vocab, [&](float l, int v) {
       if (bin_of(r, l) != bin) return;
       const uint64_t p = place_of(l, v);
       if (from < 64 && (p >> from) != prefix) return;
@@ -753,30 +722,16 @@ __device__ Found resolve(const SampleArgs& a, RowLds& s, const Row& r, const voi
   return {n, before};
 }
 
+// Draws from a row by its bins: lists the tokens that the limits can keep, if a list holds them; their
+// number. If not, draws, and returns 0.
 template <typename T>
-__global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
-  __shared__ RowLds s;
-  const int64_t row = hx::wg_x();
+__device__ int draw_by_bins(const SampleArgs& a, RowLds& s, const Row& r, int64_t row, const Limits& m, bool picked) {
   const int tid = hx::tid_x();
-  const Row r = row_of(a, row);
-  if (!r.drawn) {
-    // The first token in order; none in a row of -inf alone.
-    if (tid == 0) {
-      const bool any = (uint32_t)(r.best >> 32) > kOrderNegInf;
-      a.token_ids[row] = any ? (int64_t)(uint32_t)~(uint32_t)r.best : -1;
-      if (a.logprobs != nullptr) a.logprobs[row] = any ? 0.f : -INFINITY;
-    }
-    return;
-  }
-  const bool picked = small_top_k(a, row);
-  if (picked && a.listed[2 * row] <= (uint32_t)kList) return;  // drawn already
   const void* const logits = static_cast<const T*>(a.logits) + row * a.row_stride;
-  if (picked) {
-    fill_bins<T, kRowThreads>(s.to, r, logits, 0, a.vocab);
-  } else {
+  if (!picked) {
     for (int b = tid; b < kBins; b += kRowThreads) {
-      s.to.count[b] = a.count[row * kBins + b];
-      s.to.mass[b] = a.mass[row * kBins + b];
+      s.to.count[b] = __hip_atomic_load(&a.count[row * kBins + b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s.to.mass[b] = __hip_atomic_load(&a.mass[row * kBins + b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
   }
@@ -793,7 +748,6 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
     s.to.mass[2 * tid + 1] = m + m0 + m1;
   }
   __syncthreads();
-  const Limits m = limits_of(a, row);
   const uint32_t nk = min(m.k, s.to.count[kBins - 1]);
   const int bin_k = first_from(s.to.count, kBins, nk);
   // No kept token lies in a bin past `last`.
@@ -805,11 +759,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
     last = min(last, x < (float)(kBins - 3) ? max((int)x, 0) + 2 : kBins - 1);
   }
   const int until = m.limited && m.by_p ? bin_k : last;  // the top_k tokens' weight needs all of them
-  if (s.to.count[until] <= (uint32_t)kList) {
-    const int listed = gather<T>(a, s, r, logits, 0, until, [](uint64_t) { return true; });
-    draw_from(a, s, r, row, m, listed, s.to.mass[kBins - 1]);
-    return;
-  }
+  if (s.to.count[until] <= (uint32_t)kList) return gather<T>(a, s, r, logits, 0, until, [](uint64_t) { return true; });
   uint32_t n = nk;
   uint64_t kept = s.to.mass[kBins - 1], of = kept;
   const uint64_t* const cum = s.cum();
@@ -819,36 +769,94 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
       kept = w;
     }
   };
-  if (m.limited) {
-    const Found f = resolve<T>(a, s, r, logits, bin_k, true, nk);
-    kept = of = cum[nk - f.before - 1];
-    __syncthreads();
-  }
-  if (m.by_p) {
+  // The borders of top_k and of top_p, then the drawn token.
+#pragma nounroll
+  for (int step = m.limited ? 0 : m.by_p ? 1 : 2; step < 3; step += step == 0 && !m.by_p ? 2 : 1) {
+    if (step == 2 && m.by_min) {
+      uint64_t count = 0, mass = 0;
+      each_logit<T>(logits, 0, a.vocab, [&](float l, int) {
+        const double e = weight_of(log_weight(r, l));
+        if (e >= m.min_p) {
+          ++count;
+          mass += fixed_of(e);
+        }
+      });
+      count = block_sum(s, count);
+      mass = block_sum(s, mass);
+      fewest(max((uint32_t)count, 1u), mass);
+    }
     const double border = m.p * (double)of;
-    const int bin = min(first_from(s.to.mass, kBins, border), kBins - 1);
-    const uint64_t whole = (uint64_t)border + ((double)(uint64_t)border < border ? 1 : 0);
-    const Found f = resolve<T>(a, s, r, logits, bin, false, whole);
-    const int i = min(first_from(cum, f.n, border), f.n - 1);
-    fewest(f.before + (uint32_t)i + 1, cum[i]);
+    const uint64_t target = step == 0 ? nk : step == 2 ? m.target(kept) : (uint64_t)border + ((double)(uint64_t)border < border ? 1 : 0);
+    const int bin = step == 0 ? bin_k : min(first_from(s.to.mass, kBins, target), kBins - 1);
+    const Found f = resolve<T>(a, s, r, logits, bin, step == 0, target);
+    if (step == 0) {
+      kept = of = cum[nk - f.before - 1];
+    } else {
+      const int i = min(first_from(cum, f.n, target), f.n - 1);
+      if (step == 1) fewest(f.before + (uint32_t)i + 1, cum[i]);
+      else if (tid == 0) answer(a, r, row, s.sorted[i], kept);
+    }
     __syncthreads();
   }
-  if (m.by_min) {
-    uint64_t count = 0, mass = 0;
-    each_logit<T, kRowThreads>(logits, 0, a.vocab, [&](float l, int) {
-      const double e = weight_of(log_weight(r, l));
-      if (e >= m.min_p) {
-        ++count;
-        mass += fixed_of(e);
-      }
-    });
-    count = block_sum(s, count);
-    mass = block_sum(s, mass);
-    fewest(max((uint32_t)count, 1u), mass);
+  return 0;
+}
+
+// Whether this workgroup is the row's last, which draws. What the others gave it went past the caches,
+// each wave waits until it has arrived, and the last one reads it past the caches too: none need be
+// written back or emptied (which took 5 us over 96 rows).
+__device__ __forceinline__ bool count_done(const SampleArgs& a, RowLds& s, int64_t row) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (hx::tid_x() == 0)
+    s.crowd = __hip_atomic_fetch_add(&a.listed[2 * row + 1], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  return s.crowd == (uint32_t)a.chunks2 - 1;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
+  __shared__ RowLds s;
+  const int64_t row = hx::wg_x() / a.chunks2;
+  const int c = hx::wg_x() % a.chunks2, tid = hx::tid_x();
+  const Row r = row_of(a, row);
+  if (!r.drawn) {
+    // The first token in order; none in a row of -inf alone.
+    if (c == 0 && tid == 0) {
+      const bool any = (uint32_t)(r.best >> 32) > kOrderNegInf;
+      a.token_ids[row] = any ? (int64_t)(uint32_t)~(uint32_t)r.best : -1;
+      if (a.logprobs != nullptr) a.logprobs[row] = any ? 0.f : -INFINITY;
+    }
+    return;
   }
-  const uint64_t target = m.target(kept);
-  const Found f = resolve<T>(a, s, r, logits, first_from(s.to.mass, kBins, target), false, target);
-  if (tid == 0) answer(a, r, row, s.sorted[first_from(cum, f.n, target)], kept);
+  const int begin = min(a.vocab, c * a.chunk2), end = min(a.vocab, begin + a.chunk2);
+  const void* const logits = static_cast<const T*>(a.logits) + row * a.row_stride;
+  const bool picked = small_top_k(a, row);
+  uint32_t listed = 0;
+  if (picked) {
+    pick<T>(a, s, r, row, begin, end);
+    if (!count_done(a, s, row)) return;
+    listed = __hip_atomic_load(&a.listed[2 * row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (uint32_t i = tid; i < listed && listed <= (uint32_t)kList; i += kRowThreads)
+      s.list[i] = __hip_atomic_load(&a.mass[row * kBins + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  const bool whole = listed > 0 && listed <= (uint32_t)kList;  // (a small top_k lists a token at least)
+  const Limits m = limits_of(a, row);
+  uint64_t total = 0;
+  if (!whole) {
+    fill_bins<T>(s.to, r, logits, picked ? 0 : begin, picked ? a.vocab : end);
+    if (!picked) {
+      for (int b = tid; b < kBins; b += kRowThreads) {
+        if (!s.to.count[b]) continue;
+        atomicAdd(&a.count[row * kBins + b], s.to.count[b]);
+        if (s.to.mass[b]) atomicAdd(reinterpret_cast<unsigned long long*>(&a.mass[row * kBins + b]), s.to.mass[b]);
+      }
+      if (!count_done(a, s, row)) return;
+    }
+    listed = (uint32_t)draw_by_bins<T>(a, s, r, row, m, picked);
+    if (!listed) return;
+    total = s.to.mass[kBins - 1];
+  }
+  draw_from(a, s, r, row, m, (int)listed, total);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -865,8 +873,7 @@ void cut(int64_t rows, int32_t vocab, int64_t wgs, int32_t* chunks, int32_t* chu
 template <typename T>
 void launch(const SampleArgs& a, int64_t rows, hipStream_t s) {
   hipLaunchKernelGGL(sample_range_kernel<T>, dim3((unsigned)(rows * a.chunks)), dim3(kThreads), 0, s, a);
-  hipLaunchKernelGGL(sample_limits_kernel<T>, dim3((unsigned)(rows * a.chunks2)), dim3(kLimitThreads), 0, s, a);
-  hipLaunchKernelGGL(sample_row_kernel<T>, dim3((unsigned)rows), dim3(kRowThreads), 0, s, a);
+  hipLaunchKernelGGL(sample_row_kernel<T>, dim3((unsigned)(rows * a.chunks2)), dim3(kRowThreads), 0, s, a);
 }
 
 }  // namespace
@@ -908,7 +915,7 @@ extern "C" int hx_sample_tokens(const void* logits, int64_t logits_row_stride, i
   a.most = a.listed + rows * 2;
   a.groups = (int32_t)ceil_div(vocab, kGroup);
   cut(rows, a.vocab, 2048, &a.chunks, &a.chunk);
-  cut(rows, a.vocab, 384, &a.chunks2, &a.chunk2);
+  cut(rows, a.vocab, 256, &a.chunks2, &a.chunk2);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == HX_DTYPE_BF16) launch<__bf16>(a, rows, s);
   else if (dtype == HX_DTYPE_FP16) launch<_Float16>(a, rows, s);
