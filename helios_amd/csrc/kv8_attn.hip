@@ -9,7 +9,7 @@
 // largest element at 2^14: exact for fp16, and for bf16 down to 2^-28 of the largest element
 // (smaller ones within 2^-40 of it). Sums are fp32.
 //
-// Two kernels over a plan's work lists, and one that joins splits:
+// Two kernels over a plan's work lists, in one launch where a tick has both, and one that joins splits:
 //   few_kernel    sequences whose (row, query head) pairs of a KV head fit one MFMA's 16 columns
 //                 (decode rows, a few drafted ones), split over their keys. Bound by HBM: 64
 //                 decoders with 8 KV heads of 128, 306 MB, take 61 us with the join, 5.0 TB/s
@@ -42,8 +42,8 @@ constexpr int kFewMost = 256;     // and at most
 constexpr int kChunkUnits = 128;  // (row, head) pairs of a chunk block
 constexpr int kChunkTile = 64;
 // Workgroups below which row blocks are split, and into about as many. (512 would be on the CUs at
-// once, but partial results cost too: a tick whose blocks are 344 workgroups takes 106 us split for
-// 384, 114 for 512, 127 as it is.)
+// once, but partial results cost too: decoders beside chunks whose blocks are 344 workgroups take 96 us
+// split for 384, 97 for 512, 99 as they are, 105 for 768.)
 constexpr int kChunkWGs = 384;
 constexpr int kChunkLeast = 4;    // tiles of a split, at least
 constexpr int kShortJoin = 4;     // splits that a part of a wave joins; a workgroup does more
@@ -768,15 +768,12 @@ __device__ __forceinline__ void few_item(const RunArgs& a, FewLds<DP>& lds, cons
 }
 
 template <typename T, typename C, int DP>
-__global__ __launch_bounds__(kFewThreads, DP == 256 ? 2 : DP == 128 ? 3 : 4) void kv8_few_kernel(RunArgs a, int n_wg) {
-  __shared__ FewLds<DP> lds;
+__device__ __forceinline__ void few_items(const RunArgs& a, FewLds<DP>& lds, const int4& counts, int wg, int n_wg) {
   // All parts of one head, then of the next: a head's rows are every eighth 128 bytes of memory, say,
   // and what one head's reads bring along of its neighbours' is there when theirs come. (Heads side
   // by side: 3.9 to 5.4 TB/s of loads alone; this way 5.8 to 6.4.)
-  int4 counts;
-  if (!plan_ok(a, &counts)) return;
   const int64_t work = (int64_t)counts.x * a.s.hkv * a.z.head_blocks;
-  for (int64_t i = hx::wg_x(); i < work; i += n_wg) {
+  for (int64_t i = wg; i < work; i += n_wg) {
     const int sub = (int)((uint32_t)i / (uint32_t)counts.x), part = (int)((uint32_t)i - (uint32_t)sub * (uint32_t)counts.x);
     const int hb = sub / a.s.hkv, h = sub - hb * a.s.hkv;
     int4 e0 = uniform4(a.part + 3 * part + 1), e1 = uniform4(a.part + 3 * part + 2);
@@ -794,10 +791,29 @@ __global__ __launch_bounds__(kFewThreads, DP == 256 ? 2 : DP == 128 ? 3 : 4) voi
   }
 }
 
+template <typename T, typename C, int DP>
+__global__ __launch_bounds__(kFewThreads, DP == 256 ? 2 : DP == 128 ? 3 : 4) void kv8_few_kernel(RunArgs a, int n_wg) {
+  __shared__ FewLds<DP> lds;
+  int4 counts;
+  if (plan_ok(a, &counts)) few_items<T, C, DP>(a, lds, counts, hx::wg_x(), n_wg);
+}
+
 // ------------------------------------------------------------------------------- chunks
 constexpr int chunk_threads(int dp) { return dp == 256 ? 512 : 256; }
 constexpr float kChunkShift = 7.f;  // 2^7 times weights of up to 2^8 fits fp16
 constexpr float kLazy = 8.f;        // the reference maximum moves when exceeded by this, in log2
+
+// Rows of fp16 with 16 and 32 bytes more: 16 keys' fragments, and the 8 rows of 32 bytes that half a
+// wave reads transposed, then cover all banks once.
+constexpr int chunk_k_row(int dp) { return 2 * dp + 16; }
+constexpr int chunk_v_row(int dp) { return 2 * dp + 32; }
+
+template <int DP>
+struct ChunkLds {
+  __attribute__((aligned(16))) uint8_t k[2][kChunkTile * chunk_k_row(DP)], v[2][kChunkTile * chunk_v_row(DP)];
+  __attribute__((aligned(16))) float k_scale[2][kChunkTile], v_log[2][kChunkTile], v_inverse[2][kChunkTile];
+  uint32_t top[chunk_threads(DP) / 64];
+};
 
 // One item and KV head to a workgroup: wave w owns units 16 RB w .. + 16 RB - 1, (row, head) pairs
 // with the group's heads fastest. 64-key tiles of K and V go from HBM through registers, where the
@@ -809,7 +825,7 @@ constexpr float kLazy = 8.f;        // the reference maximum moves when exceeded
 // The weights go into P V as one fp16 (11 bits, an eighth of a bf16 output's rounding), or with
 // fp16 outputs as two.
 template <typename T, typename C, int DP>
-__global__ __launch_bounds__(chunk_threads(DP), 2) void kv8_chunk_kernel(RunArgs a, int n_wg) {
+__device__ __forceinline__ void chunk_items(const RunArgs& a, ChunkLds<DP>& lds, const int4& counts, int wg, int n_wg) {
   typedef hx::f16x8_t v8;
   typedef hx::Elem<_Float16> E;
   constexpr bool kTwo = __is_same(T, _Float16);
@@ -817,22 +833,14 @@ __global__ __launch_bounds__(chunk_threads(DP), 2) void kv8_chunk_kernel(RunArgs
   constexpr int kThreads = chunk_threads(DP), kWaves = kThreads / 64;
   constexpr int kAhead = 2;  // operands of V read before the softmax, and ahead of their products
   constexpr int kMine = 8 * DP / kThreads;  // 16-byte pieces of codes that a thread moves
-  // Rows of fp16 with 16 and 32 bytes more: 16 keys' fragments, and the 8 rows of 32 bytes that half a
-  // wave reads transposed, then cover all banks once.
-  constexpr int kKRow = 2 * DP + 16, kVRow = 2 * DP + 32;
-  __shared__ __attribute__((aligned(16))) uint8_t s_k[2][kChunkTile * kKRow];
-  __shared__ __attribute__((aligned(16))) uint8_t s_v[2][kChunkTile * kVRow];
-  __shared__ __attribute__((aligned(16))) float s_ks[2][kChunkTile], s_lv[2][kChunkTile], s_iv[2][kChunkTile];
-  __shared__ uint32_t s_top[kWaves];
+  constexpr int kKRow = chunk_k_row(DP), kVRow = chunk_v_row(DP);
   const int tid = hx::tid_x(), lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int4 counts;
-  if (!plan_ok(a, &counts)) return;
   const int D = a.s.head_dim, page = a.s.page, G = a.z.group;
   const int64_t work = (int64_t)counts.y * a.s.hkv;
   const uint32_t row_bytes = (uint32_t)a.s.hkv * (uint32_t)D;
 
-  for (int64_t i = hx::wg_x(); i < work; i += n_wg) {
+  for (int64_t i = wg; i < work; i += n_wg) {
     const int item = (int)((uint32_t)i / (uint32_t)a.s.hkv), h = (int)((uint32_t)i % (uint32_t)a.s.hkv);
     const int4 it = uniform4(a.chunk + 2 * (int64_t)item), si = uniform4(a.chunk + 2 * (int64_t)item + 1);
     const int row0 = it.y, t_begin = it.z, t_end = it.w, n = si.y, L = si.z;
@@ -868,10 +876,10 @@ __global__ __launch_bounds__(chunk_threads(DP), 2) void kv8_chunk_kernel(RunArgs
       }
       // One power of two for all units.
       for (int m = 1; m < 64; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m));
-      if (lane == 0) s_top[w] = top;
+      if (lane == 0) lds.top[w] = top;
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < kWaves; ++e) top = max(top, s_top[e]);
+      for (int e = 0; e < kWaves; ++e) top = max(top, lds.top[e]);
       top = magnitude<T>((uint32_t)__builtin_amdgcn_readfirstlane((int)top));
       const float up = fit_up(top);
 #pragma unroll
@@ -949,16 +957,16 @@ __global__ __launch_bounds__(chunk_threads(DP), 2) void kv8_chunk_kernel(RunArgs
         const int r = p / kPieces, c = p % kPieces;
         const uint2 x0 = hx8::to_f16<C>(reg[e].x), x1 = hx8::to_f16<C>(reg[e].y), x2 = hx8::to_f16<C>(reg[e].z),
                     x3 = hx8::to_f16<C>(reg[e].w);
-        uint8_t* const to = (of_v ? s_v[b] + r * kVRow : s_k[b] + r * kKRow) + 32 * c;
+        uint8_t* const to = (of_v ? lds.v[b] + r * kVRow : lds.k[b] + r * kKRow) + 32 * c;
         *reinterpret_cast<uint4*>(to) = make_uint4(x0.x, x0.y, x1.x, x1.y);
         *reinterpret_cast<uint4*>(to + 16) = make_uint4(x2.x, x2.y, x3.x, x3.y);
       }
       if (w == 0) {
-        s_ks[b][lane] = lane < cnt ? sreg * qc : 0.f;
+        lds.k_scale[b][lane] = lane < cnt ? sreg * qc : 0.f;
       } else if (w == 1) {
         const ValueScale v = value_scale(lane < cnt ? sreg : 1.f);
-        s_lv[b][lane] = v.log;
-        s_iv[b][lane] = v.inverse;
+        lds.v_log[b][lane] = v.log;
+        lds.v_inverse[b][lane] = v.inverse;
       }
     };
 
@@ -991,8 +999,8 @@ __global__ __launch_bounds__(chunk_threads(DP), 2) void kv8_chunk_kernel(RunArgs
       }
       if (key0 > any_hi || key0 + kChunkTile - 1 < any_lo) continue;
 
-      const uint8_t* const kp = s_k[b] + lr * kKRow + 16 * lg;
-      const uint8_t* const vp = s_v[b] + (4 * lg + (lr >> 2)) * kVRow + 16 * ((lr >> 1) & 1) + 8 * (lr & 1);
+      const uint8_t* const kp = lds.k[b] + lr * kKRow + 16 * lg;
+      const uint8_t* const vp = lds.v[b] + (4 * lg + (lr >> 2)) * kVRow + 16 * ((lr >> 1) & 1) + 8 * (lr & 1);
       hx::f32x4_t sc[4][RB];
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
@@ -1018,8 +1026,8 @@ __global__ __launch_bounds__(chunk_threads(DP), 2) void kv8_chunk_kernel(RunArgs
       // Lane: keys 16 kb + 4 lg + e of its units.
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) {
-        const float4 ks = *reinterpret_cast<const float4*>(&s_ks[b][16 * kb + 4 * lg]);
-        const float4 lv = *reinterpret_cast<const float4*>(&s_lv[b][16 * kb + 4 * lg]);
+        const float4 ks = *reinterpret_cast<const float4*>(&lds.k_scale[b][16 * kb + 4 * lg]);
+        const float4 lv = *reinterpret_cast<const float4*>(&lds.v_log[b][16 * kb + 4 * lg]);
         const float k4[4] = {ks.x, ks.y, ks.z, ks.w}, l4[4] = {lv.x, lv.y, lv.z, lv.w};
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
@@ -1069,7 +1077,7 @@ __global__ __launch_bounds__(chunk_threads(DP), 2) void kv8_chunk_kernel(RunArgs
         float sum = 0.f;
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
-          const float4 iv = *reinterpret_cast<const float4*>(&s_iv[b][16 * kb + 4 * lg]);
+          const float4 iv = *reinterpret_cast<const float4*>(&lds.v_inverse[b][16 * kb + 4 * lg]);
           const float i4[4] = {iv.x, iv.y, iv.z, iv.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -1135,6 +1143,30 @@ __global__ __launch_bounds__(chunk_threads(DP), 2) void kv8_chunk_kernel(RunArgs
     }
     __syncthreads();  // every wave is done with the last tile before the next item's first is stored
   }
+}
+
+template <typename T, typename C, int DP>
+__global__ __launch_bounds__(chunk_threads(DP), 2) void kv8_chunk_kernel(RunArgs a, int n_wg) {
+  __shared__ ChunkLds<DP> lds;
+  int4 counts;
+  if (plan_ok(a, &counts)) chunk_items<T, C, DP>(a, lds, counts, hx::wg_x(), n_wg);
+}
+
+// A tick of both: its few rows' reads go beside the chunks' products, up to 128 dims (where both take
+// 4 waves). 32 decoders and two chunks: 96 us, 107 in two launches, of 31 and 68.
+template <typename T, typename C, int DP>
+__global__ __launch_bounds__(kFewThreads, 2) void kv8_both_kernel(RunArgs a, int n_chunk, int n_few) {
+  static_assert(chunk_threads(DP) == kFewThreads);
+  __shared__ union Lds {
+    FewLds<DP> few;
+    ChunkLds<DP> chunk;
+    __device__ Lds() {}
+  } lds;
+  int4 counts;
+  if (!plan_ok(a, &counts)) return;
+  const int wg = hx::wg_x();
+  if (wg < n_chunk) chunk_items<T, C, DP>(a, lds.chunk, counts, wg, n_chunk);
+  else few_items<T, C, DP>(a, lds.few, counts, wg - n_chunk, n_few);
 }
 
 // -------------------------------------------------------------------------------- join
@@ -1266,16 +1298,16 @@ struct Run {
 template <typename T, typename C, int DP>
 void launch_run(const Run& r, bool few, bool chunk) {
   const RunArgs& a = r.a;
-  if (few) {
-    const int64_t most = r.l.most_parts * a.s.hkv * a.z.head_blocks;
-    const int n = (int)(most < 65536 ? most : 65536);
-    hipLaunchKernelGGL((kv8_few_kernel<T, C, DP>), dim3(n), dim3(kFewThreads), 0, r.s, a, n);
+  const int64_t most_few = r.l.most_parts * a.s.hkv * a.z.head_blocks, most_chunk = r.l.most_chunk * a.s.hkv;
+  const int n_few = (int)(most_few < 65536 ? most_few : 65536), n_chunk = (int)(most_chunk < 8192 ? most_chunk : 8192);
+  if constexpr (chunk_threads(DP) == kFewThreads) {
+    if (few && chunk) {
+      hipLaunchKernelGGL((kv8_both_kernel<T, C, DP>), dim3(n_chunk + n_few), dim3(kFewThreads), 0, r.s, a, n_chunk, n_few);
+      return;
+    }
   }
-  if (chunk) {
-    const int64_t most = r.l.most_chunk * a.s.hkv;
-    const int n = (int)(most < 8192 ? most : 8192);
-    hipLaunchKernelGGL((kv8_chunk_kernel<T, C, DP>), dim3(n), dim3(chunk_threads(DP)), 0, r.s, a, n);
-  }
+  if (few) hipLaunchKernelGGL((kv8_few_kernel<T, C, DP>), dim3(n_few), dim3(kFewThreads), 0, r.s, a, n_few);
+  if (chunk) hipLaunchKernelGGL((kv8_chunk_kernel<T, C, DP>), dim3(n_chunk), dim3(chunk_threads(DP)), 0, r.s, a, n_chunk);
 }
 
 template <typename T, typename C>
