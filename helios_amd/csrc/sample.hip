@@ -55,7 +55,7 @@ struct SampleArgs {
   const float* min_p;
   int64_t* token_ids;
   float* logprobs;
-  uint64_t* best;   // [rows][chunks]: the first token in order
+  uint64_t* best;   // [rows][chunks]: the largest logit's order, and ~ of the first 16 bytes' token that hold it
   uint32_t* least;  // [rows][chunks]: the smallest finite logit's order
   uint32_t* count;  // [rows][kBins]
   uint64_t* mass;   // [rows][kBins]; or [rows][kList], the listed tokens of a row of a small top_k
@@ -85,6 +85,15 @@ struct __attribute__((packed, aligned(sizeof(T)))) Piece {
   __device__ __forceinline__ float get(int e) const {
     if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
     else return Logit<T>::get(w[e / 2], e & 1);
+  }
+  // No infinity or NaN: no exponent of ones, which one more would carry out of.
+  __device__ __forceinline__ bool finite() const {
+    constexpr uint32_t kExp = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, _Float16) ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t kOne = sizeof(T) == 4 ? 0x00800000u : __is_same(T, _Float16) ? 0x04000400u : 0x00800080u;
+    uint32_t carry = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) carry |= (w[i] & kExp) + kOne;
+    return (carry & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u)) == 0;
   }
   // f(logit, index from `at`) for each.
   template <typename F>
@@ -166,10 +175,12 @@ __global__ __launch_bounds__(kThreads) void sample_range_kernel(SampleArgs a) {
   }
   if (c == 0 && tid < 2) a.listed[2 * row + tid] = 0;
   constexpr int kVec = Logit<T>::kVec, kLanes = kGroup / kVec, kAhead = 4;
-  uint32_t top = 0, at = 0xffffffffu, low = 0xffffffffu;
+  uint32_t top = 0, at = 0;
+  float least = INFINITY;
   const int begin = min(a.vocab, c * a.chunk), end = min(a.vocab, begin + a.chunk);
   const T* const p = static_cast<const T*>(a.logits) + row * a.row_stride;
-  // Chunks begin with a group, and every thread of a group takes each turn.
+  // Chunks begin with a group, and every thread of a group takes each turn. Finite pieces, most of all,
+  // take a maximum and a minimum an element.
   for (int v0 = begin; v0 < end; v0 += kAhead * kThreads * kVec) {
     Piece<T> u[kAhead];
 #pragma unroll
@@ -181,24 +192,32 @@ __global__ __launch_bounds__(kThreads) void sample_range_kernel(SampleArgs a) {
     for (int i = 0; i < kAhead; ++i) {
       const int v = v0 + (i * kThreads + tid) * kVec;
       uint32_t here = 0;
-      auto take = [&](float l, int v) __attribute__((always_inline)) {
-        const uint32_t o = order_of(l);
-        // Tokens come in rising order to a thread: the first of equal ones stays.
-        at = o > top ? (uint32_t)v : at;
-        top = o > top ? o : top;
-        low = o > kOrderNegInf && o < low ? o : low;
-        here = max(here, o);
-      };
-      if (v + kVec <= end) {
+      if (v + kVec <= end && u[i].finite()) {
+        float most = u[i].get(0), fewest = most;
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) take(u[i].get(e), v + e);
+        for (int e = 1; e < kVec; ++e) {
+          most = fmaxf(most, u[i].get(e));
+          fewest = fminf(fewest, u[i].get(e));
+        }
+        here = order_of(most);
+        least = fminf(least, fewest);
       } else {
-        for (int e = v; e < end; ++e) take((float)p[e], e);
+#pragma nounroll
+        for (int e = v; e < min(v + kVec, end); ++e) {
+          const float l = (float)p[e];
+          const uint32_t o = order_of(l);
+          here = max(here, o);
+          least = o > kOrderNegInf && o < kOrderInf ? fminf(least, l) : least;
+        }
       }
+      // Pieces come in rising order to a thread: the first of equal ones stays.
+      at = here > top ? (uint32_t)v : at;
+      top = max(top, here);
       here = max_of_lanes<kLanes>(here);
       if (tid % kLanes == 0 && v < end) a.most[row * a.groups + v / kGroup] = here;
     }
   }
+  uint32_t low = order_of(least);
   uint64_t best = (uint64_t)top << 32 | (uint32_t)~at;
   for (int m = 1; m < 64; m <<= 1) {
     best = max_u64(best, shfl_xor_u64(best, m));
@@ -221,7 +240,7 @@ __global__ __launch_bounds__(kThreads) void sample_range_kernel(SampleArgs a) {
 
 // ----------------------------------------------------------------------- a row's measures
 struct Row {
-  uint64_t best;    // the first token in order
+  uint64_t best;    // the largest logit's order, and ~ of the first piece's token that holds it
   float top;        // its logit
   bool drawn;       // a temperature, and a finite largest logit
   bool cut;         // the last bin's weights are all 0
@@ -822,8 +841,12 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
   if (!r.drawn) {
     // The first token in order; none in a row of -inf alone.
     if (c == 0 && tid == 0) {
-      const bool any = (uint32_t)(r.best >> 32) > kOrderNegInf;
-      a.token_ids[row] = any ? (int64_t)(uint32_t)~(uint32_t)r.best : -1;
+      const uint32_t order = (uint32_t)(r.best >> 32);
+      const bool any = order > kOrderNegInf;
+      const T* const p = static_cast<const T*>(a.logits) + row * a.row_stride;
+      int v = (int)~(uint32_t)r.best;
+      while (any && v < a.vocab - 1 && order_of((float)p[v]) != order) ++v;
+      a.token_ids[row] = any ? v : -1;
       if (a.logprobs != nullptr) a.logprobs[row] = any ? 0.f : -INFINITY;
     }
     return;
