@@ -9,8 +9,10 @@
 // [pages, kv_heads, page_size], so that attention to one head reads consecutive ones (beside the
 // codes' order a head's 4 of every 32 bytes would be read 8 times over).
 //
-// The norm and rotation are those of the 16-bit append (layers.py:30-40, :54-72), in fp32 from
-// the projections on, rounded once: to the codes, or to the queries' type.
+// The norm and rotation are those of the 16-bit append (layers.py:30-40, :54-72), rounded once: to the
+// queries' type, in fp32 from the projections on, or to the keys' codes and scales, in fp64 (fp32 keys
+// next to a border between codes fall to either side of it: 2 in 10^6, which costs 5e-5 of a tensor's
+// norm; fp64 8 % of the launch).
 
 #include "kv8_common.h"
 
@@ -83,9 +85,9 @@ __device__ __forceinline__ X over_lanes(X x, F f) {
 
 // A head row to LANES lanes, 8 elements each (lanes past head_dim idle along); a workgroup takes
 // kThreads / LANES of them, a token's query, key and value heads in turn. 2381 tokens of 32 + 8 + 8
-// heads of 128, with norms and rotation: 17.3 us, 3.3 TB/s, 11.7 without the rotation, whose weights,
+// heads of 128, with norms and rotation: 18.5 us, 3.0 TB/s, 11.7 without the rotation, whose weights,
 // cosines and sines are 6 times a row's own bytes, from L2, and whose sum and turn are chains across
-// lanes. (Two heads to a lane, which then share the cosines: 16.3, but 64 tokens 4.7 instead of 3.6.)
+// lanes. (Two heads to a lane, which then share the cosines, won 6 % there and lost 30 % at 64 tokens.)
 // Few tokens are a launch's latency.
 template <typename T, typename C, int LANES, bool ROPE, bool VEC>
 __global__ __launch_bounds__(kThreads) void kv8_write_kernel(WriteArgs a) {
@@ -112,12 +114,24 @@ __global__ __launch_bounds__(kThreads) void kv8_write_kernel(WriteArgs a) {
   if (mine)
     load8<T, VEC>(is_q ? a.q + row * a.q_row + hh * a.q_head + d
                        : which ? a.v + row * a.v_row + hh * a.v_head + d : a.k + row * a.k_row + hh * a.k_head + d, x);
+  auto store_row = [&](uint32_t lo, uint32_t hi, bool finite, float scale) __attribute__((always_inline)) {
+    if (mine) hx::st8_nt(a.codes[which] + (slot * a.hkv + hh) * a.head_dim + d, finite ? lo : 0u, finite ? hi : 0u);
+    if (lane == 0) {
+      const int64_t page = (slot >> 32) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)a.page) : slot / a.page;
+      reinterpret_cast<uint32_t*>(a.scales[which])[(page * a.hkv + hh) * a.page + (slot - page * a.page)] =
+          finite ? __float_as_uint(scale) : 0x7fc00000u;
+    }
+  };
   if (ROPE && (is_q || !which)) {
     int64_t pos = a.positions[row];
     pos = pos < 0 ? 0 : pos >= a.rope_rows ? a.rope_rows - 1 : pos;
+    const float* const norm = is_q ? a.q_norm : a.k_norm;
+    const int half = a.head_dim / 16;  // lanes of half a head row
+    const bool low = lane < half;
+    const int turn = low ? half : -half, other = (hx::tid_x() & 63) + turn;
     float w[8], c[8], s[8];
     if (mine) {
-      load8((is_q ? a.q_norm : a.k_norm) + d, w);
+      load8(norm + d, w);
       load8(a.cos + pos * a.head_dim + d, c);
       load8(a.sin + pos * a.head_dim + d, s);
     }
@@ -126,9 +140,37 @@ __global__ __launch_bounds__(kThreads) void kv8_write_kernel(WriteArgs a) {
     for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
     ss = over_lanes<LANES>(ss, [](float p, float q) { return p + q; });
     const float r = rsqrtf(ss / (float)a.head_dim + a.eps);
-    const int half = a.head_dim / 16;  // lanes of half a head row
-    const bool low = lane < half;
-    const int other = (hx::tid_x() & 63) + (low ? half : -half);
+    if (!is_q) {
+      // A key's codes follow from its elements' ratios to the largest, which r leaves as they are: those
+      // are taken in fp64, and an element next to a border between codes gets the code of its value.
+      float v[8];
+      if (mine) load8(norm + d + 8 * turn, v);
+      double z[8];
+      uint64_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float p = __shfl(x[e], other);
+        z[e] = mine ? fma((double)x[e] * w[e], (double)c[e], (double)(low ? -p : p) * v[e] * (double)s[e]) : 0.;
+        const uint64_t b = __builtin_bit_cast(uint64_t, z[e]) & 0x7fffffffffffffffull;
+        top = b > top ? b : top;
+      }
+#pragma unroll
+      for (int m = 1; m < LANES; m <<= 1) {
+        const uint64_t b = (uint64_t)(uint32_t)__shfl_xor((int)(uint32_t)top, m) |
+                           (uint64_t)(uint32_t)__shfl_xor((int)(top >> 32), m) << 32;
+        top = b > top ? b : top;
+      }
+      const double most = (double)r * __builtin_bit_cast(double, top);
+      const bool finite = top < 0x7ff0000000000000ull && (hx::raw_bits((float)most) & 0x7fffffffu) < 0x7f800000u;
+      const double scale = fmax(most * (1. / C::kMost), (double)hx8::kLeastScale);
+      const double by = (double)r / scale;
+      uint32_t code[2];
+#pragma unroll
+      for (int e = 0; e < 8; e += 4)
+        code[e / 4] = hx8::encode4<C>((float)(z[e] * by), (float)(z[e + 1] * by), (float)(z[e + 2] * by), (float)(z[e + 3] * by));
+      store_row(code[0], code[1], finite, (float)scale);
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = x[e] * r * (mine ? w[e] : 0.f);
 #pragma unroll
@@ -172,13 +214,7 @@ __global__ __launch_bounds__(kThreads) void kv8_write_kernel(WriteArgs a) {
   uint32_t code[2];
 #pragma unroll
   for (int e = 0; e < 8; e += 4) code[e / 4] = hx8::encode4<C>(x[e], x[e + 1], x[e + 2], x[e + 3]);
-  if (mine)
-    hx::st8_nt(a.codes[which] + (slot * a.hkv + hh) * a.head_dim + d, finite ? code[0] : 0u, finite ? code[1] : 0u);
-  if (lane == 0) {
-    const int64_t page = (slot >> 32) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)a.page) : slot / a.page;
-    reinterpret_cast<uint32_t*>(a.scales[which])[(page * a.hkv + hh) * a.page + (slot - page * a.page)] =
-        finite ? __float_as_uint(scale) : 0x7fc00000u;
-  }
+  store_row(code[0], code[1], finite, scale);
 }
 
 // ------------------------------------------------------------------------------ read

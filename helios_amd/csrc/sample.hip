@@ -23,8 +23,8 @@
 //          A row's last workgroup orders the list and draws, or finds the bins where the limits and
 //          the drawn position fall, gathers their tokens and orders those.
 // Bound by reading the logits from HBM, once (what is read again is in the last-level cache), and by
-// the last workgroups' chain of steps. 96 rows of 151936 fp32 logits, top_k about 1000: 43 us, of
-// which the first launch is 12; one bf16 row of them, top_k about 50: 19. (By the bins, in three
+// the last workgroups' chain of steps. 96 rows of 151936 fp32 logits, top_k about 1000: 41 us, of
+// which the first launch is 12; one bf16 row of them, top_k about 50: 18. (By the bins, in three
 // launches: 115 and 31.) 96 rows without a top_k: 75 to 130 us, of which the fp64 weights of all
 // tokens are 34 and each of the last workgroups' passes over its row 15.
 

@@ -876,9 +876,9 @@ def kv8_norm_rope_append(
 ) -> torch.Tensor:
     """``qk_norm_rope_append`` into an 8-bit cache, at any head_dim it holds: RMSNorm and position
     rotation of queries and keys, and the quantised append, in one launch. Returns the
-    normalised, rotated queries (``out`` if given). In fp32 and rounded once, to the queries'
-    dtype or to the codes (``qk_norm_rope_append`` rounds between the norm and the rotation, as
-    its reference does). Arguments as there, ``write_slots`` as for ``kv8_append``."""
+    normalised, rotated queries (``out`` if given), in fp32 and rounded once
+    (``qk_norm_rope_append`` rounds between the norm and the rotation, as its reference does).
+    Keys go on in fp64 until their scales and codes are rounded. Arguments as there, ``write_slots`` as for ``kv8_append``."""
     device = _gpu_of((queries, keys, values, q_norm_weight, k_norm_weight, cos, sin, positions, *cache, write_slots))
     code, pages, page_size, n_kv, head_dim = _check_kv8(cache)
     dtype = _check_kv8_rows(keys, values, write_slots, n_kv, head_dim)

@@ -152,6 +152,30 @@ def _tables(rows, d):
     return torch.cos(angle).float(), torch.sin(angle).float()
 
 
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("hkv,d,rows", [(4, 128, 300), (1, 256, 129), (3, 80, 65), (2, 16, 7)])
+def test_rotated_keys_have_the_codes_of_their_values(device, hkv, d, rows, code):
+    """Bit for bit those of 64 bits: both round ratios of at most 2^9 to fp32 and then to the code, from
+    values within 2^-50 of themselves, so that of the 2^17 elements here one differs with less than
+    2^17 * 2^-50 * 2^25 = 2^-8. A scale is the fp32 root of the squares' mean times one rounding."""
+    say("kv8 rotated keys' codes", hkv, d, rows, code)
+    g = torch.Generator().manual_seed(d + rows)
+    k = torch.randn(rows, hkv, d, generator=g).to(torch.bfloat16)
+    w = 1 + 0.3 * torch.randn(d, generator=g)
+    cos, sin = _tables(500, d)
+    pos = torch.randint(0, 500, (rows,), generator=g)
+    cache = _cache(-(-rows // 64), 64, hkv, d, code, device)
+    ops.kv8_norm_rope_append(*(t.to(device) for t in (k, k, k, w, w, cos, sin, pos)), cache,
+                             torch.arange(rows, device=device), 1e-6)
+    want = oracle.rotate(k, w, cos, sin, pos, 1e-6)
+    scale = want.abs().amax(dim=-1) / oracle.MOST[code]
+    ratio = (want / scale[..., None]).float()
+    codes = (ratio.round() if code == torch.int8 else ratio).to(code)
+    assert torch.equal(_u8(cache.keys.cpu().flatten(0, 1))[:rows], _u8(codes))
+    got = cache.key_scales.cpu().transpose(1, 2).flatten(0, 1)[:rows].double()
+    assert ((got - scale).abs() <= (d / 16 + 8) * 2.0 ** -24 * scale).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("code", CODES)
 @pytest.mark.parametrize("hq,hkv,d,rows", [(32, 8, 128, 65), (16, 4, 64, 7), (5, 1, 16, 1), (12, 4, 96, 40), (4, 2, 256, 20),
