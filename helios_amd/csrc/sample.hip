@@ -646,10 +646,10 @@ __device__ int gather(const SampleArgs& a, RowLds& s, const Row& r, const void* 
   __syncthreads();
   if (hx::tid_x() == 0) s.listed = 0;
   __syncthreads();
-  // (An x that is infinite, or NaN from an infinite distance and bins of no width, is in no bin.)
+  // (An infinite x, or NaN from an infinite distance and bins of no width, becomes 3.4e38: in no bin.)
   const float from = (float)first, to = last < kBins - 1 ? (float)(last + 1) : r.cut ? (float)(kBins - 1) : 3.4e38f;
   auto within = [&](float l) __attribute__((always_inline)) {
-    const float x = (r.top - l) * r.per_bin;
+    const float x = fminf((r.top - l) * r.per_bin, 3.4e38f);
     return x >= from && x < to;
   };
   auto list = [&](float l, int v) __attribute__((always_inline)) {
