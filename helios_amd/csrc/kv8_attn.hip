@@ -17,8 +17,7 @@
 //   chunk_kernel  the others: blocks of rows over 64-key tiles, split over their tiles where the
 //                 blocks alone leave CUs without work. Bound by MFMA, the reads of its operands from
 //                 LDS and the softmax, which overlap only in part: 4096 rows that see 4096 keys and
-//                 their own, 32 heads of 128, take 490 us, 840 TFLOP/s, the matrix units busy for
-//                 36 % of the time (454 without the exponentials).
+//                 their own, 32 heads of 128, take 588 us, 700 TFLOP/s.
 
 #include "kv8_common.h"
 
@@ -822,13 +821,12 @@ struct ChunkLds {
 // Up to 128 dims a workgroup is 4 waves, and the two on a CU are out of step: one's products run
 // under the other's softmax. 8 waves with 256 units halve the staging but wait in step: 1 % faster
 // on a long prompt, 11 % slower on a tick of chunks, whose blocks and splits are then twice as large.
-// The weights go into P V as one fp16 (11 bits, an eighth of a bf16 output's rounding), or with
-// fp16 outputs as two.
+// The weights go into P V as two fp16, 22 bits, as those of few rows do: one alone (11 bits) turns the
+// rounding of one bf16 output in ten, and takes 488 us for 588 on the prompt.
 template <typename T, typename C, int DP>
 __device__ __forceinline__ void chunk_items(const RunArgs& a, ChunkLds<DP>& lds, const int4& counts, int wg, int n_wg) {
   typedef hx::f16x8_t v8;
   typedef hx::Elem<_Float16> E;
-  constexpr bool kTwo = __is_same(T, _Float16);
   constexpr int RB = DP == 256 ? 1 : 2, kSteps = DP / 32, kDims = DP / 16, kPieces = DP / 16;
   constexpr int kThreads = chunk_threads(DP), kWaves = kThreads / 64;
   constexpr int kAhead = 2;  // operands of V read before the softmax, and ahead of their products
@@ -1093,12 +1091,11 @@ __device__ __forceinline__ void chunk_items(const RunArgs& a, ChunkLds<DP>& lds,
           const uint32_t p[4] = {hx::pack2_round<_Float16>(x[0], x[1]), hx::pack2_round<_Float16>(x[2], x[3]),
                                  hx::pack2_round<_Float16>(y[0], y[1]), hx::pack2_round<_Float16>(y[2], y[3])};
           pf[ks][rb] = hx::as_v8<_Float16>(make_uint4(p[0], p[1], p[2], p[3]));
-          if constexpr (kTwo)
-            pf2[ks][rb] = hx::as_v8<_Float16>(
-                make_uint4(hx::pack2_round<_Float16>(x[0] - E::lo(p[0]), x[1] - E::hi(p[0])),
-                           hx::pack2_round<_Float16>(x[2] - E::lo(p[1]), x[3] - E::hi(p[1])),
-                           hx::pack2_round<_Float16>(y[0] - E::lo(p[2]), y[1] - E::hi(p[2])),
-                           hx::pack2_round<_Float16>(y[2] - E::lo(p[3]), y[3] - E::hi(p[3]))));
+          pf2[ks][rb] = hx::as_v8<_Float16>(
+              make_uint4(hx::pack2_round<_Float16>(x[0] - E::lo(p[0]), x[1] - E::hi(p[0])),
+                         hx::pack2_round<_Float16>(x[2] - E::lo(p[1]), x[3] - E::hi(p[1])),
+                         hx::pack2_round<_Float16>(y[0] - E::lo(p[2]), y[1] - E::hi(p[2])),
+                         hx::pack2_round<_Float16>(y[2] - E::lo(p[3]), y[3] - E::hi(p[3]))));
         }
       }
       // O^T += V^T P^T
@@ -1112,7 +1109,7 @@ __device__ __forceinline__ void chunk_items(const RunArgs& a, ChunkLds<DP>& lds,
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) {
             o[d][rb] = E::mfma16x16x32(vv, pf[ks][rb], o[d][rb]);
-            if constexpr (kTwo) o[d][rb] = E::mfma16x16x32(vv, pf2[ks][rb], o[d][rb]);
+            o[d][rb] = E::mfma16x16x32(vv, pf2[ks][rb], o[d][rb]);
           }
         }
     }

@@ -1,0 +1,74 @@
+"""Attention over the 8-bit cache where single roundings show: weights that differ by half an fp16 step."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from helios_amd import ops
+from oracle import kv8 as oracle
+from tests.gpu_cases import say
+from tests.test_gpu_kv8 import CODES, DTYPES, HALF, _attend, _pool, _u8
+
+pytestmark = pytest.mark.gpu
+
+
+def _close(got, q, cache, table, cu, used, window, scale=None):
+    """One rounding of the output, whatever the rows' kind and type: weights within 2^-22 of themselves
+    (two fp16, each off by half a step, 2^-11; 2^-20 allowed), of scores whose fp32 sums of d products
+    and exponents are off by e, in the quotient's numerator and denominator; and 2^-31 of the largest
+    weight for each key, twice what fp16 loses below its smallest step."""
+    d = q.shape[2]
+    keys, vals = oracle.values(cache.keys, cache.key_scales), oracle.values(cache.values, cache.value_scales)
+    want, mag, reach, peak = oracle.attention(q, keys, vals, table, cu, used, window, scale or d ** -0.5)
+    e = (d / 2 + 16) * 2.0 ** -24 * reach + 2.0 ** -18
+    tol = HALF[q.dtype] * want.abs() + (2.0 ** -20 + 2 * e) * mag + int(used.max()) * 2.0 ** -31 * peak + 2.0 ** -25
+    off = (got.double().cpu() - want).abs()
+    bad = ~(off <= tol)
+    assert not bad.any(), (float((off / tol).max()), bad.nonzero()[:5].tolist())
+
+
+def _lengths(seqs):
+    cu = torch.tensor([0] + [n for _, n in seqs]).cumsum(0).to(torch.int32)
+    return cu, torch.tensor([c + n for c, n in seqs], dtype=torch.int32)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("rows", [1, 3, 50])
+def test_weights_half_a_step_apart(device, rows, code, dtype):
+    """Values that cancel but for weights of 1 and 2043.5 / 2048, which 11 bits take to a neighbour: 2^-12
+    of a value of 100, an eighth of what is left."""
+    say("kv8 weights half a step apart", rows, code, dtype)
+    n, d = 200 + rows, 64
+    cache, table = _pool([n], 256, 1, d, code, seed=1, stale=False)
+    _u8(cache.keys).zero_()
+    cache.keys[:, :, 0, 0] = torch.ones((), dtype=code)
+    cache.key_scales.fill_(0.0)
+    cache.key_scales[:, :, 1::2] = 8 * math.log(2043.5 / 2048)
+    top = torch.full((), 100.0 if code == torch.int8 else 104.0).to(code)
+    _u8(cache.values)[:, ::2] = _u8(top)
+    _u8(cache.values)[:, 1::2] = _u8((-top.float()).to(code))
+    cache.value_scales.fill_(1.0)
+    q = torch.zeros(rows, 2, d)
+    q[..., 0] = 1.0
+    q = q.to(dtype)
+    cu, used = _lengths([(200, rows)])
+    _, got = _attend(device, q, cache, table, cu, used, rows, n, (-1, -1), scale=1 / 8)
+    _close(got, q, cache, table, cu, used, (-1, -1), scale=1 / 8)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("code", CODES)
+def test_rows_of_every_kind_are_rounded_once(device, code, dtype):
+    """Decode rows, drafted ones and chunks of one tick, with windows and without."""
+    say("kv8 rounded once", code, dtype)
+    seqs = [(900, 1), (300, 70), (0, 129), (77, 4), (500, 16)]
+    cu, used = _lengths(seqs)
+    cache, table = _pool([c + n for c, n in seqs], 64, 2, 128, code, seed=11)
+    q = torch.randn(int(cu[-1]), 8, 128, generator=torch.Generator().manual_seed(11)).to(dtype)
+    for window in ((-1, 0), (150, 0)):
+        _, got = _attend(device, q, cache, table, cu, used, 129, int(used.max()), window)
+        _close(got, q, cache, table, cu, used, window)
