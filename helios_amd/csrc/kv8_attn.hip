@@ -5,9 +5,9 @@
 //   out = sum_j w_j v_j / sum_j (w_j / s_vj)
 // The value's scale rides on the softmax's exponent: the weights that meet the codes have their
 // maximum at 1 whatever the scales of the values are, and fit fp16 together with the codes, which
-// fp16 holds exactly. q goes into the products as fp16 too, after a power of two that puts its
-// largest element at 2^14: exact for fp16, and for bf16 down to 2^-28 of the largest element
-// (smaller ones within 2^-40 of it). Sums are fp32.
+// fp16 holds exactly. q goes into the products as fp16 too, each row and head after a power of two of
+// its own that puts its largest element at 2^14: exact for fp16, and for bf16 down to 2^-28 of that
+// element (smaller ones within 2^-39 of it). Sums are fp32.
 //
 // Two kernels over a plan's work lists, in one launch where a tick has both, and one that joins splits:
 //   few_kernel    sequences whose (row, query head) pairs of a KV head fit one MFMA's 16 columns
@@ -17,7 +17,7 @@
 //   chunk_kernel  the others: blocks of rows over 64-key tiles, split over their tiles where the
 //                 blocks alone leave CUs without work. Bound by MFMA, the reads of its operands from
 //                 LDS and the softmax, which overlap only in part: 4096 rows that see 4096 keys and
-//                 their own, 32 heads of 128, take 588 us, 700 TFLOP/s.
+//                 their own, 32 heads of 128, take 599 us, 690 TFLOP/s.
 
 #include "kv8_common.h"
 
@@ -811,7 +811,6 @@ template <int DP>
 struct ChunkLds {
   __attribute__((aligned(16))) uint8_t k[2][kChunkTile * chunk_k_row(DP)], v[2][kChunkTile * chunk_v_row(DP)];
   __attribute__((aligned(16))) float k_scale[2][kChunkTile], v_log[2][kChunkTile], v_inverse[2][kChunkTile];
-  uint32_t top[chunk_threads(DP) / 64];
 };
 
 // One item and KV head to a workgroup: wave w owns units 16 RB w .. + 16 RB - 1, (row, head) pairs
@@ -821,6 +820,8 @@ struct ChunkLds {
 // Up to 128 dims a workgroup is 4 waves, and the two on a CU are out of step: one's products run
 // under the other's softmax. 8 waves with 256 units halve the staging but wait in step: 1 % faster
 // on a long prompt, 11 % slower on a tick of chunks, whose blocks and splits are then twice as large.
+// (A power of two for all units of a block would ride on the keys' scales, 2 % of the prompt's time,
+// and lose rows that are 2^28 smaller than their neighbours.)
 // The weights go into P V as two fp16, 22 bits, as those of few rows do: one alone (11 bits) turns the
 // rounding of one bf16 output in ten, and takes 488 us for 588 on the prompt.
 template <typename T, typename C, int DP>
@@ -846,7 +847,7 @@ __device__ __forceinline__ void chunk_items(const RunArgs& a, ChunkLds<DP>& lds,
 
     // Q^T as the MFMA's B operand, and the keys each of this lane's units sees.
     v8 qf[RB][kSteps];
-    float qc;
+    float qc[RB];  // of this lane's units: log2(e) scale, and what undoes q's power of two
     int klo[RB], khi[RB], urow[RB], uhead[RB];
     bool live[RB];
 #pragma unroll
@@ -859,36 +860,32 @@ __device__ __forceinline__ void chunk_items(const RunArgs& a, ChunkLds<DP>& lds,
       klo[rb] = a.s.left >= 0 && at > a.s.left ? at - a.s.left : 0;
       khi[rb] = a.s.right >= 0 ? min(L - 1, beyond(at, a.s.right)) : L - 1;
     }
-    {
-      uint32_t top = 0;
-      uint4 raw[RB][kSteps];
+    uint4 raw[RB][kSteps];
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        const uint16_t* const qp = a.q + (int64_t)(si.x + row0 + urow[rb]) * a.q_row + (int64_t)uhead[rb] * a.q_head;
+    for (int rb = 0; rb < RB; ++rb) {
+      const uint16_t* const qp = a.q + (int64_t)(si.x + row0 + urow[rb]) * a.q_row + (int64_t)uhead[rb] * a.q_head;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const int d = 32 * s + 8 * lg;
-          raw[rb][s] = live[rb] && d < D ? *reinterpret_cast<const uint4*>(qp + d) : hx::zero4();
-          top = largest<T>(raw[rb][s], top);
-        }
+      for (int s = 0; s < kSteps; ++s) {
+        const int d = 32 * s + 8 * lg;
+        raw[rb][s] = live[rb] && d < D ? *reinterpret_cast<const uint4*>(qp + d) : hx::zero4();
       }
-      // One power of two for all units.
-      for (int m = 1; m < 64; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m));
-      if (lane == 0) lds.top[w] = top;
-      __syncthreads();
+    }
 #pragma unroll
-      for (int e = 0; e < kWaves; ++e) top = max(top, lds.top[e]);
-      top = magnitude<T>((uint32_t)__builtin_amdgcn_readfirstlane((int)top));
+    for (int rb = 0; rb < RB; ++rb) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) top = largest<T>(raw[rb][s], top);
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+      top = magnitude<T>(top);
       const float up = fit_up(top);
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          float x[8];
-          widen8<T>(raw[rb][s], x);
-          qf[rb][s] = hx::as_v8<_Float16>(pack8(x, up));
-        }
-      qc = a.scale_log2 * fit_down(top);
+      for (int s = 0; s < kSteps; ++s) {
+        float x[8];
+        widen8<T>(raw[rb][s], x);
+        qf[rb][s] = hx::as_v8<_Float16>(pack8(x, up));
+      }
+      qc[rb] = a.scale_log2 * fit_down(top);
     }
     // Keys that any unit of the wave sees, and those that all of them do.
     int any_lo = 0x7fffffff, any_hi = -1, all_lo = 0, all_hi = 0x7fffffff;
@@ -960,7 +957,7 @@ __device__ __forceinline__ void chunk_items(const RunArgs& a, ChunkLds<DP>& lds,
         *reinterpret_cast<uint4*>(to + 16) = make_uint4(x2.x, x2.y, x3.x, x3.y);
       }
       if (w == 0) {
-        lds.k_scale[b][lane] = lane < cnt ? sreg * qc : 0.f;
+        lds.k_scale[b][lane] = lane < cnt ? sreg : 0.f;
       } else if (w == 1) {
         const ValueScale v = value_scale(lane < cnt ? sreg : 1.f);
         lds.v_log[b][lane] = v.log;
@@ -1030,7 +1027,7 @@ __device__ __forceinline__ void chunk_items(const RunArgs& a, ChunkLds<DP>& lds,
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[kb][rb][e] = fmaf(sc[kb][rb][e], k4[e], l4[e]);
+          for (int e = 0; e < 4; ++e) sc[kb][rb][e] = fmaf(sc[kb][rb][e], k4[e] * qc[rb], l4[e]);
       }
       const bool whole = here == kChunkTile && key0 >= all_lo && key0 + kChunkTile - 1 <= all_hi;
       float mx[RB];

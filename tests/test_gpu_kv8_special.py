@@ -1,4 +1,5 @@
-"""Attention over the 8-bit cache where single roundings show: weights that differ by half an fp16 step."""
+"""Attention over the 8-bit cache where single roundings show: weights that differ by half an fp16 step,
+and queries of very different sizes side by side."""
 
 from __future__ import annotations
 
@@ -72,3 +73,25 @@ def test_rows_of_every_kind_are_rounded_once(device, code, dtype):
     for window in ((-1, 0), (150, 0)):
         _, got = _attend(device, q, cache, table, cu, used, 129, int(used.max()), window)
         _close(got, q, cache, table, cu, used, window)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 40, 130])
+@pytest.mark.parametrize("power", [20, 32, 40, 60, 110])
+def test_queries_far_apart(device, power, rows):
+    """Rows and heads, neighbours of one sequence, up to 2^110 apart: the small ones get their own answer
+    (not the values' mean), the large ones the value of their best key."""
+    say("kv8 queries far apart", power, rows)
+    cu, used = _lengths([(300 - rows, rows), (300 - rows, rows)])
+    cache, table = _pool([300, 300], 64, 2, 64, torch.float8_e4m3fn, seed=21)
+    g = torch.Generator().manual_seed(power + rows)
+    q = 3 * torch.randn(2 * rows, 8, 64, generator=g)
+    large = (torch.arange(2 * rows)[:, None] + torch.arange(8)) % 3 == 0
+    q = torch.where(large[..., None], q * 2.0 ** power, q).to(torch.bfloat16)
+    _, got = _attend(device, q, cache, table, cu, used, rows, 300, (-1, 0))
+    # (A large row's scores are off by more than 1: its bound holds for whatever its keys weigh.)
+    _close(got, q, cache, table, cu, used, (-1, 0))
+    assert torch.isfinite(got).all()
+    # Each row by itself has the same answer.
+    cu, used = _lengths([(299, 1)])
+    _, one = _attend(device, q[rows - 1:rows], cache, table[:1], cu, used, 1, 300, (-1, 0))
+    _close(one, q[rows - 1:rows], cache, table[:1], cu, used, (-1, 0))
