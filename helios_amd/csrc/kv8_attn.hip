@@ -6,8 +6,8 @@
 // The value's scale rides on the softmax's exponent: the weights that meet the codes have their
 // maximum at 1 whatever the scales of the values are, and fit fp16 together with the codes, which
 // fp16 holds exactly. q goes into the products as fp16 too, each row and head after a power of two of
-// its own that puts its largest element at 2^14: exact for fp16, and for bf16 down to 2^-28 of that
-// element (smaller ones within 2^-39 of it). Sums are fp32.
+// its own that puts its largest element at 2^14: exact down to 2^-28 of that element (smaller ones
+// within 2^-39 of it). Sums are fp32.
 //
 // Two kernels over a plan's work lists, in one launch where a tick has both, and one that joins splits:
 //   few_kernel    sequences whose (row, query head) pairs of a KV head fit one MFMA's 16 columns
@@ -505,8 +505,17 @@ __device__ __forceinline__ uint2 ld8_lds_tr8(const void* p) {
   return __builtin_bit_cast(uint2, r);
 }
 
-constexpr float kFewShift = 14.f;  // weights are scaled by 2^14 into fp16, and their remainders stay normal
-constexpr float kFewLazy = 1.f;    // the reference maximum moves when exceeded by this, in log2
+// The score that a softmax's weights are relative to: SHIFT below the largest, so that weights fill
+// fp16 and their remainders stay normal. It moves when a score exceeds that largest one by more than
+// LAZY; SHIFT + LAZY <= 15, all in log2. Past 2^22 fp32's steps are of their size, and its rounding
+// could take a weight past fp16: there it is the largest score itself, and moves with each larger one.
+constexpr float kStepsFit = 0x1p22f;
+__device__ __forceinline__ float reference_of(float most, float shift) {
+  return fabsf(most) < kStepsFit ? most - shift : most;
+}
+__device__ __forceinline__ float moves_past(float ref, float by) { return fabsf(ref) < kStepsFit ? ref + by : ref; }
+
+constexpr float kFewShift = 14.f, kFewLazy = 1.f;
 
 template <int DP>
 struct FewLds {
@@ -617,7 +626,7 @@ __device__ __forceinline__ void few_item(const RunArgs& a, FewLds<DP>& lds, cons
     for (int q = 0; q < kVLoads; ++q) vb[q] = hx::ld16_stream(vr, off, q * kRows * row_bytes);
   };
 
-  float m_run = -INFINITY, l_run = 0.f;
+  float ref = -INFINITY, l_run = 0.f;  // the weights' reference, and their sum
   hx::f32x4_t o[kDims];
 #pragma unroll
   for (int d = 0; d < kDims; ++d) o[d] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -680,15 +689,16 @@ __device__ __forceinline__ void few_item(const RunArgs& a, FewLds<DP>& lds, cons
 #pragma unroll
     for (int e = 2; e < 8; ++e) mx = fmaxf(mx, u[e]);
     mx = hx::max_xor32(hx::max_xor16(mx));
-    const bool move = mx > m_run + kFewLazy;
+    const bool move = mx > moves_past(ref, kFewShift + kFewLazy);
     if (__any(move)) {
-      const float alpha = move ? hx::fast_exp2(m_run - mx) : 1.f;
-      m_run = move ? mx : m_run;
+      const float to = move ? reference_of(mx, kFewShift) : ref;
+      const float alpha = move ? hx::fast_exp2(ref - to) : 1.f;
+      ref = to;
       l_run *= alpha;
 #pragma unroll
       for (int d = 0; d < kDims; ++d) o[d] *= alpha;
     }
-    const float neg = m_run == -INFINITY ? 0.f : kFewShift - m_run;
+    const float neg = ref == -INFINITY ? 0.f : -ref;
     uint32_t pw[4], pr[4];
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
@@ -732,7 +742,7 @@ __device__ __forceinline__ void few_item(const RunArgs& a, FewLds<DP>& lds, cons
     for (int d = 0; d < kDims; ++d)
       *reinterpret_cast<float4*>(&lds.o[w][lr][16 * d + 4 * lg]) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
     if (lg == 0) {
-      lds.m[w][lr] = m_run;
+      lds.m[w][lr] = ref;
       lds.l[w][lr] = l_run;
     }
   }
@@ -799,8 +809,7 @@ __global__ __launch_bounds__(kFewThreads, DP == 256 ? 2 : DP == 128 ? 3 : 4) voi
 
 // ------------------------------------------------------------------------------- chunks
 constexpr int chunk_threads(int dp) { return dp == 256 ? 512 : 256; }
-constexpr float kChunkShift = 7.f;  // 2^7 times weights of up to 2^8 fits fp16
-constexpr float kLazy = 8.f;        // the reference maximum moves when exceeded by this, in log2
+constexpr float kChunkShift = 7.f, kChunkLazy = 8.f;
 
 // Rows of fp16 with 16 and 32 bytes more: 16 keys' fragments, and the 8 rows of 32 bytes that half a
 // wave reads transposed, then cover all banks once.
@@ -970,10 +979,10 @@ __device__ __forceinline__ void chunk_items(const RunArgs& a, ChunkLds<DP>& lds,
     for (int d = 0; d < kDims; ++d)
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) o[d][rb] = hx::f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float m_run[RB], l_run[RB];
+    float ref[RB], l_run[RB];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      m_run[rb] = -INFINITY;
+      ref[rb] = -INFINITY;
       l_run[rb] = 0.f;
     }
 
@@ -1050,7 +1059,7 @@ __device__ __forceinline__ void chunk_items(const RunArgs& a, ChunkLds<DP>& lds,
         for (int kb = 1; kb < 4; ++kb)
           m = fmaxf(m, fmaxf(fmaxf(sc[kb][rb][0], sc[kb][rb][1]), fmaxf(sc[kb][rb][2], sc[kb][rb][3])));
         mx[rb] = hx::max_xor32(hx::max_xor16(m));
-        move[rb] = mx[rb] > m_run[rb] + kLazy;
+        move[rb] = mx[rb] > moves_past(ref[rb], kChunkShift + kChunkLazy);
       }
       bool moved = move[0];
 #pragma unroll
@@ -1058,8 +1067,9 @@ __device__ __forceinline__ void chunk_items(const RunArgs& a, ChunkLds<DP>& lds,
       if (__any(moved)) {
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-          const float alpha = move[rb] ? hx::fast_exp2(m_run[rb] - mx[rb]) : 1.f;
-          m_run[rb] = move[rb] ? mx[rb] : m_run[rb];
+          const float to = move[rb] ? reference_of(mx[rb], kChunkShift) : ref[rb];
+          const float alpha = move[rb] ? hx::fast_exp2(ref[rb] - to) : 1.f;
+          ref[rb] = to;
           l_run[rb] *= alpha;
 #pragma unroll
           for (int d = 0; d < kDims; ++d) o[d][rb] *= alpha;
@@ -1068,7 +1078,7 @@ __device__ __forceinline__ void chunk_items(const RunArgs& a, ChunkLds<DP>& lds,
       v8 pf[2][RB], pf2[2][RB];
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        const float neg = m_run[rb] == -INFINITY ? 0.f : kChunkShift - m_run[rb];
+        const float neg = ref[rb] == -INFINITY ? 0.f : -ref[rb];
         float sum = 0.f;
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
@@ -1132,7 +1142,7 @@ __device__ __forceinline__ void chunk_items(const RunArgs& a, ChunkLds<DP>& lds,
         for (int d = 0; d < kDims; ++d)
           if (16 * d < D)
             *reinterpret_cast<float4*>(a.part_o + p * D + 16 * d + 4 * lg) = make_float4(o[d][rb][0], o[d][rb][1], o[d][rb][2], o[d][rb][3]);
-        if (lg == 0) a.part_ml[p] = make_float2(m_run[rb], l);
+        if (lg == 0) a.part_ml[p] = make_float2(ref[rb], l);
       }
     }
     __syncthreads();  // every wave is done with the last tile before the next item's first is stored

@@ -95,3 +95,46 @@ def test_queries_far_apart(device, power, rows):
     cu, used = _lengths([(299, 1)])
     _, one = _attend(device, q[rows - 1:rows], cache, table[:1], cu, used, 1, 300, (-1, 0))
     _close(one, q[rows - 1:rows], cache, table[:1], cu, used, (-1, 0))
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_small_half_precision_queries_beside_large_ones(device, rows):
+    """The whole range of fp16 in one block, subnormal elements among them, whose keys are large."""
+    say("kv8 fp16 queries far apart", rows)
+    cu, used = _lengths([(300 - rows, rows)])
+    cache, table = _pool([300], 64, 1, 64, torch.int8, seed=22, stale=False)
+    cache.key_scales.mul_(2.0 ** 12)
+    q = torch.randn(rows, 8, 64, generator=torch.Generator().manual_seed(22))
+    q = torch.where((torch.arange(8) % 2 == 0)[:, None], q * 2.0 ** 12, q * 2.0 ** -13).to(torch.float16)
+    _, got = _attend(device, q, cache, table, cu, used, rows, 300, (-1, 0))
+    _close(got, q, cache, table, cu, used, (-1, 0))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_scores_past_the_steps_of_fp32(device, rows, dtype):
+    """Scores up to 2^40, where fp32's own steps reach those of the weights' reference: equal keys share a
+    row, all others are far below it. Scores of equal keys are equal, so the mean of their values is off
+    by the weights' and the output's rounding alone."""
+    say("kv8 large scores", rows, dtype)
+    d, n = 64, 200 + rows
+    cache, table = _pool([n], 64, 1, d, torch.int8, seed=23, stale=False)
+    _u8(cache.keys).zero_()
+    token = torch.zeros(n, dtype=torch.int8)
+    token[:] = 126
+    token[::3] = 127
+    for j in range(-(-n // 64)):
+        part = token[64 * j:64 * j + 64]
+        cache.keys[table[0, j], :part.shape[0], 0, 0] = part
+    cache.value_scales.fill_(1.0)
+    vals = cache.values[table[0].long()].flatten(0, 1)[:n, 0].double()
+    cu, used = _lengths([(200, rows)])
+    q = torch.zeros(rows, 8, d)
+    q[..., 0] = 1 + torch.arange(8) / 8  # exact in both types, scores at any part of fp32's steps
+    q = q.to(dtype)
+    want = torch.stack([vals[:200 + r + 1:3].mean(dim=0) for r in range(rows)])[:, None]
+    mag = torch.stack([vals[:200 + r + 1:3].abs().mean(dim=0) for r in range(rows)])[:, None]
+    for power in range(9, 34):  # scores of 127 * q * 2^power, in powers of two 1.44 times as much
+        cache.key_scales.fill_(2.0 ** power * (1 + 2.0 ** -9))
+        _, got = _attend(device, q, cache, table, cu, used, rows, n, (-1, 0), scale=1.0)
+        off = (got.double().cpu() - want).abs()
+        assert (off <= HALF[dtype] * want.abs() + 2.0 ** -20 * mag).all(), (power, float(off.max()))
