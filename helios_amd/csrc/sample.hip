@@ -802,7 +802,8 @@ __device__ int draw_by_bins(const SampleArgs& a, RowLds& s, const Row& r, int64_
       });
       count = block_sum(s, count);
       mass = block_sum(s, mass);
-      fewest(max((uint32_t)count, 1u), mass);
+      // (None reaches a min_p above 1: the first token stays, whose weight is 1.)
+      fewest(max((uint32_t)count, 1u), count ? mass : 1ull << kFixed);
     }
     const double border = m.p * (double)of;
     const uint64_t target = step == 0 ? nk : step == 2 ? m.target(kept) : (uint64_t)border + ((double)(uint64_t)border < border ? 1 : 0);
