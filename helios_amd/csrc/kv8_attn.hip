@@ -49,13 +49,13 @@ constexpr int kShortJoin = 4;     // splits that a part of a wave joins; a workg
 constexpr int kPlanThreads = 1024;
 
 // Plan header words.
-enum { H_PARTS = 0, H_CHUNK = 1, H_JOIN = 2, H_ERR = 3, H_STAMP = 4, H_SHORT = 12, H_WORDS = 16 };
+enum { H_PARTS = 0, H_CHUNK = 1, H_JOIN = 2, H_ERR = 3, H_STAMP = 4, H_SHORT = 12, H_STAMP2 = 13, H_WORDS = 16 };
 
 __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// What a plan is built for; its runs must agree (the first 8 words are checked on the device).
+// What a plan is built for; its runs must agree, which is checked on the device.
 struct Shape {
   int32_t batch, total_q, max_q, max_k, hq, hkv, head_dim, page;
   int32_t left, right, width;
@@ -393,6 +393,9 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_plan_kernel(PlanArgs a) {
     a.hdr[H_ERR] = err;
     const int32_t stamp[8] = {a.s.batch, a.s.total_q, a.s.max_q, a.s.max_k, a.s.hq, a.s.hkv, a.s.head_dim, a.s.page};
     for (int i = 0; i < 8; ++i) a.hdr[H_STAMP + i] = stamp[i];
+    a.hdr[H_STAMP2] = a.s.left;
+    a.hdr[H_STAMP2 + 1] = a.s.right;
+    a.hdr[H_STAMP2 + 2] = a.s.width;
   }
 }
 
@@ -425,10 +428,11 @@ struct RunArgs {
 // The plan's counts, if it was built for this shape.
 __device__ __forceinline__ bool plan_ok(const RunArgs& a, int4* counts) {
   const int4 h0 = *reinterpret_cast<const int4*>(a.hdr), h1 = *reinterpret_cast<const int4*>(a.hdr + H_STAMP),
-             h2 = *reinterpret_cast<const int4*>(a.hdr + H_STAMP + 4);
+             h2 = *reinterpret_cast<const int4*>(a.hdr + H_STAMP + 4), h3 = *reinterpret_cast<const int4*>(a.hdr + H_SHORT);
   *counts = h0;
   const bool ok = h1.x == a.s.batch && h1.y == a.s.total_q && h1.z == a.s.max_q && h1.w == a.s.max_k && h2.x == a.s.hq &&
-                  h2.y == a.s.hkv && h2.z == a.s.head_dim && h2.w == a.s.page;
+                  h2.y == a.s.hkv && h2.z == a.s.head_dim && h2.w == a.s.page && h3.y == a.s.left && h3.z == a.s.right &&
+                  h3.w == a.s.width;
   if (!ok && hx::wg_x() == 0 && hx::tid_x() == 0) atomicOr(&a.hdr[H_ERR], HX_WERR_PLAN_MISMATCH);
   return ok;
 }

@@ -725,8 +725,9 @@ int hx_kv8_gather(const void* codes, const float* scales, int32_t num_pages, int
  * rows cu_seq_q[b] .. cu_seq_q[b + 1] - 1 of q attend to the seqused_k[b] keys of sequence b, whose
  * pages are block_table[b], row i of n being at position seqused_k[b] - n + i; window_left / right
  * (-1: all) limit the keys around it. out = softmax(scale q k) v, rounded once; a row without a key
- * gets zeros. One plan serves any number of runs with its shape; runs that share a workspace must
- * be ordered. page_size is a multiple of 64, at most 128 query heads share a KV head; scales and q
+ * gets zeros. One plan serves any number of runs with its shape, windows and table width (a run with
+ * others writes nothing and sets HX_WERR_PLAN_MISMATCH); runs that share a workspace must be ordered.
+ * page_size is a multiple of 64, at most 128 query heads share a KV head; scales and q
  * are 16-byte aligned, with strides of q that are multiples of 8, out 4-byte aligned with even
  * strides. kinds (HX_KV8_*): which kinds of rows the tick has; rows of another kind stay unwritten.
  * Pages outside the pool count as no keys and, like lengths past max_q, max_k or the table, set a

@@ -1,5 +1,5 @@
-"""Attention over the 8-bit cache where single roundings show: weights that differ by half an fp16 step,
-and queries of very different sizes side by side."""
+"""Attention over the 8-bit cache where single roundings show (weights that differ by half an fp16 step,
+queries of very different sizes side by side, scores past fp32's small steps), and plans of other runs."""
 
 from __future__ import annotations
 
@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from helios_amd import ops
+from helios_amd import _capi, ops
 from oracle import kv8 as oracle
 from tests.gpu_cases import say
 from tests.test_gpu_kv8 import CODES, DTYPES, HALF, _attend, _pool, _u8
@@ -138,3 +138,26 @@ def test_scores_past_the_steps_of_fp32(device, rows, dtype):
         _, got = _attend(device, q, cache, table, cu, used, rows, n, (-1, 0), scale=1.0)
         off = (got.double().cpu() - want).abs()
         assert (off <= HALF[dtype] * want.abs() + 2.0 ** -20 * mag).all(), (power, float(off.max()))
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("windows,widths", [(((40, 0), (-1, 0)), (5, 5)), (((-1, 0), (40, 0)), (5, 5)), (((-1, 0), (-1, 7)), (5, 5)),
+                                            (((-1, 0), (-1, 0)), (5, 4)), (((-1, 0), (-1, 0)), (4, 5))])
+def test_plan_of_other_windows_or_tables_is_flagged(device, windows, widths, new):
+    """A plan's key ranges follow its windows and its table's width: a run with others writes nothing and
+    says so."""
+    say("kv8 plan of others", windows, widths, new)
+    cu, used = _lengths([(250 - new, new), (180, 1)])
+    cache, table = _pool([250, 181], 64, 1, 64, torch.int8, seed=24)
+    on = ops.Kv8Cache(*(t.to(device) for t in cache))
+    wide = torch.zeros(2, 5, dtype=torch.int32, device=device)
+    wide[:, :table.shape[1]] = table.to(device)
+    q = torch.randn(new + 1, 4, 64, device=device).to(torch.bfloat16)
+    plan = ops.Kv8AttnPlan(cu.to(device), used.to(device), total_q=new + 1, max_q=new, max_k=250, n_q_heads=4, n_kv_heads=1,
+                           head_dim=64, page_size=64, window=windows[0], block_table_width=widths[0])
+    good = plan.run(q, on, wide)
+    assert plan.error_word() == 0 and torch.isfinite(good).all()
+    plan.window, plan.width = windows[1], widths[1]
+    out = torch.full_like(q, 3.0)
+    plan.run(q, on, wide, out=out)
+    assert plan.error_word() == _capi.HX_WERR_PLAN_MISMATCH and (out == 3).all()
