@@ -1294,6 +1294,8 @@ int check_shape(const Shape& s) {
   if (s.head_dim % 16 || s.head_dim > 256 || s.page % 64 || s.hq / s.hkv > 128 || s.max_k > 0x7fffff00 - s.page ||
       (int64_t)s.hkv * s.head_dim > (1 << 22) || s.hkv > 1024)
     return HX_E_UNSUPPORTED;  // a tile must fit a buffer resource, item indexes 32 bits
+  // The plan counts the few rows' tiles and starts, and a part's past their end, in 32 bits.
+  if ((int64_t)s.batch * (s.max_k / kFewTile + 2 + kFewStart) > 0x7fffffff - 2 * kFewMost) return HX_E_UNSUPPORTED;
   return HX_OK;
 }
 

@@ -971,7 +971,7 @@ class Kv8AttnPlan:
                                                         page_size)
         if not self.ws_bytes:
             raise ValueError("Unsupported attention shape: head_dim must be a multiple of 16 from 16 to 256, page_size "
-                             "of 64, and at most 128 query heads may share a KV head.")
+                             "of 64, at most 128 query heads may share a KV head, and batch * max_k stays below 2^36.")
         self.device, self.width = device, width
         self._shape = (batch, total_q, max_q, max_k, n_q_heads, n_kv_heads, head_dim)
         self.page_size, self.window = page_size, (left, right)

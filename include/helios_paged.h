@@ -732,7 +732,8 @@ int hx_kv8_gather(const void* codes, const float* scales, int32_t num_pages, int
  * strides. kinds (HX_KV8_*): which kinds of rows the tick has; rows of another kind stay unwritten.
  * Pages outside the pool count as no keys and, like lengths past max_q, max_k or the table, set a
  * bit of the error word at hx_kv8_attn_error_word_offset() of the workspace. The workspace is
- * hx_kv8_attn_workspace_bytes() bytes (0: unsupported), 256-byte aligned.
+ * hx_kv8_attn_workspace_bytes() bytes (0: unsupported, also where batch * max_k is 2^36 or about),
+ * 256-byte aligned.
  */
 size_t hx_kv8_attn_workspace_bytes(int32_t batch, int32_t total_q, int32_t max_q, int32_t max_k,
                                    int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,

@@ -155,3 +155,15 @@ def test_oracle_sample():
     assert oracle.sample(logits, u, top_p=torch.full((8,), 0.6))[0].tolist() == [2, 2, 2, 1, 1, 1, 1, 2]
     assert oracle.sample(logits, u, min_p=torch.full((8,), 0.75))[0].tolist() == [2, 2, 2, 1, 1, 1, 1, 2]
     assert oracle.sample(logits, u, temperature=torch.zeros(8))[0].tolist() == [2] * 8
+
+
+def test_attention_refuses_more_tiles_than_the_plan_counts():
+    """Sequences of few rows are dealt by their 32-key tiles, counted in 32 bits: 2^16 sequences of up to
+    2^20 keys are 2^31 of them."""
+    lib = _capi.lib()
+    size = lib.hx_kv8_attn_workspace_bytes
+    for batch, max_k in ((1 << 16, 1 << 20), (1 << 20, 1 << 16), (40, 0x7ffffd00), (1 << 28, 1)):
+        assert size(batch, batch, 1, max_k, 1, 1, 16, 256) == 0
+        assert lib.hx_kv8_attn_plan(MIB, 2 * MIB, batch, batch, 1, max_k, 1, 1, 16, 256, 1 << 20, -1, 0, 256 * MIB, 1 << 60,
+                                    None) == NOT
+    assert size((1 << 16) - 64, 1 << 16, 1, 1 << 20, 1, 1, 16, 256) > 0 and size(31, 31, 1, 0x7ffffd00, 1, 1, 16, 256) > 0
