@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kThreads) void kv8_write_kernel(WriteArgs a) {
       for (int e = 0; e < 8; ++e) {
         const float p = __shfl(x[e], other);
         z[e] = mine ? fma((double)x[e] * w[e], (double)c[e], (double)(low ? -p : p) * v[e] * (double)s[e]) : 0.;
-        const uint64_t b = __builtin_bit_cast(uint64_t, z[e]) & 0x7fffffffffffffffull;
+        const uint64_t b = hx::raw_bits(z[e]) & 0x7fffffffffffffffull;
         top = b > top ? b : top;
       }
 #pragma unroll
