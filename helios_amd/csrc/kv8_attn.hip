@@ -17,7 +17,8 @@
 //   chunk_kernel  the others: blocks of rows over 64-key tiles, split over their tiles where the
 //                 blocks alone leave CUs without work. Bound by MFMA, the reads of its operands from
 //                 LDS and the softmax, which overlap only in part: 4096 rows that see 4096 keys and
-//                 their own, 32 heads of 128, take 599 us, 690 TFLOP/s.
+//                 their own, 32 heads of 128, take 603 us, 685 TFLOP/s, the matrix units busy for 43 %
+//                 of the time. (The 16-bit cache's kernel takes 350: a prompt is faster from there.)
 
 #include "kv8_common.h"
 
@@ -41,8 +42,8 @@ constexpr int kFewMost = 256;     // and at most
 constexpr int kChunkUnits = 128;  // (row, head) pairs of a chunk block
 constexpr int kChunkTile = 64;
 // Workgroups below which row blocks are split, and into about as many. (512 would be on the CUs at
-// once, but partial results cost too: decoders beside chunks whose blocks are 344 workgroups take 96 us
-// split for 384, 97 for 512, 99 as they are, 105 for 768.)
+// once, but partial results cost too: decoders beside chunks whose blocks are 344 workgroups take 107 us
+// split for 384, 110 for 512, 113 as they are, 115 for 768.)
 constexpr int kChunkWGs = 384;
 constexpr int kChunkLeast = 4;    // tiles of a split, at least
 constexpr int kShortJoin = 4;     // splits that a part of a wave joins; a workgroup does more
@@ -465,8 +466,10 @@ __device__ __forceinline__ uint32_t largest(uint4 u, uint32_t top) {
 template <typename T>
 __device__ __forceinline__ uint32_t magnitude(uint32_t top) { return __float_as_uint(hx::Elem<T>::lo(top)); }
 
-// A value's scale as the softmax takes it. A NaN makes the weight NaN through its logarithm, and has
-// an inverse that leaves the weight 0 of a row that does not see the key alone.
+// A value's scale as the softmax takes it. (Sums of weights over scales fit fp32 for 2^17 keys of scales
+// above 2^-96; values below those, 1e-26, may come out as 0. Weights times scales below 2^-126 of the
+// row's largest are 0.) A NaN makes the weight NaN through its logarithm, and has an inverse that
+// leaves the weight 0 of a row that does not see the key alone.
 struct ValueScale {
   float log, inverse;
 };
@@ -815,8 +818,8 @@ __global__ __launch_bounds__(kFewThreads, DP == 256 ? 2 : DP == 128 ? 3 : 4) voi
 constexpr int chunk_threads(int dp) { return dp == 256 ? 512 : 256; }
 constexpr float kChunkShift = 7.f, kChunkLazy = 8.f;
 
-// Rows of fp16 with 16 and 32 bytes more: 16 keys' fragments, and the 8 rows of 32 bytes that half a
-// wave reads transposed, then cover all banks once.
+// Rows of fp16 with 16 and 32 bytes more, so that neighbouring rows begin in other banks. Conflicts are
+// left: 51M cycles of the 357M that the CUs are busy on the prompt, by which accesses is not known.
 constexpr int chunk_k_row(int dp) { return 2 * dp + 16; }
 constexpr int chunk_v_row(int dp) { return 2 * dp + 32; }
 
@@ -832,11 +835,12 @@ struct ChunkLds {
 // loads are in flight for a whole tile, and one barrier a tile suffices.
 // Up to 128 dims a workgroup is 4 waves, and the two on a CU are out of step: one's products run
 // under the other's softmax. 8 waves with 256 units halve the staging but wait in step: 1 % faster
-// on a long prompt, 11 % slower on a tick of chunks, whose blocks and splits are then twice as large.
+// on a long prompt, 11 % slower on a tick of chunks, whose blocks and splits are then twice as large
+// (both with weights of one fp16).
 // (A power of two for all units of a block would ride on the keys' scales, 2 % of the prompt's time,
 // and lose rows that are 2^28 smaller than their neighbours.)
 // The weights go into P V as two fp16, 22 bits, as those of few rows do: one alone (11 bits) turns the
-// rounding of one bf16 output in ten, and takes 488 us for 588 on the prompt.
+// rounding of one bf16 output in ten, and takes 499 us on the prompt for 603.
 template <typename T, typename C, int DP>
 __device__ __forceinline__ void chunk_items(const RunArgs& a, ChunkLds<DP>& lds, const int4& counts, int wg, int n_wg) {
   typedef hx::f16x8_t v8;
@@ -1161,7 +1165,7 @@ __global__ __launch_bounds__(chunk_threads(DP), 2) void kv8_chunk_kernel(RunArgs
 }
 
 // A tick of both: its few rows' reads go beside the chunks' products, up to 128 dims (where both take
-// 4 waves). 32 decoders and two chunks: 96 us, 107 in two launches, of 31 and 68.
+// 4 waves). 32 decoders and two chunks: 107 us, 116 in two launches, of 31 and 84.
 template <typename T, typename C, int DP>
 __global__ __launch_bounds__(kFewThreads, 2) void kv8_both_kernel(RunArgs a, int n_chunk, int n_few) {
   static_assert(chunk_threads(DP) == kFewThreads);

@@ -1008,9 +1008,10 @@ class Kv8AttnPlan:
             out: torch.Tensor | None = None) -> torch.Tensor:
         """Attention for one layer: ``query`` ``[total_q, Hq, d]`` bfloat16 or float16, packed, over
         the pages of ``cache`` that ``block_table`` (int32 ``[batch, width]``) lists. Returns
-        ``[total_q, Hq, d]`` like ``query``: in fp32, rounded once. A row without a key gets zeros;
-        output rows behind the last sequence stay as they were. A key or value that was stored as
-        NaN makes the rows that see it NaN."""
+        ``[total_q, Hq, d]`` like ``query``: weights of 22 bits, sums in fp32, rounded once. A row without a
+        key gets zeros; output rows behind the last sequence stay as they were. A key or value that was
+        stored as NaN makes the rows that see it NaN. A key counts while its weight times its value's
+        scale is at least 2^-126 of the row's largest; outputs below 2^-80 may be 0."""
         keys, values, key_scales, value_scales = cache
         device, index = self.device, self.device.index
         for t in (query, keys, values, key_scales, value_scales, block_table):
@@ -1219,8 +1220,9 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: 
     one. The token drawn is the first in that order whose cumulative weight passes ``uniforms[r]``
     of theirs. A temperature of 0 or less takes the first token (as ``torch.argmax``, logprob 0), as
     does a row whose largest logit is +inf or NaN; a row of -inf alone gives -1 and -inf. Limits are
-    float32 (``top_k`` int32) ``[rows]``, None: none; a ``temperature`` of None is 1. Weights are
-    exact to 2^-45 of the largest and sums of them have no order: equal inputs give equal tokens."""
+    float32 (``top_k`` int32) ``[rows]``, None: none; a ``temperature`` of None is 1, and others are held
+    to [1e-30, 1e30]. Weights are within 2^-44.6 of the largest, those below 2^-45 of it count as 0, and
+    sums of them have no order: equal inputs give equal tokens."""
     device = _require_gpu(logits, uniforms)
     dtype = _capi.HX_DTYPE_FP32 if logits.dtype == torch.float32 else _SUPPORTED.get(logits.dtype)
     if dtype is None or logits.ndim != 2 or logits.shape[1] < 1:

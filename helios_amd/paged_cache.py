@@ -95,7 +95,7 @@ class KVPagePool:
     With ``kv_dtype`` (float8_e4m3fn or int8) the pool holds 8-bit codes, and
     ``key_scales[l]`` / ``value_scales[l]`` float32 ``[num_pages, n_kv_heads, page_size]`` what
     they are scaled by (``ops.Kv8Cache``; ``kv8(l)`` is a layer's): 0.52 of the 16-bit memory at
-    heads of 128. Batches write and read it through the same calls; the shared-prefix cascade,
+    heads of 128, faster decode ticks and slower chunks of prompts. Batches write and read it through the same calls; the shared-prefix cascade,
     overlapped streams and selected blocks are for 16-bit pools."""
 
     def __init__(self, config: Qwen3Config, num_pages: int, *, device: torch.device,

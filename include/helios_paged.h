@@ -725,11 +725,12 @@ int hx_kv8_gather(const void* codes, const float* scales, int32_t num_pages, int
  * rows cu_seq_q[b] .. cu_seq_q[b + 1] - 1 of q attend to the seqused_k[b] keys of sequence b, whose
  * pages are block_table[b], row i of n being at position seqused_k[b] - n + i; window_left / right
  * (-1: all) limit the keys around it. out = softmax(scale q k) v, rounded once; a row without a key
- * gets zeros. One plan serves any number of runs with its shape, windows and table width (a run with
- * others writes nothing and sets HX_WERR_PLAN_MISMATCH); runs that share a workspace must be ordered.
- * page_size is a multiple of 64, at most 128 query heads share a KV head; scales and q
- * are 16-byte aligned, with strides of q that are multiples of 8, out 4-byte aligned with even
- * strides. kinds (HX_KV8_*): which kinds of rows the tick has; rows of another kind stay unwritten.
+ * gets zeros. A key counts while its weight times its value's scale is at least 2^-126 of the row's
+ * largest; outputs below 2^-80 may be 0. One plan serves any number of runs with its shape, windows
+ * and table width (a run with others writes nothing and sets HX_WERR_PLAN_MISMATCH); runs that share a
+ * workspace must be ordered. page_size is a multiple of 64, at most 128 query heads share a KV head;
+ * scales and q are 16-byte aligned, with strides of q that are multiples of 8, out 4-byte aligned with
+ * even strides. kinds (HX_KV8_*): which kinds of rows the tick has; rows of another kind stay unwritten.
  * Pages outside the pool count as no keys and, like lengths past max_q, max_k or the table, set a
  * bit of the error word at hx_kv8_attn_error_word_offset() of the workspace. The workspace is
  * hx_kv8_attn_workspace_bytes() bytes (0: unsupported, also where batch * max_k is 2^36 or about),
@@ -789,11 +790,11 @@ int hx_logit_rules(const void* logits, int64_t logits_row_stride, int64_t rows,
  * index): the first n tokens are kept, the least of top_k[r] (<= 0: all), of the least number whose
  * weights reach top_p[r] of the first top_k tokens', and of those with e_v >= min_p[r], at least one;
  * token_ids[r] is the first whose cumulative weight passes uniforms[r] (in [0, 1)) of theirs, and
- * logprobs[r] the log of its share of them. t <= 0: the first token, 0. A row whose largest logit
- * is +inf or NaN (which counts as larger): that token, 0. A row of -inf alone: -1, -inf. Weights
- * below 2^-45 of the largest count as 0. temperature (1), top_k, top_p, min_p and logprobs may be
- * NULL. At most 2^18 tokens and 2^20 rows. The workspace is hx_sample_workspace_bytes() bytes,
- * 8-byte aligned; calls that share one must be ordered.
+ * logprobs[r] the log of its share of them. t <= 0: the first token, 0; other t are held to [1e-30,
+ * 1e30]. A row whose largest logit is +inf or NaN (which counts as larger): that token, 0. A row of
+ * -inf alone: -1, -inf. Weights below 2^-45 of the largest count as 0. temperature (1), top_k, top_p,
+ * min_p and logprobs may be NULL. At most 2^18 tokens and 2^20 rows. The workspace is
+ * hx_sample_workspace_bytes() bytes, 8-byte aligned; calls that share one must be ordered.
  */
 size_t hx_sample_workspace_bytes(int64_t rows, int64_t vocab);
 int hx_sample_tokens(const void* logits, int64_t logits_row_stride, int64_t rows, int64_t vocab,
