@@ -878,7 +878,8 @@ def kv8_norm_rope_append(
     rotation of queries and keys, and the quantised append, in one launch. Returns the
     normalised, rotated queries (``out`` if given), in fp32 and rounded once
     (``qk_norm_rope_append`` rounds between the norm and the rotation, as its reference does).
-    Keys go on in fp64 until their scales and codes are rounded. Arguments as there, ``write_slots`` as for ``kv8_append``."""
+    Keys, but for the root of their squares' mean, are in fp64 until their scales and codes are
+    rounded. Arguments as there, ``write_slots`` as for ``kv8_append``."""
     device = _gpu_of((queries, keys, values, q_norm_weight, k_norm_weight, cos, sin, positions, *cache, write_slots))
     code, pages, page_size, n_kv, head_dim = _check_kv8(cache)
     dtype = _check_kv8_rows(keys, values, write_slots, n_kv, head_dim)

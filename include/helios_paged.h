@@ -696,8 +696,9 @@ int hx_kv8_append(void* k_codes, void* v_codes, float* k_scales, float* v_scales
 /*
  * hx_qk_norm_rope_append into the 8-bit cache: RMSNorm of every query and key head, the position
  * rotation (tables of rope_rows rows of head_dim; positions are clamped to them), queries to
- * q_out in fp32, rounded once, values quantised as hx_kv8_append does, and keys in fp64 until their
- * scales and codes are rounded. Norm weights and tables are 16-byte aligned.
+ * q_out in fp32, rounded once, values quantised as hx_kv8_append does, and keys, but for the root of
+ * their squares' mean, in fp64 until their scales and codes are rounded. Norm weights and tables are
+ * 16-byte aligned.
  */
 int hx_kv8_norm_rope_append(const void* q, int64_t q_row_stride, int64_t q_head_stride,
                             const void* k, int64_t k_row_stride, int64_t k_head_stride,
