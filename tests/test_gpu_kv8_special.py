@@ -161,3 +161,33 @@ def test_plan_of_other_windows_or_tables_is_flagged(device, windows, widths, new
     out = torch.full_like(q, 3.0)
     plan.run(q, on, wide, out=out)
     assert plan.error_word() == _capi.HX_WERR_PLAN_MISMATCH and (out == 3).all()
+
+
+@pytest.mark.parametrize("power", [-78, -40, 60, 110])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_values_of_every_size(device, rows, power):
+    """Values 2^-78 to 2^110 of the usual, at 40000 keys: the outputs are as much smaller or larger. (The
+    scales' logarithms, up to 2^7, are off by 2^-17 with the scores' last places: within twice e.)"""
+    say("kv8 values of every size", rows, power)
+    n = 40000
+    cu, used = _lengths([(n - rows, rows)])
+    cache, table = _pool([n], 64, 1, 16, torch.float8_e4m3fn, seed=25, stale=False)
+    q = 2 * torch.randn(rows, 4, 16, generator=torch.Generator().manual_seed(25)).to(torch.bfloat16)
+    far = cache._replace(value_scales=cache.value_scales * 2.0 ** power)
+    _, got = _attend(device, q, far, table, cu, used, rows, n, (-1, 0))
+    _close(got.double() * 2.0 ** -power, q, cache, table, cu, used, (-1, 0))
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_rows_of_zeros_beside_large_values(device, rows):
+    """Values stored as zeros (a scale of 2^-100) count in the weights' sum beside values of 2^20."""
+    say("kv8 zeros beside large values", rows)
+    n = 3000
+    cu, used = _lengths([(n - rows, rows)])
+    cache, table = _pool([n], 64, 1, 64, torch.int8, seed=26, stale=False)
+    cache.value_scales.mul_(2.0 ** 20)
+    _u8(cache.values)[:, ::3] = 0
+    cache.value_scales[:, :, ::3] = 2.0 ** -100
+    q = torch.randn(rows, 4, 64, generator=torch.Generator().manual_seed(26)).to(torch.bfloat16)
+    _, got = _attend(device, q, cache, table, cu, used, rows, n, (-1, 0))
+    _close(got, q, cache, table, cu, used, (-1, 0))
